@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -51,11 +52,16 @@ def build_lib():
     embedded = obj_dir / 'fused_source.cpp'
     embedded.write_text('namespace cpde {\nextern const char* const kFusedSource;\n'
                         'const char* const kFusedSource = R"CPDE_SRC(' + text + ')CPDE_SRC";\n}\n')
-    objs = []
-    for src in [CSRC / 'kernels.hip', CSRC / 'api.hip', CSRC / 'tables.cpp', CSRC / 'jit.cpp', embedded]:
-        obj = obj_dir / (src.name + '.o')
+    sources = [CSRC / name for name in ('attention.hip', 'kernels.hip', 'api.hip', 'embedding.hip', 'dropout.hip',
+                                        'tables.cpp', 'jit.cpp')] + [embedded]
+    objs = [obj_dir / (src.name + '.o') for src in sources]
+
+    def compile_one(pair):
+        src, obj = pair
         _run([hipcc(), *HIP_FLAGS, '-I', ROOT / 'include', '-c', src, '-o', obj])
-        objs.append(obj)
+
+    with ThreadPoolExecutor(4) as pool:
+        list(pool.map(compile_one, zip(sources, objs)))
     tmp = LIB.with_suffix('.so.tmp')
     _run([hipcc(), *HIP_FLAGS, '-shared', '-o', tmp, *objs, '-lhiprtc'])
     os.replace(tmp, LIB)

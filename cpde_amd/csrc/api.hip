@@ -10,7 +10,6 @@
 
 #include "common.hpp"
 
-struct cpde_device_s : cpde::Device {};
 struct cpde_net_s : cpde::Net {};
 struct cpde_plan_s : cpde::Plan {};
 struct cpde_stacks_s : cpde::Stacks {};
@@ -194,29 +193,6 @@ static void swap_binding(Net& n, Plan& p, Stacks& s) {
     std::swap(n.capacity, s.capacity);
     std::swap(p.input, s.input);
     ++n.generation;
-}
-
-template <class F>
-static int guarded(F body) {
-    try {
-        body();
-        return CPDE_OK;
-    } catch (const invalid& e) {
-        set_error(e.what());
-        return CPDE_EINVAL;
-    } catch (const compile_error& e) {
-        set_error(e.what());
-        return CPDE_ECOMPILE;
-    } catch (const device_error& e) {
-        set_error(e.what());
-        return CPDE_EDEVICE;
-    } catch (const std::bad_alloc&) {
-        set_error("host allocation failed");
-        return CPDE_EDEVICE;
-    } catch (const std::exception& e) {
-        set_error(e.what());
-        return CPDE_EDEVICE;
-    }
 }
 
 // Re-raise the failure of a nested entry point with its own error class.
@@ -1450,7 +1426,8 @@ extern "C" {
 
 const char* cpde_last_error(void) { return cpde::last_error.c_str(); }
 
-int cpde_device_open(int ordinal, cpde_device** out) {
+// A device on a stream of its own, or (own false) on the caller's.
+static int open_device(int ordinal, bool own, void* stream, cpde_device** out) {
     return guarded([&] {
         require(out != nullptr, "null output");
         int count = 0;
@@ -1462,7 +1439,9 @@ int cpde_device_open(int ordinal, cpde_device** out) {
         hipDeviceProp_t prop;
         HIP_CHECK(hipGetDeviceProperties(&prop, ordinal));
         d->compute_units = prop.multiProcessorCount;
-        HIP_CHECK(hipStreamCreateWithFlags(&d->stream, hipStreamNonBlocking));
+        d->own_stream = own;
+        if (own) HIP_CHECK(hipStreamCreateWithFlags(&d->stream, hipStreamNonBlocking));
+        else d->stream = static_cast<hipStream_t>(stream);
         {
             // this GPU's address of the static scratch (the device is current)
             void* ptr = nullptr;
@@ -1479,6 +1458,12 @@ int cpde_device_open(int ordinal, cpde_device** out) {
         HIP_CHECK(hipHostMalloc(&d->host_summary, sizeof(cpde_graph_summary), hipHostMallocDefault));
         *out = d.release();
     });
+}
+
+int cpde_device_open(int ordinal, cpde_device** out) { return open_device(ordinal, true, nullptr, out); }
+
+int cpde_device_open_on(int ordinal, void* stream, cpde_device** out) {
+    return open_device(ordinal, false, stream, out);
 }
 
 int cpde_device_close(cpde_device* dev) {
@@ -1499,7 +1484,7 @@ int cpde_device_close(cpde_device* dev) {
         (void)hipFree(dev->scalar_block);
         (void)hipHostFree(dev->host_block);
         (void)hipHostFree(dev->host_summary);
-        (void)hipStreamDestroy(dev->stream);
+        if (dev->own_stream) (void)hipStreamDestroy(dev->stream);
         delete dev;
     });
 }
@@ -2434,7 +2419,8 @@ const char* cpde_trace_name(int kind) {
         "compose_forward", "compose_adjoint", "gemm_forward",   "gemm_transposed", "gemm_wgrad",
         "split_reduce",    "bias_grad",       "activate",       "cost",            "reduce",
         "optimizer",       "other",           "fused_input",    "fused_forward",   "fused_backward",
-        "fused_output_backward", "network_forward", "network_backward", "network_epoch"};
+        "fused_output_backward", "network_forward", "network_backward", "network_epoch",
+        "attention", "attention_gradient", "embedding", "dropout"};
     return kind >= 0 && kind < kTraceKinds ? names[kind] : "";
 }
 
@@ -2480,6 +2466,7 @@ int cpde_capture_begin(cpde_device* dev) {
         require(dev, "null argument");
         require(!dev->capturing, "a capture is already open on this device");
         require(!dev->tracing, "tracing times every launch with events; a capture cannot hold them");
+        require(dev->stream != nullptr, "the default stream cannot be captured: open the device on another");
         flush_reduce(*dev);
         dev->capture_nets.clear();
         for (Net* n : dev->nets) n->arena_wanted = n->separate = false;

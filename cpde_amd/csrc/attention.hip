@@ -1,0 +1,942 @@
+// Attention over sets and sequences, and its gradient.
+#include <cmath>
+
+#include "attention.hpp"
+
+namespace cpde {
+namespace {
+
+struct Attention {
+    Device* dev = nullptr;
+    cpde_attention_shape shape{};
+    float* work = nullptr;
+};
+
+// Keys of a tile of the forward and of the queries' gradients.
+template <class T>
+constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
+// Queries of a tile of the keys' gradients.
+constexpr int kQueries = 32;
+// Workgroups a CU's registers have to hold.
+template <class T, int DP>
+constexpr int kGroups = DP * sizeof(T) <= 256 ? 2 : 1;
+
+// ---- forward --------------------------------------------------------------------------
+// One pass over the keys with a running maximum and sum.  Scores are computed
+// transposed (keys x queries), so that a lane holds 16 of every 32 keys of ONE
+// query: its maximum, sum and rescaling are its own, but for one exchange with lane
+// ^ 32, and its probabilities are, in place, the fragment that multiplies the
+// transposed values into out (head columns x queries).  Queries stay in registers.
+// The reference that the exponents are taken against follows the maximum only when
+// that has grown by more than 2^8: sums stay far inside float and the rescaling of
+// the output, 16 products per 32 columns, is rare.
+template <class T, int DP>
+__global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(AttentionArgs a) {
+    constexpr int N = kKeys<T>, kSub = N / 32, kBlocks = DP / 32, kSteps = DP / 16;
+    using L = Tile<T, DP>;
+    __shared__ __align__(16) char lds[2][2][N * L::kRowBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
+    const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;  // (long rows of a causal band first)
+    const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
+    const Band band(a, b);
+    const int rows = a.queries * a.group;
+    const int row = tile * kBlockRows + wave * kWaveRows + (lane & 31);
+    const int query = row / a.group, head = kv * a.group + row % a.group;
+    const bool live = row < rows && query < band.ql;
+    const int lo = live ? band.key_lo(query) : 0, hi = live ? band.key_hi(query) : 0;
+
+    Frag<T> q[kSteps];
+    load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
+
+    // the keys that the workgroup's rows, and this wave's, see at all, and those that
+    // all of the wave's rows see
+    const auto first_row = [&](int r) { return min(r / a.group, band.ql - 1); };
+    const int block_first = tile * kBlockRows, wave_first = block_first + wave * kWaveRows;
+    const bool any = block_first / a.group < band.ql, wave_any = wave_first / a.group < band.ql;
+    int t0 = any ? band.key_lo(first_row(block_first)) / N : 0;
+    int t1 = any ? (band.key_hi(first_row(block_first + kBlockRows - 1)) + N - 1) / N : 0;
+    if (a.splits > 1) {
+        const int share = (max(t1 - t0, 0) + a.splits - 1) / a.splits;
+        t0 += split * share;
+        t1 = min(t1, t0 + share);
+    }
+    const int wave_lo = wave_any ? band.key_lo(first_row(wave_first)) : 0;
+    const int wave_hi = wave_any ? band.key_hi(first_row(wave_first + kWaveRows - 1)) : 0;
+    const int full_lo = band.key_lo(first_row(wave_first + kWaveRows - 1));
+    const int full_hi = wave_any && (wave_first + kWaveRows - 1) / a.group < band.ql ? band.key_hi(first_row(wave_first)) : 0;
+
+    TileLoader<T, DP, N> kload, vload;
+    kload.start(a.k.token, a.dim, a.wide_in);
+    vload.start(a.v.token, a.dim, a.wide_in);
+    const char* kbase = reinterpret_cast<const char*>(head_row<const T>(a.k, b, 0, kv));
+    const char* vbase = reinterpret_cast<const char*>(head_row<const T>(a.v, b, 0, kv));
+    const auto load = [&](int t, int buffer) {
+        const int64_t first = int64_t(t) * N;
+        kload.load(lds[buffer][0], kbase + first * kload.stride, band.kl - t * N, wave);
+        vload.load(lds[buffer][1], vbase + first * vload.stride, band.kl - t * N, wave);
+    };
+
+    Acc out[kBlocks] = {};
+    float reference = -INFINITY, sum = 0;
+    if (t0 < t1) {
+        for (int i = 0; i < 4; ++i) kload.clear(lds[i >> 1][i & 1]);
+        if (kload.direct && a.dim < DP) __syncthreads();
+        load(t0, 0);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int buffer = (t - t0) & 1;
+        arrived();
+        __syncthreads();
+        if (t + 1 < t1) load(t + 1, buffer ^ 1);
+        const int first = t * N;
+        if (first >= wave_hi || first + N <= wave_lo) continue;
+        const char *keys = lds[buffer][0], *values = lds[buffer][1];
+        Acc s[kSub];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            s[u] = Acc{};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) s[u] = mma(L::row(keys, 32 * u + (lane & 31), i, half), q[i], s[u]);
+        }
+        if (first < full_lo || first + N > full_hi) {
+#pragma unroll
+            for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = first + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
+                    s[u][i] = key >= lo && key < hi ? s[u][i] : -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+        top = halves_max(top) * a.scale2;
+        const bool grown = top > reference + 8.f;
+        if (__any(grown)) {
+            const float next = grown ? top : reference, by = grown ? exp2_fast(reference - next) : 1.f;
+            reference = next;
+            sum *= by;
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) out[d] *= by;
+        }
+        const float base = reference == -INFINITY ? 0.f : reference;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = exp2_fast(fmaf(s[u][i], a.scale2, -base));
+                sum += s[u][i];
+            }
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const Frag<T> p = as_fragment<T>(s[u], i);
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) out[d] = mma(L::column(values, d, 2 * u + i, lane), p, out[d]);
+            }
+    }
+    sum = halves_sum(sum);
+    if (row >= rows) return;
+    if (a.splits > 1) {
+        const int64_t at = (int64_t(split) * a.pairs + pair) * rows + row;
+        if (half == 0) {
+            a.part_stats[2 * at] = reference;
+            a.part_stats[2 * at + 1] = sum;
+        }
+        if (sum != 0)
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d)
+                store_column(a.part + at * a.dim, out[d], 1.f, d, half, a.dim, a.dim % 4 == 0);
+        return;
+    }
+    const float by = sum == 0 ? 0.f : 1.f / sum;
+    T* to = head_row<T>(a.out, b, query, head);
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) store_column(to, out[d], by, d, half, a.dim, a.wide_out);
+    if (a.lse && half == 0)
+        a.lse[(int64_t(b) * a.kv_heads * a.group + head) * a.queries + query] =
+            sum == 0 ? -INFINITY : reference * kLn2 + logf(sum);
+}
+
+// ---- few query rows: a vector kernel -----------------------------------------------------
+// Up to eight query rows of a key head read each key and value once, as they come
+// from memory: LANES lanes hold a key's columns, eight each, and every row's query.
+// Scores are summed over the lanes; each group of lanes keeps its own maximum and
+// sum, joined at the end over the groups, the waves and (through memory, in
+// attention_join_k) the splits.  Bound: HBM.
+template <int LANES>
+__device__ inline float sum_lanes(float x) {
+    // by cross-lane moves within rows of 16: neighbours, pairs, then mirror images
+    const auto move = [](float v, auto control) {
+        return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(control)::value, 0xf, 0xf, true));
+    };
+    x += move(x, std::integral_constant<int, 0xB1>{});                    // quad_perm [1,0,3,2]
+    x += move(x, std::integral_constant<int, 0x4E>{});                    // quad_perm [2,3,0,1]
+    if (LANES >= 8) x += move(x, std::integral_constant<int, 0x141>{});   // row_half_mirror
+    if (LANES >= 16) x += move(x, std::integral_constant<int, 0x140>{});  // row_mirror
+    return x;
+}
+
+template <class T>
+__device__ inline void load8(float* v, const T* p, int left, bool wide) {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int part = 0; part < 8; part += N) {
+        if (wide) {
+            vec<T, N> in = {};
+            if (part < left) in = *reinterpret_cast<const vec<T, N>*>(p + part);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[part + j] = float(in[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[part + j] = part + j < left ? float(p[part + j]) : 0.f;
+        }
+    }
+}
+
+template <class T, int LANES, int R>
+__global__ __launch_bounds__(256) void attention_step_k(AttentionArgs a) {
+    constexpr int kGroupsOfWave = 64 / LANES, kAtOnce = 4 * kGroupsOfWave, kDeep = 4;
+    __shared__ float shared[4][R][LANES * 8 + 2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in = lane % LANES, group = lane / LANES;
+    const int pair = blockIdx.x % a.pairs, split = blockIdx.x / a.pairs;
+    const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
+    const Band band(a, b);
+    const int rows = a.queries * a.group, left = a.dim - in * 8;
+    float q[R][8], acc[R][8] = {}, top[R], sum[R];
+    int lo[R], hi[R], from = band.kl, to = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int query = r / a.group;
+        const bool live = r < rows && query < band.ql;
+        lo[r] = live ? band.key_lo(query) : 0;
+        hi[r] = live ? band.key_hi(query) : 0;
+        if (lo[r] < hi[r]) {
+            from = min(from, lo[r]);
+            to = max(to, hi[r]);
+        }
+        load8(q[r], head_row<const T>(a.q, b, query, kv * a.group + r % a.group) + in * 8, live ? left : 0, a.wide_in);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[r][j] *= a.scale2;
+        top[r] = -INFINITY;
+        sum[r] = 0;
+    }
+    from = max(from, int(min(int64_t(split) * a.span, int64_t(band.kl))));
+    to = int(min(int64_t(to), int64_t(split + 1) * a.span));
+    const T* keys = head_row<const T>(a.k, b, 0, kv) + in * 8;
+    const T* values = head_row<const T>(a.v, b, 0, kv) + in * 8;
+    for (int first = from + wave * kGroupsOfWave + group; __any(first < to); first += kDeep * kAtOnce) {
+        float k[kDeep][8], v[kDeep][8], s[kDeep][R];
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+            const int key = first + u * kAtOnce;
+            load8(k[u], keys + int64_t(key) * a.k.token, key < to ? left : 0, a.wide_in);
+        }
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+            const int key = first + u * kAtOnce;
+            load8(v[u], values + int64_t(key) * a.v.token, key < to ? left : 0, a.wide_in);
+        }
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float dot = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) dot = fmaf(q[r][j], k[u][j], dot);
+                dot = sum_lanes<LANES>(dot);
+                const int key = first + u * kAtOnce;
+                s[u][r] = key >= lo[r] && key < hi[r] && key < to ? dot : -INFINITY;
+            }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float next = top[r];
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) next = fmaxf(next, s[u][r]);
+            const float base = next == -INFINITY ? 0.f : next, by = exp2_fast(top[r] - base);
+            top[r] = next;
+            sum[r] *= by;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[r][j] *= by;
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) {
+                const float p = exp2_fast(s[u][r] - base);
+                sum[r] += p;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[r][j] = fmaf(p, v[u][j], acc[r][j]);
+            }
+        }
+    }
+    // the wave's groups, then the waves
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int d = LANES; d < 64; d <<= 1) {
+            const float other = __shfl_xor(top[r], d), next = fmaxf(top[r], other);
+            const float base = next == -INFINITY ? 0.f : next;
+            const float mine = exp2_fast(top[r] - base), theirs = exp2_fast(other - base);
+            top[r] = next;
+            sum[r] = sum[r] * mine + __shfl_xor(sum[r], d) * theirs;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[r][j] = acc[r][j] * mine + __shfl_xor(acc[r][j], d) * theirs;
+        }
+        if (group == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) shared[wave][r][in * 8 + j] = acc[r][j];
+            if (in == 0) {
+                shared[wave][r][LANES * 8] = top[r];
+                shared[wave][r][LANES * 8 + 1] = sum[r];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * LANES * 8; i += 256) {
+        const int r = i / (LANES * 8), d = i % (LANES * 8);
+        if (r >= rows || d >= a.dim) continue;
+        float next = -INFINITY, total = 0, value = 0;
+        for (int w = 0; w < 4; ++w) next = fmaxf(next, shared[w][r][LANES * 8]);
+        const float base = next == -INFINITY ? 0.f : next;
+        for (int w = 0; w < 4; ++w) {
+            const float by = exp2_fast(shared[w][r][LANES * 8] - base);
+            total += shared[w][r][LANES * 8 + 1] * by;
+            value += shared[w][r][d] * by;
+        }
+        const int query = r / a.group, head = kv * a.group + r % a.group;
+        if (a.splits > 1) {
+            const int64_t at = (int64_t(split) * a.pairs + pair) * rows + r;
+            a.part[at * a.dim + d] = value;
+            if (d == 0) {
+                a.part_stats[2 * at] = next;
+                a.part_stats[2 * at + 1] = total;
+            }
+        } else {
+            head_row<T>(a.out, b, query, head)[d] = T(total == 0 ? 0.f : value / total);
+            if (a.lse && d == 0)
+                a.lse[(int64_t(b) * a.kv_heads * a.group + head) * a.queries + query] =
+                    total == 0 ? -INFINITY : next * kLn2 + logf(total);
+        }
+    }
+}
+
+// ---- joining splits -----------------------------------------------------------------------
+struct JoinArgs {
+    const float *part, *stats;  // stats null: plain sums
+    HeadView out;
+    float* lse;
+    int splits, pairs, rows, dim, kv_heads, group;
+    int per_query;  // rows of a key head (queries x group)
+    float scale;
+};
+
+// One wave a row; lanes over its columns.  Splits that saw no key wrote no output.
+template <class T>
+__global__ __launch_bounds__(64) void attention_join_k(JoinArgs a) {
+    const int pair = blockIdx.x % a.pairs, row = blockIdx.x / a.pairs;
+    const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
+    const int token = row / a.group, head = kv * a.group + row % a.group;
+    const int64_t step = int64_t(a.pairs) * a.rows, first = int64_t(pair) * a.rows + row;
+    float base = 0, total = 1;
+    if (a.stats) {
+        float top = -INFINITY;
+        for (int s = threadIdx.x; s < a.splits; s += 64) top = fmaxf(top, a.stats[2 * (first + s * step)]);
+        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        base = top == -INFINITY ? 0.f : top;
+        total = 0;
+        // (every lane the same order)
+        for (int s = 0; s < a.splits; ++s) {
+            const float* m = a.stats + 2 * (first + s * step);
+            total += m[1] * exp2_fast(m[0] - base);
+        }
+        if (a.lse && threadIdx.x == 0)
+            a.lse[(int64_t(b) * a.kv_heads * a.group + head) * (a.rows / a.group) + token] =
+                total == 0 ? -INFINITY : base * kLn2 + logf(total);
+    }
+    T* out = head_row<T>(a.out, b, token, head);
+    for (int d = threadIdx.x; d < a.dim; d += 64) {
+        float value = 0;
+#pragma unroll 8
+        for (int s = 0; s < a.splits; ++s) {
+            const int64_t at = first + s * step;
+            float weight = 1;
+            if (a.stats) weight = a.stats[2 * at + 1] == 0 ? 0.f : exp2_fast(a.stats[2 * at] - base);
+            if (weight != 0) value += a.part[at * a.dim + d] * weight;
+        }
+        out[d] = T(a.stats ? (total == 0 ? 0.f : value / total) : value * a.scale);
+    }
+}
+
+// ---- gradient ---------------------------------------------------------------------------
+// dout.out of every query row, and its statistics in base 2; sixteen lanes a row.
+template <class T>
+__global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a) {
+    const int heads = a.kv_heads * a.group;
+    const int64_t count = int64_t(a.pairs / a.kv_heads) * a.queries * heads;
+    const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) / 16;
+    const int in = threadIdx.x & 15;
+    const int64_t item = min(i, count - 1);  // (all lanes take part in the sum)
+    const int head = int(item % heads), query = int(item / heads % a.queries), b = int(item / heads / a.queries);
+    const bool live = query < length_of(a.query_lengths, b, a.queries);
+    float x[8], y[8], dot = 0;
+    const int left = live ? a.dim - in * 8 : 0;
+    load8(x, head_row<const T>(a.out, b, query, head) + in * 8, left, a.wide_in);
+    load8(y, head_row<const T>(a.dout, b, query, head) + in * 8, left, a.wide_in);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j], dot);
+    dot = sum_lanes<16>(dot);
+    if (in == 0 && i < count) {
+        const int64_t at = (int64_t(b) * heads + head) * a.queries + query;
+        const float lse = live ? a.lse[at] : -INFINITY;
+        a.row_lse[at] = lse == -INFINITY ? INFINITY : lse * kLog2e;  // (no key: every probability is 0)
+        a.row_delta[at] = dot;
+    }
+}
+
+// Gradients of keys and values: 128 keys a workgroup, 32 a wave, with their keys
+// and values in registers, over tiles of 32 queries of every head that reads them.
+// Scores lie as queries x keys, so a lane holds 16 of every 32 queries of ONE key:
+// its probabilities and its score gradients are, in place, the fragments that
+// multiply the transposed dout and queries into dv and dk.
+template <class T, int DP>
+__global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_k(AttentionArgs a) {
+    constexpr int kBlocks = DP / 32, kSteps = DP / 16;
+    using L = Tile<T, DP>;
+    __shared__ __align__(16) char lds[2][2][kQueries * L::kRowBytes];
+    __shared__ __align__(16) float stats[2][2][kQueries];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
+    const int tile = rest % a.tiles, split = rest / a.tiles;  // (a causal band's first keys are seen most)
+    const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
+    const Band band(a, b);
+    const int block_first = tile * kBlockRows, wave_first = block_first + wave * kWaveRows;
+    const int key = wave_first + (lane & 31);
+    const bool live = key < band.kl;
+    const int lo = live ? band.query_lo(key) : 0, hi = live ? band.query_hi(key) : 0;
+
+    Frag<T> k[kSteps], v[kSteps];
+    load_fragments<T, DP>(k, head_row<const T>(a.k, b, key, kv), a.dim, half, live, a.wide_in);
+    load_fragments<T, DP>(v, head_row<const T>(a.v, b, key, kv), a.dim, half, live, a.wide_in);
+
+    const auto last = [&](int j) { return min(j, band.kl - 1); };
+    const bool any = block_first < band.kl, wave_any = wave_first < band.kl;
+    const int t0 = any ? band.query_lo(block_first) / kQueries : 0;
+    const int t1 = any ? (band.query_hi(last(block_first + kBlockRows - 1)) + kQueries - 1) / kQueries : 0;
+    const int per_head = max(t1 - t0, 0);
+    int from = 0, to = per_head * a.group;
+    if (a.splits > 1) {
+        const int share = (to + a.splits - 1) / a.splits;
+        from = min(split * share, to);
+        to = min(to, from + share);
+    }
+    const int wave_lo = wave_any ? band.query_lo(wave_first) : 0;
+    const int wave_hi = wave_any ? band.query_hi(last(wave_first + kWaveRows - 1)) : 0;
+    const int full_lo = band.query_lo(last(wave_first + kWaveRows - 1));
+    const int full_hi = wave_first + kWaveRows <= band.kl ? band.query_hi(wave_first) : 0;
+
+    TileLoader<T, DP, kQueries> qload, oload;
+    qload.start(a.q.token, a.dim, a.wide_in);
+    oload.start(a.dout.token, a.dim, a.wide_in);
+    int head = per_head ? from / per_head : 0, t = t0 + from - head * per_head;  // of the next load
+    const auto load = [&](int buffer) {
+        const int first = t * kQueries, h = kv * a.group + head, valid = band.ql - first;
+        qload.load(lds[buffer][0], reinterpret_cast<const char*>(head_row<const T>(a.q, b, first, h)), valid, wave);
+        oload.load(lds[buffer][1], reinterpret_cast<const char*>(head_row<const T>(a.dout, b, first, h)), valid, wave);
+        if (wave == 0) {  // the 64 statistics, one a lane
+            const float* from = (lane < kQueries ? a.row_lse : a.row_delta) +
+                                (int64_t(b) * a.kv_heads * a.group + h) * a.queries + first;
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(from + min(lane % kQueries, valid - 1)),
+                (__attribute__((address_space(3))) void*)&stats[buffer][0][0], 4, 0, 0);
+        }
+        if (++t == t1) {
+            t = t0;
+            ++head;
+        }
+    };
+
+    Acc dk[kBlocks] = {}, dv[kBlocks] = {};
+    if (from < to) {
+        for (int i = 0; i < 4; ++i) qload.clear(lds[i >> 1][i & 1]);
+        if (qload.direct && a.dim < DP) __syncthreads();
+    }
+    int at = t;  // of the tile computed on
+    if (from < to) load(0);
+    for (int i = from; i < to; ++i) {
+        const int buffer = (i - from) & 1, first = at * kQueries;
+        if (++at == t1) at = t0;
+        arrived();
+        __syncthreads();
+        if (i + 1 < to) load(buffer ^ 1);
+        if (first >= wave_hi || first + kQueries <= wave_lo) continue;
+        const char *queries = lds[buffer][0], *douts = lds[buffer][1];
+        Acc s = {}, dp = {};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) s = mma(L::row(queries, lane & 31, i, half), k[i], s);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) dp = mma(L::row(douts, lane & 31, i, half), v[i], dp);
+        const bool hidden = first < full_lo || first + kQueries > full_hi;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const auto lse = *reinterpret_cast<const vec<float, 4>*>(&stats[buffer][0][8 * g + 4 * half]);
+            const auto delta = *reinterpret_cast<const vec<float, 4>*>(&stats[buffer][1][8 * g + 4 * half]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = 4 * g + j, query = first + 8 * g + 4 * half + j;
+                float p = exp2_fast(fmaf(s[i], a.scale2, -lse[j])), ds = p * (dp[i] - delta[j]);
+                if (hidden) {
+                    const bool seen = query >= lo && query < hi;
+                    p = seen ? p : 0.f;
+                    ds = seen ? ds : 0.f;
+                }
+                s[i] = p;
+                dp[i] = ds;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const Frag<T> p = as_fragment<T>(s, i), ds = as_fragment<T>(dp, i);
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) {
+                dv[d] = mma(L::column(douts, d, i, lane), p, dv[d]);
+                dk[d] = mma(L::column(queries, d, i, lane), ds, dk[d]);
+            }
+        }
+    }
+    if (key >= a.keys) return;
+    if (a.splits > 1) {
+        // [which][split][pair][key][dim]
+        const int64_t at = (int64_t(split) * a.pairs + pair) * a.keys + key;
+        const int64_t other = int64_t(a.splits) * a.pairs * a.keys;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d) {
+            store_column(a.part + at * a.dim, dk[d], 1.f, d, half, a.dim, a.dim % 4 == 0);
+            store_column(a.part + (other + at) * a.dim, dv[d], 1.f, d, half, a.dim, a.dim % 4 == 0);
+        }
+        return;
+    }
+    T *to_k = head_row<T>(a.dk, b, key, kv), *to_v = head_row<T>(a.dv, b, key, kv);
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) {
+        store_column(to_k, dk[d], a.scale, d, half, a.dim, a.wide_out);
+        store_column(to_v, dv[d], 1.f, d, half, a.dim, a.wide_out);
+    }
+}
+
+// Gradients of queries: the forward's shape, with queries and dout in registers.
+// (A second pass over the scores, so that no two workgroups add to one place: two
+// products of nine, for sums in a fixed order and no float copy of dq.)
+template <class T, int DP>
+__global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradient_k(AttentionArgs a) {
+    constexpr int N = kKeys<T>, kSub = N / 32, kBlocks = DP / 32, kSteps = DP / 16;
+    using L = Tile<T, DP>;
+    __shared__ __align__(16) char lds[2][2][N * L::kRowBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
+    const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
+    const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
+    const Band band(a, b);
+    const int rows = a.queries * a.group;
+    const int row = tile * kBlockRows + wave * kWaveRows + (lane & 31);
+    const int query = row / a.group, head = kv * a.group + row % a.group;
+    const bool live = row < rows && query < band.ql;
+    const int lo = live ? band.key_lo(query) : 0, hi = live ? band.key_hi(query) : 0;
+
+    Frag<T> q[kSteps], dout[kSteps];
+    load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
+    load_fragments<T, DP>(dout, head_row<const T>(a.dout, b, query, head), a.dim, half, live, a.wide_in);
+    const int64_t at_row = (int64_t(b) * a.kv_heads * a.group + head) * a.queries + query;
+    const float lse = live ? a.row_lse[at_row] : INFINITY, delta = live ? a.row_delta[at_row] : 0.f;
+
+    const auto first_row = [&](int r) { return min(r / a.group, band.ql - 1); };
+    const int block_first = tile * kBlockRows, wave_first = block_first + wave * kWaveRows;
+    const bool any = block_first / a.group < band.ql, wave_any = wave_first / a.group < band.ql;
+    int t0 = any ? band.key_lo(first_row(block_first)) / N : 0;
+    int t1 = any ? (band.key_hi(first_row(block_first + kBlockRows - 1)) + N - 1) / N : 0;
+    if (a.splits > 1) {
+        const int share = (max(t1 - t0, 0) + a.splits - 1) / a.splits;
+        t0 += split * share;
+        t1 = min(t1, t0 + share);
+    }
+    const int wave_lo = wave_any ? band.key_lo(first_row(wave_first)) : 0;
+    const int wave_hi = wave_any ? band.key_hi(first_row(wave_first + kWaveRows - 1)) : 0;
+    const int full_lo = band.key_lo(first_row(wave_first + kWaveRows - 1));
+    const int full_hi = wave_any && (wave_first + kWaveRows - 1) / a.group < band.ql ? band.key_hi(first_row(wave_first)) : 0;
+
+    TileLoader<T, DP, N> kload, vload;
+    kload.start(a.k.token, a.dim, a.wide_in);
+    vload.start(a.v.token, a.dim, a.wide_in);
+    const char* kbase = reinterpret_cast<const char*>(head_row<const T>(a.k, b, 0, kv));
+    const char* vbase = reinterpret_cast<const char*>(head_row<const T>(a.v, b, 0, kv));
+    const auto load = [&](int t, int buffer) {
+        const int64_t first = int64_t(t) * N;
+        kload.load(lds[buffer][0], kbase + first * kload.stride, band.kl - t * N, wave);
+        vload.load(lds[buffer][1], vbase + first * vload.stride, band.kl - t * N, wave);
+    };
+
+    Acc dq[kBlocks] = {};
+    if (t0 < t1) {
+        for (int i = 0; i < 4; ++i) kload.clear(lds[i >> 1][i & 1]);
+        if (kload.direct && a.dim < DP) __syncthreads();
+        load(t0, 0);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int buffer = (t - t0) & 1;
+        arrived();
+        __syncthreads();
+        if (t + 1 < t1) load(t + 1, buffer ^ 1);
+        const int first = t * N;
+        if (first >= wave_hi || first + N <= wave_lo) continue;
+        const char *keys = lds[buffer][0], *values = lds[buffer][1];
+        const bool hidden = first < full_lo || first + N > full_hi;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            Acc s = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) s = mma(L::row(keys, 32 * u + (lane & 31), i, half), q[i], s);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) dp = mma(L::row(values, 32 * u + (lane & 31), i, half), dout[i], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = first + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
+                float ds = exp2_fast(fmaf(s[i], a.scale2, -lse)) * (dp[i] - delta);
+                if (hidden) ds = key >= lo && key < hi ? ds : 0.f;
+                s[i] = ds;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const Frag<T> ds = as_fragment<T>(s, i);
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) dq[d] = mma(L::column(keys, d, 2 * u + i, lane), ds, dq[d]);
+            }
+        }
+    }
+    if (row >= rows) return;
+    if (a.splits > 1) {
+        const int64_t at = (int64_t(split) * a.pairs + pair) * rows + row;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+            store_column(a.part + at * a.dim, dq[d], 1.f, d, half, a.dim, a.dim % 4 == 0);
+        return;
+    }
+    T* to = head_row<T>(a.dq, b, query, head);
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) store_column(to, dq[d], a.scale, d, half, a.dim, a.wide_out);
+}
+
+// ---- host -----------------------------------------------------------------------------------
+int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
+
+// How the launches of a shape are cut, the same for every call: work is split over
+// the long axis and joined where whole rows would leave the device short of
+// workgroups.
+struct Cut {
+    bool step = false;   // the forward runs on the vector kernel
+    int rows = 0, row_tiles = 0, key_tiles = 0;
+    int span = 0, forward = 1, query = 1, key = 1;  // splits
+    size_t stats = 0, part = 0, part_stats = 0, floats = 0;
+};
+
+// Query rows of a key head up to which the vector kernel serves.
+constexpr int kStepRows = 8;
+
+int step_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : 16; }
+
+Cut cut(const Attention& p) {
+    const auto& s = p.shape;
+    Cut c;
+    const int64_t group = s.heads / s.kv_heads, pairs = int64_t(s.batch) * s.kv_heads;
+    c.rows = int(s.query_tokens * group);
+    c.row_tiles = ceil_div(c.rows, kBlockRows);
+    c.key_tiles = ceil_div(s.key_tokens, kBlockRows);
+    const int cus = p.dev->compute_units, keys_tile = s.dtype == CPDE_F32 ? kKeys<float> : kKeys<bf16>;
+    const auto splits = [&](int64_t blocks, int64_t steps) {
+        // two workgroups a CU, and at least four tiles a split
+        return int(std::clamp<int64_t>(blocks ? 2 * cus / blocks : 1, 1, std::max<int64_t>(steps / 4, 1)));
+    };
+    c.step = c.rows <= kStepRows;
+    if (c.step) {
+        // 16 workgroups a CU, in whole rounds of a workgroup's loads; a short list in one
+        const int round = 16 * (64 / step_lanes(s.head_dim));
+        const int64_t share = s.key_tokens <= 4 * round ? s.key_tokens : ceil_div(pairs * s.key_tokens, 16 * cus);
+        c.span = std::max(ceil_div(std::max<int64_t>(share, 1), round) * round, round);
+        c.forward = std::max(ceil_div(s.key_tokens, c.span), 1);
+    } else {
+        c.forward = splits(pairs * c.row_tiles, ceil_div(s.key_tokens, keys_tile));
+    }
+    size_t part = 0, part_stats = 0;
+    if (c.forward > 1) {
+        part = size_t(c.forward) * pairs * c.rows * s.head_dim;
+        part_stats = size_t(c.forward) * pairs * c.rows * 2;
+    }
+    if (s.backward) {
+        c.query = splits(pairs * c.row_tiles, ceil_div(s.key_tokens, keys_tile));
+        c.key = splits(pairs * c.key_tiles, group * ceil_div(s.query_tokens, kQueries));
+        if (c.query > 1) part = std::max(part, size_t(c.query) * pairs * c.rows * s.head_dim);
+        if (c.key > 1) part = std::max(part, 2 * size_t(c.key) * pairs * s.key_tokens * s.head_dim);
+        c.stats = 2 * size_t(s.batch) * s.heads * s.query_tokens;
+    }
+    const auto padded = [](size_t n) { return (n + 63) / 64 * 64; };
+    c.stats = padded(c.stats);
+    c.part = padded(part);
+    c.part_stats = padded(part_stats);
+    c.floats = c.stats + c.part + c.part_stats;
+    return c;
+}
+
+HeadView view(const cpde_heads& h) { return {static_cast<char*>(h.data), h.batch, h.token, h.head}; }
+
+// Checks a tensor's address and strides; returns whether it takes 16-byte accesses.
+bool check_heads(const cpde_attention_shape& s, const cpde_heads* h, int tokens, int heads, bool output) {
+    require(h, "null argument");
+    if (!s.batch || !tokens) return true;
+    require(h->data, "null tensor");
+    require(h->batch >= 0 && h->token >= 0 && h->head >= 0, "negative stride");
+    if (output) {
+        // from the smallest stride up, each axis steps over all of the ones before
+        std::pair<int64_t, int64_t> axes[3] = {{h->batch, s.batch}, {h->token, tokens}, {h->head, heads}};
+        std::sort(axes, axes + 3);
+        int64_t extent = s.head_dim;
+        for (auto& [stride, count] : axes) {
+            if (count == 1) continue;
+            require(stride >= extent, "output elements overlap");
+            extent = stride * (count - 1) + extent;
+        }
+    }
+    const size_t size = type_bytes(s.dtype);
+    // (a tile's rows are addressed with 32 bits)
+    return wide(h->data, h->batch, size) && wide(h->data, h->token, size) && wide(h->data, h->head, size) &&
+           s.head_dim * size % 16 == 0 && h->token * int64_t(size) < (int64_t(1) << 24);
+}
+
+AttentionArgs arguments(const Attention& p, const Cut& c, const int* query_lengths, const int* key_lengths) {
+    const auto& s = p.shape;
+    AttentionArgs a{};
+    a.query_lengths = query_lengths;
+    a.key_lengths = key_lengths;
+    a.pairs = s.batch * s.kv_heads;
+    a.kv_heads = s.kv_heads;
+    a.group = s.heads / s.kv_heads;
+    a.queries = s.query_tokens;
+    a.keys = s.key_tokens;
+    a.dim = s.head_dim;
+    a.left = s.left;
+    a.right = s.right;
+    a.scale = s.scale;
+    a.scale2 = s.scale * kLog2e;
+    a.span = c.span;
+    a.row_lse = p.work;
+    a.row_delta = p.work + c.stats / 2;
+    a.part = p.work + c.stats;
+    a.part_stats = a.part + c.part;
+    return a;
+}
+
+template <class T>
+void join(Device& d, const AttentionArgs& a, const float* part, const float* stats, const HeadView& out, float* lse,
+          int rows, int group, float scale) {
+    JoinArgs j{};
+    j.part = part;
+    j.stats = stats;
+    j.out = out;
+    j.lse = lse;
+    j.splits = a.splits;
+    j.pairs = a.pairs;
+    j.rows = rows;
+    j.dim = a.dim;
+    j.kv_heads = a.kv_heads;
+    j.group = group;
+    j.scale = scale;
+    hipLaunchKernelGGL((attention_join_k<T>), unsigned(a.pairs) * unsigned(rows), 64, 0, d.stream, j);
+}
+
+template <class F>
+void with_width(int dim, F body) {
+    if (dim <= 32) body(std::integral_constant<int, 32>{});
+    else if (dim <= 64) body(std::integral_constant<int, 64>{});
+    else if (dim <= 96) body(std::integral_constant<int, 96>{});
+    else body(std::integral_constant<int, 128>{});
+}
+
+template <class T>
+void step(Device& d, const AttentionArgs& a, int rows) {
+    const unsigned blocks = unsigned(a.pairs) * unsigned(a.splits);
+    const auto launch = [&](auto lanes, auto most) {
+        hipLaunchKernelGGL((attention_step_k<T, decltype(lanes)::value, decltype(most)::value>), blocks, 256, 0, d.stream, a);
+    };
+    const auto with_rows = [&](auto lanes) {
+        if (rows == 1) launch(lanes, std::integral_constant<int, 1>{});
+        else if (rows == 2) launch(lanes, std::integral_constant<int, 2>{});
+        else if (rows <= 4) launch(lanes, std::integral_constant<int, 4>{});
+        else launch(lanes, std::integral_constant<int, 8>{});
+    };
+    const int lanes = step_lanes(a.dim);
+    if (lanes == 4) with_rows(std::integral_constant<int, 4>{});
+    else if (lanes == 8) with_rows(std::integral_constant<int, 8>{});
+    else with_rows(std::integral_constant<int, 16>{});
+}
+
+}  // namespace
+}  // namespace cpde
+
+struct cpde_attention_s : cpde::Attention {};
+using namespace cpde;
+
+extern "C" {
+
+int cpde_attention_create(cpde_device* dev, const cpde_attention_shape* shape, cpde_attention** out) {
+    return guarded([&] {
+        require(dev && shape && out, "null argument");
+        *out = nullptr;
+        cpde_attention_shape s = *shape;
+        check_dtype(s.dtype);
+        require(s.batch >= 0 && s.query_tokens >= 0 && s.key_tokens >= 0, "negative size");
+        require(s.heads >= 1 && s.kv_heads >= 1 && s.heads % s.kv_heads == 0,
+                "query heads are a whole number of times the key heads");
+        require(s.head_dim >= 1 && s.head_dim <= kMaxHeadDim, "a head is 1 to 128 wide");
+        require(std::isfinite(s.scale) && s.scale >= 0, "the scale is positive, or 0 for 1/sqrt(head_dim)");
+        constexpr int64_t kMost = int64_t(1) << 30;  // (row and key numbers, and sums of two, stay inside 32 bits)
+        require(int64_t(s.query_tokens) * (s.heads / s.kv_heads) <= kMost && s.key_tokens <= kMost, "too many tokens");
+        if (s.scale == 0) s.scale = 1.f / std::sqrt(float(s.head_dim));
+        s.left = s.left < 0 ? -1 : int(std::min<int64_t>(s.left, kMost));
+        s.right = s.right < 0 ? -1 : int(std::min<int64_t>(s.right, kMost));
+        require(!dev->capturing, "a capture is open on this device");
+        auto p = std::make_unique<cpde_attention_s>();
+        p->dev = dev;
+        p->shape = s;
+        const Cut c = cut(*p);
+        const int64_t pairs = int64_t(s.batch) * s.kv_heads;
+        const int64_t most = std::max({int64_t(c.row_tiles) * std::max(c.forward, c.query), int64_t(c.key_tiles) * c.key,
+                                       c.forward > 1 || c.query > 1 ? int64_t(c.rows) : 1,
+                                       c.key > 1 ? int64_t(s.key_tokens) : 1, int64_t(c.forward)});
+        require(pairs <= kMost && pairs * most <= kMost &&
+                    int64_t(s.batch) * s.heads * s.query_tokens <= kMost * 8,
+                "too many workgroups: split the batch");
+        HIP_CHECK(hipMalloc(&p->work, std::max<size_t>(c.floats, 64) * sizeof(float)));
+        *out = p.release();
+    });
+}
+
+int cpde_attention_destroy(cpde_attention* attention) {
+    return guarded([&] {
+        if (!attention) return;
+        sync_stream(*attention->dev, __LINE__);
+        ++attention->dev->layout;
+        HIP_CHECK(hipFree(attention->work));
+        delete attention;
+    });
+}
+
+int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const cpde_heads* k, const cpde_heads* v,
+                           const cpde_heads* out, float* lse, const int32_t* query_lengths,
+                           const int32_t* key_lengths) {
+    return guarded([&] {
+        require(attention, "null argument");
+        const Attention& p = *attention;
+        const auto& s = p.shape;
+        const Cut c = cut(p);
+        AttentionArgs a = arguments(p, c, query_lengths, key_lengths);
+        const bool wq = check_heads(s, q, s.query_tokens, s.heads, false);
+        const bool wk = check_heads(s, k, s.key_tokens, s.kv_heads, false);
+        const bool wv = check_heads(s, v, s.key_tokens, s.kv_heads, false);
+        a.wide_in = wq && wk && wv;
+        a.wide_out = check_heads(s, out, s.query_tokens, s.heads, true);
+        if (!a.pairs || !c.rows) return;
+        a.q = view(*q);
+        a.k = view(*k);
+        a.v = view(*v);
+        a.out = view(*out);
+        a.lse = lse;
+        a.splits = c.forward;
+        a.tiles = c.row_tiles;
+        Device& d = *p.dev;
+        flush_reduce(d);
+        TraceScope trace(d, kTraceAttention, 4.0 * s.batch * s.heads * double(s.query_tokens) * s.key_tokens * s.head_dim);
+        with_type(s.dtype, [&](auto element) {
+            using T = decltype(element);
+            if (c.step) step<T>(d, a, c.rows);
+            else
+                with_width(a.dim, [&](auto width) {
+                    hipLaunchKernelGGL((attention_forward_k<T, decltype(width)::value>),
+                                       unsigned(a.pairs) * a.tiles * a.splits, 256, 0, d.stream, a);
+                });
+            HIP_CHECK(hipGetLastError());
+            if (a.splits > 1) join<T>(d, a, a.part, a.part_stats, a.out, lse, c.rows, a.group, 1.f);
+        });
+        HIP_CHECK(hipGetLastError());
+    });
+}
+
+int cpde_attention_backward(cpde_attention* attention, const cpde_heads* q, const cpde_heads* k, const cpde_heads* v,
+                            const cpde_heads* out, const float* lse, const cpde_heads* dout, const cpde_heads* dq,
+                            const cpde_heads* dk, const cpde_heads* dv, const int32_t* query_lengths,
+                            const int32_t* key_lengths) {
+    return guarded([&] {
+        require(attention, "null argument");
+        const Attention& p = *attention;
+        const auto& s = p.shape;
+        require(s.backward, "the attention was created without a backward");
+        const Cut c = cut(p);
+        AttentionArgs a = arguments(p, c, query_lengths, key_lengths);
+        const bool in[] = {check_heads(s, q, s.query_tokens, s.heads, false),
+                           check_heads(s, k, s.key_tokens, s.kv_heads, false),
+                           check_heads(s, v, s.key_tokens, s.kv_heads, false),
+                           check_heads(s, out, s.query_tokens, s.heads, false),
+                           check_heads(s, dout, s.query_tokens, s.heads, false)};
+        const bool to[] = {check_heads(s, dq, s.query_tokens, s.heads, true),
+                           check_heads(s, dk, s.key_tokens, s.kv_heads, true),
+                           check_heads(s, dv, s.key_tokens, s.kv_heads, true)};
+        require(lse || !a.pairs || !c.rows, "null statistics");
+        a.wide_in = in[0] && in[1] && in[2] && in[3] && in[4];
+        a.wide_out = to[0] && to[1] && to[2];
+        a.q = view(*q);
+        a.k = view(*k);
+        a.v = view(*v);
+        a.out = view(*out);
+        a.dout = view(*dout);
+        a.dq = view(*dq);
+        a.dk = view(*dk);
+        a.dv = view(*dv);
+        a.lse = const_cast<float*>(lse);
+        if (!a.pairs) return;
+        Device& d = *p.dev;
+        flush_reduce(d);
+        TraceScope trace(d, kTraceAttentionGradient,
+                         10.0 * s.batch * s.heads * double(s.query_tokens) * s.key_tokens * s.head_dim);
+        with_type(s.dtype, [&](auto element) {
+            using T = decltype(element);
+            const int64_t count = int64_t(s.batch) * s.heads * s.query_tokens;
+            if (count)
+                hipLaunchKernelGGL((attention_delta_k<T>), unsigned((count * 16 + 255) / 256), 256, 0, d.stream, a);
+            HIP_CHECK(hipGetLastError());
+            with_width(a.dim, [&](auto width) {
+                constexpr int DP = decltype(width)::value;
+                if (s.key_tokens) {
+                    a.splits = c.key;
+                    a.tiles = c.key_tiles;
+                    hipLaunchKernelGGL((attention_key_gradient_k<T, DP>), unsigned(a.pairs) * a.tiles * a.splits, 256, 0,
+                                       d.stream, a);
+                    HIP_CHECK(hipGetLastError());
+                    if (a.splits > 1) {
+                        join<T>(d, a, a.part, nullptr, a.dk, nullptr, s.key_tokens, 1, a.scale);
+                        join<T>(d, a, a.part + size_t(a.splits) * a.pairs * s.key_tokens * s.head_dim, nullptr, a.dv,
+                                nullptr, s.key_tokens, 1, 1.f);
+                    }
+                }
+                if (c.rows) {
+                    a.splits = c.query;
+                    a.tiles = c.row_tiles;
+                    hipLaunchKernelGGL((attention_query_gradient_k<T, DP>), unsigned(a.pairs) * a.tiles * a.splits, 256, 0,
+                                       d.stream, a);
+                    HIP_CHECK(hipGetLastError());
+                    if (a.splits > 1) join<T>(d, a, a.part, nullptr, a.dq, nullptr, c.rows, a.group, a.scale);
+                }
+            });
+        });
+        HIP_CHECK(hipGetLastError());
+    });
+}
+
+}  // extern "C"

@@ -4,6 +4,7 @@
 
 #include <cstdint>
 #include <memory>
+#include <new>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -29,6 +30,29 @@ void check_hip(hipError_t status, const char* what, const char* file, int line);
 #define HIP_CHECK(expr) ::cpde::check_hip((expr), #expr, __FILE__, __LINE__)
 inline void require(bool ok, const char* message) {
     if (!ok) throw invalid(message);
+}
+// Runs an entry point's body and turns what it throws into the C ABI's status.
+template <class F>
+int guarded(F body) {
+    try {
+        body();
+        return CPDE_OK;
+    } catch (const invalid& e) {
+        set_error(e.what());
+        return CPDE_EINVAL;
+    } catch (const compile_error& e) {
+        set_error(e.what());
+        return CPDE_ECOMPILE;
+    } catch (const device_error& e) {
+        set_error(e.what());
+        return CPDE_EDEVICE;
+    } catch (const std::bad_alloc&) {
+        set_error("host allocation failed");
+        return CPDE_EDEVICE;
+    } catch (const std::exception& e) {
+        set_error(e.what());
+        return CPDE_EDEVICE;
+    }
 }
 
 constexpr int kMaxOrder = 6;
@@ -258,7 +282,7 @@ enum TraceKind {
     kTraceComposeForward, kTraceComposeAdjoint, kTraceGemm, kTraceGemmTransposed, kTraceWgrad, kTraceSplitReduce,
     kTraceBiasGrad, kTraceActivate, kTraceCost, kTraceReduce, kTraceOptimizer, kTraceOther, kTraceFusedInput,
     kTraceFusedForward, kTraceFusedBackward, kTraceFusedOutput, kTraceNetworkForward, kTraceNetworkBackward,
-    kTraceNetworkEpoch, kTraceKinds
+    kTraceNetworkEpoch, kTraceAttention, kTraceAttentionGradient, kTraceEmbedding, kTraceDropout, kTraceKinds
 };
 // A one-pass epoch launch held back so that the next one can share it (api.hip).
 struct HeldEpoch;
@@ -273,6 +297,7 @@ struct Device {
     int ordinal = 0;
     int compute_units = 0;
     hipStream_t stream = nullptr;
+    bool own_stream = true;  // false: the caller's (cpde_device_open_on)
     // this GPU's copy of the library's static scratch array (api.hip), or null
     // with the reason when its address could not be taken
     unsigned char* static_scratch = nullptr;
@@ -526,3 +551,5 @@ GraphLaunch graph_launch(Device& d, const cpde_scalar_node* nodes, int count, in
 void launch_graph(Device& d, const GraphLaunch& g);
 
 }  // namespace cpde
+
+struct cpde_device_s : cpde::Device {};

@@ -1,0 +1,610 @@
+// Rows of a table by token, scaled, and the table's gradient by sorted tokens.
+#include "sequence.hpp"
+
+namespace cpde {
+namespace {
+
+constexpr int kSmallSort = 4096;     // tokens sorted by one workgroup in LDS
+constexpr int kDigitBits = 10;       // at most, of one pass over longer lists
+constexpr int kSortTokens = 4096;    // per workgroup of such a pass
+constexpr uint32_t kFan = 32;             // sorted tokens of a partial sum, and partial sums of one of the second level
+
+struct Embedding {
+    Device* dev = nullptr;
+    int dtype = 0, rows = 0, width = 0, index_bytes = 0;
+    int64_t tokens = 0;
+    char* work = nullptr;  // of the gradient, see layout()
+};
+
+// The gradient's workspace.
+struct Layout {
+    size_t keys[2], places[2], counts, sums1, sums2, bytes;
+};
+int bit_width(uint32_t v) {
+    int bits = 0;
+    while (v) v >>= 1, ++bits;
+    return bits;
+}
+int sort_passes(int rows) { return (bit_width(uint32_t(rows)) + kDigitBits - 1) / kDigitBits; }
+int digit_bits(int rows) { return (bit_width(uint32_t(rows)) + sort_passes(rows) - 1) / sort_passes(rows); }
+
+Layout layout(const Embedding& e) {
+    Layout l{};
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t begin = at;
+        at += (bytes + 255) / 256 * 256;
+        return begin;
+    };
+    const size_t n = size_t(e.tokens);
+    for (int i = 0; i < 2; ++i) {
+        l.keys[i] = take(4 * n);
+        l.places[i] = take(4 * n);
+    }
+    l.counts = take(4 * ((n + kSortTokens - 1) / kSortTokens << digit_bits(e.rows)));
+    l.sums1 = take(4 * (n / kFan) * size_t(e.width));
+    l.sums2 = take(4 * (n / (kFan * kFan)) * size_t(e.width));
+    l.bytes = std::max<size_t>(at, 256);
+    return l;
+}
+
+// An id as a sort key: ids outside the table sort behind every row.
+template <class I>
+__device__ inline uint32_t key_of(I id, int rows) {
+    return id >= 0 && id < I(rows) ? uint32_t(id) : uint32_t(rows);
+}
+
+// Eight values of 16 bits, or four floats, of a row as floats: in one load where
+// the rows are aligned, else one by one; values at or past `left` are zeros.
+template <class T>
+constexpr int kLane = 16 / sizeof(T);
+template <class T>
+__device__ inline void load_lane(float* v, const T* p, int64_t left, bool aligned) {
+    if (aligned) {
+        const vec<T, kLane<T>> in = *reinterpret_cast<const vec<T, kLane<T>>*>(p);
+#pragma unroll
+        for (int j = 0; j < kLane<T>; ++j) v[j] = float(in[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLane<T>; ++j) v[j] = j < left ? float(p[j]) : 0.f;
+    }
+}
+
+// ---- lookup ---------------------------------------------------------------------------
+// A lane copies 16 bytes of one row.  Bound: HBM (the rows written; rows of common
+// tokens come from the caches).
+template <class T, class I>
+__global__ __launch_bounds__(256) void embedding_lookup_k(const I* ids, uint64_t lanes, uint32_t per_row, const T* table,
+                                                          int64_t table_stride, int rows, int width, float scale, T* out,
+                                                          int64_t out_stride, bool aligned) {
+    constexpr int N = kLane<T>;
+    const uint64_t step = uint64_t(gridDim.x) * 256;
+    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < lanes; i += step) {
+        const uint64_t token = lanes <= 0xffffffffull ? uint32_t(i) / per_row : i / per_row;
+        const int column = int(i - token * per_row) * N;
+        const uint32_t row = key_of(ids[token], rows);
+        float v[N] = {};
+        if (row < uint32_t(rows)) load_lane(v, table + int64_t(row) * table_stride + column, width - column, aligned);
+        T* to = out + int64_t(token) * out_stride + column;
+        if (aligned) {
+            vec<T, N> o;
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[j] = T(v[j] * scale);
+            *reinterpret_cast<vec<T, N>*>(to) = o;
+        } else {
+            for (int j = 0; j < N && column + j < width; ++j) to[j] = T(v[j] * scale);
+        }
+    }
+}
+
+// ---- sorting tokens by row ------------------------------------------------------------
+// A stable radix sort of (row, place) pairs, so that a row's tokens stay in order.
+// Lanes of a wave with the same digit find one another by one ballot a bit; the
+// first of them takes their places from the wave's counter of that digit.
+__device__ inline uint64_t same_digit(uint32_t digit, int bits, bool live) {
+    uint64_t peers = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const bool set = (digit >> b) & 1;
+        const uint64_t with = __ballot(set);
+        peers &= set ? with : ~with;
+    }
+    return peers;
+}
+__device__ inline int take_place(int* counter, uint64_t peers, int lane) {
+    const int first = __ffsll(static_cast<unsigned long long>(peers)) - 1;
+    int base = 0;
+    if (lane == first) base = atomicAdd(counter, __popcll(peers));
+    return __shfl(base, first) + __popcll(peers & ((1ull << lane) - 1));
+}
+
+// Exclusive sums of a value a thread over a workgroup of 1024; returns the total.
+__device__ inline int scan_block(int value, int& before, int* waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sum = value;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(sum, d);
+        if (lane >= d) sum += other;
+    }
+    __syncthreads();
+    if (lane == 63) waves[wave] = sum;
+    __syncthreads();
+    int base = 0, total = 0;
+    for (int w = 0; w < 16; ++w) {
+        if (w < wave) base += waves[w];
+        total += waves[w];
+    }
+    before = base + sum - value;
+    return total;
+}
+
+// Up to 4,096 tokens in one workgroup: six bits a pass, the pairs in LDS.  Bound:
+// the passes' latency.
+template <class I>
+__global__ __launch_bounds__(1024) void embedding_sort_small_k(const I* ids, int tokens, int rows, int bits,
+                                                               uint32_t* keys, uint32_t* places) {
+    __shared__ uint32_t key[kSmallSort];
+    __shared__ uint16_t place[kSmallSort];
+    __shared__ int counter[16 * 64];  // [wave][digit]
+    __shared__ int waves[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // wave w holds tokens [w * share, (w + 1) * share), in rounds of 64
+    const int rounds = (tokens + 1023) / 1024, begin = wave * rounds * 64 + lane;
+    uint32_t k[4];
+    uint32_t p[4];
+    bool live[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        p[r] = begin + r * 64;
+        live[r] = r < rounds && int(p[r]) < tokens;
+        k[r] = live[r] ? key_of(ids[p[r]], rows) : 0;
+    }
+    for (int shift = 0; shift < bits; shift += 6) {
+        counter[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (live[r]) atomicAdd(&counter[wave * 64 + ((k[r] >> shift) & 63)], 1);
+        __syncthreads();
+        // places in the order (digit, wave): thread t owns digit t / 16 of wave t % 16
+        int* own = &counter[(threadIdx.x & 15) * 64 + (threadIdx.x >> 4)];
+        int before;
+        scan_block(*own, before, waves);
+        *own = before;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t digit = (k[r] >> shift) & 63;
+            const uint64_t peers = same_digit(digit, 6, live[r]);
+            if (live[r]) {
+                const int to = take_place(&counter[wave * 64 + digit], peers, lane);
+                key[to] = k[r];
+                place[to] = uint16_t(p[r]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (live[r]) {
+                k[r] = key[begin + r * 64];
+                p[r] = place[begin + r * 64];
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (live[r]) {
+            keys[begin + r * 64] = k[r];
+            places[begin + r * 64] = p[r];
+        }
+    }
+}
+
+// Longer lists: per pass, digits counted per 4,096 tokens, the counts' running
+// sums, and the pairs moved.  `ids` is null after the first pass.
+template <class I>
+__global__ __launch_bounds__(256) void embedding_count_k(const I* ids, const uint32_t* keys, uint32_t tokens, int rows,
+                                                         int shift, int bits, int* counts) {
+    __shared__ int counter[1 << kDigitBits];
+    const int bins = 1 << bits;
+    for (int b = threadIdx.x; b < bins; b += 256) counter[b] = 0;
+    __syncthreads();
+    const uint32_t begin = blockIdx.x * uint32_t(kSortTokens);
+#pragma unroll 4
+    for (uint32_t j = 0; j < kSortTokens; j += 256) {
+        const uint32_t i = begin + j + threadIdx.x;
+        if (i < tokens) atomicAdd(&counter[((ids ? key_of(ids[i], rows) : keys[i]) >> shift) & (bins - 1)], 1);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += 256) counts[size_t(b) * gridDim.x + blockIdx.x] = counter[b];
+}
+
+__global__ __launch_bounds__(1024) void embedding_scan_k(int* counts, int64_t count) {
+    __shared__ int waves[16];
+    int carry = 0;
+    for (int64_t i = 0; i < count; i += 4096) {
+        int v[4], sum = 0, before;
+        const int64_t at = i + threadIdx.x * 4;
+        for (int j = 0; j < 4; ++j) sum += v[j] = at + j < count ? counts[at + j] : 0;
+        const int total = scan_block(sum, before, waves);
+        before += carry;
+        for (int j = 0; j < 4; ++j) {
+            if (at + j < count) counts[at + j] = before;
+            before += v[j];
+        }
+        carry += total;
+    }
+}
+
+template <class I>
+__global__ __launch_bounds__(256) void embedding_move_k(const I* ids, const uint32_t* keys, const uint32_t* places,
+                                                        uint32_t tokens, int rows, int shift, int bits,
+                                                        const int* counts, uint32_t* to_keys, uint32_t* to_places) {
+    __shared__ int counter[4][1 << kDigitBits];
+    const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kRounds = kSortTokens / 256;  // of a wave's quarter
+    for (int b = threadIdx.x; b < bins; b += 256)
+        for (int w = 0; w < 4; ++w) counter[w][b] = 0;
+    const uint32_t begin = blockIdx.x * uint32_t(kSortTokens) + wave * (kSortTokens / 4) + lane;
+    uint32_t k[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const uint32_t i = begin + r * 64;
+        k[r] = i < tokens ? ids ? key_of(ids[i], rows) : keys[i] : 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+        if (begin + r * 64 < tokens) atomicAdd(&counter[wave][(k[r] >> shift) & (bins - 1)], 1);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += 256) {
+        int at = counts[size_t(b) * gridDim.x + blockIdx.x];
+        for (int w = 0; w < 4; ++w) {
+            const int n = counter[w][b];
+            counter[w][b] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const uint32_t i = begin + r * 64;
+        const bool live = i < tokens;
+        const uint32_t digit = (k[r] >> shift) & (bins - 1);
+        const uint64_t peers = same_digit(digit, bits, live);
+        if (live) {
+            const int to = take_place(&counter[wave][digit], peers, lane);
+            to_keys[to] = k[r];
+            to_places[to] = ids ? i : places[i];
+        }
+    }
+}
+
+// ---- sums of sorted tokens ------------------------------------------------------------
+struct SumArgs {
+    const uint32_t *keys, *places;
+    const void* dout;
+    int64_t dout_stride;
+    float* dtable;
+    int64_t dtable_stride;
+    float *sums1, *sums2;  // of whole runs of kFan and kFan^2 tokens, [run][width]
+    uint32_t tokens;
+    int rows, width, accumulate, group_rows, lanes;  // lanes a row of `width` takes in one slice (a power of two)
+    float scale;
+    bool aligned, aligned_out;
+};
+
+// A lane's values of a partial sum, whose rows are `width` floats.
+template <int N>
+__device__ inline void load_sum(float* v, const float* p, int left, int width) {
+    if (width % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const vec<float, 4> in = j < left ? *reinterpret_cast<const vec<float, 4>*>(p + j) : vec<float, 4>{};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[j + q] = in[q];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = j < left ? p[j] : 0.f;
+    }
+}
+
+// Partial sums of the aligned runs of kFan tokens (level 1), or of kFan level-1
+// sums (level 2), that lie whole inside one row: a common token's row is then the
+// sum of few terms, whatever its count.  One group of lanes a run and slice.
+template <class T>
+__global__ __launch_bounds__(256) void embedding_partial_k(SumArgs a, uint32_t runs, int level) {
+    constexpr int N = kLane<T>;
+    const uint64_t run = (uint64_t(blockIdx.x) * 256 + threadIdx.x) / unsigned(a.lanes);
+    const int column = (blockIdx.y * a.lanes + threadIdx.x % a.lanes) * N, left = a.width - column;
+    if (run >= runs || left <= 0) return;
+    const uint32_t span = level == 1 ? kFan : kFan * kFan, first = uint32_t(run) * span;
+    const uint32_t row = a.keys[first];
+    if (row >= uint32_t(a.rows) || row != a.keys[first + span - 1]) return;
+    float acc[N] = {};
+    for (uint32_t i = 0; i < kFan; i += 8) {
+        float v[8][N];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u) {
+            if (level == 1)
+                load_lane(v[u], static_cast<const T*>(a.dout) + int64_t(a.places[first + i + u]) * a.dout_stride + column,
+                          left, a.aligned);
+            else load_sum<N>(v[u], a.sums1 + (size_t(run) * kFan + i + u) * a.width + column, left, a.width);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+    }
+    float* to = (level == 1 ? a.sums1 : a.sums2) + size_t(run) * a.width + column;
+    for (int j = 0; j < N && j < left; ++j) to[j] = acc[j];
+}
+
+// First sorted token whose row is at least `row`, by a group of `lanes` lanes: each
+// step probes `lanes` places at once.  All lanes of the wave take part.
+__device__ inline uint32_t first_of(const uint32_t* keys, uint32_t tokens, uint32_t row, int lanes) {
+    const int lane = threadIdx.x & 63, in = lane & (lanes - 1);
+    const uint64_t group = (lanes == 64 ? ~0ull : (1ull << lanes) - 1) << (lane - in);
+    uint32_t low = 0, high = tokens;  // the answer lies in [low, high]
+    while (__any(low < high)) {
+        const uint64_t left = high - low;
+        const auto probe = [&](int i) { return low + uint32_t(left * uint64_t(i + 1) / uint64_t(lanes + 1)); };
+        const bool less = low < high && keys[probe(in)] < row;
+        const int below = __popcll(__ballot(less) & group);  // probes 0..below-1 are less
+        if (low < high) {
+            const uint32_t to = below == lanes ? high : probe(below);
+            if (below) low = probe(below - 1) + 1;
+            high = to;
+        }
+    }
+    return low;
+}
+
+// The table's gradient: a group of lanes takes `group_rows` rows and their sorted
+// tokens, eight loads in flight whatever rows they belong to, and writes each row
+// once, the sum of its tokens (or zeros).  Where a whole run of kFan tokens, or of
+// kFan such runs, belongs to one row, its partial sum stands for it: the order of
+// a sum depends on the tokens alone.  Bound: HBM.
+template <class T>
+__global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
+    constexpr int N = kLane<T>;
+    const uint64_t group = (uint64_t(blockIdx.x) * 256 + threadIdx.x) / unsigned(a.lanes);
+    const int column = (blockIdx.y * a.lanes + threadIdx.x % a.lanes) * N;
+    const uint64_t begin_row = std::min(group * uint64_t(a.group_rows), uint64_t(a.rows));
+    const uint32_t end_row = uint32_t(std::min(begin_row + a.group_rows, uint64_t(a.rows)));
+    uint32_t at = first_of(a.keys, a.tokens, uint32_t(begin_row), a.lanes);
+    const uint32_t end = first_of(a.keys, a.tokens, end_row, a.lanes);
+    if (column >= a.width) return;
+    const T* base = static_cast<const T*>(a.dout) + column;
+    const int left = a.width - column;
+    uint32_t row = uint32_t(begin_row);
+    float acc[N] = {};
+    const auto finish_before = [&](uint32_t next) {
+        for (; row < next; ++row) {
+            float* out = a.dtable + int64_t(row) * a.dtable_stride + column;
+            if (a.aligned_out) {
+#pragma unroll
+                for (int j = 0; j < N; j += 4) {
+                    vec<float, 4>* p = reinterpret_cast<vec<float, 4>*>(out + j);
+                    vec<float, 4> v = {acc[j] * a.scale, acc[j + 1] * a.scale, acc[j + 2] * a.scale, acc[j + 3] * a.scale};
+                    if (a.accumulate) v += *p;
+                    *p = v;
+                }
+            } else {
+                for (int j = 0; j < N && j < left; ++j) out[j] = (a.accumulate ? out[j] : 0.f) + acc[j] * a.scale;
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] = 0.f;
+        }
+    };
+    while (at < end) {
+        const uint32_t key = a.keys[at];
+        const auto whole = [&](uint32_t from, uint32_t span) {
+            return from % span == 0 && from + span <= end && a.keys[from + span - 1] == key;
+        };
+        if (whole(at, kFan)) {
+            const bool second = whole(at, kFan * kFan);
+            const uint32_t span = second ? kFan * kFan : kFan;
+            const float* sums = (second ? a.sums2 : a.sums1) + column;
+            finish_before(key);
+            int runs = 1;
+            while (runs < 8 && whole(at + runs * span, span)) ++runs;
+            float v[8][N];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) load_sum<N>(v[u], sums + size_t(at / span + (u < runs ? u : 0)) * a.width, left, a.width);
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (u < runs)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+            at += runs * span;
+        } else {
+            // to the next place where a whole run may begin
+            const int count = int(std::min(std::min(end - at, kFan - at % kFan), 8u));
+            uint32_t key8[8];
+            float v[8][N];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const uint32_t i = at + (u < count ? u : 0);
+                key8[u] = a.keys[i];
+                load_lane(v[u], base + int64_t(a.places[i]) * a.dout_stride, left, a.aligned);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                if (u < count) {
+                    finish_before(key8[u]);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+                }
+            }
+            at += count;
+        }
+    }
+    finish_before(end_row);
+}
+
+template <class T, class I>
+void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
+    Device& d = *e.dev;
+    const Layout l = layout(e);
+    const auto part = [&](size_t at) { return reinterpret_cast<uint32_t*>(e.work + at); };
+    const int bits = bit_width(uint32_t(e.rows));
+    int now = 0;
+    if (tokens <= kSmallSort) {
+        if (tokens)
+            hipLaunchKernelGGL((embedding_sort_small_k<I>), 1, 1024, 0, d.stream, ids, int(tokens), e.rows, bits,
+                               part(l.keys[0]), part(l.places[0]));
+    } else {
+        const int digit = digit_bits(e.rows), passes = sort_passes(e.rows);
+        const unsigned blocks = (tokens + kSortTokens - 1) / kSortTokens;
+        int* counts = reinterpret_cast<int*>(e.work + l.counts);
+        for (int p = 0; p < passes; ++p) {
+            const I* source = p ? nullptr : ids;
+            hipLaunchKernelGGL((embedding_count_k<I>), blocks, 256, 0, d.stream, source, part(l.keys[now]), tokens, e.rows,
+                               p * digit, digit, counts);
+            hipLaunchKernelGGL(embedding_scan_k, 1, 1024, 0, d.stream, counts, int64_t(blocks) << digit);
+            hipLaunchKernelGGL((embedding_move_k<I>), blocks, 256, 0, d.stream, source, part(l.keys[now]),
+                               part(l.places[now]), tokens, e.rows, p * digit, digit, counts, part(l.keys[1 - now]),
+                               part(l.places[1 - now]));
+            now = 1 - now;
+        }
+    }
+    a.keys = part(l.keys[now]);
+    a.places = part(l.places[now]);
+    a.sums1 = reinterpret_cast<float*>(part(l.sums1));
+    a.sums2 = reinterpret_cast<float*>(part(l.sums2));
+    a.tokens = tokens;
+    constexpr int N = kLane<T>;
+    const int per_row = (e.width + N - 1) / N;
+    a.lanes = 1;
+    while (a.lanes < per_row && a.lanes < 64) a.lanes <<= 1;
+    const unsigned slices = unsigned((per_row + a.lanes - 1) / a.lanes);
+    for (int level = 1; level <= 2; ++level) {
+        const uint32_t runs = tokens / (level == 1 ? kFan : kFan * kFan);
+        if (runs)
+            hipLaunchKernelGGL((embedding_partial_k<T>), dim3(unsigned((uint64_t(runs) * a.lanes + 255) / 256), slices),
+                               256, 0, d.stream, a, runs, level);
+    }
+    // rows a group: 16 where there are many (a search serves them all), fewer where
+    // that would leave the device short of waves
+    const int64_t groups_wanted = int64_t(d.compute_units) * 16 * (64 / a.lanes) / slices;
+    a.group_rows = int(std::clamp<int64_t>(e.rows / std::max<int64_t>(groups_wanted, 1), 1, 16));
+    const uint64_t groups = (uint64_t(e.rows) + a.group_rows - 1) / a.group_rows;
+    hipLaunchKernelGGL((embedding_sum_k<T>), dim3(unsigned((groups * unsigned(a.lanes) + 255) / 256), slices), 256, 0, d.stream, a);
+}
+
+void check_rows(const cpde_rows* r, int64_t count, int width, bool output) {
+    require(r, "null argument");
+    require(r->data || count == 0, "null tensor");
+    require(r->stride >= 0, "negative stride");
+    require(!output || count <= 1 || r->stride >= width, "output rows overlap");
+}
+
+}  // namespace
+}  // namespace cpde
+
+struct cpde_embedding_s : cpde::Embedding {};
+using namespace cpde;
+
+extern "C" {
+
+int cpde_embedding_create(cpde_device* dev, int dtype, int rows, int width, int64_t tokens, int index_bytes,
+                          cpde_embedding** out) {
+    return guarded([&] {
+        require(dev && out, "null argument");
+        *out = nullptr;
+        check_dtype(dtype);
+        require(rows >= 1 && rows < (1 << 30) && width >= 1 && width <= (1 << 24), "invalid table size");
+        require(tokens >= 0 && tokens < (int64_t(1) << 31) - kSortTokens, "invalid token count");
+        require(index_bytes == 4 || index_bytes == 8, "ids are 4 or 8 bytes");
+        auto e = std::make_unique<cpde_embedding_s>();
+        e->dev = dev;
+        e->dtype = dtype;
+        e->rows = rows;
+        e->width = width;
+        e->tokens = tokens;
+        e->index_bytes = index_bytes;
+        require(!dev->capturing, "a capture is open on this device");
+        HIP_CHECK(hipMalloc(&e->work, layout(*e).bytes));
+        *out = e.release();
+    });
+}
+
+int cpde_embedding_destroy(cpde_embedding* embedding) {
+    return guarded([&] {
+        if (!embedding) return;
+        sync_stream(*embedding->dev, __LINE__);
+        ++embedding->dev->layout;
+        HIP_CHECK(hipFree(embedding->work));
+        delete embedding;
+    });
+}
+
+int cpde_embedding_forward(cpde_embedding* embedding, const void* ids, int64_t tokens, const cpde_rows* table,
+                           float scale, const cpde_rows* out) {
+    return guarded([&] {
+        require(embedding, "null argument");
+        const Embedding& e = *embedding;
+        require(tokens >= 0 && tokens <= e.tokens, "more tokens than the embedding was created for");
+        require(ids || tokens == 0, "null tensor");
+        check_rows(table, e.rows, e.width, false);
+        check_rows(out, tokens, e.width, true);
+        if (!tokens) return;
+        const size_t size = type_bytes(e.dtype);
+        const bool aligned = wide(table->data, table->stride, size) && wide(out->data, out->stride, size) &&
+                             e.width * size % 16 == 0;
+        flush_reduce(*e.dev);
+        TraceScope trace(*e.dev, kTraceEmbedding, double(tokens) * (2.0 * e.width * double(size) + e.index_bytes));
+        with_type(e.dtype, [&](auto element) {
+            using T = decltype(element);
+            const uint32_t per_row = uint32_t((e.width + kLane<T> - 1) / kLane<T>);
+            const uint64_t lanes = uint64_t(tokens) * per_row;
+            const unsigned blocks =
+                unsigned(std::min<uint64_t>((lanes + 255) / 256, uint64_t(e.dev->compute_units) * 64));
+            const auto launch = [&](auto* at) {
+                using I = std::remove_const_t<std::remove_pointer_t<decltype(at)>>;
+                hipLaunchKernelGGL((embedding_lookup_k<T, I>), blocks, 256, 0, e.dev->stream, at, lanes, per_row,
+                                   static_cast<const T*>(table->data), table->stride, e.rows, e.width, scale,
+                                   static_cast<T*>(out->data), out->stride, aligned);
+            };
+            if (e.index_bytes == 4) launch(static_cast<const int32_t*>(ids));
+            else launch(static_cast<const int64_t*>(ids));
+        });
+        HIP_CHECK(hipGetLastError());
+    });
+}
+
+int cpde_embedding_backward(cpde_embedding* embedding, const void* ids, int64_t tokens, const cpde_rows* dout,
+                            float scale, const cpde_rows* dtable, int accumulate) {
+    return guarded([&] {
+        require(embedding, "null argument");
+        const Embedding& e = *embedding;
+        require(tokens >= 0 && tokens <= e.tokens, "more tokens than the embedding was created for");
+        require(ids || tokens == 0, "null tensor");
+        check_rows(dout, tokens, e.width, false);
+        check_rows(dtable, e.rows, e.width, true);
+        const size_t size = type_bytes(e.dtype);
+        SumArgs a{};
+        a.dout = dout->data;
+        a.dout_stride = dout->stride;
+        a.dtable = static_cast<float*>(dtable->data);
+        a.dtable_stride = dtable->stride;
+        a.rows = e.rows;
+        a.width = e.width;
+        a.accumulate = accumulate != 0;
+        a.scale = scale;
+        a.aligned = wide(dout->data, dout->stride, size) && e.width * size % 16 == 0;
+        a.aligned_out = wide(dtable->data, dtable->stride, 4) && e.width * size % 16 == 0;
+        flush_reduce(*e.dev);
+        TraceScope trace(*e.dev, kTraceEmbedding,
+                         double(tokens) * (double(size) * e.width + e.index_bytes) + 4.0 * e.rows * double(e.width));
+        with_type(e.dtype, [&](auto element) {
+            using T = decltype(element);
+            if (e.index_bytes == 4) gradient<T>(e, static_cast<const int32_t*>(ids), uint32_t(tokens), a);
+            else gradient<T>(e, static_cast<const int64_t*>(ids), uint32_t(tokens), a);
+        });
+        HIP_CHECK(hipGetLastError());
+    });
+}
+
+}  // extern "C"

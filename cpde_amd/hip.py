@@ -26,6 +26,38 @@ class GradientStats(ctypes.Structure):
                 ('nonfinite_count', ctypes.c_uint64), ('first_nonfinite', ctypes.c_int32), ('pad_', ctypes.c_int32)]
 
 
+class Heads(ctypes.Structure):
+    """cpde_heads: a device tensor [batch][token][head][head_dim] by its element
+    strides, the last axis contiguous."""
+    _fields_ = [('data', ctypes.c_void_p), ('batch', ctypes.c_int64), ('token', ctypes.c_int64),
+                ('head', ctypes.c_int64)]
+
+    @classmethod
+    def of(cls, tensor):
+        """The view of a tensor with data_ptr() and stride() (torch's), which the caller keeps."""
+        batch, token, head, last = tensor.stride()
+        if last != 1 and tensor.shape[-1] > 1:
+            raise ValueError('the last axis is not contiguous')
+        return cls(tensor.data_ptr(), batch, token, head)
+
+
+class Rows(ctypes.Structure):
+    """cpde_rows: a device matrix by its row stride in elements, columns contiguous."""
+    _fields_ = [('data', ctypes.c_void_p), ('stride', ctypes.c_int64)]
+
+    @classmethod
+    def of(cls, tensor):
+        stride, last = tensor.stride()
+        if last != 1 and tensor.shape[-1] > 1:
+            raise ValueError('the last axis is not contiguous')
+        return cls(tensor.data_ptr(), stride)
+
+
+class AttentionShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ('dtype', 'batch', 'query_tokens', 'key_tokens', 'heads', 'kv_heads',
+                                              'head_dim', 'left', 'right', 'backward')] + [('scale', ctypes.c_float)]
+
+
 class CpdeError(RuntimeError):
     def __init__(self, code, message):
         super().__init__(f'[{code}] {message}')
@@ -36,10 +68,17 @@ _lib = None
 vp = ctypes.c_void_p
 i32 = ctypes.c_int
 f32 = ctypes.c_float
+i64 = ctypes.c_int64
+u64 = ctypes.c_uint64
+heads_p = ctypes.POINTER(Heads)
+rows_p = ctypes.POINTER(Rows)
+
+F32, F16, BF16 = 0, 1, 2    # element types of the operators on sequences
 
 SIGNATURES = {
     'cpde_last_error': (ctypes.c_char_p, []),
     'cpde_device_open': (i32, [i32, ctypes.POINTER(vp)]),
+    'cpde_device_open_on': (i32, [i32, vp, ctypes.POINTER(vp)]),
     'cpde_device_close': (i32, [vp]),
     'cpde_device_synchronize': (i32, [vp]),
     'cpde_device_info': (i32, [vp, ctypes.c_char_p, ctypes.c_size_t, ctypes.POINTER(i32)]),
@@ -93,6 +132,16 @@ SIGNATURES = {
     'cpde_program_destroy': (i32, [vp]),
     'cpde_cost_expression': (i32, [vp, vp, vp, vp, i32, i32, i32, vp, vp, i32, i32, i32]),
     'cpde_epoch_expression': (i32, [vp, vp, vp, vp, i32, i32, i32, vp, vp, i32, i32, i32]),
+    'cpde_attention_create': (i32, [vp, ctypes.POINTER(AttentionShape), ctypes.POINTER(vp)]),
+    'cpde_attention_destroy': (i32, [vp]),
+    'cpde_attention_forward': (i32, [vp, heads_p, heads_p, heads_p, heads_p, vp, vp, vp]),
+    'cpde_attention_backward': (i32, [vp, heads_p, heads_p, heads_p, heads_p, vp, heads_p, heads_p, heads_p, heads_p,
+                                      vp, vp]),
+    'cpde_embedding_create': (i32, [vp, i32, i32, i32, i64, i32, ctypes.POINTER(vp)]),
+    'cpde_embedding_destroy': (i32, [vp]),
+    'cpde_embedding_forward': (i32, [vp, vp, i64, rows_p, f32, rows_p]),
+    'cpde_embedding_backward': (i32, [vp, vp, i64, rows_p, f32, rows_p, i32]),
+    'cpde_dropout': (i32, [vp, i32, i64, i64, rows_p, rows_p, rows_p, ctypes.c_double, u64, u64]),
     'cpde_capture_begin': (i32, [vp]),
     'cpde_capture_end': (i32, [vp, i32, vp]),
     'cpde_replay_launch': (i32, [vp]),
@@ -142,6 +191,13 @@ def _ptr(a):
     return ctypes.c_void_p(a.ctypes.data)
 
 
+def _address(a):
+    """The device address of a Buffer, a tensor with data_ptr() (torch's), a pointer, or None."""
+    if a is None or isinstance(a, (int, ctypes.c_void_p)):
+        return a
+    return a.ptr if isinstance(a, Buffer) else a.data_ptr()
+
+
 class Buffer:
     """A device allocation (bytes); upload/download take numpy arrays."""
 
@@ -175,9 +231,16 @@ class Buffer:
 
 
 class Device:
-    def __init__(self, ordinal=0):
+    """An open GPU.  stream: None for a stream of the library's own, or the handle
+    of one of the caller's (0: the default stream), so that the library's work is
+    in order with what else runs there."""
+
+    def __init__(self, ordinal=0, stream=None):
         h = vp()
-        check(load().cpde_device_open(ordinal, ctypes.byref(h)))
+        if stream is None:
+            check(load().cpde_device_open(ordinal, ctypes.byref(h)))
+        else:
+            check(load().cpde_device_open_on(ordinal, stream, ctypes.byref(h)))
         self.handle = h
 
     def info(self):
@@ -228,6 +291,11 @@ class Device:
             if n.value:
                 out[lib.cpde_trace_name(k).decode()] = (n.value, ms.value, work.value)
         return out
+
+    def dropout(self, dtype, rows, columns, x, y, probability, seed, offset=0, residual=None):
+        """y = dropout(x) (+ residual), Rows of one type; the gradient is the same
+        call on y's gradient with the same probability, seed and offset."""
+        check(load().cpde_dropout(self.handle, dtype, rows, columns, x, residual, y, probability, seed, offset))
 
     def capture_begin(self):
         check(load().cpde_capture_begin(self.handle))
@@ -430,6 +498,55 @@ class Plan:
     def destroy(self):
         if self.handle:
             check(load().cpde_plan_destroy(self.handle))
+            self.handle = None
+
+
+class Attention:
+    """Attention of one shape and type (cpde_attention_shape).  Tensors are Heads,
+    lse and the lengths device addresses (or tensors, or Buffers)."""
+
+    def __init__(self, device, dtype, batch, query_tokens, key_tokens, heads, kv_heads, head_dim, scale=0.0, left=-1,
+                 right=-1, backward=True):
+        self.device = device
+        shape = AttentionShape(dtype, batch, query_tokens, key_tokens, heads, kv_heads, head_dim, left, right,
+                               int(backward), scale)
+        h = vp()
+        check(load().cpde_attention_create(device.handle, ctypes.byref(shape), ctypes.byref(h)))
+        self.handle = h
+
+    def forward(self, q, k, v, out, lse=None, query_lengths=None, key_lengths=None):
+        check(load().cpde_attention_forward(self.handle, q, k, v, out, _address(lse), _address(query_lengths),
+                                            _address(key_lengths)))
+
+    def backward(self, q, k, v, out, lse, dout, dq, dk, dv, query_lengths=None, key_lengths=None):
+        check(load().cpde_attention_backward(self.handle, q, k, v, out, _address(lse), dout, dq, dk, dv,
+                                             _address(query_lengths), _address(key_lengths)))
+
+    def destroy(self):
+        if self.handle:
+            check(load().cpde_attention_destroy(self.handle))
+            self.handle = None
+
+
+class Embedding:
+    """Lookups of at most `tokens` ids a call in a table of rows x width, and the
+    table's gradient.  ids are a device address (or tensor, or Buffer), the others Rows."""
+
+    def __init__(self, device, dtype, rows, width, tokens, index_bytes=4):
+        self.device = device
+        h = vp()
+        check(load().cpde_embedding_create(device.handle, dtype, rows, width, tokens, index_bytes, ctypes.byref(h)))
+        self.handle = h
+
+    def forward(self, ids, tokens, table, out, scale=1.0):
+        check(load().cpde_embedding_forward(self.handle, _address(ids), tokens, table, scale, out))
+
+    def backward(self, ids, tokens, dout, dtable, scale=1.0, accumulate=False):
+        check(load().cpde_embedding_backward(self.handle, _address(ids), tokens, dout, scale, dtable, int(accumulate)))
+
+    def destroy(self):
+        if self.handle:
+            check(load().cpde_embedding_destroy(self.handle))
             self.handle = None
 
 

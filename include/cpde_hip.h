@@ -43,6 +43,8 @@ typedef struct cpde_plan_s cpde_plan;
 typedef struct cpde_program_s cpde_program;
 typedef struct cpde_stacks_s cpde_stacks;
 typedef struct cpde_replay_s cpde_replay;
+typedef struct cpde_attention_s cpde_attention;
+typedef struct cpde_embedding_s cpde_embedding;
 
 /* Per-cost reduction result: signed double sum and the first bad (sample,
  * component); component -1 means the objective itself
@@ -85,6 +87,11 @@ const char* cpde_last_error(void);
 /* ---- device, stream and buffers (replaces cudaSetDevice/cudaStreamCreate/
  *      cudaMalloc/cudaMemcpy uses, cuda/cpde_engine.cuh:23-87, cuda/cpde_server.cu:26-33) */
 int cpde_device_open(int ordinal, cpde_device** out);
+/* The same on a stream of the caller's (a hipStream_t of that GPU; NULL: the
+ * default stream), which the caller keeps until the device is closed: work
+ * that the caller issues on it is in order with the library's, without a wait.
+ * A device on the default stream cannot be captured (cpde_capture_begin). */
+int cpde_device_open_on(int ordinal, void* stream, cpde_device** out);
 int cpde_device_close(cpde_device* dev);
 int cpde_device_synchronize(cpde_device* dev);
 /* Name and compute-unit count of the open device. */
@@ -373,6 +380,97 @@ int cpde_graph_execute(cpde_device* dev, const cpde_scalar_node* nodes, int coun
  * compile (cuda/expression_program.hpp:104-121), done lazily at first use. */
 int cpde_jit_prepare(int rows, int variables, const int* table, int layers, const int* neurons, int width,
                      int compute_units, const char* arch, char* log, size_t log_capacity);
+
+/* ---- operators on sequences -------------------------------------------------------
+ * No counterpart in the reference, whose networks see one point at a time: what a
+ * network needs to read sets and sequences of points or tokens, each with its
+ * gradient.  All of them run on the device's stream, return before the work is
+ * done, allocate nothing after their create call (so they can be recorded) and
+ * sum in a fixed order: the same call on the same inputs gives the same bits.
+ * Tensors are device memory of one of the three types; sums, softmax statistics
+ * and table gradients are held in 32 bits, and results are rounded once, except
+ * where a comment says so.  Outputs must not overlap inputs or each other, but
+ * for cpde_dropout, whose output may be one of its inputs. */
+#define CPDE_F32 0
+#define CPDE_F16 1
+#define CPDE_BF16 2
+
+/* A tensor [batch][token][head][head_dim]: strides in elements, the last axis
+ * contiguous.  Any order of the first three axes; an input may have strides of
+ * zero (broadcast), an output may not have two elements in one place.  Strides
+ * and addresses that are whole multiples of 16 bytes, and so head_dim, are read
+ * 16 bytes at a time; others one element at a time. */
+typedef struct {
+    void* data;
+    int64_t batch, token, head;
+} cpde_heads;
+
+/* A matrix: stride in elements from row to row, columns contiguous. */
+typedef struct {
+    void* data;
+    int64_t stride;
+} cpde_rows;
+
+/* Attention of `heads` query heads on `kv_heads` key heads (a whole number of
+ * query heads each: query head h reads key head h / (heads / kv_heads)), head_dim
+ * at most 128.  Query i of batch entry b sees key j where
+ *   i < ql, j < kl and -left <= j - (i + kl - ql) <= right,
+ * with ql and kl the entry's lengths (query_tokens and key_tokens where the call
+ * gives none): the last query stands on the last key.  A negative left or right
+ * is no bound, right = 0 is causal.  scale > 0 multiplies the scores; 0 stands for
+ * 1/sqrt(head_dim). */
+typedef struct {
+    int32_t dtype, batch, query_tokens, key_tokens, heads, kv_heads, head_dim;
+    int32_t left, right;
+    int32_t backward; /* 0: cpde_attention_backward will not be called */
+    float scale;
+} cpde_attention_shape;
+
+int cpde_attention_create(cpde_device* dev, const cpde_attention_shape* shape, cpde_attention** out);
+int cpde_attention_destroy(cpde_attention* attention);
+/* out_i = sum_j p_ij v_j with p_ij = exp(s_ij - lse_i) over the keys that i sees,
+ * s_ij = scale q_i.k_j, lse_i = log sum_j exp(s_ij).  lse [batch][heads][query_tokens]
+ * float (may be NULL).  query_lengths, key_lengths: int32 [batch] on the device, or
+ * NULL; values outside 0..tokens count as the nearest of the two.  Keys and queries
+ * at or past the lengths are not read.  A query that sees no key, or past its
+ * length, gives zeros and lse = -inf.  Probabilities are rounded to the tensors'
+ * type before they multiply v. */
+int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const cpde_heads* k, const cpde_heads* v,
+                           const cpde_heads* out, float* lse, const int32_t* query_lengths,
+                           const int32_t* key_lengths);
+/* The gradients of q, k and v from dout, with out and lse as the forward gave them
+ * on the same inputs: the probabilities are recomputed.  Keys' gradients are summed
+ * over the query heads that share them.  Rows at or past the lengths, queries that
+ * see no key and keys that no query sees get zeros. */
+int cpde_attention_backward(cpde_attention* attention, const cpde_heads* q, const cpde_heads* k, const cpde_heads* v,
+                            const cpde_heads* out, const float* lse, const cpde_heads* dout, const cpde_heads* dq,
+                            const cpde_heads* dk, const cpde_heads* dv, const int32_t* query_lengths,
+                            const int32_t* key_lengths);
+
+/* A table of `rows` x `width` values looked up by at most `tokens` ids a call, of
+ * index_bytes 4 or 8 (signed). */
+int cpde_embedding_create(cpde_device* dev, int dtype, int rows, int width, int64_t tokens, int index_bytes,
+                          cpde_embedding** out);
+int cpde_embedding_destroy(cpde_embedding* embedding);
+/* out_t = scale * table[ids_t]; an id outside [0, rows) gives zeros. */
+int cpde_embedding_forward(cpde_embedding* embedding, const void* ids, int64_t tokens, const cpde_rows* table,
+                           float scale, const cpde_rows* out);
+/* dtable_r (+)= scale * sum of dout_t over the tokens t with ids_t = r, for every
+ * row r, in float whatever dout's type; ids outside [0, rows) have no share.
+ * accumulate=0 overwrites the whole table gradient, 1 adds to it. */
+int cpde_embedding_backward(cpde_embedding* embedding, const void* ids, int64_t tokens, const cpde_rows* dout,
+                            float scale, const cpde_rows* dtable, int accumulate);
+
+/* y = x / (1 - probability) where an element is kept, 0 where it is dropped, plus
+ * residual (may be NULL); the gradient of x is the same call on y's gradient
+ * without a residual.  Element e = row * columns + column takes word e % 4 of the
+ * generator Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random
+ * numbers: as easy as 1, 2, 3", 2011) at counter offset + e / 4 with key `seed`, and
+ * is kept where the word is at least round(probability * 2^32): nothing of the
+ * mask is stored.  A call uses up (rows * columns + 3) / 4 counters.
+ * probability 1 drops everything. */
+int cpde_dropout(cpde_device* dev, int dtype, int64_t rows, int64_t columns, const cpde_rows* x,
+                 const cpde_rows* residual, const cpde_rows* y, double probability, uint64_t seed, uint64_t offset);
 
 /* ---- captured epochs ------------------------------------------------------------- */
 /* No counterpart in the reference, whose server issues every launch of every
