@@ -71,10 +71,10 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
     vload.start(a.v.token, a.dim, a.wide_in);
     const char* kbase = reinterpret_cast<const char*>(head_row<const T>(a.k, b, 0, kv));
     const char* vbase = reinterpret_cast<const char*>(head_row<const T>(a.v, b, 0, kv));
-    const auto load = [&](int t, int buffer) {
+    const auto load = [&](int t, char* to_keys, char* to_values) {
         const int64_t first = int64_t(t) * N;
-        kload.load(lds[buffer][0], kbase + first * kload.stride, band.kl - t * N, wave);
-        vload.load(lds[buffer][1], vbase + first * vload.stride, band.kl - t * N, wave);
+        kload.load(to_keys, kbase + first * kload.stride, band.kl - t * N, wave);
+        vload.load(to_values, vbase + first * vload.stride, band.kl - t * N, wave);
     };
 
     Acc out[kBlocks] = {};
@@ -82,16 +82,15 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
     if (t0 < t1) {
         for (int i = 0; i < 4; ++i) kload.clear(lds[i >> 1][i & 1]);
         if (kload.direct && a.dim < DP) __syncthreads();
-        load(t0, 0);
+        load(t0, lds[0][0], lds[0][1]);
     }
-    for (int t = t0; t < t1; ++t) {
-        const int buffer = (t - t0) & 1;
-        arrived();
-        __syncthreads();
-        if (t + 1 < t1) load(t + 1, buffer ^ 1);
+    // (the tile read and the tiles written do not overlap, which the compiler has to
+    // know so as not to wait for the loads under way before it reads)
+    const auto step = [&](int t, const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next_keys,
+                          char* __restrict__ next_values) __attribute__((always_inline)) {
+        if (t + 1 < t1) load(t + 1, next_keys, next_values);
         const int first = t * N;
-        if (first >= wave_hi || first + N <= wave_lo) continue;
-        const char *keys = lds[buffer][0], *values = lds[buffer][1];
+        if (first >= wave_hi || first + N <= wave_lo) return;
         Acc s[kSub];
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
@@ -138,6 +137,12 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) out[d] = mma(L::column(values, d, 2 * u + i, lane), p, out[d]);
             }
+    };
+    for (int t = t0; t < t1; ++t) {
+        const int now = (t - t0) & 1, next = now ^ 1;
+        arrived();
+        __syncthreads();
+        step(t, lds[now][0], lds[now][1], lds[next][0], lds[next][1]);
     }
     sum = halves_sum(sum);
     if (row >= rows) return;
@@ -328,49 +333,93 @@ struct JoinArgs {
     HeadView out;
     float* lse;
     int splits, pairs, rows, dim, kv_heads, group;
-    int per_query;  // rows of a key head (queries x group)
+    int teams;  // of 32 lanes a row, each with every teams-th split (a power of two)
+    int wide_part, wide_out;
     float scale;
 };
 
-// One wave a row; lanes over its columns.  Splits that saw no key wrote no output.
+// 32 lanes hold a row, four columns each; `teams` of them share its splits, with a
+// running maximum each, and are joined through LDS in order.  Splits that saw no
+// key wrote no output.  Bound: HBM (the parts read once).
 template <class T>
-__global__ __launch_bounds__(64) void attention_join_k(JoinArgs a) {
-    const int pair = blockIdx.x % a.pairs, row = blockIdx.x / a.pairs;
+__global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
+    __shared__ float shared[8][32][6];
+    const int lane = threadIdx.x & 31, team = threadIdx.x / 32, in = team & (a.teams - 1);
+    const int64_t count = int64_t(a.pairs) * a.rows;
+    const int64_t item = int64_t(blockIdx.x) * (8 / a.teams) + team / a.teams, at = min(item, count - 1);
+    const int d = lane * 4;
+    float top = -INFINITY, total = 0;
+    vec<float, 4> value = {};
+#pragma unroll 4
+    for (int s = in; s < a.splits; s += a.teams) {
+        const int64_t from = s * count + at;
+        float m = 0, l = 1;
+        if (a.stats) {
+            const auto both = *reinterpret_cast<const vec<float, 2>*>(a.stats + 2 * from);
+            m = both[0];
+            l = both[1];
+        }
+        vec<float, 4> v = {};
+        const float* p = a.part + from * a.dim + d;
+        if (a.wide_part) {
+            if (d < a.dim) v = *reinterpret_cast<const vec<float, 4>*>(p);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (d + j < a.dim) v[j] = p[j];
+        }
+        if (a.stats) {
+            const float next = fmaxf(top, m), base = next == -INFINITY ? 0.f : next;
+            const float mine = exp2_fast(top - base), theirs = exp2_fast(m - base);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) value[j] = value[j] * mine + (l == 0 ? 0.f : v[j] * theirs);
+            total = total * mine + l * theirs;
+            top = next;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) value[j] += v[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) shared[team][lane][j] = value[j];
+    shared[team][lane][4] = top;
+    shared[team][lane][5] = total;
+    __syncthreads();
+    if (in != 0 || item >= count) return;
+    for (int t = 1; t < a.teams; ++t) {
+        const float* other = shared[team + t][lane];
+        if (a.stats) {
+            const float next = fmaxf(top, other[4]), base = next == -INFINITY ? 0.f : next;
+            const float mine = exp2_fast(top - base), theirs = exp2_fast(other[4] - base);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) value[j] = value[j] * mine + other[j] * theirs;
+            total = total * mine + other[5] * theirs;
+            top = next;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) value[j] += other[j];
+        }
+    }
+    const int pair = int(item / a.rows), row = int(item % a.rows);
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
     const int token = row / a.group, head = kv * a.group + row % a.group;
-    const int64_t step = int64_t(a.pairs) * a.rows, first = int64_t(pair) * a.rows + row;
-    float base = 0, total = 1;
-    if (a.stats) {
-        float top = -INFINITY;
-        for (int s = threadIdx.x; s < a.splits; s += 64) top = fmaxf(top, a.stats[2 * (first + s * step)]);
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        base = top == -INFINITY ? 0.f : top;
-        total = 0;
-        // (every lane the same order)
-        for (int s = 0; s < a.splits; ++s) {
-            const float* m = a.stats + 2 * (first + s * step);
-            total += m[1] * exp2_fast(m[0] - base);
-        }
-        if (a.lse && threadIdx.x == 0)
-            a.lse[(int64_t(b) * a.kv_heads * a.group + head) * (a.rows / a.group) + token] =
-                total == 0 ? -INFINITY : base * kLn2 + logf(total);
+    const float by = a.stats ? (total == 0 ? 0.f : 1.f / total) : a.scale;
+    T* out = head_row<T>(a.out, b, token, head) + d;
+    if (a.wide_out) {
+        value *= by;
+        if (d < a.dim) *reinterpret_cast<vec<T, 4>*>(out) = __builtin_convertvector(value, vec<T, 4>);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (d + j < a.dim) out[j] = T(value[j] * by);
     }
-    T* out = head_row<T>(a.out, b, token, head);
-    for (int d = threadIdx.x; d < a.dim; d += 64) {
-        float value = 0;
-#pragma unroll 8
-        for (int s = 0; s < a.splits; ++s) {
-            const int64_t at = first + s * step;
-            float weight = 1;
-            if (a.stats) weight = a.stats[2 * at + 1] == 0 ? 0.f : exp2_fast(a.stats[2 * at] - base);
-            if (weight != 0) value += a.part[at * a.dim + d] * weight;
-        }
-        out[d] = T(a.stats ? (total == 0 ? 0.f : value / total) : value * a.scale);
-    }
+    if (a.lse && lane == 0)
+        a.lse[(int64_t(b) * a.kv_heads * a.group + head) * (a.rows / a.group) + token] =
+            total == 0 ? -INFINITY : top * kLn2 + logf(total);
 }
 
 // ---- gradient ---------------------------------------------------------------------------
-// dout.out of every query row, and its statistics in base 2; sixteen lanes a row.
+// dout.out of every query row, and its lse in the scores' units (over the scale); sixteen lanes a row.
 template <class T>
 __global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a) {
     const int heads = a.kv_heads * a.group;
@@ -390,7 +439,7 @@ __global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a) {
     if (in == 0 && i < count) {
         const int64_t at = (int64_t(b) * heads + head) * a.queries + query;
         const float lse = live ? a.lse[at] : -INFINITY;
-        a.row_lse[at] = lse == -INFINITY ? INFINITY : lse * kLog2e;  // (no key: every probability is 0)
+        a.row_lse[at] = lse == -INFINITY ? INFINITY : lse / a.scale;  // (no key: every probability is 0)
         a.row_delta[at] = dot;
     }
 }
@@ -408,13 +457,14 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
     __shared__ __align__(16) float stats[2][2][kQueries];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
-    const int tile = rest % a.tiles, split = rest / a.tiles;  // (a causal band's first keys are seen most)
+    // (a causal band's first keys are seen most; a second round of workgroups comes to
+    // the CUs of the first in the same order, so it goes the other way)
+    const int split = rest / a.tiles, tile = split & 1 ? a.tiles - 1 - rest % a.tiles : rest % a.tiles;
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
     const Band band(a, b);
     const int block_first = tile * kBlockRows, wave_first = block_first + wave * kWaveRows;
     const int key = wave_first + (lane & 31);
     const bool live = key < band.kl;
-    const int lo = live ? band.query_lo(key) : 0, hi = live ? band.query_hi(key) : 0;
 
     Frag<T> k[kSteps], v[kSteps];
     load_fragments<T, DP>(k, head_row<const T>(a.k, b, key, kv), a.dim, half, live, a.wide_in);
@@ -439,21 +489,35 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
     TileLoader<T, DP, kQueries> qload, oload;
     qload.start(a.q.token, a.dim, a.wide_in);
     oload.start(a.dout.token, a.dim, a.wide_in);
-    int head = per_head ? from / per_head : 0, t = t0 + from - head * per_head;  // of the next load
-    const auto load = [&](int buffer) {
-        const int first = t * kQueries, h = kv * a.group + head, valid = band.ql - first;
-        qload.load(lds[buffer][0], reinterpret_cast<const char*>(head_row<const T>(a.q, b, first, h)), valid, wave);
-        oload.load(lds[buffer][1], reinterpret_cast<const char*>(head_row<const T>(a.dout, b, first, h)), valid, wave);
-        if (wave == 0) {  // the 64 statistics, one a lane
-            const float* from = (lane < kQueries ? a.row_lse : a.row_delta) +
-                                (int64_t(b) * a.kv_heads * a.group + h) * a.queries + first;
+    // the next load: tile t of a head, and where it lies; after a head's last tile the
+    // next head's first
+    const int head = per_head ? from / per_head : 0;
+    int t = t0 + from - head * per_head;
+    const int first_head = kv * a.group + head;
+    const char* at_q = reinterpret_cast<const char*>(head_row<const T>(a.q, b, int64_t(t) * kQueries, first_head));
+    const char* at_o = reinterpret_cast<const char*>(head_row<const T>(a.dout, b, int64_t(t) * kQueries, first_head));
+    int64_t at_s = (int64_t(b) * a.kv_heads * a.group + first_head) * a.queries + int64_t(t) * kQueries;
+    const int64_t back_q = a.q.head * int64_t(sizeof(T)) - int64_t(per_head) * kQueries * qload.stride;
+    const int64_t back_o = a.dout.head * int64_t(sizeof(T)) - int64_t(per_head) * kQueries * oload.stride;
+    const auto load = [&](char* to_queries, char* to_douts, float* to_stats) {
+        const int valid = band.ql - t * kQueries;
+        qload.load(to_queries, at_q, valid, wave);
+        oload.load(to_douts, at_o, valid, wave);
+        if (wave < 2 * kQueries / 64) {  // the statistics, one a lane
+            const int i = wave * 64 + fresh(lane);
+            const float* from = (i < kQueries ? a.row_lse : a.row_delta) + at_s;
             __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)(from + min(lane % kQueries, valid - 1)),
-                (__attribute__((address_space(3))) void*)&stats[buffer][0][0], 4, 0, 0);
+                (const __attribute__((address_space(1))) void*)(from + min(i % kQueries, valid - 1)),
+                (__attribute__((address_space(3))) void*)(to_stats + wave * 64), 4, 0, 0);
         }
+        at_q += kQueries * qload.stride;
+        at_o += kQueries * oload.stride;
+        at_s += kQueries;
         if (++t == t1) {
             t = t0;
-            ++head;
+            at_q += back_q;
+            at_o += back_o;
+            at_s += a.queries - per_head * kQueries;
         }
     };
 
@@ -463,30 +527,46 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
         if (qload.direct && a.dim < DP) __syncthreads();
     }
     int at = t;  // of the tile computed on
-    if (from < to) load(0);
-    for (int i = from; i < to; ++i) {
-        const int buffer = (i - from) & 1, first = at * kQueries;
+    if (from < to) load(lds[0][0], lds[0][1], stats[0][0]);
+    const auto step = [&](bool more, const char* __restrict__ queries, const char* __restrict__ douts,
+                          const float* __restrict__ statistics, char* __restrict__ next_queries,
+                          char* __restrict__ next_douts, float* __restrict__ next_statistics) __attribute__((always_inline)) {
+        const int first = at * kQueries;
         if (++at == t1) at = t0;
-        arrived();
-        __syncthreads();
-        if (i + 1 < to) load(buffer ^ 1);
-        if (first >= wave_hi || first + kQueries <= wave_lo) continue;
-        const char *queries = lds[buffer][0], *douts = lds[buffer][1];
-        Acc s = {}, dp = {};
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) s = mma(L::row(queries, lane & 31, i, half), k[i], s);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) dp = mma(L::row(douts, lane & 31, i, half), v[i], dp);
+        if (more) load(next_queries, next_douts, next_statistics);
+        if (first >= wave_hi || first + kQueries <= wave_lo) return;
         const bool hidden = first < full_lo || first + kQueries > full_hi;
+        const int now = fresh(lane);
+        int lo = 0, hi = band.ql;
+        if (hidden) {
+            lo = live ? band.query_lo(key) : 0;
+            hi = live ? band.query_hi(key) : 0;
+        }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const auto lse = *reinterpret_cast<const vec<float, 4>*>(&stats[buffer][0][8 * g + 4 * half]);
-            const auto delta = *reinterpret_cast<const vec<float, 4>*>(&stats[buffer][1][8 * g + 4 * half]);
+        for (int u = 0; u < kQueries / 32; ++u) {
+            // The products start from the rows' statistics (lse in the scores' units), which
+            // so take no registers of their own.
+            Acc s, dp;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = 4 * g + j, query = first + 8 * g + 4 * half + j;
-                float p = exp2_fast(fmaf(s[i], a.scale2, -lse[j])), ds = p * (dp[i] - delta[j]);
+            for (int g = 0; g < 4; ++g) {
+                const int at = 32 * u + 8 * g + 4 * (now >> 5);
+                const auto lse = *reinterpret_cast<const vec<float, 4>*>(statistics + at);
+                const auto delta = *reinterpret_cast<const vec<float, 4>*>(statistics + kQueries + at);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[4 * g + j] = -lse[j];
+                    dp[4 * g + j] = -delta[j];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) s = mma(L::row(queries, 32 * u + (now & 31), i, now >> 5), k[i], s);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) dp = mma(L::row(douts, 32 * u + (now & 31), i, now >> 5), v[i], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float p = exp2_fast(s[i] * a.scale2), ds = p * dp[i];
                 if (hidden) {
+                    const int query = first + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
                     const bool seen = query >= lo && query < hi;
                     p = seen ? p : 0.f;
                     ds = seen ? ds : 0.f;
@@ -494,34 +574,41 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
                 s[i] = p;
                 dp[i] = ds;
             }
-        }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const Frag<T> p = as_fragment<T>(s, i), ds = as_fragment<T>(dp, i);
+            for (int i = 0; i < 2; ++i) {
+                const Frag<T> p = as_fragment<T>(s, i), ds = as_fragment<T>(dp, i);
 #pragma unroll
-            for (int d = 0; d < kBlocks; ++d) {
-                dv[d] = mma(L::column(douts, d, i, lane), p, dv[d]);
-                dk[d] = mma(L::column(queries, d, i, lane), ds, dk[d]);
+                for (int d = 0; d < kBlocks; ++d) {
+                    dv[d] = mma(L::column(douts, d, 2 * u + i, now), p, dv[d]);
+                    dk[d] = mma(L::column(queries, d, 2 * u + i, now), ds, dk[d]);
+                }
             }
         }
+    };
+    for (int i = from; i < to; ++i) {
+        const int now = (i - from) & 1, next = now ^ 1;
+        arrived();
+        __syncthreads();
+        step(i + 1 < to, lds[now][0], lds[now][1], stats[now][0], lds[next][0], lds[next][1], stats[next][0]);
     }
-    if (key >= a.keys) return;
+    const int end = fresh(lane), last_key = wave_first + (end & 31), last_half = end >> 5;
+    if (last_key >= a.keys) return;
     if (a.splits > 1) {
         // [which][split][pair][key][dim]
-        const int64_t at = (int64_t(split) * a.pairs + pair) * a.keys + key;
+        const int64_t at = (int64_t(split) * a.pairs + pair) * a.keys + last_key;
         const int64_t other = int64_t(a.splits) * a.pairs * a.keys;
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) {
-            store_column(a.part + at * a.dim, dk[d], 1.f, d, half, a.dim, a.dim % 4 == 0);
-            store_column(a.part + (other + at) * a.dim, dv[d], 1.f, d, half, a.dim, a.dim % 4 == 0);
+            store_column(a.part + at * a.dim, dk[d], 1.f, d, last_half, a.dim, a.dim % 4 == 0);
+            store_column(a.part + (other + at) * a.dim, dv[d], 1.f, d, last_half, a.dim, a.dim % 4 == 0);
         }
         return;
     }
-    T *to_k = head_row<T>(a.dk, b, key, kv), *to_v = head_row<T>(a.dv, b, key, kv);
+    T *to_k = head_row<T>(a.dk, b, last_key, kv), *to_v = head_row<T>(a.dv, b, last_key, kv);
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d) {
-        store_column(to_k, dk[d], a.scale, d, half, a.dim, a.wide_out);
-        store_column(to_v, dv[d], 1.f, d, half, a.dim, a.wide_out);
+        store_column(to_k, dk[d], a.scale, d, last_half, a.dim, a.wide_out);
+        store_column(to_v, dv[d], 1.f, d, last_half, a.dim, a.wide_out);
     }
 }
 
@@ -570,26 +657,23 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradien
     vload.start(a.v.token, a.dim, a.wide_in);
     const char* kbase = reinterpret_cast<const char*>(head_row<const T>(a.k, b, 0, kv));
     const char* vbase = reinterpret_cast<const char*>(head_row<const T>(a.v, b, 0, kv));
-    const auto load = [&](int t, int buffer) {
+    const auto load = [&](int t, char* to_keys, char* to_values) {
         const int64_t first = int64_t(t) * N;
-        kload.load(lds[buffer][0], kbase + first * kload.stride, band.kl - t * N, wave);
-        vload.load(lds[buffer][1], vbase + first * vload.stride, band.kl - t * N, wave);
+        kload.load(to_keys, kbase + first * kload.stride, band.kl - t * N, wave);
+        vload.load(to_values, vbase + first * vload.stride, band.kl - t * N, wave);
     };
 
     Acc dq[kBlocks] = {};
     if (t0 < t1) {
         for (int i = 0; i < 4; ++i) kload.clear(lds[i >> 1][i & 1]);
         if (kload.direct && a.dim < DP) __syncthreads();
-        load(t0, 0);
+        load(t0, lds[0][0], lds[0][1]);
     }
-    for (int t = t0; t < t1; ++t) {
-        const int buffer = (t - t0) & 1;
-        arrived();
-        __syncthreads();
-        if (t + 1 < t1) load(t + 1, buffer ^ 1);
+    const auto step = [&](int t, const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next_keys,
+                          char* __restrict__ next_values) __attribute__((always_inline)) {
+        if (t + 1 < t1) load(t + 1, next_keys, next_values);
         const int first = t * N;
-        if (first >= wave_hi || first + N <= wave_lo) continue;
-        const char *keys = lds[buffer][0], *values = lds[buffer][1];
+        if (first >= wave_hi || first + N <= wave_lo) return;
         const bool hidden = first < full_lo || first + N > full_hi;
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
@@ -601,7 +685,7 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradien
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = first + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
-                float ds = exp2_fast(fmaf(s[i], a.scale2, -lse)) * (dp[i] - delta);
+                float ds = exp2_fast((s[i] - lse) * a.scale2) * (dp[i] - delta);
                 if (hidden) ds = key >= lo && key < hi ? ds : 0.f;
                 s[i] = ds;
             }
@@ -612,6 +696,12 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradien
                 for (int d = 0; d < kBlocks; ++d) dq[d] = mma(L::column(keys, d, 2 * u + i, lane), ds, dq[d]);
             }
         }
+    };
+    for (int t = t0; t < t1; ++t) {
+        const int now = (t - t0) & 1, next = now ^ 1;
+        arrived();
+        __syncthreads();
+        step(t, lds[now][0], lds[now][1], lds[next][0], lds[next][1]);
     }
     if (row >= rows) return;
     if (a.splits > 1) {
@@ -749,7 +839,11 @@ void join(Device& d, const AttentionArgs& a, const float* part, const float* sta
     j.kv_heads = a.kv_heads;
     j.group = group;
     j.scale = scale;
-    hipLaunchKernelGGL((attention_join_k<T>), unsigned(a.pairs) * unsigned(rows), 64, 0, d.stream, j);
+    j.wide_part = a.dim % 4 == 0;
+    j.wide_out = a.wide_out;
+    j.teams = 1;
+    while (j.teams < 8 && 2 * j.teams < a.splits) j.teams *= 2;
+    hipLaunchKernelGGL((attention_join_k<T>), ceil_div(int64_t(a.pairs) * rows, 8 / j.teams), 256, 0, d.stream, j);
 }
 
 template <class F>

@@ -28,7 +28,7 @@ struct AttentionArgs {
     float scale, scale2;         // of the scores; the same times log2 e
     int wide_in, wide_out;       // 16-byte loads and stores
     float *part, *part_stats;    // [split][pair][row][dim], [split][pair][row][2]
-    float *row_lse, *row_delta;  // [batch][head][query]: lse times log2 e, dout.out
+    float *row_lse, *row_delta;  // [batch][head][query]: lse over scale, dout.out
 };
 
 // Lengths of a batch entry.
@@ -98,7 +98,11 @@ struct Tile {
     // Fragment of row `row`, inner indices the columns 16 s + 8 half + j.
     __device__ static Frag<T> row(const char* tile, int row, int s, int half) {
         const char* p = tile + row * kRowBytes;
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (sizeof(T) == 2 && (kChunks & (kChunks - 1)) == 0) {
+            // (the same place, by one exclusive or a fragment)
+            const int at = (row * kRowBytes + ((half ^ turn(row)) << 4)) ^ (s << 5);
+            return *reinterpret_cast<const Frag<T>*>(tile + at);
+        } else if constexpr (sizeof(T) == 2) {
             return *reinterpret_cast<const Frag<T>*>(p + (((2 * s + half) ^ turn(row)) << 4));
         } else {
             const auto lo = *reinterpret_cast<const vec<T, 4>*>(p + (((4 * s + 2 * half) ^ turn(row)) << 4));
@@ -135,15 +139,25 @@ struct Tile {
     }
 };
 
+// A number that the compiler takes for a new one each time: what is derived from it
+// is computed where it is used, not kept in registers through a loop.
+__device__ inline int fresh(int i) {
+    asm volatile("" : "+v"(i));
+    return i;
+}
+
 // Brings ROWS rows of a tensor into a tile, 256 lanes.  Rows past `valid` repeat
 // the last valid one (the caller hides them): memory past the lengths is not read.
 template <class T, int DP, int ROWS>
 struct TileLoader {
     using L = Tile<T, DP>;
     static constexpr int kSlots = ROWS * L::kChunks, kSteps = (kSlots + 255) / 256;
-    uint32_t offset[kSteps];  // of a full tile
-    int chunks;               // that hold values
-    int64_t stride;           // bytes from row to row
+    // Where 256 slots are whole rows in eights, a lane's slots differ by whole rows:
+    // one lane's offset and a step that is the same in every lane.
+    static constexpr bool kRegular = 256 % (8 * L::kChunks) == 0;
+    uint32_t offset[kRegular ? 1 : kSteps];  // of a full tile
+    int chunks;                              // that hold values
+    int64_t stride;                          // bytes from row to row
     int dim;
     bool direct;
 
@@ -153,7 +167,7 @@ struct TileLoader {
         chunks = dim / L::kChunk;
         direct = wide;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
+        for (int i = 0; i < (kRegular ? 1 : kSteps); ++i) {
             const int slot = i * 256 + threadIdx.x, row = slot / L::kChunks;
             offset[i] = uint32_t(row * uint32_t(stride)) + (((slot % L::kChunks) ^ L::turn(row)) << 4);
         }
@@ -168,20 +182,27 @@ struct TileLoader {
     // wave: this wave's number, the same in every lane.  The loads have arrived
     // after arrived() and a barrier.
     __device__ void load(char* tile, const char* base, int valid, int wave) const {
-        if (direct) {
+        const auto bring = [&](int i, const char* from) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                             (__attribute__((address_space(3))) void*)(tile + (i * 256 + wave * 64) * 16),
+                                             16, 0, 0);
+        };
+        if (direct && valid >= ROWS && chunks == L::kChunks) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                const int slot = i * 256 + threadIdx.x, row = slot / L::kChunks;
-                if (i * 256 + wave * 64 >= kSlots) break;
-                uint32_t at = offset[i];
-                if (row >= valid) at -= uint32_t(row - valid + 1) * uint32_t(stride);
-                if (chunks == L::kChunks || ((slot % L::kChunks) ^ L::turn(row)) < chunks)
-                    __builtin_amdgcn_global_load_lds(
-                        (const __attribute__((address_space(1))) void*)(base + at),
-                        (__attribute__((address_space(3))) void*)(tile + (i * 256 + wave * 64) * 16), 16, 0, 0);
+                if (kSlots % 256 && i * 256 + wave * 64 >= kSlots) break;
+                if constexpr (kRegular) bring(i, base + i * (256 / L::kChunks) * stride + offset[0]);
+                else bring(i, base + offset[i]);
+            }
+        } else if (direct) {
+            const int lane = fresh(threadIdx.x);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int slot = i * 256 + lane, row = slot / L::kChunks, chunk = (slot % L::kChunks) ^ L::turn(row);
+                if (slot < kSlots && chunk < chunks) bring(i, base + int64_t(min(row, valid - 1)) * stride + chunk * 16);
             }
         } else {
-            for (int slot = threadIdx.x; slot < kSlots; slot += 256) {
+            for (int slot = fresh(threadIdx.x); slot < kSlots; slot += 256) {
                 const int row = slot / L::kChunks, column = ((slot % L::kChunks) ^ L::turn(row)) * L::kChunk;
                 const T* p = reinterpret_cast<const T*>(base + int64_t(min(row, valid - 1)) * stride);
                 vec<T, L::kChunk> v;
