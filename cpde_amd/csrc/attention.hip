@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
     vload.start(a.v.token, a.dim, a.wide_in);
     const char* kbase = reinterpret_cast<const char*>(head_row<const T>(a.k, b, 0, kv));
     const char* vbase = reinterpret_cast<const char*>(head_row<const T>(a.v, b, 0, kv));
-    const auto load = [&](int t, char* to_keys, char* to_values) {
+    const auto load = [&](int t, char* to_keys, char* to_values) __attribute__((always_inline)) {
         const int64_t first = int64_t(t) * N;
         kload.load(to_keys, kbase + first * kload.stride, band.kl - t * N, wave);
         vload.load(to_values, vbase + first * vload.stride, band.kl - t * N, wave);
@@ -167,12 +167,13 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
             sum == 0 ? -INFINITY : reference * kLn2 + logf(sum);
 }
 
-// ---- few query rows: a vector kernel -----------------------------------------------------
-// Up to eight query rows of a key head read each key and value once, as they come
+// ---- one or two query rows: a vector kernel -------------------------------------------------
+// One or two query rows of a key head read each key and value once, as they come
 // from memory: LANES lanes hold a key's columns, eight each, and every row's query.
 // Scores are summed over the lanes; each group of lanes keeps its own maximum and
 // sum, joined at the end over the groups, the waves and (through memory, in
-// attention_join_k) the splits.  Bound: HBM.
+// attention_join_k) the splits.  Bound: HBM, and for short lists the latency of a
+// launch and of a few rounds of loads, of which 16 waves need fewest.
 template <int LANES>
 __device__ inline float sum_lanes(float x) {
     // by cross-lane moves within rows of 16: neighbours, pairs, then mirror images
@@ -203,10 +204,11 @@ __device__ inline void load8(float* v, const T* p, int left, bool wide) {
     }
 }
 
-template <class T, int LANES, int R>
-__global__ __launch_bounds__(256) void attention_step_k(AttentionArgs a) {
-    constexpr int kGroupsOfWave = 64 / LANES, kAtOnce = 4 * kGroupsOfWave, kDeep = 4;
-    __shared__ float shared[4][R][LANES * 8 + 2];
+constexpr int kStepDeep = 4;  // keys a group of lanes has under way
+template <class T, int LANES, int R, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attention_step_k(AttentionArgs a) {
+    constexpr int kGroupsOfWave = 64 / LANES, kAtOnce = WAVES * kGroupsOfWave, kDeep = kStepDeep;
+    __shared__ float shared[WAVES][R][LANES * 8 + 2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in = lane % LANES, group = lane / LANES;
     const int pair = blockIdx.x % a.pairs, split = blockIdx.x / a.pairs;
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
@@ -299,13 +301,13 @@ __global__ __launch_bounds__(256) void attention_step_k(AttentionArgs a) {
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < R * LANES * 8; i += 256) {
+    for (int i = threadIdx.x; i < R * LANES * 8; i += 64 * WAVES) {
         const int r = i / (LANES * 8), d = i % (LANES * 8);
         if (r >= rows || d >= a.dim) continue;
         float next = -INFINITY, total = 0, value = 0;
-        for (int w = 0; w < 4; ++w) next = fmaxf(next, shared[w][r][LANES * 8]);
+        for (int w = 0; w < WAVES; ++w) next = fmaxf(next, shared[w][r][LANES * 8]);
         const float base = next == -INFINITY ? 0.f : next;
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float by = exp2_fast(shared[w][r][LANES * 8] - base);
             total += shared[w][r][LANES * 8 + 1] * by;
             value += shared[w][r][d] * by;
@@ -322,6 +324,127 @@ __global__ __launch_bounds__(256) void attention_step_k(AttentionArgs a) {
             head_row<T>(a.out, b, query, head)[d] = T(total == 0 ? 0.f : value / total);
             if (a.lse && d == 0)
                 a.lse[(int64_t(b) * a.kv_heads * a.group + head) * a.queries + query] =
+                    total == 0 ? -INFINITY : next * kLn2 + logf(total);
+        }
+    }
+}
+
+// ---- up to 32 query rows: matrix tiles on waves' own keys -----------------------------------
+// All query rows of a key head are one matrix tile's columns, so every wave of a
+// split holds them all and the waves share out the KEYS: each brings tiles of 32 to
+// its own part of LDS and computes on them in turn, with no barrier until their
+// outputs are joined; eight waves a CU keep its share of memory busy.  Bound: HBM.
+template <class T, int DP>
+constexpr int kRowWaves = DP * sizeof(T) <= 256 ? 4 : 2;
+template <class T, int DP>
+__global__ __launch_bounds__((64 * kRowWaves<T, DP>), 2) void attention_rows_k(AttentionArgs a) {
+    constexpr int kWaves = kRowWaves<T, DP>, kBlocks = DP / 32, kSteps = DP / 16;
+    constexpr int kHalf = 32 * DP * int(sizeof(T));  // bytes of a tile of keys
+    constexpr int kPitch = DP + 4;                   // floats of a row of a wave's output in LDS
+    using L = Tile<T, DP>;
+    __shared__ __align__(16) char lds[kWaves][2 * kHalf > 32 * kPitch * 4 ? 2 * kHalf : 32 * kPitch * 4];
+    __shared__ float joined[kWaves][2][32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int pair = blockIdx.x % a.pairs, split = blockIdx.x / a.pairs;
+    const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
+    const Band band(a, b);
+    const int rows = a.queries * a.group, row = lane & 31;
+    const int query = row / a.group, head = kv * a.group + row % a.group;
+    const bool live = row < rows && query < band.ql;
+    const int lo = live ? band.key_lo(query) : 0, hi = live ? band.key_hi(query) : 0;
+    // keys that any row, and that all rows, see (the rows that count are the first)
+    const int last = min(a.queries, band.ql) - 1;
+    const int from = last < 0 ? 0 : max(band.key_lo(0), int(min(int64_t(split) * a.span, int64_t(band.kl))));
+    const int to = last < 0 ? 0 : int(min(int64_t(band.key_hi(last)), int64_t(split + 1) * a.span));
+    const int full_lo = last < 0 ? 0 : band.key_lo(last), full_hi = last < 0 ? 0 : band.key_hi(0);
+    const int t0 = from / 32, t1 = from < to ? (to + 31) / 32 : t0;
+
+    Frag<T> q[kSteps];
+    load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
+    WaveLoader<T, DP, 32> kload, vload;
+    kload.start(a.k.token, a.dim, a.wide_in, lane);
+    vload.start(a.v.token, a.dim, a.wide_in, lane);
+    const char* kbase = reinterpret_cast<const char*>(head_row<const T>(a.k, b, 0, kv));
+    const char* vbase = reinterpret_cast<const char*>(head_row<const T>(a.v, b, 0, kv));
+    char* tile = lds[wave];
+    const char* values = tile + kHalf;
+    Acc out[kBlocks] = {};
+    float reference = -INFINITY, sum = 0;
+    for (int t = t0 + wave; t < t1; t += kWaves) {
+        kload.load(tile, kbase + int64_t(t) * 32 * kload.stride, band.kl - t * 32, lane);
+        vload.load(tile + kHalf, vbase + int64_t(t) * 32 * vload.stride, band.kl - t * 32, lane);
+        arrived();
+        Acc s = {};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) s = mma(L::row(tile, lane & 31, i, half), q[i], s);
+        const int first = t * 32;
+        if (first < max(full_lo, from) || first + 32 > min(full_hi, to)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = first + 8 * (i >> 2) + 4 * half + (i & 3);
+                s[i] = key >= max(lo, from) && key < min(hi, to) ? s[i] : -INFINITY;
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top = halves_max(top) * a.scale2;
+        const bool grown = top > reference + 8.f;
+        if (__any(grown)) {
+            const float next = grown ? top : reference, by = grown ? exp2_fast(reference - next) : 1.f;
+            reference = next;
+            sum *= by;
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) out[d] *= by;
+        }
+        const float base = reference == -INFINITY ? 0.f : reference;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = exp2_fast(fmaf(s[i], a.scale2, -base));
+            sum += s[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const Frag<T> p = as_fragment<T>(s, i);
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) out[d] = mma(L::column(values, d, i, lane), p, out[d]);
+        }
+    }
+    sum = halves_sum(sum);
+    // the waves' outputs side by side
+    float* own = reinterpret_cast<float*>(tile);
+    if (half == 0) {
+        joined[wave][0][row] = reference;
+        joined[wave][1][row] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) store_column(own + row * kPitch, out[d], 1.f, d, half, DP, true);
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * DP; i += 64 * kWaves) {
+        const int r = i / DP, d = i % DP;
+        if (d >= a.dim) continue;
+        float next = -INFINITY, total = 0, value = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) next = fmaxf(next, joined[w][0][r]);
+        const float base = next == -INFINITY ? 0.f : next;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float by = exp2_fast(joined[w][0][r] - base);
+            total += joined[w][1][r] * by;
+            value += reinterpret_cast<const float*>(lds[w])[r * kPitch + d] * by;
+        }
+        const int q = r / a.group, h = kv * a.group + r % a.group;
+        if (a.splits > 1) {
+            const int64_t at = (int64_t(split) * a.pairs + pair) * rows + r;
+            a.part[at * a.dim + d] = value;
+            if (d == 0) {
+                a.part_stats[2 * at] = next;
+                a.part_stats[2 * at + 1] = total;
+            }
+        } else {
+            head_row<T>(a.out, b, q, h)[d] = T(total == 0 ? 0.f : value / total);
+            if (a.lse && d == 0)
+                a.lse[(int64_t(b) * a.kv_heads * a.group + h) * a.queries + q] =
                     total == 0 ? -INFINITY : next * kLn2 + logf(total);
         }
     }
@@ -499,7 +622,7 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
     int64_t at_s = (int64_t(b) * a.kv_heads * a.group + first_head) * a.queries + int64_t(t) * kQueries;
     const int64_t back_q = a.q.head * int64_t(sizeof(T)) - int64_t(per_head) * kQueries * qload.stride;
     const int64_t back_o = a.dout.head * int64_t(sizeof(T)) - int64_t(per_head) * kQueries * oload.stride;
-    const auto load = [&](char* to_queries, char* to_douts, float* to_stats) {
+    const auto load = [&](char* to_queries, char* to_douts, float* to_stats) __attribute__((always_inline)) {
         const int valid = band.ql - t * kQueries;
         qload.load(to_queries, at_q, valid, wave);
         oload.load(to_douts, at_o, valid, wave);
@@ -657,7 +780,7 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradien
     vload.start(a.v.token, a.dim, a.wide_in);
     const char* kbase = reinterpret_cast<const char*>(head_row<const T>(a.k, b, 0, kv));
     const char* vbase = reinterpret_cast<const char*>(head_row<const T>(a.v, b, 0, kv));
-    const auto load = [&](int t, char* to_keys, char* to_values) {
+    const auto load = [&](int t, char* to_keys, char* to_values) __attribute__((always_inline)) {
         const int64_t first = int64_t(t) * N;
         kload.load(to_keys, kbase + first * kload.stride, band.kl - t * N, wave);
         vload.load(to_values, vbase + first * vload.stride, band.kl - t * N, wave);
@@ -723,14 +846,15 @@ int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 // the long axis and joined where whole rows would leave the device short of
 // workgroups.
 struct Cut {
-    bool step = false;   // the forward runs on the vector kernel
+    bool step = false, brief = false;  // the forward runs on the vector kernel, of 16 waves
+    bool few = false;                  // on the kernel of up to 32 rows
     int rows = 0, row_tiles = 0, key_tiles = 0;
     int span = 0, forward = 1, query = 1, key = 1;  // splits
     size_t stats = 0, part = 0, part_stats = 0, floats = 0;
 };
 
 // Query rows of a key head up to which the vector kernel serves.
-constexpr int kStepRows = 8;
+constexpr int kStepRows = 2;
 
 int step_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : 16; }
 
@@ -746,12 +870,24 @@ Cut cut(const Attention& p) {
         // two workgroups a CU, and at least four tiles a split
         return int(std::clamp<int64_t>(blocks ? 2 * cus / blocks : 1, 1, std::max<int64_t>(steps / 4, 1)));
     };
-    c.step = c.rows <= kStepRows;
+    // The vector kernel takes one or two rows of floats, or of a list short enough for
+    // one workgroup's few rounds; matrix tiles the others (us, vector and tiles; 8 x 8192
+    // keys of 4 heads: f32, 128 wide, 1 row 61 and 75, 4 rows 75 and 77; bf16, 1 row 50
+    // and 32, 2 rows 55 and 32; 729 keys of 4 heads: bf16, 128 wide, 1 row 8.6 and 11.2).
+    const int round = kStepDeep * 16 * (64 / step_lanes(s.head_dim));
+    const bool brief = s.key_tokens <= 2 * round;
+    c.step = c.rows <= kStepRows && (brief || s.dtype == CPDE_F32);
     if (c.step) {
-        // 16 workgroups a CU, in whole rounds of a workgroup's loads; a short list in one
-        const int round = 16 * (64 / step_lanes(s.head_dim));
-        const int64_t share = s.key_tokens <= 4 * round ? s.key_tokens : ceil_div(pairs * s.key_tokens, 16 * cus);
-        c.span = std::max(ceil_div(std::max<int64_t>(share, 1), round) * round, round);
+        // 16 workgroups of four waves a CU, in whole rounds of a workgroup's loads; a
+        // short list in one of 16 waves
+        const int64_t share = brief ? s.key_tokens : ceil_div(pairs * s.key_tokens, 16 * cus);
+        c.brief = brief;
+        c.span = std::max(ceil_div(std::max<int64_t>(share, 1), round / 4) * (round / 4), round / 4);
+        c.forward = std::max(ceil_div(s.key_tokens, c.span), 1);
+    } else if ((c.few = c.rows <= kWaveRows)) {
+        const int round = 32 * (s.head_dim * type_bytes(s.dtype) <= 256 ? 4 : 2);
+        const int64_t share = std::max<int64_t>(ceil_div(pairs * s.key_tokens, 8 * cus), 4 * round);
+        c.span = ceil_div(share, round) * round;
         c.forward = std::max(ceil_div(s.key_tokens, c.span), 1);
     } else {
         c.forward = splits(pairs * c.row_tiles, ceil_div(s.key_tokens, keys_tile));
@@ -855,16 +991,20 @@ void with_width(int dim, F body) {
 }
 
 template <class T>
-void step(Device& d, const AttentionArgs& a, int rows) {
+void step(Device& d, const AttentionArgs& a, int rows, bool brief) {
     const unsigned blocks = unsigned(a.pairs) * unsigned(a.splits);
-    const auto launch = [&](auto lanes, auto most) {
-        hipLaunchKernelGGL((attention_step_k<T, decltype(lanes)::value, decltype(most)::value>), blocks, 256, 0, d.stream, a);
+    const auto launch = [&](auto lanes, auto most, auto waves) {
+        constexpr int kWaves = decltype(waves)::value;
+        hipLaunchKernelGGL((attention_step_k<T, decltype(lanes)::value, decltype(most)::value, kWaves>), blocks,
+                           64 * kWaves, 0, d.stream, a);
+    };
+    const auto with_waves = [&](auto lanes, auto most) {
+        if (brief) launch(lanes, most, std::integral_constant<int, 16>{});
+        else if constexpr (sizeof(T) == 4) launch(lanes, most, std::integral_constant<int, 4>{});
     };
     const auto with_rows = [&](auto lanes) {
-        if (rows == 1) launch(lanes, std::integral_constant<int, 1>{});
-        else if (rows == 2) launch(lanes, std::integral_constant<int, 2>{});
-        else if (rows <= 4) launch(lanes, std::integral_constant<int, 4>{});
-        else launch(lanes, std::integral_constant<int, 8>{});
+        if (rows == 1) with_waves(lanes, std::integral_constant<int, 1>{});
+        else with_waves(lanes, std::integral_constant<int, 2>{});
     };
     const int lanes = step_lanes(a.dim);
     if (lanes == 4) with_rows(std::integral_constant<int, 4>{});
@@ -950,9 +1090,15 @@ int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const
         TraceScope trace(d, kTraceAttention, 4.0 * s.batch * s.heads * double(s.query_tokens) * s.key_tokens * s.head_dim);
         with_type(s.dtype, [&](auto element) {
             using T = decltype(element);
-            if (c.step) step<T>(d, a, c.rows);
+            if (c.step) step<T>(d, a, c.rows, c.brief);
             else
                 with_width(a.dim, [&](auto width) {
+                    if (c.few) {
+                        constexpr int DP = decltype(width)::value;
+                        hipLaunchKernelGGL((attention_rows_k<T, DP>), unsigned(a.pairs) * a.splits, (64 * kRowWaves<T, DP>),
+                                           0, d.stream, a);
+                        return;
+                    }
                     hipLaunchKernelGGL((attention_forward_k<T, decltype(width)::value>),
                                        unsigned(a.pairs) * a.tiles * a.splits, 256, 0, d.stream, a);
                 });

@@ -181,7 +181,7 @@ struct TileLoader {
     }
     // wave: this wave's number, the same in every lane.  The loads have arrived
     // after arrived() and a barrier.
-    __device__ void load(char* tile, const char* base, int valid, int wave) const {
+    __device__ __attribute__((always_inline)) void load(char* tile, const char* base, int valid, int wave) const {
         const auto bring = [&](int i, const char* from) {
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                              (__attribute__((address_space(3))) void*)(tile + (i * 256 + wave * 64) * 16),
@@ -213,6 +213,57 @@ struct TileLoader {
         }
     }
 };
+// The same for one wave and a tile of its own: 64 lanes, ROWS rows.
+template <class T, int DP, int ROWS>
+struct WaveLoader {
+    using L = Tile<T, DP>;
+    static constexpr int kSteps = ROWS * L::kChunks / 64;
+    uint32_t offset[kSteps];
+    int chunks, dim;
+    int64_t stride;
+    bool direct;
+
+    __device__ void start(int64_t token, int dim_, bool wide, int lane) {
+        stride = token * int64_t(sizeof(T));
+        dim = dim_;
+        chunks = dim / L::kChunk;
+        direct = wide;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int slot = i * 64 + lane, row = slot / L::kChunks;
+            offset[i] = uint32_t(row * uint32_t(stride)) + (((slot % L::kChunks) ^ L::turn(row)) << 4);
+        }
+    }
+    // The loads have arrived after arrived().
+    __device__ __attribute__((always_inline)) void load(char* tile, const char* base, int valid, int lane) const {
+        const auto bring = [&](int i, const char* from) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                             (__attribute__((address_space(3))) void*)(tile + i * 1024), 16, 0, 0);
+        };
+        if (direct && valid >= ROWS && chunks == L::kChunks) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) bring(i, base + offset[i]);
+            return;
+        }
+        for (int i = 0; i < kSteps; ++i) {
+            const int slot = i * 64 + fresh(lane), row = slot / L::kChunks, chunk = (slot % L::kChunks) ^ L::turn(row);
+            const char* from = base + int64_t(min(row, valid - 1)) * stride;
+            if (direct && chunk < chunks) {
+                bring(i, from + chunk * 16);
+            } else {
+                // (columns past the head's width are zeros)
+                vec<T, L::kChunk> v;
+#pragma unroll
+                for (int j = 0; j < L::kChunk; ++j) {
+                    const int column = chunk * L::kChunk + j;
+                    v[j] = !direct && column < dim ? reinterpret_cast<const T*>(from)[column] : T(0.f);
+                }
+                *reinterpret_cast<vec<T, L::kChunk>*>(tile + slot * 16) = v;
+            }
+        }
+    }
+};
+
 __device__ inline void arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0), the other counters open
 
 // A row's fragments straight from memory: inner indices the columns 16 s + 8 half + j,

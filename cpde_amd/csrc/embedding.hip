@@ -6,7 +6,7 @@ namespace {
 
 constexpr int kSmallSort = 4096;     // tokens sorted by one workgroup in LDS
 constexpr int kDigitBits = 10;       // at most, of one pass over longer lists
-constexpr int kSortTokens = 4096;    // per workgroup of such a pass
+constexpr int kSortTokens = 1024;    // per workgroup of such a pass
 constexpr uint32_t kFan = 32;             // sorted tokens of a partial sum, and partial sums of one of the second level
 
 struct Embedding {
@@ -18,7 +18,7 @@ struct Embedding {
 
 // The gradient's workspace.
 struct Layout {
-    size_t keys[2], places[2], counts, sums1, sums2, bytes;
+    size_t keys[2], places[2], counts, totals, sums1, sums2, bytes;
 };
 int bit_width(uint32_t v) {
     int bits = 0;
@@ -42,6 +42,7 @@ Layout layout(const Embedding& e) {
         l.places[i] = take(4 * n);
     }
     l.counts = take(4 * ((n + kSortTokens - 1) / kSortTokens << digit_bits(e.rows)));
+    l.totals = take(4 << kDigitBits);
     l.sums1 = take(4 * (n / kFan) * size_t(e.width));
     l.sums2 = take(4 * (n / (kFan * kFan)) * size_t(e.width));
     l.bytes = std::max<size_t>(at, 256);
@@ -199,8 +200,9 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_k(const I* ids, int
     }
 }
 
-// Longer lists: per pass, digits counted per 4,096 tokens, the counts' running
-// sums, and the pairs moved.  `ids` is null after the first pass.
+// Longer lists: per pass, the digits of every 1,024 tokens counted, the counts'
+// running sums over those blocks (one wave a digit), and the pairs moved.  `ids` is
+// null after the first pass.
 template <class I>
 __global__ __launch_bounds__(256) void embedding_count_k(const I* ids, const uint32_t* keys, uint32_t tokens, int rows,
                                                          int shift, int bits, int* counts) {
@@ -208,73 +210,100 @@ __global__ __launch_bounds__(256) void embedding_count_k(const I* ids, const uin
     const int bins = 1 << bits;
     for (int b = threadIdx.x; b < bins; b += 256) counter[b] = 0;
     __syncthreads();
-    const uint32_t begin = blockIdx.x * uint32_t(kSortTokens);
-#pragma unroll 4
-    for (uint32_t j = 0; j < kSortTokens; j += 256) {
-        const uint32_t i = begin + j + threadIdx.x;
-        if (i < tokens) atomicAdd(&counter[((ids ? key_of(ids[i], rows) : keys[i]) >> shift) & (bins - 1)], 1);
-    }
+    const uint32_t begin = blockIdx.x * uint32_t(kSortTokens) + threadIdx.x;
+#pragma unroll
+    for (uint32_t j = 0; j < kSortTokens; j += 256)
+        if (begin + j < tokens)
+            atomicAdd(&counter[((ids ? key_of(ids[begin + j], rows) : keys[begin + j]) >> shift) & (bins - 1)], 1);
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += 256) counts[size_t(b) * gridDim.x + blockIdx.x] = counter[b];
 }
 
-__global__ __launch_bounds__(1024) void embedding_scan_k(int* counts, int64_t count) {
-    __shared__ int waves[16];
+// counts[digit][block] to sums over the blocks before, totals[digit] the whole row.
+__global__ __launch_bounds__(256) void embedding_scan_k(int* counts, int* totals, int bins, uint32_t blocks) {
+    const int lane = threadIdx.x & 63, bin = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (bin >= bins) return;
+    int* row = counts + size_t(bin) * blocks;
     int carry = 0;
-    for (int64_t i = 0; i < count; i += 4096) {
-        int v[4], sum = 0, before;
-        const int64_t at = i + threadIdx.x * 4;
-        for (int j = 0; j < 4; ++j) sum += v[j] = at + j < count ? counts[at + j] : 0;
-        const int total = scan_block(sum, before, waves);
-        before += carry;
-        for (int j = 0; j < 4; ++j) {
-            if (at + j < count) counts[at + j] = before;
-            before += v[j];
+    for (uint32_t first = 0; first < blocks; first += 64) {
+        const uint32_t i = first + lane;
+        const int value = i < blocks ? row[i] : 0;
+        int sum = value;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int other = __shfl_up(sum, d);
+            if (lane >= d) sum += other;
         }
-        carry += total;
+        if (i < blocks) row[i] = carry + sum - value;
+        carry += __shfl(sum, 63);
     }
+    if (lane == 0) totals[bin] = carry;
 }
 
 template <class I>
 __global__ __launch_bounds__(256) void embedding_move_k(const I* ids, const uint32_t* keys, const uint32_t* places,
                                                         uint32_t tokens, int rows, int shift, int bits,
-                                                        const int* counts, uint32_t* to_keys, uint32_t* to_places) {
+                                                        const int* counts, const int* totals, uint32_t* to_keys,
+                                                        uint32_t* to_places) {
     __shared__ int counter[4][1 << kDigitBits];
+    __shared__ int waves[4];
     const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     constexpr int kRounds = kSortTokens / 256;  // of a wave's quarter
+    constexpr int kBins = (1 << kDigitBits) / 256;
     for (int b = threadIdx.x; b < bins; b += 256)
         for (int w = 0; w < 4; ++w) counter[w][b] = 0;
     const uint32_t begin = blockIdx.x * uint32_t(kSortTokens) + wave * (kSortTokens / 4) + lane;
-    uint32_t k[kRounds];
+    uint32_t k[kRounds], p[kRounds];
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
         const uint32_t i = begin + r * 64;
         k[r] = i < tokens ? ids ? key_of(ids[i], rows) : keys[i] : 0;
+        p[r] = i < tokens && !ids ? places[i] : i;
     }
+    // a lane's digits are neighbours: kBins of them from kBins * thread
+    int total[kBins], before[kBins], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kBins; ++j) {
+        const int b = threadIdx.x * kBins + j;
+        total[j] = b < bins ? totals[b] : 0;
+        before[j] = b < bins ? counts[size_t(b) * gridDim.x + blockIdx.x] : 0;
+        sum += total[j];
+    }
+    int running = sum;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(running, d);
+        if (lane >= d) running += other;
+    }
+    if (lane == 63) waves[wave] = running;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kRounds; ++r)
         if (begin + r * 64 < tokens) atomicAdd(&counter[wave][(k[r] >> shift) & (bins - 1)], 1);
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 256) {
-        int at = counts[size_t(b) * gridDim.x + blockIdx.x];
-        for (int w = 0; w < 4; ++w) {
-            const int n = counter[w][b];
-            counter[w][b] = at;
-            at += n;
+    running -= sum;
+    for (int w = 0; w < wave; ++w) running += waves[w];
+#pragma unroll
+    for (int j = 0; j < kBins; ++j) {
+        const int b = threadIdx.x * kBins + j;
+        if (b < bins) {
+            int at = running + before[j];
+            for (int w = 0; w < 4; ++w) {
+                const int n = counter[w][b];
+                counter[w][b] = at;
+                at += n;
+            }
         }
+        running += total[j];
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-        const uint32_t i = begin + r * 64;
-        const bool live = i < tokens;
+        const bool live = begin + r * 64 < tokens;
         const uint32_t digit = (k[r] >> shift) & (bins - 1);
         const uint64_t peers = same_digit(digit, bits, live);
         if (live) {
             const int to = take_place(&counter[wave][digit], peers, lane);
             to_keys[to] = k[r];
-            to_places[to] = ids ? i : places[i];
+            to_places[to] = p[r];
         }
     }
 }
@@ -309,87 +338,125 @@ __device__ inline void load_sum(float* v, const float* p, int left, int width) {
     }
 }
 
-// Partial sums of the aligned runs of kFan tokens (level 1), or of kFan level-1
-// sums (level 2), that lie whole inside one row: a common token's row is then the
-// sum of few terms, whatever its count.  One group of lanes a run and slice.
+// Sixteen bytes of a row as they are in memory (or as many single values), added later.
 template <class T>
-__global__ __launch_bounds__(256) void embedding_partial_k(SumArgs a, uint32_t runs, int level) {
+__device__ inline vec<T, kLane<T>> load_raw(const T* p, int left, bool aligned) {
+    vec<T, kLane<T>> v = {};
+    if (aligned) {
+        if (left > 0) v = *reinterpret_cast<const vec<T, kLane<T>>*>(p);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLane<T>; ++j)
+            if (j < left) v[j] = p[j];
+    }
+    return v;
+}
+
+// Partial sums of the aligned runs of kFan tokens that lie whole inside one row: a
+// common token's row is then the sum of few terms, whatever its count.  A group of
+// lanes a run, so that a common token's runs spread over the device.
+template <class T>
+__global__ __launch_bounds__(256) void embedding_partial_k(SumArgs a, uint32_t runs) {
     constexpr int N = kLane<T>;
     const uint64_t run = (uint64_t(blockIdx.x) * 256 + threadIdx.x) / unsigned(a.lanes);
-    const int column = (blockIdx.y * a.lanes + threadIdx.x % a.lanes) * N, left = a.width - column;
+    const int column = (blockIdx.y * a.lanes + (threadIdx.x & (a.lanes - 1))) * N, left = a.width - column;
     if (run >= runs || left <= 0) return;
-    const uint32_t span = level == 1 ? kFan : kFan * kFan, first = uint32_t(run) * span;
-    const uint32_t row = a.keys[first];
-    if (row >= uint32_t(a.rows) || row != a.keys[first + span - 1]) return;
+    const uint32_t first = uint32_t(run) * kFan, row = a.keys[first];
+    if (row >= uint32_t(a.rows) || row != a.keys[first + kFan - 1]) return;
     float acc[N] = {};
-    for (uint32_t i = 0; i < kFan; i += 8) {
-        float v[8][N];
+#pragma unroll 1
+    for (uint32_t i = 0; i < kFan; i += 16) {
+        vec<T, N> v[16];
 #pragma unroll
-        for (uint32_t u = 0; u < 8; ++u) {
-            if (level == 1)
-                load_lane(v[u], static_cast<const T*>(a.dout) + int64_t(a.places[first + i + u]) * a.dout_stride + column,
-                          left, a.aligned);
-            else load_sum<N>(v[u], a.sums1 + (size_t(run) * kFan + i + u) * a.width + column, left, a.width);
-        }
+        for (uint32_t u = 0; u < 16; ++u)
+            v[u] = load_raw(static_cast<const T*>(a.dout) + int64_t(a.places[first + i + u]) * a.dout_stride + column, left,
+                            a.aligned);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < 16; ++u)
 #pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+            for (int j = 0; j < N; ++j) acc[j] += float(v[u][j]);
     }
-    float* to = (level == 1 ? a.sums1 : a.sums2) + size_t(run) * a.width + column;
+    float* to = a.sums1 + size_t(run) * a.width + column;
     for (int j = 0; j < N && j < left; ++j) to[j] = acc[j];
 }
 
-// First sorted token whose row is at least `row`, by a group of `lanes` lanes: each
-// step probes `lanes` places at once.  All lanes of the wave take part.
-__device__ inline uint32_t first_of(const uint32_t* keys, uint32_t tokens, uint32_t row, int lanes) {
+// The same of kFan such runs; a workgroup each.
+__global__ __launch_bounds__(256) void embedding_partial2_k(SumArgs a) {
+    const uint32_t first = blockIdx.x * kFan * kFan, row = a.keys[first];
+    if (row >= uint32_t(a.rows) || row != a.keys[first + kFan * kFan - 1]) return;
+    for (int column = threadIdx.x; column < a.width; column += 256) {
+        const float* from = a.sums1 + size_t(blockIdx.x) * kFan * a.width + column;
+        float sum = 0;
+#pragma unroll
+        for (uint32_t r = 0; r < kFan; ++r) sum += from[size_t(r) * a.width];
+        a.sums2[size_t(blockIdx.x) * a.width + column] = sum;
+    }
+}
+
+// First sorted tokens whose rows are at least `row` and `end`, by a group of `lanes`
+// lanes: each step probes `lanes` places of both searches at once.  All lanes of the
+// wave take part.
+__device__ inline void first_of(const uint32_t* keys, uint32_t tokens, uint32_t row, uint32_t end, int lanes,
+                                uint32_t& first, uint32_t& last) {
     const int lane = threadIdx.x & 63, in = lane & (lanes - 1);
     const uint64_t group = (lanes == 64 ? ~0ull : (1ull << lanes) - 1) << (lane - in);
-    uint32_t low = 0, high = tokens;  // the answer lies in [low, high]
-    while (__any(low < high)) {
-        const uint64_t left = high - low;
-        const auto probe = [&](int i) { return low + uint32_t(left * uint64_t(i + 1) / uint64_t(lanes + 1)); };
-        const bool less = low < high && keys[probe(in)] < row;
-        const int below = __popcll(__ballot(less) & group);  // probes 0..below-1 are less
-        if (low < high) {
-            const uint32_t to = below == lanes ? high : probe(below);
-            if (below) low = probe(below - 1) + 1;
-            high = to;
+    uint32_t low[2] = {0, 0}, high[2] = {tokens, tokens};  // the answers lie in [low, high]
+    const uint32_t want[2] = {row, end};
+    while (__any(low[0] < high[0] || low[1] < high[1])) {
+        uint32_t key[2];
+        const auto probe = [&](int s, int i) {
+            return low[s] + uint32_t((high[s] - low[s]) * uint64_t(i + 1) / uint64_t(lanes + 1));
+        };
+#pragma unroll
+        for (int s = 0; s < 2; ++s) key[s] = low[s] < high[s] ? keys[probe(s, in)] : 0;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const bool open = low[s] < high[s];
+            const int below = __popcll(__ballot(open && key[s] < want[s]) & group);  // probes 0..below-1 are less
+            if (open) {
+                const uint32_t to = below == lanes ? high[s] : probe(s, below);
+                if (below) low[s] = probe(s, below - 1) + 1;
+                high[s] = to;
+            }
         }
     }
-    return low;
+    first = low[0];
+    last = low[1];
 }
 
 // The table's gradient: a group of lanes takes `group_rows` rows and their sorted
-// tokens, eight loads in flight whatever rows they belong to, and writes each row
-// once, the sum of its tokens (or zeros).  Where a whole run of kFan tokens, or of
-// kFan such runs, belongs to one row, its partial sum stands for it: the order of
-// a sum depends on the tokens alone.  Bound: HBM.
+// tokens and writes each row once, the sum of its tokens (or zeros).  Tokens come
+// `lanes` at a time, a lane each, and their rows of dout in eights, the next eight
+// under way while one is added, whatever rows of the table they belong to.  Where a
+// whole run of kFan tokens, or of kFan such runs, belongs to one row, its partial
+// sum stands for it: the order of a sum depends on the tokens alone.  Bound: HBM.
 template <class T>
 __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
     constexpr int N = kLane<T>;
+    const int lane = threadIdx.x & 63, in = lane & (a.lanes - 1), begin_lane = lane - in;
+    const uint64_t mine = (a.lanes == 64 ? ~0ull : (1ull << a.lanes) - 1) << begin_lane;
     const uint64_t group = (uint64_t(blockIdx.x) * 256 + threadIdx.x) / unsigned(a.lanes);
-    const int column = (blockIdx.y * a.lanes + threadIdx.x % a.lanes) * N;
+    const int column = (blockIdx.y * a.lanes + in) * N, left = a.width - column;
     const uint64_t begin_row = std::min(group * uint64_t(a.group_rows), uint64_t(a.rows));
     const uint32_t end_row = uint32_t(std::min(begin_row + a.group_rows, uint64_t(a.rows)));
-    uint32_t at = first_of(a.keys, a.tokens, uint32_t(begin_row), a.lanes);
-    const uint32_t end = first_of(a.keys, a.tokens, end_row, a.lanes);
-    if (column >= a.width) return;
+    uint32_t at, end;
+    first_of(a.keys, a.tokens, uint32_t(begin_row), end_row, a.lanes, at, end);
     const T* base = static_cast<const T*>(a.dout) + column;
-    const int left = a.width - column;
     uint32_t row = uint32_t(begin_row);
     float acc[N] = {};
     const auto finish_before = [&](uint32_t next) {
         for (; row < next; ++row) {
             float* out = a.dtable + int64_t(row) * a.dtable_stride + column;
             if (a.aligned_out) {
+                if (left > 0)
 #pragma unroll
-                for (int j = 0; j < N; j += 4) {
-                    vec<float, 4>* p = reinterpret_cast<vec<float, 4>*>(out + j);
-                    vec<float, 4> v = {acc[j] * a.scale, acc[j + 1] * a.scale, acc[j + 2] * a.scale, acc[j + 3] * a.scale};
-                    if (a.accumulate) v += *p;
-                    *p = v;
-                }
+                    for (int j = 0; j < N; j += 4) {
+                        vec<float, 4>* p = reinterpret_cast<vec<float, 4>*>(out + j);
+                        vec<float, 4> v = {acc[j] * a.scale, acc[j + 1] * a.scale, acc[j + 2] * a.scale,
+                                           acc[j + 3] * a.scale};
+                        if (a.accumulate) v += *p;
+                        *p = v;
+                    }
             } else {
                 for (int j = 0; j < N && j < left; ++j) out[j] = (a.accumulate ? out[j] : 0.f) + acc[j] * a.scale;
             }
@@ -398,47 +465,75 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
         }
     };
     while (at < end) {
-        const uint32_t key = a.keys[at];
-        const auto whole = [&](uint32_t from, uint32_t span) {
-            return from % span == 0 && from + span <= end && a.keys[from + span - 1] == key;
-        };
-        if (whole(at, kFan)) {
-            const bool second = whole(at, kFan * kFan);
-            const uint32_t span = second ? kFan * kFan : kFan;
-            const float* sums = (second ? a.sums2 : a.sums1) + column;
-            finish_before(key);
-            int runs = 1;
-            while (runs < 8 && whole(at + runs * span, span)) ++runs;
-            float v[8][N];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) load_sum<N>(v[u], sums + size_t(at / span + (u < runs ? u : 0)) * a.width, left, a.width);
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (u < runs)
-#pragma unroll
-                    for (int j = 0; j < N; ++j) acc[j] += v[u][j];
-            at += runs * span;
-        } else {
-            // to the next place where a whole run may begin
-            const int count = int(std::min(std::min(end - at, kFan - at % kFan), 8u));
-            uint32_t key8[8];
-            float v[8][N];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const uint32_t i = at + (u < count ? u : 0);
-                key8[u] = a.keys[i];
-                load_lane(v[u], base + int64_t(a.places[i]) * a.dout_stride, left, a.aligned);
+        // the next tokens, a lane each, to the next place where a whole run may begin;
+        // and, where one begins here, how many follow one another
+        const uint32_t here = std::min(std::min(end - at, kFan - at % kFan), uint32_t(a.lanes));
+        const uint32_t i = at + std::min(uint32_t(in), here - 1);
+        const uint32_t my_key = a.keys[i], my_place = a.places[i];
+        uint32_t span = 0;
+        int runs = 0;
+        if (at % kFan == 0 && at + kFan <= end) {
+            const uint32_t key = __shfl(my_key, begin_lane);
+            const auto follow = [&](uint32_t s) {
+                const uint64_t last = uint64_t(at) + uint64_t(in + 1) * s;
+                const uint64_t no = ~__ballot(last <= end && a.keys[last <= end ? last - 1 : at] == key) & mine;
+                return no ? __ffsll(static_cast<unsigned long long>(no)) - 1 - begin_lane : a.lanes;
+            };
+            if (at % (kFan * kFan) == 0) {
+                span = kFan * kFan;
+                runs = follow(span);
             }
+            if (!runs) {
+                span = kFan;
+                runs = follow(span);
+            }
+            if (runs) finish_before(key);
+        }
+        if (runs) {
+            if (span == kFan)  // (up to where the second level may take over)
+                runs = std::min(runs, int((kFan * kFan - at % (kFan * kFan)) / kFan));
+            const float* sums = (span == kFan ? a.sums1 : a.sums2) + size_t(at / span) * a.width + column;
+            for (int r = 0; r < runs; r += 4) {
+                float v[4][N];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                if (u < count) {
-                    finish_before(key8[u]);
+                for (int u = 0; u < 4; ++u) load_sum<N>(v[u], sums + size_t(std::min(r + u, runs - 1)) * a.width, left, a.width);
 #pragma unroll
-                    for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+                for (int u = 0; u < 4; ++u)
+                    if (r + u < runs)
+#pragma unroll
+                        for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+            }
+            at += runs * span;
+            continue;
+        }
+        constexpr int kBatch = 8;
+        vec<T, N> v[2][kBatch];
+        const auto load = [&](vec<T, N>* to, uint32_t from) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const uint32_t place = __shfl(my_place, begin_lane + int(std::min(from + u, here - 1)));
+                to[u] = load_raw(base + int64_t(place) * a.dout_stride, left, a.aligned);
+            }
+        };
+        const auto add = [&](const vec<T, N>* from, uint32_t first) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const uint32_t key = __shfl(my_key, begin_lane + int(std::min(first + u, here - 1)));
+                if (first + u < here) {
+                    finish_before(key);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += float(from[u][j]);
                 }
             }
-            at += count;
+        };
+        load(v[0], 0);
+        for (uint32_t n = 0; n < here; n += 2 * kBatch) {
+            if (n + kBatch < here) load(v[1], n + kBatch);
+            add(v[0], n);
+            if (n + 2 * kBatch < here) load(v[0], n + 2 * kBatch);
+            if (n + kBatch < here) add(v[1], n + kBatch);
         }
+        at += here;
     }
     finish_before(end_row);
 }
@@ -457,15 +552,15 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
     } else {
         const int digit = digit_bits(e.rows), passes = sort_passes(e.rows);
         const unsigned blocks = (tokens + kSortTokens - 1) / kSortTokens;
-        int* counts = reinterpret_cast<int*>(e.work + l.counts);
+        int *counts = reinterpret_cast<int*>(e.work + l.counts), *totals = reinterpret_cast<int*>(e.work + l.totals);
         for (int p = 0; p < passes; ++p) {
             const I* source = p ? nullptr : ids;
             hipLaunchKernelGGL((embedding_count_k<I>), blocks, 256, 0, d.stream, source, part(l.keys[now]), tokens, e.rows,
                                p * digit, digit, counts);
-            hipLaunchKernelGGL(embedding_scan_k, 1, 1024, 0, d.stream, counts, int64_t(blocks) << digit);
+            hipLaunchKernelGGL(embedding_scan_k, (1u << digit) / 4 + 1, 256, 0, d.stream, counts, totals, 1 << digit, blocks);
             hipLaunchKernelGGL((embedding_move_k<I>), blocks, 256, 0, d.stream, source, part(l.keys[now]),
-                               part(l.places[now]), tokens, e.rows, p * digit, digit, counts, part(l.keys[1 - now]),
-                               part(l.places[1 - now]));
+                               part(l.places[now]), tokens, e.rows, p * digit, digit, counts, totals,
+                               part(l.keys[1 - now]), part(l.places[1 - now]));
             now = 1 - now;
         }
     }
@@ -479,15 +574,15 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
     a.lanes = 1;
     while (a.lanes < per_row && a.lanes < 64) a.lanes <<= 1;
     const unsigned slices = unsigned((per_row + a.lanes - 1) / a.lanes);
-    for (int level = 1; level <= 2; ++level) {
-        const uint32_t runs = tokens / (level == 1 ? kFan : kFan * kFan);
-        if (runs)
-            hipLaunchKernelGGL((embedding_partial_k<T>), dim3(unsigned((uint64_t(runs) * a.lanes + 255) / 256), slices),
-                               256, 0, d.stream, a, runs, level);
-    }
-    // rows a group: 16 where there are many (a search serves them all), fewer where
-    // that would leave the device short of waves
-    const int64_t groups_wanted = int64_t(d.compute_units) * 16 * (64 / a.lanes) / slices;
+    const uint32_t runs = tokens / kFan;
+    if (runs)
+        hipLaunchKernelGGL((embedding_partial_k<T>), dim3(unsigned((uint64_t(runs) * a.lanes + 255) / 256), slices), 256, 0,
+                           d.stream, a, runs);
+    if (runs / kFan) hipLaunchKernelGGL(embedding_partial2_k, runs / kFan, 256, 0, d.stream, a);
+    // Rows a group: enough that a search serves several, few enough that common tokens
+    // do not hold a wave back (131,072 uneven tokens of 65,536 rows x 512: 4 rows 126
+    // us, 8 rows 133, 16 rows 143).
+    const int64_t groups_wanted = int64_t(d.compute_units) * 64 * (64 / a.lanes) / slices;
     a.group_rows = int(std::clamp<int64_t>(e.rows / std::max<int64_t>(groups_wanted, 1), 1, 16));
     const uint64_t groups = (uint64_t(e.rows) + a.group_rows - 1) / a.group_rows;
     hipLaunchKernelGGL((embedding_sum_k<T>), dim3(unsigned((groups * unsigned(a.lanes) + 255) / 256), slices), 256, 0, d.stream, a);
