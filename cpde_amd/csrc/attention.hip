@@ -1,5 +1,6 @@
 // Attention over sets and sequences, and its gradient.
 #include <cmath>
+#include <initializer_list>
 
 #include "attention.hpp"
 
@@ -46,8 +47,6 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
     const bool live = row < rows && query < band.ql;
     const int lo = live ? band.key_lo(query) : 0, hi = live ? band.key_hi(query) : 0;
 
-    Frag<T> q[kSteps];
-    load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
 
     // the keys that the workgroup's rows, and this wave's, see at all, and those that
     // all of the wave's rows see
@@ -84,6 +83,8 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
         if (kload.direct && a.dim < DP) __syncthreads();
         load(t0, lds[0][0], lds[0][1]);
     }
+    Frag<T> q[kSteps];
+    load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
     // (the tile read and the tiles written do not overlap, which the compiler has to
     // know so as not to wait for the loads under way before it reads)
     const auto step = [&](int t, const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next_keys,
@@ -451,14 +452,18 @@ __global__ __launch_bounds__((64 * kRowWaves<T, DP>), 2) void attention_rows_k(A
 }
 
 // ---- joining splits -----------------------------------------------------------------------
-struct JoinArgs {
-    const float *part, *stats;  // stats null: plain sums
+struct Join {
+    const float* part;
     HeadView out;
-    float* lse;
-    int splits, pairs, rows, dim, kv_heads, group;
+    int splits, rows, group, blocks;
     int teams;  // of 32 lanes a row, each with every teams-th split (a power of two)
-    int wide_part, wide_out;
     float scale;
+};
+struct JoinArgs {
+    Join joins[3];
+    const float* stats;  // null: plain sums
+    float* lse;
+    int pairs, dim, kv_heads, wide_part, wide_out;
 };
 
 // 32 lanes hold a row, four columns each; `teams` of them share its splits, with a
@@ -466,15 +471,18 @@ struct JoinArgs {
 // key wrote no output.  Bound: HBM (the parts read once).
 template <class T>
 __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
+    int block = blockIdx.x, which = 0;
+    while (block >= a.joins[which].blocks) block -= a.joins[which++].blocks;
+    const Join c = a.joins[which];
     __shared__ float shared[8][32][6];
-    const int lane = threadIdx.x & 31, team = threadIdx.x / 32, in = team & (a.teams - 1);
-    const int64_t count = int64_t(a.pairs) * a.rows;
-    const int64_t item = int64_t(blockIdx.x) * (8 / a.teams) + team / a.teams, at = min(item, count - 1);
+    const int lane = threadIdx.x & 31, team = threadIdx.x / 32, in = team & (c.teams - 1);
+    const int64_t count = int64_t(a.pairs) * c.rows;
+    const int64_t item = int64_t(block) * (8 / c.teams) + team / c.teams, at = min(item, count - 1);
     const int d = lane * 4;
     float top = -INFINITY, total = 0;
     vec<float, 4> value = {};
 #pragma unroll 4
-    for (int s = in; s < a.splits; s += a.teams) {
+    for (int s = in; s < c.splits; s += c.teams) {
         const int64_t from = s * count + at;
         float m = 0, l = 1;
         if (a.stats) {
@@ -483,7 +491,7 @@ __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
             l = both[1];
         }
         vec<float, 4> v = {};
-        const float* p = a.part + from * a.dim + d;
+        const float* p = c.part + from * a.dim + d;
         if (a.wide_part) {
             if (d < a.dim) v = *reinterpret_cast<const vec<float, 4>*>(p);
         } else {
@@ -509,7 +517,7 @@ __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
     shared[team][lane][5] = total;
     __syncthreads();
     if (in != 0 || item >= count) return;
-    for (int t = 1; t < a.teams; ++t) {
+    for (int t = 1; t < c.teams; ++t) {
         const float* other = shared[team + t][lane];
         if (a.stats) {
             const float next = fmaxf(top, other[4]), base = next == -INFINITY ? 0.f : next;
@@ -523,11 +531,11 @@ __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
             for (int j = 0; j < 4; ++j) value[j] += other[j];
         }
     }
-    const int pair = int(item / a.rows), row = int(item % a.rows);
+    const int pair = int(item / c.rows), row = int(item % c.rows);
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
-    const int token = row / a.group, head = kv * a.group + row % a.group;
-    const float by = a.stats ? (total == 0 ? 0.f : 1.f / total) : a.scale;
-    T* out = head_row<T>(a.out, b, token, head) + d;
+    const int token = row / c.group, head = kv * c.group + row % c.group;
+    const float by = a.stats ? (total == 0 ? 0.f : 1.f / total) : c.scale;
+    T* out = head_row<T>(c.out, b, token, head) + d;
     if (a.wide_out) {
         value *= by;
         if (d < a.dim) *reinterpret_cast<vec<T, 4>*>(out) = __builtin_convertvector(value, vec<T, 4>);
@@ -537,7 +545,7 @@ __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
             if (d + j < a.dim) out[j] = T(value[j] * by);
     }
     if (a.lse && lane == 0)
-        a.lse[(int64_t(b) * a.kv_heads * a.group + head) * (a.rows / a.group) + token] =
+        a.lse[(int64_t(b) * a.kv_heads * c.group + head) * (c.rows / c.group) + token] =
             total == 0 ? -INFINITY : top * kLn2 + logf(total);
 }
 
@@ -573,25 +581,27 @@ __global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a) {
 // its probabilities and its score gradients are, in place, the fragments that
 // multiply the transposed dout and queries into dv and dk.
 template <class T, int DP>
-__global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_k(AttentionArgs a) {
+struct KeyShared {
+    char tiles[2][2][kQueries * Tile<T, DP>::kRowBytes];
+    float stats[2][2][kQueries];
+};
+template <class T, int DP>
+__device__ __attribute__((always_inline)) inline void key_gradient(const AttentionArgs& a, int block, KeyShared<T, DP>& shared) {
     constexpr int kBlocks = DP / 32, kSteps = DP / 16;
     using L = Tile<T, DP>;
-    __shared__ __align__(16) char lds[2][2][kQueries * L::kRowBytes];
-    __shared__ __align__(16) float stats[2][2][kQueries];
+    auto& lds = shared.tiles;
+    auto& stats = shared.stats;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
+    const int pair = block % a.pairs, rest = block / a.pairs;
     // (a causal band's first keys are seen most; a second round of workgroups comes to
     // the CUs of the first in the same order, so it goes the other way)
-    const int split = rest / a.tiles, tile = split & 1 ? a.tiles - 1 - rest % a.tiles : rest % a.tiles;
+    const int split = rest / a.key_tiles, place = rest % a.key_tiles, tile = split & 1 ? a.key_tiles - 1 - place : place;
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
     const Band band(a, b);
     const int block_first = tile * kBlockRows, wave_first = block_first + wave * kWaveRows;
     const int key = wave_first + (lane & 31);
     const bool live = key < band.kl;
 
-    Frag<T> k[kSteps], v[kSteps];
-    load_fragments<T, DP>(k, head_row<const T>(a.k, b, key, kv), a.dim, half, live, a.wide_in);
-    load_fragments<T, DP>(v, head_row<const T>(a.v, b, key, kv), a.dim, half, live, a.wide_in);
 
     const auto last = [&](int j) { return min(j, band.kl - 1); };
     const bool any = block_first < band.kl, wave_any = wave_first < band.kl;
@@ -599,8 +609,8 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
     const int t1 = any ? (band.query_hi(last(block_first + kBlockRows - 1)) + kQueries - 1) / kQueries : 0;
     const int per_head = max(t1 - t0, 0);
     int from = 0, to = per_head * a.group;
-    if (a.splits > 1) {
-        const int share = (to + a.splits - 1) / a.splits;
+    if (a.key_splits > 1) {
+        const int share = (to + a.key_splits - 1) / a.key_splits;
         from = min(split * share, to);
         to = min(to, from + share);
     }
@@ -651,6 +661,9 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
     }
     int at = t;  // of the tile computed on
     if (from < to) load(lds[0][0], lds[0][1], stats[0][0]);
+    Frag<T> k[kSteps], v[kSteps];
+    load_fragments<T, DP>(k, head_row<const T>(a.k, b, key, kv), a.dim, half, live, a.wide_in);
+    load_fragments<T, DP>(v, head_row<const T>(a.v, b, key, kv), a.dim, half, live, a.wide_in);
     const auto step = [&](bool more, const char* __restrict__ queries, const char* __restrict__ douts,
                           const float* __restrict__ statistics, char* __restrict__ next_queries,
                           char* __restrict__ next_douts, float* __restrict__ next_statistics) __attribute__((always_inline)) {
@@ -716,14 +729,14 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
     }
     const int end = fresh(lane), last_key = wave_first + (end & 31), last_half = end >> 5;
     if (last_key >= a.keys) return;
-    if (a.splits > 1) {
+    if (a.key_splits > 1) {
         // [which][split][pair][key][dim]
         const int64_t at = (int64_t(split) * a.pairs + pair) * a.keys + last_key;
-        const int64_t other = int64_t(a.splits) * a.pairs * a.keys;
+        const int64_t other = int64_t(a.key_splits) * a.pairs * a.keys;
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) {
-            store_column(a.part + at * a.dim, dk[d], 1.f, d, last_half, a.dim, a.dim % 4 == 0);
-            store_column(a.part + (other + at) * a.dim, dv[d], 1.f, d, last_half, a.dim, a.dim % 4 == 0);
+            store_column(a.key_part + at * a.dim, dk[d], 1.f, d, last_half, a.dim, a.dim % 4 == 0);
+            store_column(a.key_part + (other + at) * a.dim, dv[d], 1.f, d, last_half, a.dim, a.dim % 4 == 0);
         }
         return;
     }
@@ -739,12 +752,16 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_key_gradient_
 // (A second pass over the scores, so that no two workgroups add to one place: two
 // products of nine, for sums in a fixed order and no float copy of dq.)
 template <class T, int DP>
-__global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradient_k(AttentionArgs a) {
+struct QueryShared {
+    char tiles[2][2][kKeys<T> * Tile<T, DP>::kRowBytes];
+};
+template <class T, int DP>
+__device__ __attribute__((always_inline)) inline void query_gradient(const AttentionArgs& a, int block, QueryShared<T, DP>& shared) {
     constexpr int N = kKeys<T>, kSub = N / 32, kBlocks = DP / 32, kSteps = DP / 16;
     using L = Tile<T, DP>;
-    __shared__ __align__(16) char lds[2][2][N * L::kRowBytes];
+    auto& lds = shared.tiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
+    const int pair = block % a.pairs, rest = block / a.pairs;
     const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
     const Band band(a, b);
@@ -754,11 +771,6 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradien
     const bool live = row < rows && query < band.ql;
     const int lo = live ? band.key_lo(query) : 0, hi = live ? band.key_hi(query) : 0;
 
-    Frag<T> q[kSteps], dout[kSteps];
-    load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
-    load_fragments<T, DP>(dout, head_row<const T>(a.dout, b, query, head), a.dim, half, live, a.wide_in);
-    const int64_t at_row = (int64_t(b) * a.kv_heads * a.group + head) * a.queries + query;
-    const float lse = live ? a.row_lse[at_row] : INFINITY, delta = live ? a.row_delta[at_row] : 0.f;
 
     const auto first_row = [&](int r) { return min(r / a.group, band.ql - 1); };
     const int block_first = tile * kBlockRows, wave_first = block_first + wave * kWaveRows;
@@ -792,6 +804,11 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradien
         if (kload.direct && a.dim < DP) __syncthreads();
         load(t0, lds[0][0], lds[0][1]);
     }
+    Frag<T> q[kSteps], dout[kSteps];
+    load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
+    load_fragments<T, DP>(dout, head_row<const T>(a.dout, b, query, head), a.dim, half, live, a.wide_in);
+    const int64_t at_row = (int64_t(b) * a.kv_heads * a.group + head) * a.queries + query;
+    const float lse = live ? a.row_lse[at_row] : INFINITY, delta = live ? a.row_delta[at_row] : 0.f;
     const auto step = [&](int t, const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next_keys,
                           char* __restrict__ next_values) __attribute__((always_inline)) {
         if (t + 1 < t1) load(t + 1, next_keys, next_values);
@@ -839,6 +856,18 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_query_gradien
     for (int d = 0; d < kBlocks; ++d) store_column(to, dq[d], a.scale, d, half, a.dim, a.wide_out);
 }
 
+// Both in one launch, the keys' workgroups first (four products to three): where
+// either would leave the device short of workgroups the other fills it.
+template <class T, int DP>
+__global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_gradient_k(AttentionArgs a) {
+    __shared__ __align__(16) union {
+        KeyShared<T, DP> key;
+        QueryShared<T, DP> query;
+    } shared;
+    if (int(blockIdx.x) < a.key_blocks) key_gradient<T, DP>(a, blockIdx.x, shared.key);
+    else query_gradient<T, DP>(a, blockIdx.x - a.key_blocks, shared.query);
+}
+
 // ---- host -----------------------------------------------------------------------------------
 int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
@@ -850,7 +879,7 @@ struct Cut {
     bool few = false;                  // on the kernel of up to 32 rows
     int rows = 0, row_tiles = 0, key_tiles = 0;
     int span = 0, forward = 1, query = 1, key = 1;  // splits
-    size_t stats = 0, part = 0, part_stats = 0, floats = 0;
+    size_t stats = 0, part = 0, part_stats = 0, key_part = 0, floats = 0;
 };
 
 // Query rows of a key head up to which the vector kernel serves.
@@ -901,14 +930,14 @@ Cut cut(const Attention& p) {
         c.query = splits(pairs * c.row_tiles, ceil_div(s.key_tokens, keys_tile));
         c.key = splits(pairs * c.key_tiles, group * ceil_div(s.query_tokens, kQueries));
         if (c.query > 1) part = std::max(part, size_t(c.query) * pairs * c.rows * s.head_dim);
-        if (c.key > 1) part = std::max(part, 2 * size_t(c.key) * pairs * s.key_tokens * s.head_dim);
+        if (c.key > 1) c.key_part = 2 * size_t(c.key) * pairs * s.key_tokens * s.head_dim;
         c.stats = 2 * size_t(s.batch) * s.heads * s.query_tokens;
     }
     const auto padded = [](size_t n) { return (n + 63) / 64 * 64; };
     c.stats = padded(c.stats);
     c.part = padded(part);
     c.part_stats = padded(part_stats);
-    c.floats = c.stats + c.part + c.part_stats;
+    c.floats = c.stats + c.part + c.part_stats + c.key_part;
     return c;
 }
 
@@ -957,29 +986,33 @@ AttentionArgs arguments(const Attention& p, const Cut& c, const int* query_lengt
     a.row_delta = p.work + c.stats / 2;
     a.part = p.work + c.stats;
     a.part_stats = a.part + c.part;
+    a.key_part = a.part_stats + c.part_stats;
     return a;
 }
 
+Join join_of(const float* part, const HeadView& out, int pairs, int splits, int rows, int group, float scale) {
+    Join j{part, out, splits, rows, group, 0, 1, scale};
+    while (j.teams < 8 && 2 * j.teams < splits) j.teams *= 2;
+    j.blocks = splits > 1 ? ceil_div(int64_t(pairs) * rows, 8 / j.teams) : 0;
+    return j;
+}
 template <class T>
-void join(Device& d, const AttentionArgs& a, const float* part, const float* stats, const HeadView& out, float* lse,
-          int rows, int group, float scale) {
+void join(Device& d, const AttentionArgs& a, std::initializer_list<Join> joins, const float* stats, float* lse) {
     JoinArgs j{};
-    j.part = part;
+    int n = 0, blocks = 0;
+    for (const Join& one : joins) {
+        j.joins[n++] = one;
+        blocks += one.blocks;
+    }
+    if (!blocks) return;
     j.stats = stats;
-    j.out = out;
     j.lse = lse;
-    j.splits = a.splits;
     j.pairs = a.pairs;
-    j.rows = rows;
     j.dim = a.dim;
     j.kv_heads = a.kv_heads;
-    j.group = group;
-    j.scale = scale;
     j.wide_part = a.dim % 4 == 0;
     j.wide_out = a.wide_out;
-    j.teams = 1;
-    while (j.teams < 8 && 2 * j.teams < a.splits) j.teams *= 2;
-    hipLaunchKernelGGL((attention_join_k<T>), ceil_div(int64_t(a.pairs) * rows, 8 / j.teams), 256, 0, d.stream, j);
+    hipLaunchKernelGGL((attention_join_k<T>), unsigned(blocks), 256, 0, d.stream, j);
 }
 
 template <class F>
@@ -1103,7 +1136,7 @@ int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const
                                        unsigned(a.pairs) * a.tiles * a.splits, 256, 0, d.stream, a);
                 });
             HIP_CHECK(hipGetLastError());
-            if (a.splits > 1) join<T>(d, a, a.part, a.part_stats, a.out, lse, c.rows, a.group, 1.f);
+            join<T>(d, a, {join_of(a.part, a.out, a.pairs, a.splits, c.rows, a.group, 1.f)}, a.part_stats, lse);
         });
         HIP_CHECK(hipGetLastError());
     });
@@ -1151,29 +1184,23 @@ int cpde_attention_backward(cpde_attention* attention, const cpde_heads* q, cons
             if (count)
                 hipLaunchKernelGGL((attention_delta_k<T>), unsigned((count * 16 + 255) / 256), 256, 0, d.stream, a);
             HIP_CHECK(hipGetLastError());
+            a.tiles = c.row_tiles;
+            a.splits = c.query;
+            a.key_tiles = c.key_tiles;
+            a.key_splits = c.key;
+            a.key_blocks = a.pairs * c.key_tiles * c.key;
+            const unsigned blocks = unsigned(a.key_blocks) + unsigned(a.pairs) * unsigned(c.row_tiles * c.query);
+            if (!blocks) return;
             with_width(a.dim, [&](auto width) {
-                constexpr int DP = decltype(width)::value;
-                if (s.key_tokens) {
-                    a.splits = c.key;
-                    a.tiles = c.key_tiles;
-                    hipLaunchKernelGGL((attention_key_gradient_k<T, DP>), unsigned(a.pairs) * a.tiles * a.splits, 256, 0,
-                                       d.stream, a);
-                    HIP_CHECK(hipGetLastError());
-                    if (a.splits > 1) {
-                        join<T>(d, a, a.part, nullptr, a.dk, nullptr, s.key_tokens, 1, a.scale);
-                        join<T>(d, a, a.part + size_t(a.splits) * a.pairs * s.key_tokens * s.head_dim, nullptr, a.dv,
-                                nullptr, s.key_tokens, 1, 1.f);
-                    }
-                }
-                if (c.rows) {
-                    a.splits = c.query;
-                    a.tiles = c.row_tiles;
-                    hipLaunchKernelGGL((attention_query_gradient_k<T, DP>), unsigned(a.pairs) * a.tiles * a.splits, 256, 0,
-                                       d.stream, a);
-                    HIP_CHECK(hipGetLastError());
-                    if (a.splits > 1) join<T>(d, a, a.part, nullptr, a.dq, nullptr, c.rows, a.group, a.scale);
-                }
+                hipLaunchKernelGGL((attention_gradient_k<T, decltype(width)::value>), blocks, 256, 0, d.stream, a);
             });
+            HIP_CHECK(hipGetLastError());
+            const float* second = a.key_part + size_t(c.key) * a.pairs * s.key_tokens * s.head_dim;
+            join<T>(d, a,
+                    {join_of(a.key_part, a.dk, a.pairs, c.key, s.key_tokens, 1, a.scale),
+                     join_of(second, a.dv, a.pairs, c.key, s.key_tokens, 1, 1.f),
+                     join_of(a.part, a.dq, a.pairs, c.query, c.rows, a.group, a.scale)},
+                    nullptr, nullptr);
         });
         HIP_CHECK(hipGetLastError());
     });

@@ -21,13 +21,16 @@ struct AttentionArgs {
     float* lse;
     const int *query_lengths, *key_lengths;
     int pairs, kv_heads, group;  // pairs: batch entries x key heads
+    int key_blocks;              // workgroups of the keys' gradients, the first of their launch
     int queries, keys, dim;
     int left, right;             // negative: unbounded
-    int tiles, splits;
+    int tiles, splits;           // of query rows
+    int key_tiles, key_splits;   // of keys, in their gradients
     int span;                    // keys of a split of the vector kernel
     float scale, scale2;         // of the scores; the same times log2 e
     int wide_in, wide_out;       // 16-byte loads and stores
     float *part, *part_stats;    // [split][pair][row][dim], [split][pair][row][2]
+    float* key_part;             // dk, then dv: [split][pair][key][dim] each
     float *row_lse, *row_delta;  // [batch][head][query]: lse over scale, dout.out
 };
 
@@ -155,6 +158,7 @@ struct TileLoader {
     // Where 256 slots are whole rows in eights, a lane's slots differ by whole rows:
     // one lane's offset and a step that is the same in every lane.
     static constexpr bool kRegular = 256 % (8 * L::kChunks) == 0;
+    static constexpr uint32_t kNone = ~0u;   // a column past the head's width
     uint32_t offset[kRegular ? 1 : kSteps];  // of a full tile
     int chunks;                              // that hold values
     int64_t stride;                          // bytes from row to row
@@ -168,8 +172,8 @@ struct TileLoader {
         direct = wide;
 #pragma unroll
         for (int i = 0; i < (kRegular ? 1 : kSteps); ++i) {
-            const int slot = i * 256 + threadIdx.x, row = slot / L::kChunks;
-            offset[i] = uint32_t(row * uint32_t(stride)) + (((slot % L::kChunks) ^ L::turn(row)) << 4);
+            const int slot = i * 256 + threadIdx.x, row = slot / L::kChunks, chunk = (slot % L::kChunks) ^ L::turn(row);
+            offset[i] = chunk < chunks ? uint32_t(row * uint32_t(stride)) + (chunk << 4) : kNone;
         }
     }
     // Columns past the head's width are zeros: written once where rows are loaded
@@ -187,12 +191,12 @@ struct TileLoader {
                                              (__attribute__((address_space(3))) void*)(tile + (i * 256 + wave * 64) * 16),
                                              16, 0, 0);
         };
-        if (direct && valid >= ROWS && chunks == L::kChunks) {
+        if (direct && valid >= ROWS) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 if (kSlots % 256 && i * 256 + wave * 64 >= kSlots) break;
-                if constexpr (kRegular) bring(i, base + i * (256 / L::kChunks) * stride + offset[0]);
-                else bring(i, base + offset[i]);
+                const uint32_t at = offset[kRegular ? 0 : i];
+                if (at != kNone) bring(i, base + (kRegular ? i * (256 / L::kChunks) * stride : 0) + at);
             }
         } else if (direct) {
             const int lane = fresh(threadIdx.x);
