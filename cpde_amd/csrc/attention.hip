@@ -7,9 +7,21 @@
 namespace cpde {
 namespace {
 
+// How the launches of a shape are cut (cut_launches).
+struct Cut {
+    bool step = false, brief = false;  // the forward runs on the vector kernel, of 16 waves
+    bool few = false;                  // on the kernel of up to 32 rows
+    int rows = 0, row_tiles = 0, key_tiles = 0;
+    int span = 0, forward = 1, query = 1, key = 1;                   // splits (of `span` keys on the first two)
+    size_t stats = 0, part = 0, part_stats = 0, key_part = 0, floats = 0;  // of the workspace
+};
+// Query rows of a key head up to which the vector kernel serves.
+constexpr int kStepRows = 2;
+
 struct Attention {
     Device* dev = nullptr;
     cpde_attention_shape shape{};
+    Cut cut;
     float* work = nullptr;
 };
 
@@ -38,7 +50,9 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
     __shared__ __align__(16) char lds[2][2][N * L::kRowBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
-    const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;  // (long rows of a causal band first)
+    // (long rows of a causal band first; a second round of workgroups comes to the CUs of
+    // the first in the same order, so it goes the other way)
+    const int split = rest / a.tiles, place = rest % a.tiles, tile = split & 1 ? place : a.tiles - 1 - place;
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
     const Band band(a, b);
     const int rows = a.queries * a.group;
@@ -762,7 +776,7 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
     auto& lds = shared.tiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int pair = block % a.pairs, rest = block / a.pairs;
-    const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
+    const int split = rest / a.tiles, place = rest % a.tiles, tile = split & 1 ? place : a.tiles - 1 - place;
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
     const Band band(a, b);
     const int rows = a.queries * a.group;
@@ -871,64 +885,101 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_gradient_k(At
 // ---- host -----------------------------------------------------------------------------------
 int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
+int step_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : 16; }
+
+// What a launch of `blocks` workgroups in `splits` each takes, in us: the longest
+// workgroup on a CU of its own, or all of them on the CUs they share, with their
+// starts; then the join, whose parts are written and read once.  Measured on 729 to
+// 8192 rows and keys, within about 15%.
+struct Work {
+    int64_t blocks = 0;               // before splitting
+    double longest = 0, mean = 0;     // steps of 32 keys (or queries) of a workgroup
+    double alone = 0, shared = 0;     // us a step, on a CU of its own and in its share of a full one
+    double part_bytes = 0;            // a split writes
+};
+double launch_time(const Work* w, const int* splits, int count, int cus) {
+    double longest = 0, all = 0, blocks = 0, join = 0;
+    for (int i = 0; i < count; ++i) {
+        longest = std::max(longest, w[i].longest / splits[i] * w[i].alone);
+        all += w[i].blocks * w[i].mean * w[i].shared / cus;
+        blocks += double(w[i].blocks) * splits[i];
+        if (splits[i] > 1) join = std::max(join, 6.0) + w[i].part_bytes * splits[i] / 1e6;
+    }
+    const double rounds = std::ceil(blocks / cus);
+    if (count == 1) all = rounds * w[0].mean / splits[0] * w[0].shared;
+    return std::max(longest, all) + 2.5 * rounds + join;
+}
+
 // How the launches of a shape are cut, the same for every call: work is split over
 // the long axis and joined where whole rows would leave the device short of
 // workgroups.
-struct Cut {
-    bool step = false, brief = false;  // the forward runs on the vector kernel, of 16 waves
-    bool few = false;                  // on the kernel of up to 32 rows
-    int rows = 0, row_tiles = 0, key_tiles = 0;
-    int span = 0, forward = 1, query = 1, key = 1;  // splits
-    size_t stats = 0, part = 0, part_stats = 0, key_part = 0, floats = 0;
-};
-
-// Query rows of a key head up to which the vector kernel serves.
-constexpr int kStepRows = 2;
-
-int step_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : 16; }
-
-Cut cut(const Attention& p) {
+void cut_launches(Attention& p) {
     const auto& s = p.shape;
-    Cut c;
+    Cut& c = p.cut;
     const int64_t group = s.heads / s.kv_heads, pairs = int64_t(s.batch) * s.kv_heads;
     c.rows = int(s.query_tokens * group);
     c.row_tiles = ceil_div(c.rows, kBlockRows);
     c.key_tiles = ceil_div(s.key_tokens, kBlockRows);
-    const int cus = p.dev->compute_units, keys_tile = s.dtype == CPDE_F32 ? kKeys<float> : kKeys<bf16>;
-    const auto splits = [&](int64_t blocks, int64_t steps) {
-        // two workgroups a CU, and at least four tiles a split
-        return int(std::clamp<int64_t>(blocks ? 2 * cus / blocks : 1, 1, std::max<int64_t>(steps / 4, 1)));
+    const int cus = p.dev->compute_units;
+    const bool floats = s.dtype == CPDE_F32;
+    // us of a step of two products (32 queries of every wave on 32 keys)
+    const double alone = floats ? 0.35 + 0.0344 * s.head_dim : 0.4 + 0.004 * s.head_dim;
+    const double shared = floats ? 0.0355 * s.head_dim : 0.15 + 0.0037 * s.head_dim;
+    // a band bounded on one side shows half of the other axis on average, on both sides its width
+    const auto seen = [&](double steps) {
+        const double width = s.left >= 0 && s.right >= 0 ? (double(s.left) + s.right + kBlockRows) / 32 : 2 * steps;
+        return std::min({steps, width, s.left >= 0 || s.right >= 0 ? std::max(steps / 2, 1.0) : steps});
     };
+    const double key_steps = ceil_div(s.key_tokens, 32), query_steps = ceil_div(s.query_tokens, 32);
+    const Work rows{pairs * c.row_tiles, s.left >= 0 && s.right >= 0 ? seen(key_steps) : key_steps, seen(key_steps), alone,
+                    shared, 4.0 * double(pairs) * c.rows * s.head_dim};
+    constexpr int kMostSplits = 64;
     // The vector kernel takes one or two rows of floats, or of a list short enough for
     // one workgroup's few rounds; matrix tiles the others (us, vector and tiles; 8 x 8192
     // keys of 4 heads: f32, 128 wide, 1 row 61 and 75, 4 rows 75 and 77; bf16, 1 row 50
     // and 32, 2 rows 55 and 32; 729 keys of 4 heads: bf16, 128 wide, 1 row 8.6 and 11.2).
     const int round = kStepDeep * 16 * (64 / step_lanes(s.head_dim));
-    const bool brief = s.key_tokens <= 2 * round;
-    c.step = c.rows <= kStepRows && (brief || s.dtype == CPDE_F32);
+    c.brief = s.key_tokens <= 2 * round;
+    c.step = c.rows <= kStepRows && (c.brief || floats);
+    c.few = !c.step && c.rows <= kWaveRows;
     if (c.step) {
         // 16 workgroups of four waves a CU, in whole rounds of a workgroup's loads; a
         // short list in one of 16 waves
-        const int64_t share = brief ? s.key_tokens : ceil_div(pairs * s.key_tokens, 16 * cus);
-        c.brief = brief;
+        const int64_t share = c.brief ? s.key_tokens : ceil_div(pairs * s.key_tokens, 16 * cus);
         c.span = std::max(ceil_div(std::max<int64_t>(share, 1), round / 4) * (round / 4), round / 4);
         c.forward = std::max(ceil_div(s.key_tokens, c.span), 1);
-    } else if ((c.few = c.rows <= kWaveRows)) {
-        const int round = 32 * (s.head_dim * type_bytes(s.dtype) <= 256 ? 4 : 2);
-        const int64_t share = std::max<int64_t>(ceil_div(pairs * s.key_tokens, 8 * cus), 4 * round);
-        c.span = ceil_div(share, round) * round;
+    } else if (c.few) {
+        // eight workgroups a CU, of at least four tiles a wave
+        const int tiles = 32 * (s.head_dim * type_bytes(s.dtype) <= 256 ? 4 : 2);
+        const int64_t share = std::max<int64_t>(ceil_div(pairs * s.key_tokens, 8 * cus), 4 * tiles);
+        c.span = ceil_div(share, tiles) * tiles;
         c.forward = std::max(ceil_div(s.key_tokens, c.span), 1);
     } else {
-        c.forward = splits(pairs * c.row_tiles, ceil_div(s.key_tokens, keys_tile));
+        double best = 0;
+        for (int n = 1; n <= std::clamp<int>(int(key_steps) / 4, 1, kMostSplits); ++n) {
+            const double time = launch_time(&rows, &n, 1, cus);
+            if (n == 1 || time < best) best = time, c.forward = n;
+        }
     }
-    size_t part = 0, part_stats = 0;
+    size_t part = 0;
     if (c.forward > 1) {
         part = size_t(c.forward) * pairs * c.rows * s.head_dim;
-        part_stats = size_t(c.forward) * pairs * c.rows * 2;
+        c.part_stats = size_t(c.forward) * pairs * c.rows * 2;
     }
     if (s.backward) {
-        c.query = splits(pairs * c.row_tiles, ceil_div(s.key_tokens, keys_tile));
-        c.key = splits(pairs * c.key_tiles, group * ceil_div(s.query_tokens, kQueries));
+        const double per_head = s.left >= 0 && s.right >= 0 ? seen(query_steps) : query_steps;
+        const Work both[2] = {{pairs * c.key_tiles, group * per_head, group * seen(query_steps), 2 * alone, 2 * shared,
+                               8.0 * double(pairs) * s.key_tokens * s.head_dim},
+                              {rows.blocks, rows.longest, rows.mean, 1.5 * alone, 1.5 * shared, rows.part_bytes}};
+        double best = 0;
+        const int most_keys = std::clamp<int>(int(std::min(group * query_steps, 1e6)) / 4, 1, kMostSplits);
+        const int most_queries = std::clamp<int>(int(key_steps) / 4, 1, kMostSplits);
+        for (int k = 1; k <= most_keys; ++k)
+            for (int q = 1; q <= most_queries; ++q) {
+                const int n[2] = {k, q};
+                const double time = launch_time(both, n, 2, cus);
+                if ((k == 1 && q == 1) || time < best) best = time, c.key = k, c.query = q;
+            }
         if (c.query > 1) part = std::max(part, size_t(c.query) * pairs * c.rows * s.head_dim);
         if (c.key > 1) c.key_part = 2 * size_t(c.key) * pairs * s.key_tokens * s.head_dim;
         c.stats = 2 * size_t(s.batch) * s.heads * s.query_tokens;
@@ -936,9 +987,8 @@ Cut cut(const Attention& p) {
     const auto padded = [](size_t n) { return (n + 63) / 64 * 64; };
     c.stats = padded(c.stats);
     c.part = padded(part);
-    c.part_stats = padded(part_stats);
+    c.part_stats = padded(c.part_stats);
     c.floats = c.stats + c.part + c.part_stats + c.key_part;
-    return c;
 }
 
 HeadView view(const cpde_heads& h) { return {static_cast<char*>(h.data), h.batch, h.token, h.head}; }
@@ -966,8 +1016,9 @@ bool check_heads(const cpde_attention_shape& s, const cpde_heads* h, int tokens,
            s.head_dim * size % 16 == 0 && h->token * int64_t(size) < (int64_t(1) << 24);
 }
 
-AttentionArgs arguments(const Attention& p, const Cut& c, const int* query_lengths, const int* key_lengths) {
+AttentionArgs arguments(const Attention& p, const int* query_lengths, const int* key_lengths) {
     const auto& s = p.shape;
+    const Cut& c = p.cut;
     AttentionArgs a{};
     a.query_lengths = query_lengths;
     a.key_lengths = key_lengths;
@@ -1073,7 +1124,8 @@ int cpde_attention_create(cpde_device* dev, const cpde_attention_shape* shape, c
         auto p = std::make_unique<cpde_attention_s>();
         p->dev = dev;
         p->shape = s;
-        const Cut c = cut(*p);
+        cut_launches(*p);
+        const Cut& c = p->cut;
         const int64_t pairs = int64_t(s.batch) * s.kv_heads;
         const int64_t most = std::max({int64_t(c.row_tiles) * std::max(c.forward, c.query), int64_t(c.key_tiles) * c.key,
                                        c.forward > 1 || c.query > 1 ? int64_t(c.rows) : 1,
@@ -1103,8 +1155,8 @@ int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const
         require(attention, "null argument");
         const Attention& p = *attention;
         const auto& s = p.shape;
-        const Cut c = cut(p);
-        AttentionArgs a = arguments(p, c, query_lengths, key_lengths);
+        const Cut& c = p.cut;
+        AttentionArgs a = arguments(p, query_lengths, key_lengths);
         const bool wq = check_heads(s, q, s.query_tokens, s.heads, false);
         const bool wk = check_heads(s, k, s.key_tokens, s.kv_heads, false);
         const bool wv = check_heads(s, v, s.key_tokens, s.kv_heads, false);
@@ -1151,8 +1203,8 @@ int cpde_attention_backward(cpde_attention* attention, const cpde_heads* q, cons
         const Attention& p = *attention;
         const auto& s = p.shape;
         require(s.backward, "the attention was created without a backward");
-        const Cut c = cut(p);
-        AttentionArgs a = arguments(p, c, query_lengths, key_lengths);
+        const Cut& c = p.cut;
+        AttentionArgs a = arguments(p, query_lengths, key_lengths);
         const bool in[] = {check_heads(s, q, s.query_tokens, s.heads, false),
                            check_heads(s, k, s.key_tokens, s.kv_heads, false),
                            check_heads(s, v, s.key_tokens, s.kv_heads, false),
