@@ -72,28 +72,47 @@ __device__ inline void load_lane(float* v, const T* p, int64_t left, bool aligne
 }
 
 // ---- lookup ---------------------------------------------------------------------------
-// A lane copies 16 bytes of one row.  Bound: HBM (the rows written; rows of common
-// tokens come from the caches).
+// A lane copies 16 bytes of each of two rows, so that two ids and then two rows
+// are under way.  Bound: HBM (the rows written; rows of common tokens come from the
+// caches, which the rows written pass by: 32,768 uneven tokens of 1,024 16-bit values
+// 19 us, 34 where they do not, 25 with one row a lane, 24 with four).
 template <class T, class I>
 __global__ __launch_bounds__(256) void embedding_lookup_k(const I* ids, uint64_t lanes, uint32_t per_row, const T* table,
                                                           int64_t table_stride, int rows, int width, float scale, T* out,
                                                           int64_t out_stride, bool aligned) {
-    constexpr int N = kLane<T>;
+    constexpr int N = kLane<T>, kDeep = 2;
     const uint64_t step = uint64_t(gridDim.x) * 256;
-    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < lanes; i += step) {
-        const uint64_t token = lanes <= 0xffffffffull ? uint32_t(i) / per_row : i / per_row;
-        const int column = int(i - token * per_row) * N;
-        const uint32_t row = key_of(ids[token], rows);
-        float v[N] = {};
-        if (row < uint32_t(rows)) load_lane(v, table + int64_t(row) * table_stride + column, width - column, aligned);
-        T* to = out + int64_t(token) * out_stride + column;
-        if (aligned) {
-            vec<T, N> o;
+    for (uint64_t first = uint64_t(blockIdx.x) * 256 + threadIdx.x; first < lanes; first += kDeep * step) {
+        uint64_t token[kDeep];
+        uint32_t row[kDeep];
+        int column[kDeep];
+        float v[kDeep][N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) o[j] = T(v[j] * scale);
-            *reinterpret_cast<vec<T, N>*>(to) = o;
-        } else {
-            for (int j = 0; j < N && column + j < width; ++j) to[j] = T(v[j] * scale);
+        for (int u = 0; u < kDeep; ++u) {
+            const uint64_t i = first + u * step;
+            token[u] = lanes <= 0xffffffffull ? uint32_t(i) / per_row : i / per_row;
+            column[u] = int(i - token[u] * per_row) * N;
+            row[u] = i < lanes ? key_of(ids[token[u]], rows) : uint32_t(rows);
+        }
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[u][j] = 0.f;
+            if (row[u] < uint32_t(rows))
+                load_lane(v[u], table + int64_t(row[u]) * table_stride + column[u], width - column[u], aligned);
+        }
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+            if (first + u * step >= lanes) break;
+            T* to = out + int64_t(token[u]) * out_stride + column[u];
+            if (aligned) {
+                vec<T, N> o;
+#pragma unroll
+                for (int j = 0; j < N; ++j) o[j] = T(v[u][j] * scale);
+                __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), reinterpret_cast<u32x4*>(to));
+            } else {
+                for (int j = 0; j < N && column[u] + j < width; ++j) to[j] = T(v[u][j] * scale);
+            }
         }
     }
 }
@@ -455,7 +474,7 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
                         vec<float, 4> v = {acc[j] * a.scale, acc[j + 1] * a.scale, acc[j + 2] * a.scale,
                                            acc[j + 3] * a.scale};
                         if (a.accumulate) v += *p;
-                        *p = v;
+                        __builtin_nontemporal_store(v, p);
                     }
             } else {
                 for (int j = 0; j < N && j < left; ++j) out[j] = (a.accumulate ? out[j] : 0.f) + acc[j] * a.scale;
