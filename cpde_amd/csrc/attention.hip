@@ -10,7 +10,7 @@ namespace {
 // How the launches of a shape are cut (cut_launches).
 struct Cut {
     bool step = false, brief = false;  // the forward runs on the vector kernel, of 16 waves
-    bool few = false;                  // on the kernel of up to 32 rows
+    bool few = false;                  // on the kernel of 32 rows a workgroup
     int rows = 0, row_tiles = 0, key_tiles = 0;
     int span = 0, forward = 1, query = 1, key = 1;                   // splits (of `span` keys on the first two)
     size_t stats = 0, part = 0, part_stats = 0, key_part = 0, floats = 0;  // of the workspace
@@ -344,11 +344,13 @@ __global__ __launch_bounds__(64 * WAVES) void attention_step_k(AttentionArgs a) 
     }
 }
 
-// ---- up to 32 query rows: matrix tiles on waves' own keys -----------------------------------
-// All query rows of a key head are one matrix tile's columns, so every wave of a
-// split holds them all and the waves share out the KEYS: each brings tiles of 32 to
-// its own part of LDS and computes on them in turn, with no barrier until their
-// outputs are joined; eight waves a CU keep its share of memory busy.  Bound: HBM.
+// ---- 32 query rows a workgroup: matrix tiles on waves' own keys ------------------------------
+// 32 query rows of a key head are one matrix tile's columns, so every wave of the
+// workgroup holds them all and the waves share out the KEYS: each brings tiles of 32
+// to its own part of LDS and computes on them in turn, with no barrier until their
+// outputs are joined.  For one token, or a few, on long lists eight such waves a CU
+// keep its share of memory busy (bound: HBM); small sets get four times the
+// workgroups of 128 rows, and waves that wait for different things.
 template <class T, int DP>
 constexpr int kRowWaves = DP * sizeof(T) <= 256 ? 4 : 2;
 template <class T, int DP>
@@ -360,18 +362,21 @@ __global__ __launch_bounds__((64 * kRowWaves<T, DP>), 2) void attention_rows_k(A
     __shared__ __align__(16) char lds[kWaves][2 * kHalf > 32 * kPitch * 4 ? 2 * kHalf : 32 * kPitch * 4];
     __shared__ float joined[kWaves][2][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int pair = blockIdx.x % a.pairs, split = blockIdx.x / a.pairs;
+    const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
+    const int first_row = (a.tiles - 1 - rest % a.tiles) * kWaveRows, split = rest / a.tiles;
     const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
     const Band band(a, b);
-    const int rows = a.queries * a.group, row = lane & 31;
+    const int rows = a.queries * a.group, row = first_row + (lane & 31);
     const int query = row / a.group, head = kv * a.group + row % a.group;
     const bool live = row < rows && query < band.ql;
     const int lo = live ? band.key_lo(query) : 0, hi = live ? band.key_hi(query) : 0;
     // keys that any row, and that all rows, see (the rows that count are the first)
-    const int last = min(a.queries, band.ql) - 1;
-    const int from = last < 0 ? 0 : max(band.key_lo(0), int(min(int64_t(split) * a.span, int64_t(band.kl))));
-    const int to = last < 0 ? 0 : int(min(int64_t(band.key_hi(last)), int64_t(split + 1) * a.span));
-    const int full_lo = last < 0 ? 0 : band.key_lo(last), full_hi = last < 0 ? 0 : band.key_hi(0);
+    const int top_query = first_row / a.group, last_query = (min(first_row + kWaveRows, rows) - 1) / a.group;
+    const bool any = top_query < band.ql;
+    const int last = min(last_query, band.ql - 1);
+    const int from = any ? max(band.key_lo(top_query), int(min(int64_t(split) * a.span, int64_t(band.kl)))) : 0;
+    const int to = any ? int(min(int64_t(band.key_hi(last)), int64_t(split + 1) * a.span)) : 0;
+    const int full_lo = any ? band.key_lo(last) : 0, full_hi = any ? band.key_hi(top_query) : 0;
     const int t0 = from / 32, t1 = from < to ? (to + 31) / 32 : t0;
 
     Frag<T> q[kSteps];
@@ -385,6 +390,8 @@ __global__ __launch_bounds__((64 * kRowWaves<T, DP>), 2) void attention_rows_k(A
     const char* values = tile + kHalf;
     Acc out[kBlocks] = {};
     float reference = -INFINITY, sum = 0;
+    kload.clear(tile, lane);
+    vload.clear(tile + kHalf, lane);
     for (int t = t0 + wave; t < t1; t += kWaves) {
         kload.load(tile, kbase + int64_t(t) * 32 * kload.stride, band.kl - t * 32, lane);
         vload.load(tile + kHalf, vbase + int64_t(t) * 32 * vload.stride, band.kl - t * 32, lane);
@@ -429,13 +436,13 @@ __global__ __launch_bounds__((64 * kRowWaves<T, DP>), 2) void attention_rows_k(A
     // the waves' outputs side by side
     float* own = reinterpret_cast<float*>(tile);
     if (half == 0) {
-        joined[wave][0][row] = reference;
-        joined[wave][1][row] = sum;
+        joined[wave][0][lane] = reference;
+        joined[wave][1][lane] = sum;
     }
 #pragma unroll
-    for (int d = 0; d < kBlocks; ++d) store_column(own + row * kPitch, out[d], 1.f, d, half, DP, true);
+    for (int d = 0; d < kBlocks; ++d) store_column(own + (lane & 31) * kPitch, out[d], 1.f, d, half, DP, true);
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * DP; i += 64 * kWaves) {
+    for (int i = threadIdx.x; i < min(kWaveRows, rows - first_row) * DP; i += 64 * kWaves) {
         const int r = i / DP, d = i % DP;
         if (d >= a.dim) continue;
         float next = -INFINITY, total = 0, value = 0;
@@ -448,9 +455,9 @@ __global__ __launch_bounds__((64 * kRowWaves<T, DP>), 2) void attention_rows_k(A
             total += joined[w][1][r] * by;
             value += reinterpret_cast<const float*>(lds[w])[r * kPitch + d] * by;
         }
-        const int q = r / a.group, h = kv * a.group + r % a.group;
+        const int at_row = first_row + r, q = at_row / a.group, h = kv * a.group + at_row % a.group;
         if (a.splits > 1) {
-            const int64_t at = (int64_t(split) * a.pairs + pair) * rows + r;
+            const int64_t at = (int64_t(split) * a.pairs + pair) * rows + at_row;
             a.part[at * a.dim + d] = value;
             if (d == 0) {
                 a.part_stats[2 * at] = next;
@@ -941,24 +948,34 @@ void cut_launches(Attention& p) {
     const int round = kStepDeep * 16 * (64 / step_lanes(s.head_dim));
     c.brief = s.key_tokens <= 2 * round;
     c.step = c.rows <= kStepRows && (c.brief || floats);
-    c.few = !c.step && c.rows <= kWaveRows;
     if (c.step) {
         // 16 workgroups of four waves a CU, in whole rounds of a workgroup's loads; a
         // short list in one of 16 waves
         const int64_t share = c.brief ? s.key_tokens : ceil_div(pairs * s.key_tokens, 16 * cus);
         c.span = std::max(ceil_div(std::max<int64_t>(share, 1), round / 4) * (round / 4), round / 4);
         c.forward = std::max(ceil_div(s.key_tokens, c.span), 1);
-    } else if (c.few) {
-        // eight workgroups a CU, of at least four tiles a wave
-        const int tiles = 32 * (s.head_dim * type_bytes(s.dtype) <= 256 ? 4 : 2);
-        const int64_t share = std::max<int64_t>(ceil_div(pairs * s.key_tokens, 8 * cus), 4 * tiles);
-        c.span = ceil_div(share, tiles) * tiles;
-        c.forward = std::max(ceil_div(s.key_tokens, c.span), 1);
     } else {
         double best = 0;
         for (int n = 1; n <= std::clamp<int>(int(key_steps) / 4, 1, kMostSplits); ++n) {
             const double time = launch_time(&rows, &n, 1, cus);
             if (n == 1 || time < best) best = time, c.forward = n;
+        }
+        // 32 rows a workgroup, its waves sharing the keys: the steps of 128 rows' workgroups
+        // over waves, each a little dearer, as many of them, and waves to join
+        const int tiles = 32 * (s.head_dim * type_bytes(s.dtype) <= 256 ? 4 : 2), waves = tiles / 32;
+        const double blocks = double(pairs) * ceil_div(c.rows, kWaveRows), steps = std::ceil(key_steps / waves);
+        const double dearer = floats ? 1.2 : 1.45, fixed = 3.5 + 1.5 * std::ceil(blocks / cus);
+        const double few = std::max(steps * alone, blocks * std::ceil(seen(key_steps) / waves) * waves / 4 * dearer * shared / cus) + fixed;
+        if (c.rows <= kWaveRows) {
+            // memory's time, not a wave's: eight workgroups a CU, of at least four tiles a wave
+            c.few = true;
+            const int64_t share = std::max<int64_t>(ceil_div(pairs * s.key_tokens, 8 * cus), 4 * tiles);
+            c.span = ceil_div(share, tiles) * tiles;
+            c.forward = std::max(ceil_div(s.key_tokens, c.span), 1);
+        } else if (few < best) {
+            c.few = true;
+            c.span = std::max(ceil_div(s.key_tokens, tiles), 1) * tiles;
+            c.forward = 1;
         }
     }
     size_t part = 0;
@@ -1180,8 +1197,9 @@ int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const
                 with_width(a.dim, [&](auto width) {
                     if (c.few) {
                         constexpr int DP = decltype(width)::value;
-                        hipLaunchKernelGGL((attention_rows_k<T, DP>), unsigned(a.pairs) * a.splits, (64 * kRowWaves<T, DP>),
-                                           0, d.stream, a);
+                        a.tiles = ceil_div(c.rows, kWaveRows);
+                        hipLaunchKernelGGL((attention_rows_k<T, DP>), unsigned(a.pairs) * a.tiles * a.splits,
+                                           (64 * kRowWaves<T, DP>), 0, d.stream, a);
                         return;
                     }
                     hipLaunchKernelGGL((attention_forward_k<T, decltype(width)::value>),

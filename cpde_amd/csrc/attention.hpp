@@ -222,6 +222,7 @@ template <class T, int DP, int ROWS>
 struct WaveLoader {
     using L = Tile<T, DP>;
     static constexpr int kSteps = ROWS * L::kChunks / 64;
+    static constexpr uint32_t kNone = ~0u;  // a column past the head's width
     uint32_t offset[kSteps];
     int chunks, dim;
     int64_t stride;
@@ -234,9 +235,15 @@ struct WaveLoader {
         direct = wide;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const int slot = i * 64 + lane, row = slot / L::kChunks;
-            offset[i] = uint32_t(row * uint32_t(stride)) + (((slot % L::kChunks) ^ L::turn(row)) << 4);
+            const int slot = i * 64 + lane, row = slot / L::kChunks, chunk = (slot % L::kChunks) ^ L::turn(row);
+            offset[i] = chunk < chunks ? uint32_t(row * uint32_t(stride)) + (chunk << 4) : kNone;
         }
+    }
+    // Columns past the head's width: zeros, which direct loads leave alone.
+    __device__ void clear(char* tile, int lane) const {
+        if (direct && chunks < L::kChunks)
+            for (int slot = lane; slot < ROWS * L::kChunks; slot += 64)
+                *reinterpret_cast<u32x4*>(tile + slot * 16) = u32x4{0, 0, 0, 0};
     }
     // The loads have arrived after arrived().
     __device__ __attribute__((always_inline)) void load(char* tile, const char* base, int valid, int lane) const {
@@ -244,23 +251,23 @@ struct WaveLoader {
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                              (__attribute__((address_space(3))) void*)(tile + i * 1024), 16, 0, 0);
         };
-        if (direct && valid >= ROWS && chunks == L::kChunks) {
+        if (direct && valid >= ROWS) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) bring(i, base + offset[i]);
+            for (int i = 0; i < kSteps; ++i)
+                if (offset[i] != kNone) bring(i, base + offset[i]);
             return;
         }
         for (int i = 0; i < kSteps; ++i) {
             const int slot = i * 64 + fresh(lane), row = slot / L::kChunks, chunk = (slot % L::kChunks) ^ L::turn(row);
             const char* from = base + int64_t(min(row, valid - 1)) * stride;
-            if (direct && chunk < chunks) {
-                bring(i, from + chunk * 16);
+            if (direct) {
+                if (chunk < chunks) bring(i, from + chunk * 16);
             } else {
-                // (columns past the head's width are zeros)
                 vec<T, L::kChunk> v;
 #pragma unroll
                 for (int j = 0; j < L::kChunk; ++j) {
                     const int column = chunk * L::kChunk + j;
-                    v[j] = !direct && column < dim ? reinterpret_cast<const T*>(from)[column] : T(0.f);
+                    v[j] = column < dim ? reinterpret_cast<const T*>(from)[column] : T(0.f);
                 }
                 *reinterpret_cast<vec<T, L::kChunk>*>(tile + slot * 16) = v;
             }
