@@ -11,6 +11,7 @@ namespace {
 struct Cut {
     bool step = false, brief = false;  // the forward runs on the vector kernel, of 16 waves
     bool few = false;                  // on the kernel of 32 rows a workgroup
+    bool few_gradient = false;         // the backward on the one of 32 keys or rows
     int rows = 0, row_tiles = 0, key_tiles = 0;
     int span = 0, forward = 1, query = 1, key = 1;                   // splits (of `span` keys on the first two)
     size_t stats = 0, part = 0, part_stats = 0, key_part = 0, floats = 0;  // of the workspace
@@ -596,11 +597,118 @@ __global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a) {
     }
 }
 
-// Gradients of keys and values: 128 keys a workgroup, 32 a wave, with their keys
-// and values in registers, over tiles of 32 queries of every head that reads them.
-// Scores lie as queries x keys, so a lane holds 16 of every 32 queries of ONE key:
-// its probabilities and its score gradients are, in place, the fragments that
-// multiply the transposed dout and queries into dv and dk.
+// The statistics of a tile of queries, lse then delta, one a lane of one wave.
+__device__ __attribute__((always_inline)) inline void load_statistics(const AttentionArgs& a, float* to, int64_t at, int valid,
+                                                                      int lane) {
+    const int i = fresh(lane);
+    const float* from = (i < kQueries ? a.row_lse : a.row_delta) + at + min(i % kQueries, valid - 1);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 4, 0, 0);
+}
+
+// One tile of the gradients of a wave's 32 keys and values, which are in registers,
+// over 32 queries: scores lie as queries x keys, so a lane holds 16 of the 32
+// queries of ONE key, and its probabilities and score gradients are, in place, the
+// fragments that multiply the transposed dout and queries into dv and dk.
+template <class T, int DP>
+__device__ __attribute__((always_inline)) inline void key_tile(const AttentionArgs& a, const Band& band, Acc* dk, Acc* dv,
+                                                               const Frag<T>* k, const Frag<T>* v, const char* queries,
+                                                               const char* douts, const float* statistics, int first,
+                                                               int key, bool hidden, int lane) {
+    using L = Tile<T, DP>;
+    const int now = fresh(lane), half = now >> 5;  // (addresses made anew: the gradients leave no registers for them)
+    int lo = 0, hi = band.ql;
+    if (hidden) {
+        lo = key < band.kl ? band.query_lo(key) : 0;
+        hi = key < band.kl ? band.query_hi(key) : 0;
+    }
+    // The products start from the rows' statistics (lse in the scores' units), which
+    // so take no registers of their own.
+    Acc s, dp;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const auto lse = *reinterpret_cast<const vec<float, 4>*>(statistics + 8 * g + 4 * half);
+        const auto delta = *reinterpret_cast<const vec<float, 4>*>(statistics + kQueries + 8 * g + 4 * half);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s[4 * g + j] = -lse[j];
+            dp[4 * g + j] = -delta[j];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) s = mma(L::row(queries, now & 31, i, half), k[i], s);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) dp = mma(L::row(douts, now & 31, i, half), v[i], dp);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float p = exp2_fast(s[i] * a.scale2), ds = p * dp[i];
+        if (hidden) {
+            const int query = first + 8 * (i >> 2) + 4 * half + (i & 3);
+            const bool seen = query >= lo && query < hi;
+            p = seen ? p : 0.f;
+            ds = seen ? ds : 0.f;
+        }
+        s[i] = p;
+        dp[i] = ds;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const Frag<T> p = as_fragment<T>(s, i), ds = as_fragment<T>(dp, i);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+            dv[d] = mma(L::column(douts, d, i, now), p, dv[d]);
+            dk[d] = mma(L::column(queries, d, i, now), ds, dk[d]);
+        }
+    }
+}
+
+// One tile of 32 keys of the gradient of a wave's 32 query rows: the forward's
+// shape, with queries and dout in registers.
+template <class T, int DP>
+__device__ __attribute__((always_inline)) inline void query_tile(const AttentionArgs& a, Acc* dq, const Frag<T>* q,
+                                                                 const Frag<T>* dout, const char* keys,
+                                                                 const char* values, int at, int first, int lo, int hi,
+                                                                 bool hidden, float lse, float delta, int lane) {
+    using L = Tile<T, DP>;
+    const int half = lane >> 5;
+    Acc s = {}, dp = {};
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) s = mma(L::row(keys, at + (lane & 31), i, half), q[i], s);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) dp = mma(L::row(values, at + (lane & 31), i, half), dout[i], dp);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int key = first + 8 * (i >> 2) + 4 * half + (i & 3);
+        float ds = exp2_fast((s[i] - lse) * a.scale2) * (dp[i] - delta);
+        if (hidden) ds = key >= lo && key < hi ? ds : 0.f;
+        s[i] = ds;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const Frag<T> ds = as_fragment<T>(s, i);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) dq[d] = mma(L::column(keys, d, at / 16 + i, lane), ds, dq[d]);
+    }
+}
+
+// A wave's gradient columns (32 rows of DP) into its place in LDS, and the four
+// waves' sums of it by all of them: column(row, d, value).
+template <int DP>
+constexpr int kPitch = DP + 4;  // floats of a row there
+template <int DP, class F>
+__device__ inline void join_waves(float* const (&places)[4], const Acc* c, int wave, int lane, int rows, int dim, F column) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) store_column(places[wave] + (lane & 31) * kPitch<DP>, c[d], 1.f, d, lane >> 5, DP, true);
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * DP; i += 256) {
+        const int row = i / DP, d = i % DP, at = row * kPitch<DP> + d;
+        if (d < dim) column(row, d, (places[0][at] + places[1][at]) + (places[2][at] + places[3][at]));
+    }
+    __syncthreads();
+}
+
+// Gradients of keys and values.  128 keys a workgroup, 32 a wave, over tiles of 32
+// queries of every head that reads them, one ahead in LDS of the one computed on.
 template <class T, int DP>
 struct KeyShared {
     char tiles[2][2][kQueries * Tile<T, DP>::kRowBytes];
@@ -609,7 +717,6 @@ struct KeyShared {
 template <class T, int DP>
 __device__ __attribute__((always_inline)) inline void key_gradient(const AttentionArgs& a, int block, KeyShared<T, DP>& shared) {
     constexpr int kBlocks = DP / 32, kSteps = DP / 16;
-    using L = Tile<T, DP>;
     auto& lds = shared.tiles;
     auto& stats = shared.stats;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
@@ -622,7 +729,6 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
     const int block_first = tile * kBlockRows, wave_first = block_first + wave * kWaveRows;
     const int key = wave_first + (lane & 31);
     const bool live = key < band.kl;
-
 
     const auto last = [&](int j) { return min(j, band.kl - 1); };
     const bool any = block_first < band.kl, wave_any = wave_first < band.kl;
@@ -657,13 +763,7 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
         const int valid = band.ql - t * kQueries;
         qload.load(to_queries, at_q, valid, wave);
         oload.load(to_douts, at_o, valid, wave);
-        if (wave < 2 * kQueries / 64) {  // the statistics, one a lane
-            const int i = wave * 64 + fresh(lane);
-            const float* from = (i < kQueries ? a.row_lse : a.row_delta) + at_s;
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)(from + min(i % kQueries, valid - 1)),
-                (__attribute__((address_space(3))) void*)(to_stats + wave * 64), 4, 0, 0);
-        }
+        if (wave == 0) load_statistics(a, to_stats, at_s, valid, lane);
         at_q += kQueries * qload.stride;
         at_o += kQueries * oload.stride;
         at_s += kQueries;
@@ -692,55 +792,8 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
         if (++at == t1) at = t0;
         if (more) load(next_queries, next_douts, next_statistics);
         if (first >= wave_hi || first + kQueries <= wave_lo) return;
-        const bool hidden = first < full_lo || first + kQueries > full_hi;
-        const int now = fresh(lane);
-        int lo = 0, hi = band.ql;
-        if (hidden) {
-            lo = live ? band.query_lo(key) : 0;
-            hi = live ? band.query_hi(key) : 0;
-        }
-#pragma unroll
-        for (int u = 0; u < kQueries / 32; ++u) {
-            // The products start from the rows' statistics (lse in the scores' units), which
-            // so take no registers of their own.
-            Acc s, dp;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int at = 32 * u + 8 * g + 4 * (now >> 5);
-                const auto lse = *reinterpret_cast<const vec<float, 4>*>(statistics + at);
-                const auto delta = *reinterpret_cast<const vec<float, 4>*>(statistics + kQueries + at);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[4 * g + j] = -lse[j];
-                    dp[4 * g + j] = -delta[j];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) s = mma(L::row(queries, 32 * u + (now & 31), i, now >> 5), k[i], s);
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) dp = mma(L::row(douts, 32 * u + (now & 31), i, now >> 5), v[i], dp);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float p = exp2_fast(s[i] * a.scale2), ds = p * dp[i];
-                if (hidden) {
-                    const int query = first + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
-                    const bool seen = query >= lo && query < hi;
-                    p = seen ? p : 0.f;
-                    ds = seen ? ds : 0.f;
-                }
-                s[i] = p;
-                dp[i] = ds;
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const Frag<T> p = as_fragment<T>(s, i), ds = as_fragment<T>(dp, i);
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    dv[d] = mma(L::column(douts, d, 2 * u + i, now), p, dv[d]);
-                    dk[d] = mma(L::column(queries, d, 2 * u + i, now), ds, dk[d]);
-                }
-            }
-        }
+        key_tile<T, DP>(a, band, dk, dv, k, v, queries, douts, statistics, first, key,
+                        first < full_lo || first + kQueries > full_hi, lane);
     };
     for (int i = from; i < to; ++i) {
         const int now = (i - from) & 1, next = now ^ 1;
@@ -769,17 +822,16 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
     }
 }
 
-// Gradients of queries: the forward's shape, with queries and dout in registers.
-// (A second pass over the scores, so that no two workgroups add to one place: two
-// products of nine, for sums in a fixed order and no float copy of dq.)
+// Gradients of queries, 128 rows a workgroup.  (A second pass over the scores, so
+// that no two workgroups add to one place: two products of nine, for sums in a fixed
+// order and no float copy of dq.)
 template <class T, int DP>
 struct QueryShared {
     char tiles[2][2][kKeys<T> * Tile<T, DP>::kRowBytes];
 };
 template <class T, int DP>
 __device__ __attribute__((always_inline)) inline void query_gradient(const AttentionArgs& a, int block, QueryShared<T, DP>& shared) {
-    constexpr int N = kKeys<T>, kSub = N / 32, kBlocks = DP / 32, kSteps = DP / 16;
-    using L = Tile<T, DP>;
+    constexpr int N = kKeys<T>, kBlocks = DP / 32, kSteps = DP / 16;
     auto& lds = shared.tiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int pair = block % a.pairs, rest = block / a.pairs;
@@ -791,7 +843,6 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
     const int query = row / a.group, head = kv * a.group + row % a.group;
     const bool live = row < rows && query < band.ql;
     const int lo = live ? band.key_lo(query) : 0, hi = live ? band.key_hi(query) : 0;
-
 
     const auto first_row = [&](int r) { return min(r / a.group, band.ql - 1); };
     const int block_first = tile * kBlockRows, wave_first = block_first + wave * kWaveRows;
@@ -837,26 +888,8 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
         if (first >= wave_hi || first + N <= wave_lo) return;
         const bool hidden = first < full_lo || first + N > full_hi;
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-            Acc s = {}, dp = {};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) s = mma(L::row(keys, 32 * u + (lane & 31), i, half), q[i], s);
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) dp = mma(L::row(values, 32 * u + (lane & 31), i, half), dout[i], dp);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = first + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
-                float ds = exp2_fast((s[i] - lse) * a.scale2) * (dp[i] - delta);
-                if (hidden) ds = key >= lo && key < hi ? ds : 0.f;
-                s[i] = ds;
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const Frag<T> ds = as_fragment<T>(s, i);
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) dq[d] = mma(L::column(keys, d, 2 * u + i, lane), ds, dq[d]);
-            }
-        }
+        for (int u = 0; u < N; u += 32)
+            query_tile<T, DP>(a, dq, q, dout, keys, values, u, first + u, lo, hi, hidden, lse, delta, lane);
     };
     for (int t = t0; t < t1; ++t) {
         const int now = (t - t0) & 1, next = now ^ 1;
@@ -889,6 +922,112 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_gradient_k(At
     else query_gradient<T, DP>(a, blockIdx.x - a.key_blocks, shared.query);
 }
 
+// The same for small sets, 32 keys or rows a workgroup, whose waves share out the
+// tiles of the other axis, each in its own part of LDS, and are joined at the end:
+// four times the workgroups, nothing to join in memory.
+template <class T, int DP>
+struct FewShared {
+    static constexpr int kTiles = 2 * 32 * Tile<T, DP>::kRowBytes, kOut = 32 * kPitch<DP> * 4;
+    char tiles[4][kTiles > kOut ? kTiles : kOut];
+    float stats[4][2][kQueries];
+};
+template <class T, int DP>
+__device__ __attribute__((always_inline)) inline void few_keys_gradient(const AttentionArgs& a, int block, FewShared<T, DP>& shared) {
+    constexpr int kBlocks = DP / 32, kSteps = DP / 16, kHalf = 32 * Tile<T, DP>::kRowBytes;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int pair = block % a.pairs, first_key = block / a.pairs * kWaveRows;
+    const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
+    const Band band(a, b);
+    const int key = first_key + (lane & 31), last = min(first_key + kWaveRows, band.kl) - 1;
+    const bool any = first_key < band.kl, live = key < band.kl;
+    const int lo = any ? band.query_lo(first_key) : 0, hi = any ? band.query_hi(last) : 0;
+    const int full_lo = any ? band.query_lo(last) : 0;
+    const int full_hi = first_key + kWaveRows <= band.kl ? band.query_hi(first_key) : 0;
+    const int t0 = lo / kQueries, per_head = lo < hi ? (hi + kQueries - 1) / kQueries - t0 : 0;
+
+    Frag<T> k[kSteps], v[kSteps];
+    load_fragments<T, DP>(k, head_row<const T>(a.k, b, key, kv), a.dim, half, live, a.wide_in);
+    load_fragments<T, DP>(v, head_row<const T>(a.v, b, key, kv), a.dim, half, live, a.wide_in);
+    WaveLoader<T, DP, 32> qload, oload;
+    qload.start(a.q.token, a.dim, a.wide_in, lane);
+    oload.start(a.dout.token, a.dim, a.wide_in, lane);
+    char* tile = shared.tiles[wave];
+    float* stats = shared.stats[wave][0];
+    qload.clear(tile, lane);
+    oload.clear(tile + kHalf, lane);
+    Acc dk[kBlocks] = {}, dv[kBlocks] = {};
+    for (int i = wave; i < per_head * a.group; i += 4) {
+        const int head = kv * a.group + i / per_head, first = (t0 + i % per_head) * kQueries, valid = band.ql - first;
+        qload.load(tile, reinterpret_cast<const char*>(head_row<const T>(a.q, b, first, head)), valid, lane);
+        oload.load(tile + kHalf, reinterpret_cast<const char*>(head_row<const T>(a.dout, b, first, head)), valid, lane);
+        load_statistics(a, stats, (int64_t(b) * a.kv_heads * a.group + head) * a.queries + first, valid, lane);
+        arrived();
+        key_tile<T, DP>(a, band, dk, dv, k, v, tile, tile + kHalf, stats, first, key,
+                        first < full_lo || first + kQueries > full_hi, lane);
+    }
+    float* const places[4] = {reinterpret_cast<float*>(shared.tiles[0]), reinterpret_cast<float*>(shared.tiles[1]),
+                              reinterpret_cast<float*>(shared.tiles[2]), reinterpret_cast<float*>(shared.tiles[3])};
+    const int rows = min(kWaveRows, a.keys - first_key);
+    join_waves<DP>(places, dk, wave, lane, rows, a.dim, [&](int r, int d, float x) {
+        head_row<T>(a.dk, b, first_key + r, kv)[d] = T(x * a.scale);
+    });
+    join_waves<DP>(places, dv, wave, lane, rows, a.dim, [&](int r, int d, float x) {
+        head_row<T>(a.dv, b, first_key + r, kv)[d] = T(x);
+    });
+}
+template <class T, int DP>
+__device__ __attribute__((always_inline)) inline void few_rows_gradient(const AttentionArgs& a, int block, FewShared<T, DP>& shared) {
+    constexpr int kBlocks = DP / 32, kSteps = DP / 16, kHalf = 32 * Tile<T, DP>::kRowBytes;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int pair = block % a.pairs, first_row = (a.tiles - 1 - block / a.pairs) * kWaveRows;
+    const int b = pair / a.kv_heads, kv = pair % a.kv_heads;
+    const Band band(a, b);
+    const int rows = a.queries * a.group, row = first_row + (lane & 31);
+    const int query = row / a.group, head = kv * a.group + row % a.group;
+    const bool live = row < rows && query < band.ql;
+    const int lo = live ? band.key_lo(query) : 0, hi = live ? band.key_hi(query) : 0;
+    const int top_query = first_row / a.group, last_query = (min(first_row + kWaveRows, rows) - 1) / a.group;
+    const bool any = top_query < band.ql;
+    const int last = min(last_query, band.ql - 1);
+    const int from = any ? band.key_lo(top_query) : 0, to = any ? band.key_hi(last) : 0;
+    const int full_lo = any ? band.key_lo(last) : 0, full_hi = any ? band.key_hi(top_query) : 0;
+
+    Frag<T> q[kSteps], dout[kSteps];
+    load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
+    load_fragments<T, DP>(dout, head_row<const T>(a.dout, b, query, head), a.dim, half, live, a.wide_in);
+    const int64_t at_row = (int64_t(b) * a.kv_heads * a.group + head) * a.queries + query;
+    const float lse = live ? a.row_lse[at_row] : INFINITY, delta = live ? a.row_delta[at_row] : 0.f;
+    WaveLoader<T, DP, 32> kload, vload;
+    kload.start(a.k.token, a.dim, a.wide_in, lane);
+    vload.start(a.v.token, a.dim, a.wide_in, lane);
+    const char* kbase = reinterpret_cast<const char*>(head_row<const T>(a.k, b, 0, kv));
+    const char* vbase = reinterpret_cast<const char*>(head_row<const T>(a.v, b, 0, kv));
+    char* tile = shared.tiles[wave];
+    kload.clear(tile, lane);
+    vload.clear(tile + kHalf, lane);
+    Acc dq[kBlocks] = {};
+    for (int t = from / 32 + wave; t * 32 < to; t += 4) {
+        const int first = t * 32;
+        kload.load(tile, kbase + int64_t(first) * kload.stride, band.kl - first, lane);
+        vload.load(tile + kHalf, vbase + int64_t(first) * vload.stride, band.kl - first, lane);
+        arrived();
+        query_tile<T, DP>(a, dq, q, dout, tile, tile + kHalf, 0, first, lo, hi, first < full_lo || first + 32 > full_hi, lse,
+                          delta, lane);
+    }
+    float* const places[4] = {reinterpret_cast<float*>(shared.tiles[0]), reinterpret_cast<float*>(shared.tiles[1]),
+                              reinterpret_cast<float*>(shared.tiles[2]), reinterpret_cast<float*>(shared.tiles[3])};
+    join_waves<DP>(places, dq, wave, lane, min(kWaveRows, rows - first_row), a.dim, [&](int r, int d, float x) {
+        const int at = first_row + r;
+        head_row<T>(a.dq, b, at / a.group, kv * a.group + at % a.group)[d] = T(x * a.scale);
+    });
+}
+template <class T, int DP>
+__global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_few_gradient_k(AttentionArgs a) {
+    __shared__ __align__(16) FewShared<T, DP> shared;
+    if (int(blockIdx.x) < a.key_blocks) few_keys_gradient<T, DP>(a, blockIdx.x, shared);
+    else few_rows_gradient<T, DP>(a, blockIdx.x - a.key_blocks, shared);
+}
+
 // ---- host -----------------------------------------------------------------------------------
 int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
@@ -913,7 +1052,7 @@ double launch_time(const Work* w, const int* splits, int count, int cus) {
         if (splits[i] > 1) join = std::max(join, 6.0) + w[i].part_bytes * splits[i] / 1e6;
     }
     const double rounds = std::ceil(blocks / cus);
-    if (count == 1) all = rounds * w[0].mean / splits[0] * w[0].shared;
+    if (blocks > 0) all *= rounds * cus / blocks;  // (the last round leaves CUs idle)
     return std::max(longest, all) + 2.5 * rounds + join;
 }
 
@@ -997,6 +1136,14 @@ void cut_launches(Attention& p) {
                 const double time = launch_time(both, n, 2, cus);
                 if ((k == 1 && q == 1) || time < best) best = time, c.key = k, c.query = q;
             }
+        // 32 keys or rows a workgroup, as above; two outputs to join
+        const double blocks[2] = {double(pairs) * ceil_div(s.key_tokens, kWaveRows), double(pairs) * ceil_div(c.rows, kWaveRows)};
+        const double few = std::max({std::ceil(both[0].longest / 4) * both[0].alone, std::ceil(both[1].longest / 4) * both[1].alone,
+                                     (blocks[0] * std::ceil(both[0].mean / 4) * both[0].shared +
+                                      blocks[1] * std::ceil(both[1].mean / 4) * both[1].shared) * (floats ? 1.1 : 1.45) / cus}) +
+                           3.5 + 2 * std::ceil((blocks[0] + blocks[1]) / cus);
+        c.few_gradient = few < best;
+        if (c.few_gradient) c.key = c.query = 1;
         if (c.query > 1) part = std::max(part, size_t(c.query) * pairs * c.rows * s.head_dim);
         if (c.key > 1) c.key_part = 2 * size_t(c.key) * pairs * s.key_tokens * s.head_dim;
         c.stats = 2 * size_t(s.batch) * s.heads * s.query_tokens;
@@ -1258,11 +1405,17 @@ int cpde_attention_backward(cpde_attention* attention, const cpde_heads* q, cons
             a.splits = c.query;
             a.key_tiles = c.key_tiles;
             a.key_splits = c.key;
-            a.key_blocks = a.pairs * c.key_tiles * c.key;
-            const unsigned blocks = unsigned(a.key_blocks) + unsigned(a.pairs) * unsigned(c.row_tiles * c.query);
+            if (c.few_gradient) {
+                a.tiles = ceil_div(c.rows, kWaveRows);
+                a.key_tiles = ceil_div(s.key_tokens, kWaveRows);
+            }
+            a.key_blocks = a.pairs * a.key_tiles * c.key;
+            const unsigned blocks = unsigned(a.key_blocks) + unsigned(a.pairs) * unsigned(a.tiles * c.query);
             if (!blocks) return;
             with_width(a.dim, [&](auto width) {
-                hipLaunchKernelGGL((attention_gradient_k<T, decltype(width)::value>), blocks, 256, 0, d.stream, a);
+                constexpr int DP = decltype(width)::value;
+                if (c.few_gradient) hipLaunchKernelGGL((attention_few_gradient_k<T, DP>), blocks, 256, 0, d.stream, a);
+                else hipLaunchKernelGGL((attention_gradient_k<T, DP>), blocks, 256, 0, d.stream, a);
             });
             HIP_CHECK(hipGetLastError());
             const float* second = a.key_part + size_t(c.key) * a.pairs * s.key_tokens * s.head_dim;
