@@ -377,7 +377,8 @@ __global__ __launch_bounds__((64 * kRowWaves<T, DP>), 2) void attention_rows_k(A
     const int last = min(last_query, band.ql - 1);
     const int from = any ? max(band.key_lo(top_query), int(min(int64_t(split) * a.span, int64_t(band.kl)))) : 0;
     const int to = any ? int(min(int64_t(band.key_hi(last)), int64_t(split + 1) * a.span)) : 0;
-    const int full_lo = any ? band.key_lo(last) : 0, full_hi = any ? band.key_hi(top_query) : 0;
+    // (rows past the length see none: a tile with such rows is never whole)
+    const int full_lo = any ? band.key_lo(last) : 0, full_hi = any && last_query < band.ql ? band.key_hi(top_query) : 0;
     const int t0 = from / 32, t1 = from < to ? (to + 31) / 32 : t0;
 
     Frag<T> q[kSteps];
@@ -622,23 +623,33 @@ __device__ __attribute__((always_inline)) inline void key_tile(const AttentionAr
         lo = key < band.kl ? band.query_lo(key) : 0;
         hi = key < band.kl ? band.query_hi(key) : 0;
     }
-    // The products start from the rows' statistics (lse in the scores' units), which
-    // so take no registers of their own.
-    Acc s, dp;
+    // In 16 bits the products start from the rows' statistics (lse in the scores'
+    // units), which so take no registers of their own; floats keep the bits that a
+    // sum from a large start would round off.
+    constexpr bool kFromStatistics = sizeof(T) == 2;
+    Acc s = {}, dp = {}, lse, delta;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const auto lse = *reinterpret_cast<const vec<float, 4>*>(statistics + 8 * g + 4 * half);
-        const auto delta = *reinterpret_cast<const vec<float, 4>*>(statistics + kQueries + 8 * g + 4 * half);
+        const auto l = *reinterpret_cast<const vec<float, 4>*>(statistics + 8 * g + 4 * half);
+        const auto d = *reinterpret_cast<const vec<float, 4>*>(statistics + kQueries + 8 * g + 4 * half);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            s[4 * g + j] = -lse[j];
-            dp[4 * g + j] = -delta[j];
+            lse[4 * g + j] = -l[j];
+            delta[4 * g + j] = -d[j];
         }
+    }
+    if constexpr (kFromStatistics) {
+        s = lse;
+        dp = delta;
     }
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) s = mma(L::row(queries, now & 31, i, half), k[i], s);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) dp = mma(L::row(douts, now & 31, i, half), v[i], dp);
+    if constexpr (!kFromStatistics) {
+        s += lse;
+        dp += delta;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         float p = exp2_fast(s[i] * a.scale2), ds = p * dp[i];

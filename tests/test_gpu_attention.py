@@ -111,6 +111,17 @@ def test_lengths(device, dtype, queries, keys, right):
     c.against(right=right, ql=ql, kl=kl)
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('right', [-1, 0])
+@pytest.mark.parametrize('queries,keys', [(6, 700), (2, 4000)])
+def test_lengths_of_few_rows(device, dtype, right, queries, keys):
+    """Tiles of keys that every live row sees whole, and rows past the lengths beside them."""
+    c = Case(dtype, 4, queries, keys, 6, 2, 64)
+    ql, kl = [queries, queries // 2, 1, 0], [keys, keys - 100, 33, keys]
+    c.run(device, right=right, ql=ql, kl=kl)
+    c.against(right=right, ql=ql, kl=kl)
+
+
 @pytest.mark.parametrize('dtype', ['f32', 'f16', 'bf16'])
 @pytest.mark.parametrize('order', ['bhtd', 'tbhd', 'htbd'])
 @pytest.mark.parametrize('dim,offset', [(32, 0), (64, 3), (7, 0), (33, 1), (1, 0), (90, 0)])
@@ -131,11 +142,48 @@ def test_one_row_layouts(device):
         c.against()
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('dim', [24, 64, 96, 128])
+@pytest.mark.parametrize('left,right', [(-1, -1), (-1, 0), (50, 9)])
+@pytest.mark.parametrize('queries,keys', [(330, 300), (300, 340)])
+def test_workgroups_of_32_rows(device, dtype, dim, left, right, queries, keys):
+    """Sets large enough for the kernels whose waves share out the other axis."""
+    print(f'[case] 32 rows {dtype} {queries} x {keys} dim={dim} left={left} right={right}', flush=True)
+    c = Case(dtype, 1, queries, keys, 4, 2, dim)
+    c.run(device, left, right)
+    c.against(left, right)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('order,dim,offset', [('bhtd', 40, 0), ('tbhd', 33, 0), ('bthd', 64, 1), ('htbd', 100, 0)])
+def test_workgroups_of_32_rows_layouts(device, dtype, order, dim, offset):
+    """The same on ragged batches (an empty entry on either side, NaN past the lengths) and other layouts."""
+    print(f'[case] 32 rows {dtype} {order} dim={dim} offset={offset}', flush=True)
+    c = Case(dtype, 4, 330, 340, 2, 1, dim, order=order, offset=offset)
+    ql, kl = [330, 0, 201, 77], [340, 340, 0, 129]
+    for b, (n, m) in enumerate(zip(ql, kl)):
+        for t, x in ((c.q, n), (c.dout, n), (c.k, m), (c.v, m)):
+            t[b, x:] = math.nan
+    c.run(device, right=0, ql=ql, kl=kl)
+    c.against(right=0, ql=ql, kl=kl)
+
+
+@pytest.mark.parametrize('dtype,dim', [('f32', 32), ('f32', 64), ('f32', 96), ('f32', 128), ('f16', 32), ('f16', 64), ('f16', 96),
+                                       ('f16', 128), ('bf16', 32), ('bf16', 64), ('bf16', 96), ('bf16', 128)])
+def test_workgroups_of_128_rows(device, dtype, dim):
+    """Many rows and keys: every workgroup resident more than once over."""
+    c = Case(dtype, 4, 700, 900, 16, 8, dim)
+    c.run(device, right=0)
+    c.against(right=0)
+
+
 @pytest.mark.parametrize('dtype', ['f32', 'bf16'])
 @pytest.mark.parametrize('shape', [
     (1, 20, 3000, 2, 2, 64),     # few rows, many keys: forward and queries' gradients split
     (1, 3000, 20, 2, 1, 32),     # few keys, many rows: the keys' gradients split
     (1, 1, 5000, 2, 1, 128),     # one row over splits of the vector kernel
+    (2, 1, 5000, 2, 2, 32),
+    (1, 1, 3000, 2, 1, 50),
     (3, 2, 9000, 8, 2, 30),      # the same with lengths that leave splits empty, unaligned
 ])
 def test_splits(device, dtype, shape):

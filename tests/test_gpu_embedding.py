@@ -89,6 +89,11 @@ def test_gradient_layouts(device, dtype, pad, offset, width):
     gradient(device, dtype, 2000, 300, width, 'skewed', torch.int64, pad=pad, offset=offset)
 
 
+def test_gradient_of_wide_ids(device):
+    """A list for the passes in memory, ids of eight bytes, some outside the table."""
+    gradient(device, 'f16', 9000, 5000, 40, 'outside', torch.int64)
+
+
 @pytest.mark.parametrize('tokens', [900, 6000])
 def test_gradient_adds(device, tokens):
     gradient(device, 'bf16', tokens, 2000, 72, 'skewed', accumulate=True)
