@@ -4,8 +4,10 @@
 namespace cpde {
 namespace {
 
-constexpr int kSmallSort = 4096;     // tokens sorted by one workgroup in LDS
-constexpr int kDigitBits = 10;       // at most, of one pass over longer lists
+constexpr int kShort = 4096;         // tokens up to which every workgroup looks for its rows' tokens itself
+constexpr size_t kShortBytes = 2 << 20;  // and their rows' bytes: one row may have all of them, and so one CU
+constexpr int kShortRows = 256;      // table rows of such a workgroup, at most
+constexpr int kDigitBits = 10;       // at most, of one pass of the sort
 constexpr int kSortTokens = 1024;    // per workgroup of such a pass
 constexpr uint32_t kFan = 32;             // sorted tokens of a partial sum, and partial sums of one of the second level
 
@@ -137,89 +139,7 @@ __device__ inline int take_place(int* counter, uint64_t peers, int lane) {
     return __shfl(base, first) + __popcll(peers & ((1ull << lane) - 1));
 }
 
-// Exclusive sums of a value a thread over a workgroup of 1024; returns the total.
-__device__ inline int scan_block(int value, int& before, int* waves) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sum = value;
-    for (int d = 1; d < 64; d <<= 1) {
-        const int other = __shfl_up(sum, d);
-        if (lane >= d) sum += other;
-    }
-    __syncthreads();
-    if (lane == 63) waves[wave] = sum;
-    __syncthreads();
-    int base = 0, total = 0;
-    for (int w = 0; w < 16; ++w) {
-        if (w < wave) base += waves[w];
-        total += waves[w];
-    }
-    before = base + sum - value;
-    return total;
-}
-
-// Up to 4,096 tokens in one workgroup: six bits a pass, the pairs in LDS.  Bound:
-// the passes' latency.
-template <class I>
-__global__ __launch_bounds__(1024) void embedding_sort_small_k(const I* ids, int tokens, int rows, int bits,
-                                                               uint32_t* keys, uint32_t* places) {
-    __shared__ uint32_t key[kSmallSort];
-    __shared__ uint16_t place[kSmallSort];
-    __shared__ int counter[16 * 64];  // [wave][digit]
-    __shared__ int waves[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // wave w holds tokens [w * share, (w + 1) * share), in rounds of 64
-    const int rounds = (tokens + 1023) / 1024, begin = wave * rounds * 64 + lane;
-    uint32_t k[4];
-    uint32_t p[4];
-    bool live[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        p[r] = begin + r * 64;
-        live[r] = r < rounds && int(p[r]) < tokens;
-        k[r] = live[r] ? key_of(ids[p[r]], rows) : 0;
-    }
-    for (int shift = 0; shift < bits; shift += 6) {
-        counter[threadIdx.x] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (live[r]) atomicAdd(&counter[wave * 64 + ((k[r] >> shift) & 63)], 1);
-        __syncthreads();
-        // places in the order (digit, wave): thread t owns digit t / 16 of wave t % 16
-        int* own = &counter[(threadIdx.x & 15) * 64 + (threadIdx.x >> 4)];
-        int before;
-        scan_block(*own, before, waves);
-        *own = before;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t digit = (k[r] >> shift) & 63;
-            const uint64_t peers = same_digit(digit, 6, live[r]);
-            if (live[r]) {
-                const int to = take_place(&counter[wave * 64 + digit], peers, lane);
-                key[to] = k[r];
-                place[to] = uint16_t(p[r]);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (live[r]) {
-                k[r] = key[begin + r * 64];
-                p[r] = place[begin + r * 64];
-            }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        if (live[r]) {
-            keys[begin + r * 64] = k[r];
-            places[begin + r * 64] = p[r];
-        }
-    }
-}
-
-// Longer lists: per pass, the digits of every 1,024 tokens counted, the counts'
+// Per pass, the digits of every 1,024 tokens counted, the counts'
 // running sums over those blocks (one wave a digit), and the pairs moved.  `ids` is
 // null after the first pass.
 template <class I>
@@ -412,6 +332,135 @@ __global__ __launch_bounds__(256) void embedding_partial2_k(SumArgs a) {
     }
 }
 
+// A lane's columns of one row of the table's gradient.
+template <int N>
+__device__ inline void write_row(const SumArgs& a, int64_t row, int column, const float* sum) {
+    float* out = a.dtable + row * a.dtable_stride + column;
+    const int left = a.width - column;
+    if (a.aligned_out) {
+        if (left > 0)
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                vec<float, 4>* p = reinterpret_cast<vec<float, 4>*>(out + j);
+                vec<float, 4> v = {sum[j] * a.scale, sum[j + 1] * a.scale, sum[j + 2] * a.scale, sum[j + 3] * a.scale};
+                if (a.accumulate) v += *p;
+                __builtin_nontemporal_store(v, p);
+            }
+    } else {
+        for (int j = 0; j < N && j < left; ++j) out[j] = (a.accumulate ? out[j] : 0.f) + sum[j] * a.scale;
+    }
+}
+
+// Short lists, in one launch without a sort: a workgroup reads all ids, keeps its
+// rows' tokens in LDS in their order, and a group of lanes sums each row's; a row of
+// more than kFan tokens is shared by all groups, in shares by its tokens' order.
+template <class T, class I>
+__global__ __launch_bounds__(256) void embedding_short_k(SumArgs a, const I* ids, int block_rows) {
+    constexpr int N = kLane<T>, kRounds = kShort / 256;
+    __shared__ uint32_t list[kShort];  // row in the workgroup << 16, token
+    __shared__ int count[kShortRows];
+    __shared__ int waves[4];
+    __shared__ float shares[256 * N];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t first = blockIdx.x * block_rows;
+    const int rows = int(std::min<uint32_t>(block_rows, a.rows - first));
+    for (int r = threadIdx.x; r < rows; r += 256) count[r] = 0;
+    // wave w reads tokens [w * share, (w + 1) * share), in rounds of 64
+    const int rounds = (a.tokens + 255) / 256, begin = wave * rounds * 64 + lane;
+    uint32_t key[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const uint32_t i = begin + r * 64;
+        const bool live = r < rounds && i < a.tokens;
+        // (an id outside the table, or of other rows, becomes one past the workgroup's)
+        key[r] = live ? std::min<uint32_t>(key_of(ids[i], a.rows) - first, kShortRows) : kShortRows;
+        if (int(key[r]) >= rows) key[r] = kShortRows;
+    }
+    __syncthreads();
+    int mine_before = 0;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        if (r >= rounds) break;
+        mine_before += __popcll(__ballot(key[r] < kShortRows));
+        if (key[r] < kShortRows) atomicAdd(&count[key[r]], 1);
+    }
+    if (lane == 0) waves[wave] = mine_before;
+    __syncthreads();
+    int at = 0, total = 0;
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) at += waves[w];
+        total += waves[w];
+    }
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        if (r >= rounds) break;
+        const uint64_t in = __ballot(key[r] < kShortRows);
+        if (key[r] < kShortRows) list[at + __popcll(in & ((1ull << lane) - 1))] = key[r] << 16 | uint32_t(begin + r * 64);
+        at += __popcll(in);
+    }
+    __syncthreads();
+    const int in = lane & (a.lanes - 1), begin_lane = lane - in, group = threadIdx.x / a.lanes, groups = 256 / a.lanes;
+    const uint64_t mine = (a.lanes == 64 ? ~0ull : (1ull << a.lanes) - 1) << begin_lane;
+    // acc += tokens number from .. to of a row, in order, eight under way
+    const auto sum = [&](float* acc, uint32_t row, int from, int to, int column) {
+        const T* base = static_cast<const T*>(a.dout) + column;
+        const int left = a.width - column;
+        int seen = 0;
+        for (int p = 0; p < total && seen < to; p += a.lanes) {
+            const uint32_t entry = p + in < total ? list[p + in] : ~0u;
+            uint64_t hits = __ballot(entry >> 16 == row) & mine;
+            const int n = __popcll(hits);
+            for (int skip = min(max(from - seen, 0), n); skip > 0; --skip) hits &= hits - 1;
+            int left_over = min(n, to - seen) - min(max(from - seen, 0), n);
+            seen += n;
+            while (left_over > 0) {
+                vec<T, N> v[8];
+                const int now = min(left_over, 8);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    if (u < now) {
+                        const int who = __ffsll(static_cast<unsigned long long>(hits)) - 1;
+                        hits &= hits - 1;
+                        v[u] = load_raw(base + int64_t(__shfl(entry, who) & 0xffff) * a.dout_stride, left, a.aligned);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (u < now)
+#pragma unroll
+                        for (int j = 0; j < N; ++j) acc[j] += float(v[u][j]);
+                left_over -= now;
+            }
+        }
+    };
+    for (int slice = 0; slice * a.lanes * N < a.width; ++slice) {
+        const int column = (slice * a.lanes + in) * N;
+        for (int r = group; r < rows; r += groups) {
+            const int tokens = count[r];
+            if (tokens > int(kFan)) continue;
+            float acc[N] = {};
+            if (tokens) sum(acc, r, 0, tokens, column);
+            write_row<N>(a, first + r, column, acc);
+        }
+        for (int r = 0; r < rows; ++r) {
+            const int tokens = count[r];
+            if (tokens <= int(kFan)) continue;
+            float acc[N] = {};
+            sum(acc, r, int(int64_t(tokens) * group / groups), int(int64_t(tokens) * (group + 1) / groups), column);
+#pragma unroll
+            for (int j = 0; j < N; ++j) shares[threadIdx.x * N + j] = acc[j];
+            __syncthreads();
+            if (group == 0) {
+                for (int g = 1; g < groups; ++g)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += shares[(g * a.lanes + in) * N + j];
+                write_row<N>(a, first + r, column, acc);
+            }
+            __syncthreads();
+        }
+    }
+}
+
 // First sorted tokens whose rows are at least `row` and `end`, by a group of `lanes`
 // lanes: each step probes `lanes` places of both searches at once.  All lanes of the
 // wave take part.
@@ -465,20 +514,7 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
     float acc[N] = {};
     const auto finish_before = [&](uint32_t next) {
         for (; row < next; ++row) {
-            float* out = a.dtable + int64_t(row) * a.dtable_stride + column;
-            if (a.aligned_out) {
-                if (left > 0)
-#pragma unroll
-                    for (int j = 0; j < N; j += 4) {
-                        vec<float, 4>* p = reinterpret_cast<vec<float, 4>*>(out + j);
-                        vec<float, 4> v = {acc[j] * a.scale, acc[j + 1] * a.scale, acc[j + 2] * a.scale,
-                                           acc[j + 3] * a.scale};
-                        if (a.accumulate) v += *p;
-                        __builtin_nontemporal_store(v, p);
-                    }
-            } else {
-                for (int j = 0; j < N && j < left; ++j) out[j] = (a.accumulate ? out[j] : 0.f) + acc[j] * a.scale;
-            }
+            write_row<N>(a, row, column, acc);
 #pragma unroll
             for (int j = 0; j < N; ++j) acc[j] = 0.f;
         }
@@ -562,36 +598,36 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
     Device& d = *e.dev;
     const Layout l = layout(e);
     const auto part = [&](size_t at) { return reinterpret_cast<uint32_t*>(e.work + at); };
-    const int bits = bit_width(uint32_t(e.rows));
-    int now = 0;
-    if (tokens <= kSmallSort) {
-        if (tokens)
-            hipLaunchKernelGGL((embedding_sort_small_k<I>), 1, 1024, 0, d.stream, ids, int(tokens), e.rows, bits,
-                               part(l.keys[0]), part(l.places[0]));
-    } else {
-        const int digit = digit_bits(e.rows), passes = sort_passes(e.rows);
-        const unsigned blocks = (tokens + kSortTokens - 1) / kSortTokens;
-        int *counts = reinterpret_cast<int*>(e.work + l.counts), *totals = reinterpret_cast<int*>(e.work + l.totals);
-        for (int p = 0; p < passes; ++p) {
-            const I* source = p ? nullptr : ids;
-            hipLaunchKernelGGL((embedding_count_k<I>), blocks, 256, 0, d.stream, source, part(l.keys[now]), tokens, e.rows,
-                               p * digit, digit, counts);
-            hipLaunchKernelGGL(embedding_scan_k, (1u << digit) / 4 + 1, 256, 0, d.stream, counts, totals, 1 << digit, blocks);
-            hipLaunchKernelGGL((embedding_move_k<I>), blocks, 256, 0, d.stream, source, part(l.keys[now]),
-                               part(l.places[now]), tokens, e.rows, p * digit, digit, counts, totals,
-                               part(l.keys[1 - now]), part(l.places[1 - now]));
-            now = 1 - now;
-        }
-    }
-    a.keys = part(l.keys[now]);
-    a.places = part(l.places[now]);
-    a.sums1 = reinterpret_cast<float*>(part(l.sums1));
-    a.sums2 = reinterpret_cast<float*>(part(l.sums2));
     a.tokens = tokens;
     constexpr int N = kLane<T>;
     const int per_row = (e.width + N - 1) / N;
     a.lanes = 1;
     while (a.lanes < per_row && a.lanes < 64) a.lanes <<= 1;
+    if (tokens <= kShort && size_t(tokens) * e.width * sizeof(T) <= kShortBytes) {
+        // four workgroups a CU (2,187 tokens of 1,000 rows x 128 floats: 7.1 us, 18.7 sorted
+        // first; 4,096 uneven ones of 1,000 rows x 512 in 16 bits, 4 MB of which a fifth
+        // is one row's: 54 and 39)
+        const int rows = int(std::clamp<int64_t>((int64_t(e.rows) + 4 * d.compute_units - 1) / (4 * d.compute_units), 1, kShortRows));
+        hipLaunchKernelGGL((embedding_short_k<T, I>), unsigned((e.rows + rows - 1) / rows), 256, 0, d.stream, a, ids, rows);
+        return;
+    }
+    const int digit = digit_bits(e.rows), passes = sort_passes(e.rows);
+    const unsigned blocks = (tokens + kSortTokens - 1) / kSortTokens;
+    int *counts = reinterpret_cast<int*>(e.work + l.counts), *totals = reinterpret_cast<int*>(e.work + l.totals);
+    int now = 0;
+    for (int p = 0; p < passes; ++p) {
+        const I* source = p ? nullptr : ids;
+        hipLaunchKernelGGL((embedding_count_k<I>), blocks, 256, 0, d.stream, source, part(l.keys[now]), tokens, e.rows,
+                           p * digit, digit, counts);
+        hipLaunchKernelGGL(embedding_scan_k, ((1u << digit) + 3) / 4, 256, 0, d.stream, counts, totals, 1 << digit, blocks);
+        hipLaunchKernelGGL((embedding_move_k<I>), blocks, 256, 0, d.stream, source, part(l.keys[now]), part(l.places[now]),
+                           tokens, e.rows, p * digit, digit, counts, totals, part(l.keys[1 - now]), part(l.places[1 - now]));
+        now = 1 - now;
+    }
+    a.keys = part(l.keys[now]);
+    a.places = part(l.places[now]);
+    a.sums1 = reinterpret_cast<float*>(part(l.sums1));
+    a.sums2 = reinterpret_cast<float*>(part(l.sums2));
     const unsigned slices = unsigned((per_row + a.lanes - 1) / a.lanes);
     const uint32_t runs = tokens / kFan;
     if (runs)
