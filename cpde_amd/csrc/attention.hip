@@ -43,7 +43,13 @@ constexpr int kGroups = DP * sizeof(T) <= 256 ? 2 : 1;
 // transposed values into out (head columns x queries).  Queries stay in registers.
 // The reference that the exponents are taken against follows the maximum only when
 // that has grown by more than 2^8: sums stay far inside float and the rescaling of
-// the output, 16 products per 32 columns, is rare.
+// the output, 16 products per 32 columns, is rare.  Probabilities are rounded to the
+// tensors' type for the second product (one rounding of each, of relative size
+// 2^-9 in bf16); their sum is of the unrounded ones.
+// A tile's keys and values go from memory to LDS without registers, one tile ahead.
+// Bound: matrix instructions, and LDS at the same rate (a wave reads a tile's 32 KB
+// for 1,024 cycles of products).  Measured: 2 x 8192 causal, 16 heads of 128, bf16:
+// 565 us, 973 TFLOP/s (a large library product on the same card: 1,144).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(AttentionArgs a) {
     constexpr int N = kKeys<T>, kSub = N / 32, kBlocks = DP / 32, kSteps = DP / 16;
@@ -350,8 +356,11 @@ __global__ __launch_bounds__(64 * WAVES) void attention_step_k(AttentionArgs a) 
 // workgroup holds them all and the waves share out the KEYS: each brings tiles of 32
 // to its own part of LDS and computes on them in turn, with no barrier until their
 // outputs are joined.  For one token, or a few, on long lists eight such waves a CU
-// keep its share of memory busy (bound: HBM); small sets get four times the
-// workgroups of 128 rows, and waves that wait for different things.
+// keep its share of memory busy (bound: HBM; 16 sequences of up to 32,768 keys, 4
+// heads of 128, bf16: 537 MB in 113 us of this kernel, 4.8 TB/s); small sets get four times the
+// workgroups of 128 rows, and waves that wait for different things (4 x 729 rows on
+// 729 keys, 32 wide, f32: 20.6 us, 31 with 128 rows a workgroup; bound: the float
+// instruction, 8.2 us, and the waves' own latencies).
 template <class T, int DP>
 constexpr int kRowWaves = DP * sizeof(T) <= 256 ? 4 : 2;
 template <class T, int DP>
@@ -491,7 +500,8 @@ struct JoinArgs {
 
 // 32 lanes hold a row, four columns each; `teams` of them share its splits, with a
 // running maximum each, and are joined through LDS in order.  Splits that saw no
-// key wrote no output.  Bound: HBM (the parts read once).
+// key wrote no output.  Bound: HBM (the parts read once; 64 splits of 256 rows of 128:
+// 5.4 us).
 template <class T>
 __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
     int block = blockIdx.x, which = 0;
@@ -573,7 +583,8 @@ __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
 }
 
 // ---- gradient ---------------------------------------------------------------------------
-// dout.out of every query row, and its lse in the scores' units (over the scale); sixteen lanes a row.
+// dout.out of every query row, and its lse in the scores' units (over the scale);
+// sixteen lanes a row.  Bound: HBM (2 x 4096 x 16 rows of 128, bf16: 67 MB in 16.6 us).
 template <class T>
 __global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a) {
     const int heads = a.kv_heads * a.group;
@@ -922,7 +933,11 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
 }
 
 // Both in one launch, the keys' workgroups first (four products to three): where
-// either would leave the device short of workgroups the other fills it.
+// either would leave the device short of workgroups the other fills it.  Score
+// gradients are rounded to the tensors' type for the products that sum them.  Bound:
+// as the forward's; at 128 columns of 16 bits a wave's keys, values and their
+// gradients leave 32 of its 256 registers.  Measured: 2 x 4096 causal, 16 heads on
+// 4, 128 wide, bf16: 560 us for seven products, 860 TFLOP/s.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_gradient_k(AttentionArgs a) {
     __shared__ __align__(16) union {
@@ -935,7 +950,9 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_gradient_k(At
 
 // The same for small sets, 32 keys or rows a workgroup, whose waves share out the
 // tiles of the other axis, each in its own part of LDS, and are joined at the end:
-// four times the workgroups, nothing to join in memory.
+// four times the workgroups, nothing to join in memory.  (8 x 729 points, 4 heads of
+// 32, f32: 88 us with the launch before it, 107 with 128 a workgroup; bound: the
+// float instruction, 50 us for seven products.)
 template <class T, int DP>
 struct FewShared {
     static constexpr int kTiles = 2 * 32 * Tile<T, DP>::kRowBytes, kOut = 32 * kPitch<DP> * 4;

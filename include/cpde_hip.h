@@ -433,8 +433,9 @@ int cpde_attention_destroy(cpde_attention* attention);
  * float (may be NULL).  query_lengths, key_lengths: int32 [batch] on the device, or
  * NULL; values outside 0..tokens count as the nearest of the two.  Keys and queries
  * at or past the lengths are not read.  A query that sees no key, or past its
- * length, gives zeros and lse = -inf.  Probabilities are rounded to the tensors'
- * type before they multiply v. */
+ * length, gives zeros and lse = -inf.  Where matrix instructions multiply them,
+ * probabilities are rounded to the tensors' type first.  A key that a query does
+ * not see has weight zero in it: finite values there leave no trace. */
 int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const cpde_heads* k, const cpde_heads* v,
                            const cpde_heads* out, float* lse, const int32_t* query_lengths,
                            const int32_t* key_lengths);
