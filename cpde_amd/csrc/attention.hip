@@ -1306,12 +1306,13 @@ int cpde_attention_create(cpde_device* dev, const cpde_attention_shape* shape, c
         require(s.heads >= 1 && s.kv_heads >= 1 && s.heads % s.kv_heads == 0,
                 "query heads are a whole number of times the key heads");
         require(s.head_dim >= 1 && s.head_dim <= kMaxHeadDim, "a head is 1 to 128 wide");
-        require(std::isfinite(s.scale) && s.scale >= 0, "the scale is positive, or 0 for 1/sqrt(head_dim)");
+        // (the backward divides by it, the forward takes it times log2 e)
+        require(s.scale == 0 || (s.scale >= 1e-30f && s.scale <= 1e30f), "the scale is positive, or 0 for 1/sqrt(head_dim)");
         constexpr int64_t kMost = int64_t(1) << 30;  // (row and key numbers, and sums of two, stay inside 32 bits)
         require(int64_t(s.query_tokens) * (s.heads / s.kv_heads) <= kMost && s.key_tokens <= kMost, "too many tokens");
         if (s.scale == 0) s.scale = 1.f / std::sqrt(float(s.head_dim));
-        s.left = s.left < 0 ? -1 : int(std::min<int64_t>(s.left, kMost));
-        s.right = s.right < 0 ? -1 : int(std::min<int64_t>(s.right, kMost));
+        s.left = s.left < 0 ? -1 : int(std::min<int64_t>(s.left, kMost - 2));
+        s.right = s.right < 0 ? -1 : int(std::min<int64_t>(s.right, kMost - 2));
         require(!dev->capturing, "a capture is open on this device");
         auto p = std::make_unique<cpde_attention_s>();
         p->dev = dev;
@@ -1319,10 +1320,11 @@ int cpde_attention_create(cpde_device* dev, const cpde_attention_shape* shape, c
         cut_launches(*p);
         const Cut& c = p->cut;
         const int64_t pairs = int64_t(s.batch) * s.kv_heads;
-        const int64_t most = std::max({int64_t(c.row_tiles) * std::max(c.forward, c.query), int64_t(c.key_tiles) * c.key,
-                                       c.forward > 1 || c.query > 1 ? int64_t(c.rows) : 1,
-                                       c.key > 1 ? int64_t(s.key_tokens) : 1, int64_t(c.forward)});
-        require(pairs <= kMost && pairs * most <= kMost &&
+        // workgroups of the largest launch: of rows, of keys, of joins
+        const int64_t rows = (c.few || c.few_gradient ? ceil_div(c.rows, kWaveRows) : c.row_tiles) * int64_t(std::max(c.forward, c.query));
+        const int64_t keys = (c.few_gradient ? ceil_div(s.key_tokens, kWaveRows) : c.key_tiles) * int64_t(c.key);
+        const int64_t joins = (c.forward > 1 || c.query > 1 ? int64_t(c.rows) : 0) + (c.key > 1 ? 2 * int64_t(s.key_tokens) : 0);
+        require(pairs <= kMost && pairs * std::max(rows + keys, joins) <= kMost &&
                     int64_t(s.batch) * s.heads * s.query_tokens <= kMost * 8,
                 "too many workgroups: split the batch");
         HIP_CHECK(hipMalloc(&p->work, std::max<size_t>(c.floats, 64) * sizeof(float)));

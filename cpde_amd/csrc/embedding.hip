@@ -666,7 +666,7 @@ int cpde_embedding_create(cpde_device* dev, int dtype, int rows, int width, int6
         require(dev && out, "null argument");
         *out = nullptr;
         check_dtype(dtype);
-        require(rows >= 1 && rows < (1 << 30) && width >= 1 && width <= (1 << 24), "invalid table size");
+        require(rows >= 1 && rows < (1 << 30) && width >= 1 && width <= (1 << 22), "invalid table size");
         require(tokens >= 0 && tokens < (int64_t(1) << 31) - kSortTokens, "invalid token count");
         require(index_bytes == 4 || index_bytes == 8, "ids are 4 or 8 bytes");
         auto e = std::make_unique<cpde_embedding_s>();

@@ -342,7 +342,10 @@ def test_refusals(device):
     refused('negative size', lambda: make(hip.F32, 1, -1, 8, 2, 2, 32))
     refused('scale', lambda: make(hip.F32, 1, 8, 8, 2, 2, 32, scale=-1.0))
     refused('scale', lambda: make(hip.F32, 1, 8, 8, 2, 2, 32, scale=math.nan))
+    refused('scale', lambda: make(hip.F32, 1, 8, 8, 2, 2, 32, scale=1e-35))
+    refused('scale', lambda: make(hip.F32, 1, 8, 8, 2, 2, 32, scale=math.inf))
     refused('too many', lambda: make(hip.F32, 1, 1 << 30, 8, 4, 2, 32))
+    refused('too many workgroups', lambda: make(hip.F32, 1 << 20, 1 << 20, 8, 2, 2, 32))
     c = Case('f32', 2, 8, 9, 2, 2, 32)
     plan = make(c.type, *c.shape, backward=False)
     q, k, v, out, dout, dq, dk, dv = c.view('q', 'k', 'v', 'out', 'dout', 'dq', 'dk', 'dv')

@@ -187,6 +187,7 @@ def test_refusals(device):
     refused('element type', lambda: make(-1, 8, 8, 8))
     refused('table size', lambda: make(hip.F32, 0, 8, 8))
     refused('table size', lambda: make(hip.F32, 8, 0, 8))
+    refused('table size', lambda: make(hip.F32, 8, 1 << 23, 8))
     refused('token count', lambda: make(hip.F32, 8, 8, -1))
     refused('4 or 8', lambda: make(hip.F32, 8, 8, 8, index_bytes=2))
     plan = make(hip.F32, 8, 8, 10)
