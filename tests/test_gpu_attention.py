@@ -284,6 +284,30 @@ def test_gradient_against_differences(device, which):
     assert abs(slope - float((grad * d).sum())) < 1e-3 * float(grad.norm() * d.norm())
 
 
+@pytest.mark.parametrize('shape', [(2, 1, 40, 2, 1, 64), (1, 20, 3000, 2, 2, 64), (2, 60, 70, 2, 1, 64), (4, 700, 900, 16, 8, 64)])
+def test_statistics_are_optional(device, shape):
+    """Inference asks for none; the outputs are the same bits."""
+    c = Case('bf16', *shape)
+    c.run(device, backward=False)
+    out = c.out.clone()
+    c.out.fill_(math.nan)
+    c.lse = None
+    c.run(device, backward=False)
+    assert torch.equal(c.out, out)
+
+
+def test_traced(device):
+    """Tracing counts the operators' launches in classes of their own."""
+    device.trace(True)
+    c = Case('bf16', 1, 50, 60, 2, 1, 64)
+    c.run(device)
+    report = device.trace_report()
+    device.trace(False)
+    assert report['attention'][0] == 1 and report['attention_gradient'][0] == 1
+    assert report['attention'][2] == 4 * 2 * 50 * 60 * 64
+    c.against()
+
+
 def test_callers_stream():
     """A device on a stream of torch's: ordered with torch's work there without a wait."""
     stream = torch.cuda.Stream()

@@ -128,6 +128,22 @@ def test_past_32_bits(device):
     assert torch.equal(y[:4].cpu() != 0, keep(4, columns, 0.5, 11))
 
 
+def test_recorded(device):
+    x, r = matrix(300, 64, 'bf16'), matrix(300, 64, 'bf16', seed=2)
+    y = dropped(device, 'bf16', x, 0.3, 5, residual=r)
+    device.capture_begin()
+    device.dropout(hip.BF16, 300, 64, rows_of(x), rows_of(y), 0.3, 5, residual=rows_of(r))
+    replay = device.capture_end()
+    device.synchronize()
+    for _ in range(3):
+        x.mul_(0.5)
+        torch.cuda.synchronize()
+        replay.launch()
+        device.synchronize()
+        against(y, x, 'bf16', 0.3, 5, residual=r)
+    replay.destroy()
+
+
 def refused(match, call):
     with pytest.raises(hip.CpdeError, match=match) as err:
         call()
