@@ -4,8 +4,9 @@
 namespace cpde {
 namespace {
 
-constexpr int kShort = 4096;         // tokens up to which every workgroup looks for its rows' tokens itself
-constexpr size_t kShortBytes = 2 << 20;  // and their rows' bytes: one row may have all of them, and so one CU
+constexpr int kShort = 8192;         // tokens up to which every workgroup looks for its rows' tokens itself
+constexpr int kLong = 16384;         // the same where they are few workgroups
+constexpr int64_t kShortBytes = 4 << 20;  // and their rows' bytes in a workgroup's columns: one row may have all of them
 constexpr int kShortRows = 256;      // table rows of such a workgroup, at most
 constexpr int kDigitBits = 10;       // at most, of one pass of the sort
 constexpr int kSortTokens = 1024;    // per workgroup of such a pass
@@ -261,13 +262,21 @@ struct SumArgs {
     bool aligned, aligned_out;
 };
 
-// A lane's values of a partial sum, whose rows are `width` floats.
+// Four floats of any alignment.
+__device__ inline vec<float, 4> load_floats(const float* p) {
+    vec<float, 4> v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+// A lane's values of a partial sum, whose rows are `width` floats; those at or past
+// `left` are zeros.
 template <int N>
 __device__ inline void load_sum(float* v, const float* p, int left, int width) {
     if (width % 4 == 0) {
 #pragma unroll
         for (int j = 0; j < N; j += 4) {
-            const vec<float, 4> in = j < left ? *reinterpret_cast<const vec<float, 4>*>(p + j) : vec<float, 4>{};
+            const vec<float, 4> in = j < left ? load_floats(p + j) : vec<float, 4>{};
 #pragma unroll
             for (int q = 0; q < 4; ++q) v[j + q] = in[q];
         }
@@ -277,12 +286,23 @@ __device__ inline void load_sum(float* v, const float* p, int left, int width) {
     }
 }
 
-// Sixteen bytes of a row as they are in memory (or as many single values), added later.
+// Sixteen bytes of a row as they are in memory, added later; values at or past `left`
+// are zeros.  Rows that are not on multiples of 16 bytes are read by unaligned loads,
+// a row's last ones from its last 16 bytes, and only rows shorter than that value by
+// value (4,000 tokens of 3 rows x 1,023 in 16 bits: 20 us, 71 value by value).
 template <class T>
-__device__ inline vec<T, kLane<T>> load_raw(const T* p, int left, bool aligned) {
+__device__ inline vec<T, kLane<T>> load_raw(const T* p, int left, bool aligned, int width) {
     vec<T, kLane<T>> v = {};
     if (aligned) {
         if (left > 0) v = *reinterpret_cast<const vec<T, kLane<T>>*>(p);
+    } else if (width >= kLane<T>) {
+        if (left > 0) {
+            const int past = left < kLane<T> ? kLane<T> - left : 0;
+            unsigned __int128 bits;
+            __builtin_memcpy(&bits, p - past, 16);
+            bits >>= past * int(sizeof(T)) * 8;
+            __builtin_memcpy(&v, &bits, 16);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < kLane<T>; ++j)
@@ -309,7 +329,7 @@ __global__ __launch_bounds__(256) void embedding_partial_k(SumArgs a, uint32_t r
 #pragma unroll
         for (uint32_t u = 0; u < 16; ++u)
             v[u] = load_raw(static_cast<const T*>(a.dout) + int64_t(a.places[first + i + u]) * a.dout_stride + column, left,
-                            a.aligned);
+                            a.aligned, a.width);
 #pragma unroll
         for (int u = 0; u < 16; ++u)
 #pragma unroll
@@ -347,113 +367,139 @@ __device__ inline void write_row(const SumArgs& a, int64_t row, int column, cons
                 __builtin_nontemporal_store(v, p);
             }
     } else {
-        for (int j = 0; j < N && j < left; ++j) out[j] = (a.accumulate ? out[j] : 0.f) + sum[j] * a.scale;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            if (j + 4 <= left) {
+                vec<float, 4> v = {sum[j] * a.scale, sum[j + 1] * a.scale, sum[j + 2] * a.scale, sum[j + 3] * a.scale};
+                if (a.accumulate) v += load_floats(out + j);
+                __builtin_memcpy(out + j, &v, 16);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (j + q < left) out[j + q] = (a.accumulate ? out[j + q] : 0.f) + sum[j + q] * a.scale;
+            }
+        }
     }
 }
 
-// Short lists, in one launch without a sort: a workgroup reads all ids, keeps its
-// rows' tokens in LDS in their order, and a group of lanes sums each row's; a row of
-// more than kFan tokens is shared by all groups, in shares by its tokens' order.
-template <class T, class I>
-__global__ __launch_bounds__(256) void embedding_short_k(SumArgs a, const I* ids, int block_rows) {
-    constexpr int N = kLane<T>, kRounds = kShort / 256;
-    __shared__ uint32_t list[kShort];  // row in the workgroup << 16, token
-    __shared__ int count[kShortRows];
-    __shared__ int waves[4];
-    __shared__ float shares[256 * N];
+// Short lists, in one launch without a sort of the whole: a workgroup reads all ids
+// and puts its rows' tokens into LDS by row (stably: counted, then moved, a wave each),
+// and a group of lanes sums each row's, eight loads under way.  A row of more tokens
+// than `alone` is shared by all groups, in shares by its tokens' order, joined in a
+// tree.  Workgroups along y take slices of the columns.
+template <class T, class I, int LIST>
+__global__ __launch_bounds__(256) void embedding_short_k(SumArgs a, const I* ids, int block_rows, int alone) {
+    constexpr int N = kLane<T>, kRounds = 16;
+    __shared__ uint16_t order[LIST];  // tokens by row
+    __shared__ int counter[4][kShortRows], places[4][kShortRows], start[kShortRows + 1];
+    __shared__ float shares[4 * 64 * N];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t first = blockIdx.x * block_rows;
     const int rows = int(std::min<uint32_t>(block_rows, a.rows - first));
-    for (int r = threadIdx.x; r < rows; r += 256) count[r] = 0;
     // wave w reads tokens [w * share, (w + 1) * share), in rounds of 64
     const int rounds = (a.tokens + 255) / 256, begin = wave * rounds * 64 + lane;
-    uint32_t key[kRounds];
+    uint32_t key[kRounds], some = 0;  // keys of 16 rounds; the rounds that have any of the workgroup's rows
+    const auto load = [&](int from) {
+        some = 0;
+        uint64_t in[kRounds];
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-        const uint32_t i = begin + r * 64;
-        const bool live = r < rounds && i < a.tokens;
-        // (an id outside the table, or of other rows, becomes one past the workgroup's)
-        key[r] = live ? std::min<uint32_t>(key_of(ids[i], a.rows) - first, kShortRows) : kShortRows;
-        if (int(key[r]) >= rows) key[r] = kShortRows;
-    }
-    __syncthreads();
-    int mine_before = 0;
+        for (int r = 0; r < kRounds; ++r)
+            if (from + r < rounds) in[r] = uint64_t(int64_t(ids[std::min<uint32_t>(begin + (from + r) * 64, a.tokens - 1)]));
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-        if (r >= rounds) break;
-        mine_before += __popcll(__ballot(key[r] < kShortRows));
-        if (key[r] < kShortRows) atomicAdd(&count[key[r]], 1);
-    }
-    if (lane == 0) waves[wave] = mine_before;
-    __syncthreads();
-    int at = 0, total = 0;
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) at += waves[w];
-        total += waves[w];
-    }
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-        if (r >= rounds) break;
-        const uint64_t in = __ballot(key[r] < kShortRows);
-        if (key[r] < kShortRows) list[at + __popcll(in & ((1ull << lane) - 1))] = key[r] << 16 | uint32_t(begin + r * 64);
-        at += __popcll(in);
-    }
-    __syncthreads();
-    const int in = lane & (a.lanes - 1), begin_lane = lane - in, group = threadIdx.x / a.lanes, groups = 256 / a.lanes;
-    const uint64_t mine = (a.lanes == 64 ? ~0ull : (1ull << a.lanes) - 1) << begin_lane;
-    // acc += tokens number from .. to of a row, in order, eight under way
-    const auto sum = [&](float* acc, uint32_t row, int from, int to, int column) {
-        const T* base = static_cast<const T*>(a.dout) + column;
-        const int left = a.width - column;
-        int seen = 0;
-        for (int p = 0; p < total && seen < to; p += a.lanes) {
-            const uint32_t entry = p + in < total ? list[p + in] : ~0u;
-            uint64_t hits = __ballot(entry >> 16 == row) & mine;
-            const int n = __popcll(hits);
-            for (int skip = min(max(from - seen, 0), n); skip > 0; --skip) hits &= hits - 1;
-            int left_over = min(n, to - seen) - min(max(from - seen, 0), n);
-            seen += n;
-            while (left_over > 0) {
-                vec<T, N> v[8];
-                const int now = min(left_over, 8);
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    if (u < now) {
-                        const int who = __ffsll(static_cast<unsigned long long>(hits)) - 1;
-                        hits &= hits - 1;
-                        v[u] = load_raw(base + int64_t(__shfl(entry, who) & 0xffff) * a.dout_stride, left, a.aligned);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if (u < now)
-#pragma unroll
-                        for (int j = 0; j < N; ++j) acc[j] += float(v[u][j]);
-                left_over -= now;
-            }
+        for (int r = 0; r < kRounds; ++r) {
+            if (from + r >= rounds) continue;
+            // (ids outside the table, too, are no less than `rows` from `first` on)
+            const uint64_t row = in[r] - first;
+            const bool live = row < uint32_t(rows) && begin + (from + r) * 64 < a.tokens;
+            key[r] = live ? uint32_t(row) : kShortRows;
+            if (__any(live)) some |= 1u << r;
         }
     };
-    for (int slice = 0; slice * a.lanes * N < a.width; ++slice) {
-        const int column = (slice * a.lanes + in) * N;
+    load(0);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) counter[w][threadIdx.x] = 0;
+    __syncthreads();
+    for (int from = 0; from < rounds; from += kRounds) {
+        if (from) load(from);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r)
+            if (some >> r & 1 && key[r] < kShortRows) atomicAdd(&counter[wave][key[r]], 1);
+    }
+    __syncthreads();
+    // (every wave makes the running sums for itself: no barrier before the move)
+    for (int c = 0, carry = 0; c < rows; c += 64) {
+        int n[4], tokens = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) tokens += n[w] = counter[w][c + lane];
+        int before = tokens;
+        for (int step = 1; step < 64; step <<= 1) {
+            const int other = __shfl_up(before, step);
+            if (lane >= step) before += other;
+        }
+        const int sum = __shfl(before, 63);
+        before += carry - tokens;
+        if (wave == 0) {
+            start[c + lane] = before;
+            if (lane == 63) start[c + 64] = before + tokens;
+        }
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+            if (w < wave) before += n[w];
+        places[wave][c + lane] = before;
+        carry += sum;
+    }
+    const int bits = block_rows > 1 ? 32 - __clz(block_rows - 1) : 0;
+    for (int from = 0; from < rounds; from += kRounds) {
+        if (rounds > kRounds) load(from);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            if (!(some >> r & 1)) continue;
+            const bool live = key[r] < kShortRows;
+            const uint64_t peers = same_digit(key[r], bits, live);
+            if (live) order[take_place(&places[wave][key[r]], peers, lane)] = uint16_t(begin + (from + r) * 64);
+        }
+    }
+    __syncthreads();
+    const int in = lane & (a.lanes - 1), group = threadIdx.x / a.lanes, groups = 256 / a.lanes;
+    for (int slice = blockIdx.y; slice * a.lanes * N < a.width; slice += gridDim.y) {
+        const int column = (slice * a.lanes + in) * N, left = a.width - column;
+        const T* base = static_cast<const T*>(a.dout) + column;
+        // acc += the tokens at [from, to) of the order
+        const auto sum = [&](float* acc, int from, int to) {
+            for (int p = from; p < to; p += 8) {
+                vec<T, N> v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (p + u < to) v[u] = load_raw(base + int64_t(order[p + u]) * a.dout_stride, left, a.aligned, a.width);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (p + u < to)
+#pragma unroll
+                        for (int j = 0; j < N; ++j) acc[j] += float(v[u][j]);
+            }
+        };
         for (int r = group; r < rows; r += groups) {
-            const int tokens = count[r];
-            if (tokens > int(kFan)) continue;
+            if (start[r + 1] - start[r] > alone) continue;
             float acc[N] = {};
-            if (tokens) sum(acc, r, 0, tokens, column);
+            sum(acc, start[r], start[r + 1]);
             write_row<N>(a, first + r, column, acc);
         }
         for (int r = 0; r < rows; ++r) {
-            const int tokens = count[r];
-            if (tokens <= int(kFan)) continue;
+            const int tokens = start[r + 1] - start[r];
+            if (tokens <= alone) continue;
             float acc[N] = {};
-            sum(acc, r, int(int64_t(tokens) * group / groups), int(int64_t(tokens) * (group + 1) / groups), column);
+            sum(acc, start[r] + tokens * group / groups, start[r] + tokens * (group + 1) / groups);
+            for (int step = a.lanes; step < 64; step <<= 1)
 #pragma unroll
-            for (int j = 0; j < N; ++j) shares[threadIdx.x * N + j] = acc[j];
+                for (int j = 0; j < N; ++j) acc[j] += __shfl_xor(acc[j], step);
+            if (lane < a.lanes)
+#pragma unroll
+                for (int j = 0; j < N; ++j) shares[(wave * 64 + in) * N + j] = acc[j];
             __syncthreads();
             if (group == 0) {
-                for (int g = 1; g < groups; ++g)
+                for (int w = 1; w < 4; ++w)
 #pragma unroll
-                    for (int j = 0; j < N; ++j) acc[j] += shares[(g * a.lanes + in) * N + j];
+                    for (int j = 0; j < N; ++j) acc[j] += shares[(w * 64 + in) * N + j];
                 write_row<N>(a, first + r, column, acc);
             }
             __syncthreads();
@@ -550,12 +596,14 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
             if (span == kFan)  // (up to where the second level may take over)
                 runs = std::min(runs, int((kFan * kFan - at % (kFan * kFan)) / kFan));
             const float* sums = (span == kFan ? a.sums1 : a.sums2) + size_t(at / span) * a.width + column;
-            for (int r = 0; r < runs; r += 4) {
-                float v[4][N];
+            constexpr int kSums = 32 / N;
+            for (int r = 0; r < runs; r += kSums) {
+                float v[kSums][N];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) load_sum<N>(v[u], sums + size_t(std::min(r + u, runs - 1)) * a.width, left, a.width);
+                for (int u = 0; u < kSums; ++u)
+                    load_sum<N>(v[u], sums + size_t(std::min(r + u, runs - 1)) * a.width, left, a.width);
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < kSums; ++u)
                     if (r + u < runs)
 #pragma unroll
                         for (int j = 0; j < N; ++j) acc[j] += v[u][j];
@@ -569,7 +617,7 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 const uint32_t place = __shfl(my_place, begin_lane + int(std::min(from + u, here - 1)));
-                to[u] = load_raw(base + int64_t(place) * a.dout_stride, left, a.aligned);
+                to[u] = load_raw(base + int64_t(place) * a.dout_stride, left, a.aligned, a.width);
             }
         };
         const auto add = [&](const vec<T, N>* from, uint32_t first) {
@@ -605,13 +653,21 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
     const int per_row = (e.width + N - 1) / N;
     a.lanes = 1;
     while (a.lanes < per_row && a.lanes < 64) a.lanes <<= 1;
-    if (tokens <= kShort && size_t(tokens) * e.width * sizeof(T) <= kShortBytes) {
-        // four workgroups a CU (2,187 tokens of 1,000 rows x 128 floats: 7.1 us, 18.7 sorted
-        // first; 4,096 uneven ones of 1,000 rows x 512 in 16 bits, 4 MB of which a fifth
-        // is one row's: 54 and 39)
-        const int rows = int(std::clamp<int64_t>((int64_t(e.rows) + 4 * d.compute_units - 1) / (4 * d.compute_units), 1, kShortRows));
-        hipLaunchKernelGGL((embedding_short_k<T, I>), unsigned((e.rows + rows - 1) / rows), 256, 0, d.stream, a, ids, rows);
-        return;
+    if (tokens <= kLong) {
+        const int fill = 4 * d.compute_units;  // workgroups
+        const int rows = int(std::clamp<int64_t>((int64_t(e.rows) + fill - 1) / fill, 1, kShortRows));
+        const int blocks = (e.rows + rows - 1) / rows;
+        // tables of few rows: more workgroups by slices of the columns, of 64 bytes at least
+        int lanes = a.lanes;
+        const auto slices = [&] { return 2 * blocks <= fill ? std::min((per_row + lanes - 1) / lanes, 65535) : 1; };
+        while (lanes > 4 && 2 * int64_t(blocks) * slices() <= fill) lanes >>= 1;
+        if ((tokens <= kShort || blocks * slices() <= d.compute_units) &&
+            int64_t(tokens) * e.width * int64_t(sizeof(T)) <= kShortBytes * slices()) {
+            a.lanes = lanes;
+            const auto kernel = tokens <= kShort ? embedding_short_k<T, I, kShort> : embedding_short_k<T, I, kLong>;
+            hipLaunchKernelGGL(kernel, dim3(blocks, slices()), 256, 0, d.stream, a, ids, rows, rows > 4 ? 32 : 8);
+            return;
+        }
     }
     const int digit = digit_bits(e.rows), passes = sort_passes(e.rows);
     const unsigned blocks = (tokens + kSortTokens - 1) / kSortTokens;
@@ -636,6 +692,8 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
         hipLaunchKernelGGL((embedding_partial_k<T>), dim3(unsigned((uint64_t(runs) * a.lanes + 255) / 256), slices), 256, 0,
                            d.stream, a, runs);
     if (runs / kFan) hipLaunchKernelGGL(embedding_partial2_k, runs / kFan, 256, 0, d.stream, a);
+    // A group's lanes also look through the tokens, so narrow rows have idle ones.
+    a.lanes = std::max(a.lanes, 16);
     // Rows a group: enough that a search serves several, few enough that common tokens
     // do not hold a wave back (131,072 uneven tokens of 65,536 rows x 512: 4 rows 126
     // us, 8 rows 133, 16 rows 143).

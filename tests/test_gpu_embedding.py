@@ -64,6 +64,17 @@ def gradient(device, dtype, tokens, rows, width, kind='uniform', index=torch.int
     assert (off <= far).all(), float((off / far.clamp(min=1e-300)).max())
 
 
+@pytest.mark.parametrize('tokens', [257, 4095, 5000, 16384, 16385])
+@pytest.mark.parametrize('rows,width', [(3, 9), (8, 8), (303, 12), (12, 203), (1500, 31), (66000, 5)])
+@pytest.mark.parametrize('kind', ['uniform', 'skewed', 'one', 'outside'])
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_gradient_narrow_and_odd_rows(device, dtype, kind, tokens, rows, width):
+    """Rows narrower than a wave's loads, tables of few rows, widths off every alignment; common tokens."""
+    print(f'[case] narrow gradient {dtype} {kind} tokens={tokens} rows={rows} width={width}', flush=True)
+    gradient(device, dtype, tokens, rows, width, kind, index=torch.int64 if width % 2 else torch.int32,
+             accumulate=rows == 12, pad=3 if rows == 303 else 0, offset=1 if rows == 1500 else 0)
+
+
 @pytest.mark.parametrize('tokens', [0, 1, 63, 65, 1000, 4096, 4097, 10000, 70001])
 @pytest.mark.parametrize('rows,width', [(1, 64), (2, 3), (63, 512), (1000, 130), (1025, 8), (70000, 16)])
 def test_gradient_sizes(device, tokens, rows, width):
