@@ -259,7 +259,7 @@ struct SumArgs {
     uint32_t tokens;
     int rows, width, accumulate, group_rows, lanes;  // lanes a row of `width` takes in one slice (a power of two)
     float scale;
-    bool aligned, aligned_out;
+    bool aligned_out;
 };
 
 // Four floats of any alignment.
@@ -286,35 +286,53 @@ __device__ inline void load_sum(float* v, const float* p, int left, int width) {
     }
 }
 
-// Sixteen bytes of a row as they are in memory, added later; values at or past `left`
-// are zeros.  Rows that are not on multiples of 16 bytes are read by unaligned loads,
-// a row's last ones from its last 16 bytes, and only rows shorter than that value by
-// value (4,000 tokens of 3 rows x 1,023 in 16 bits: 20 us, 71 value by value).
-template <class T>
-__device__ inline vec<T, kLane<T>> load_raw(const T* p, int left, bool aligned, int width) {
-    vec<T, kLane<T>> v = {};
-    if (aligned) {
-        if (left > 0) v = *reinterpret_cast<const vec<T, kLane<T>>*>(p);
-    } else if (width >= kLane<T>) {
-        if (left > 0) {
-            const int past = left < kLane<T> ? kLane<T> - left : 0;
+// A lane's columns of dout: sixteen bytes of a row as they are in memory, by one load
+// of any alignment; a row's last ones are the last of its last 16 bytes, moved down when
+// they are added (a move behind the load would wait for it).  Rows shorter than that
+// are read value by value.  Lanes past the width read the row's last bytes and are not
+// used.  (4,000 tokens of 400 rows x 1,023 in 16 bits: 39 us; value by value 89.)
+// The form is a template's, as a branch between two loads waits for the first.
+template <class T, bool WIDE>
+struct Columns {
+    static constexpr int N = kLane<T>;
+    const T* base;
+    int64_t stride;
+    int left, shift;  // values from the lane's column on; bits of the move
+    bool moved;
+    __device__ Columns(const SumArgs& a, int column) : stride(a.dout_stride), left(a.width - column) {
+        moved = WIDE && a.width % N;
+        const int back = WIDE ? std::max(0, N - left) : 0;
+        shift = left > 0 ? back * int(sizeof(T)) * 8 : 0;
+        base = static_cast<const T*>(a.dout) + column - back;
+    }
+    __device__ vec<T, N> load(int64_t token) const {
+        const T* p = base + token * stride;
+        vec<T, N> v = {};
+        if constexpr (WIDE) {
+            __builtin_memcpy(&v, p, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < left) v[j] = p[j];
+        }
+        return v;
+    }
+    __device__ void add(float* acc, vec<T, N> v) const {
+        if (moved) {
             unsigned __int128 bits;
-            __builtin_memcpy(&bits, p - past, 16);
-            bits >>= past * int(sizeof(T)) * 8;
+            __builtin_memcpy(&bits, &v, 16);
+            bits >>= shift;
             __builtin_memcpy(&v, &bits, 16);
         }
-    } else {
 #pragma unroll
-        for (int j = 0; j < kLane<T>; ++j)
-            if (j < left) v[j] = p[j];
+        for (int j = 0; j < N; ++j) acc[j] += float(v[j]);
     }
-    return v;
-}
+};
 
 // Partial sums of the aligned runs of kFan tokens that lie whole inside one row: a
 // common token's row is then the sum of few terms, whatever its count.  A group of
 // lanes a run, so that a common token's runs spread over the device.
-template <class T>
+template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void embedding_partial_k(SumArgs a, uint32_t runs) {
     constexpr int N = kLane<T>;
     const uint64_t run = (uint64_t(blockIdx.x) * 256 + threadIdx.x) / unsigned(a.lanes);
@@ -322,18 +340,19 @@ __global__ __launch_bounds__(256) void embedding_partial_k(SumArgs a, uint32_t r
     if (run >= runs || left <= 0) return;
     const uint32_t first = uint32_t(run) * kFan, row = a.keys[first];
     if (row >= uint32_t(a.rows) || row != a.keys[first + kFan - 1]) return;
+    const Columns<T, WIDE> columns(a, column);
     float acc[N] = {};
 #pragma unroll 1
     for (uint32_t i = 0; i < kFan; i += 16) {
+        uint32_t place[16];
         vec<T, N> v[16];
 #pragma unroll
+        for (uint32_t u = 0; u < 16; ++u) place[u] = a.places[first + i + u];
+#pragma unroll
         for (uint32_t u = 0; u < 16; ++u)
-            v[u] = load_raw(static_cast<const T*>(a.dout) + int64_t(a.places[first + i + u]) * a.dout_stride + column, left,
-                            a.aligned, a.width);
+            v[u] = columns.load(place[u]);
 #pragma unroll
-        for (int u = 0; u < 16; ++u)
-#pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] += float(v[u][j]);
+        for (int u = 0; u < 16; ++u) columns.add(acc, v[u]);
     }
     float* to = a.sums1 + size_t(run) * a.width + column;
     for (int j = 0; j < N && j < left; ++j) to[j] = acc[j];
@@ -387,7 +406,7 @@ __device__ inline void write_row(const SumArgs& a, int64_t row, int column, cons
 // and a group of lanes sums each row's, eight loads under way.  A row of more tokens
 // than `alone` is shared by all groups, in shares by its tokens' order, joined in a
 // tree.  Workgroups along y take slices of the columns.
-template <class T, class I, int LIST>
+template <class T, class I, int LIST, bool WIDE>
 __global__ __launch_bounds__(256) void embedding_short_k(SumArgs a, const I* ids, int block_rows, int alone) {
     constexpr int N = kLane<T>, kRounds = 16;
     __shared__ uint16_t order[LIST];  // tokens by row
@@ -462,20 +481,25 @@ __global__ __launch_bounds__(256) void embedding_short_k(SumArgs a, const I* ids
     __syncthreads();
     const int in = lane & (a.lanes - 1), group = threadIdx.x / a.lanes, groups = 256 / a.lanes;
     for (int slice = blockIdx.y; slice * a.lanes * N < a.width; slice += gridDim.y) {
-        const int column = (slice * a.lanes + in) * N, left = a.width - column;
-        const T* base = static_cast<const T*>(a.dout) + column;
+        const int column = (slice * a.lanes + in) * N;
+        const Columns<T, WIDE> columns(a, column);
         // acc += the tokens at [from, to) of the order
         const auto sum = [&](float* acc, int from, int to) {
-            for (int p = from; p < to; p += 8) {
+            int p = from;
+            for (; p + 8 <= to; p += 8) {
                 vec<T, N> v[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if (p + u < to) v[u] = load_raw(base + int64_t(order[p + u]) * a.dout_stride, left, a.aligned, a.width);
+                for (int u = 0; u < 8; ++u) v[u] = columns.load(order[p + u]);
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if (p + u < to)
+                for (int u = 0; u < 8; ++u) columns.add(acc, v[u]);
+            }
+            for (; p < to; p += 4) {
+                vec<T, N> v[4];
 #pragma unroll
-                        for (int j = 0; j < N; ++j) acc[j] += float(v[u][j]);
+                for (int u = 0; u < 4; ++u) v[u] = columns.load(order[std::min(p + u, to - 1)]);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (p + u < to) columns.add(acc, v[u]);
             }
         };
         for (int r = group; r < rows; r += groups) {
@@ -546,7 +570,7 @@ __device__ inline void first_of(const uint32_t* keys, uint32_t tokens, uint32_t 
 // sum stands for it: the order of a sum depends on the tokens alone.  Bound: HBM
 // (131,072 uneven tokens of 65,536 rows x 512, bf16: 56 us, 218 MB; with the sort's 32
 // us and the partial sums' 20 the gradient takes 122).
-template <class T>
+template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
     constexpr int N = kLane<T>;
     const int lane = threadIdx.x & 63, in = lane & (a.lanes - 1), begin_lane = lane - in;
@@ -557,7 +581,7 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
     const uint32_t end_row = uint32_t(std::min(begin_row + a.group_rows, uint64_t(a.rows)));
     uint32_t at, end;
     first_of(a.keys, a.tokens, uint32_t(begin_row), end_row, a.lanes, at, end);
-    const T* base = static_cast<const T*>(a.dout) + column;
+    const Columns<T, WIDE> columns(a, column);
     uint32_t row = uint32_t(begin_row);
     float acc[N] = {};
     const auto finish_before = [&](uint32_t next) {
@@ -617,7 +641,7 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 const uint32_t place = __shfl(my_place, begin_lane + int(std::min(from + u, here - 1)));
-                to[u] = load_raw(base + int64_t(place) * a.dout_stride, left, a.aligned, a.width);
+                to[u] = columns.load(place);
             }
         };
         const auto add = [&](const vec<T, N>* from, uint32_t first) {
@@ -626,8 +650,7 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
                 const uint32_t key = __shfl(my_key, begin_lane + int(std::min(first + u, here - 1)));
                 if (first + u < here) {
                     finish_before(key);
-#pragma unroll
-                    for (int j = 0; j < N; ++j) acc[j] += float(from[u][j]);
+                    columns.add(acc, from[u]);
                 }
             }
         };
@@ -643,7 +666,7 @@ __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
     finish_before(end_row);
 }
 
-template <class T, class I>
+template <class T, class I, bool WIDE>
 void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
     Device& d = *e.dev;
     const Layout l = layout(e);
@@ -658,13 +681,15 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
         const int rows = int(std::clamp<int64_t>((int64_t(e.rows) + fill - 1) / fill, 1, kShortRows));
         const int blocks = (e.rows + rows - 1) / rows;
         // tables of few rows: more workgroups by slices of the columns, of 64 bytes at least
+        const int64_t bytes = int64_t(tokens) * e.width * int64_t(sizeof(T));
+        const int wanted = bytes > 2 << 20 ? 2 * fill : fill;
         int lanes = a.lanes;
-        const auto slices = [&] { return 2 * blocks <= fill ? std::min((per_row + lanes - 1) / lanes, 65535) : 1; };
-        while (lanes > 4 && 2 * int64_t(blocks) * slices() <= fill) lanes >>= 1;
+        const auto slices = [&] { return 2 * blocks <= wanted ? std::min((per_row + lanes - 1) / lanes, 65535) : 1; };
+        while (lanes > 4 && 2 * int64_t(blocks) * slices() <= wanted) lanes >>= 1;
         if ((tokens <= kShort || blocks * slices() <= d.compute_units) &&
-            int64_t(tokens) * e.width * int64_t(sizeof(T)) <= kShortBytes * slices()) {
+            bytes <= kShortBytes * slices()) {
             a.lanes = lanes;
-            const auto kernel = tokens <= kShort ? embedding_short_k<T, I, kShort> : embedding_short_k<T, I, kLong>;
+            const auto kernel = tokens <= kShort ? embedding_short_k<T, I, kShort, WIDE> : embedding_short_k<T, I, kLong, WIDE>;
             hipLaunchKernelGGL(kernel, dim3(blocks, slices()), 256, 0, d.stream, a, ids, rows, rows > 4 ? 32 : 8);
             return;
         }
@@ -689,7 +714,7 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
     const unsigned slices = unsigned((per_row + a.lanes - 1) / a.lanes);
     const uint32_t runs = tokens / kFan;
     if (runs)
-        hipLaunchKernelGGL((embedding_partial_k<T>), dim3(unsigned((uint64_t(runs) * a.lanes + 255) / 256), slices), 256, 0,
+        hipLaunchKernelGGL((embedding_partial_k<T, WIDE>), dim3(unsigned((uint64_t(runs) * a.lanes + 255) / 256), slices), 256, 0,
                            d.stream, a, runs);
     if (runs / kFan) hipLaunchKernelGGL(embedding_partial2_k, runs / kFan, 256, 0, d.stream, a);
     // A group's lanes also look through the tokens, so narrow rows have idle ones.
@@ -697,10 +722,10 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
     // Rows a group: enough that a search serves several, few enough that common tokens
     // do not hold a wave back (131,072 uneven tokens of 65,536 rows x 512: 4 rows 126
     // us, 8 rows 133, 16 rows 143).
-    const int64_t groups_wanted = int64_t(d.compute_units) * 64 * (64 / a.lanes) / slices;
+    const int64_t groups_wanted = int64_t(d.compute_units) * 64 / slices;
     a.group_rows = int(std::clamp<int64_t>(e.rows / std::max<int64_t>(groups_wanted, 1), 1, 16));
     const uint64_t groups = (uint64_t(e.rows) + a.group_rows - 1) / a.group_rows;
-    hipLaunchKernelGGL((embedding_sum_k<T>), dim3(unsigned((groups * unsigned(a.lanes) + 255) / 256), slices), 256, 0, d.stream, a);
+    hipLaunchKernelGGL((embedding_sum_k<T, WIDE>), dim3(unsigned((groups * unsigned(a.lanes) + 255) / 256), slices), 256, 0, d.stream, a);
 }
 
 void check_rows(const cpde_rows* r, int64_t count, int width, bool output) {
@@ -803,15 +828,19 @@ int cpde_embedding_backward(cpde_embedding* embedding, const void* ids, int64_t 
         a.width = e.width;
         a.accumulate = accumulate != 0;
         a.scale = scale;
-        a.aligned = wide(dout->data, dout->stride, size) && e.width * size % 16 == 0;
         a.aligned_out = wide(dtable->data, dtable->stride, 4) && e.width * size % 16 == 0;
         flush_reduce(*e.dev);
         TraceScope trace(*e.dev, kTraceEmbedding,
                          double(tokens) * (double(size) * e.width + e.index_bytes) + 4.0 * e.rows * double(e.width));
         with_type(e.dtype, [&](auto element) {
             using T = decltype(element);
-            if (e.index_bytes == 4) gradient<T>(e, static_cast<const int32_t*>(ids), uint32_t(tokens), a);
-            else gradient<T>(e, static_cast<const int64_t*>(ids), uint32_t(tokens), a);
+            const auto run = [&](auto wide) {
+                constexpr bool WIDE = decltype(wide)::value;
+                if (e.index_bytes == 4) gradient<T, int32_t, WIDE>(e, static_cast<const int32_t*>(ids), uint32_t(tokens), a);
+                else gradient<T, int64_t, WIDE>(e, static_cast<const int64_t*>(ids), uint32_t(tokens), a);
+            };
+            if (e.width >= kLane<T>) run(std::true_type{});
+            else run(std::false_type{});
         });
         HIP_CHECK(hipGetLastError());
     });
