@@ -4,9 +4,16 @@
 namespace cpde {
 namespace {
 
-constexpr int kShort = 8192;         // tokens up to which every workgroup looks for its rows' tokens itself
-constexpr int kLong = 16384;         // the same where they are few workgroups
-constexpr int64_t kShortBytes = 4 << 20;  // and their rows' bytes in a workgroup's columns: one row may have all of them
+// Tokens up to which every workgroup looks for its rows' tokens itself (8,000 uneven ones
+// of 1,000 rows x 32: 20 us, 51 sorted first), and up to which it does where there are no
+// more workgroups than CUs, as a longer list leaves room for fewer (16,000 of 200 rows x
+// 32: 38 us, 43 sorted; 16,384 of 20 rows x 200: 35 and 49; lists of 16,384 for all,
+// 2,187 of 1,000 rows x 128: 15 us, 11 with lists of 8,192 then).
+constexpr int kShort = 8192, kLong = 16384;
+// And their rows' bytes in a workgroup's columns, as one row may have all of them (in 4
+// MB, not in 2: 4,096 tokens of 3,000 rows x 512 15 us, 33 sorted; of 1,000 x 1,023 29
+// and 41; but of 20,000 x 1,024 55 and 52).
+constexpr int64_t kShortBytes = 4 << 20;
 constexpr int kShortRows = 256;      // table rows of such a workgroup, at most
 constexpr int kDigitBits = 10;       // at most, of one pass of the sort
 constexpr int kSortTokens = 1024;    // per workgroup of such a pass
@@ -290,8 +297,10 @@ __device__ inline void load_sum(float* v, const float* p, int left, int width) {
 // of any alignment; a row's last ones are the last of its last 16 bytes, moved down when
 // they are added (a move behind the load would wait for it).  Rows shorter than that
 // are read value by value.  Lanes past the width read the row's last bytes and are not
-// used.  (4,000 tokens of 400 rows x 1,023 in 16 bits: 39 us; value by value 89.)
-// The form is a template's, as a branch between two loads waits for the first.
+// used.
+// The form is a template's, as a branch between two loads waits for the first (4,000
+// tokens of 400 rows x 1,023 in 16 bits 26 us, 52 with branches; 131,072 of 65,536 x 512
+// 116 and 125).
 template <class T, bool WIDE>
 struct Columns {
     static constexpr int N = kLane<T>;
@@ -568,8 +577,9 @@ __device__ inline void first_of(const uint32_t* keys, uint32_t tokens, uint32_t 
 // under way while one is added, whatever rows of the table they belong to.  Where a
 // whole run of kFan tokens, or of kFan such runs, belongs to one row, its partial
 // sum stands for it: the order of a sum depends on the tokens alone.  Bound: HBM
-// (131,072 uneven tokens of 65,536 rows x 512, bf16: 56 us, 218 MB; with the sort's 32
-// us and the partial sums' 20 the gradient takes 122).
+// (131,072 uneven tokens of 65,536 rows x 512, bf16: 54 us, 218 MB, where
+// calls repeat on the same inputs; the sort's 33 us and the partial sums' 17 come before;
+// 116 the whole on changing inputs).
 template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
     constexpr int N = kLane<T>;
@@ -680,7 +690,10 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
         const int fill = 4 * d.compute_units;  // workgroups
         const int rows = int(std::clamp<int64_t>((int64_t(e.rows) + fill - 1) / fill, 1, kShortRows));
         const int blocks = (e.rows + rows - 1) / rows;
-        // tables of few rows: more workgroups by slices of the columns, of 64 bytes at least
+        // Tables of few rows: more workgroups by slices of the columns, of 64 bytes at
+        // least; twice as many where the rows of common tokens are what takes the time
+        // (4,000 tokens of 400 rows x 1,023: 26 us, 31 with `fill` ones; 2,187 of 1,000 x 128,
+        // 1 MB: 7.1, 11.9 with twice as many).
         const int64_t bytes = int64_t(tokens) * e.width * int64_t(sizeof(T));
         const int wanted = bytes > 2 << 20 ? 2 * fill : fill;
         int lanes = a.lanes;
@@ -690,6 +703,8 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
             bytes <= kShortBytes * slices()) {
             a.lanes = lanes;
             const auto kernel = tokens <= kShort ? embedding_short_k<T, I, kShort, WIDE> : embedding_short_k<T, I, kLong, WIDE>;
+            // (few rows a workgroup leave groups of lanes idle, so shorter ones are shared: 242
+            // tokens of 11 rows x 344 5.3 us, 6.9 where rows of up to 32 tokens are not)
             hipLaunchKernelGGL(kernel, dim3(blocks, slices()), 256, 0, d.stream, a, ids, rows, rows > 4 ? 32 : 8);
             return;
         }
@@ -717,11 +732,12 @@ void gradient(const Embedding& e, const I* ids, uint32_t tokens, SumArgs a) {
         hipLaunchKernelGGL((embedding_partial_k<T, WIDE>), dim3(unsigned((uint64_t(runs) * a.lanes + 255) / 256), slices), 256, 0,
                            d.stream, a, runs);
     if (runs / kFan) hipLaunchKernelGGL(embedding_partial2_k, runs / kFan, 256, 0, d.stream, a);
-    // A group's lanes also look through the tokens, so narrow rows have idle ones.
+    // A group's lanes also look through the tokens, so narrow rows have idle ones (60,000
+    // tokens of 20 rows x 8: 59 us with 16 lanes, 64 with 8; 30,000 of 64 x 32 72 and 87).
     a.lanes = std::max(a.lanes, 16);
     // Rows a group: enough that a search serves several, few enough that common tokens
-    // do not hold a wave back (131,072 uneven tokens of 65,536 rows x 512: 4 rows 126
-    // us, 8 rows 133, 16 rows 143).
+    // do not hold a wave back (131,072 uneven tokens of 65,536 rows x 512: 4 rows 116 us, 2
+    // rows 127, 8 rows 129).
     const int64_t groups_wanted = int64_t(d.compute_units) * 64 / slices;
     a.group_rows = int(std::clamp<int64_t>(e.rows / std::max<int64_t>(groups_wanted, 1), 1, 16));
     const uint64_t groups = (uint64_t(e.rows) + a.group_rows - 1) / a.group_rows;
