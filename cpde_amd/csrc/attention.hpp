@@ -239,11 +239,13 @@ struct WaveLoader {
             offset[i] = chunk < chunks ? uint32_t(row * uint32_t(stride)) + (chunk << 4) : kNone;
         }
     }
-    // Columns past the head's width: zeros, which direct loads leave alone.
+    // Columns past the head's width: zeros.  Only the chunks that direct loads leave
+    // alone are written, as nothing orders a wave's stores to LDS and its loads into it.
     __device__ void clear(char* tile, int lane) const {
         if (direct && chunks < L::kChunks)
             for (int slot = lane; slot < ROWS * L::kChunks; slot += 64)
-                *reinterpret_cast<u32x4*>(tile + slot * 16) = u32x4{0, 0, 0, 0};
+                if (((slot % L::kChunks) ^ L::turn(slot / L::kChunks)) >= chunks)
+                    *reinterpret_cast<u32x4*>(tile + slot * 16) = u32x4{0, 0, 0, 0};
     }
     // The loads have arrived after arrived().
     __device__ __attribute__((always_inline)) void load(char* tile, const char* base, int valid, int lane) const {
