@@ -10,6 +10,7 @@ with dropout and added onto what it read for.  The linear layers between are tor
 a device opened on torch's stream keeps both sides' work in order.
 """
 import argparse
+import functools
 import math
 import sys
 from pathlib import Path
@@ -20,6 +21,19 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 from cpde_amd import hip  # noqa: E402
 
 MODES, LEVELS, DIFFUSIVITY = 8, 16, 0.05
+
+
+def once(backward):
+    """Gradients come from kernels that autograd does not see into: asked for with
+    create_graph=True, whose second derivatives would silently lack their share (torch's
+    once_differentiable lets that pass where the incoming gradient is a constant), they
+    are refused."""
+    @functools.wraps(backward)
+    def checked(ctx, *grads):
+        if torch.is_grad_enabled():
+            raise RuntimeError('the operators on sequences have first derivatives only (create_graph=True)')
+        return backward(ctx, *grads)
+    return checked
 
 
 class Lookup(torch.autograd.Function):
@@ -34,6 +48,7 @@ class Lookup(torch.autograd.Function):
         return out.view(*ids.shape, -1)
 
     @staticmethod
+    @once
     def backward(ctx, dout):
         ids, = ctx.saved_tensors
         dout = dout.reshape(ids.numel(), -1).contiguous()
@@ -55,6 +70,7 @@ class Attend(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
         dout = dout.contiguous()
@@ -77,6 +93,7 @@ class Dropout(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once
     def backward(ctx, dy):
         device, probability, seed, offset = ctx.args
         dy = dy.contiguous()
