@@ -26,31 +26,78 @@ class GradientStats(ctypes.Structure):
                 ('nonfinite_count', ctypes.c_uint64), ('first_nonfinite', ctypes.c_int32), ('pad_', ctypes.c_int32)]
 
 
+_type_names = {}
+
+
+def _type_name(dtype):
+    name = _type_names.get(dtype)
+    if name is None:
+        name = _type_names[dtype] = str(dtype).rpartition('.')[2]
+    return name
+
+
+def _held(tensor):
+    """(element type, GPU, sizes...) of a tensor."""
+    if tensor.device.type == 'cpu':
+        raise ValueError('the tensor is not on a GPU')
+    return (_type_name(tensor.dtype), tensor.get_device(), *tensor.shape)
+
+
+def _holds(name, view, want):
+    """Refuses the view of a tensor of another type or GPU than `want`, or of less than its sizes."""
+    held = view.held if view is not None else None
+    if held != want and held is not None:  # (None: of an address)
+        if held[:2] != want[:2]:
+            raise ValueError(f'{name} is a tensor of {held[0]} on GPU {held[1]}, not of {want[0]} on GPU {want[1]}')
+        if any(h < w for h, w in zip(held[2:], want[2:])):
+            raise ValueError(f'{name} has the sizes {held[2:]}, less than {want[2:]}')
+
+
+def _list_holds(name, a, kind, gpu, count):
+    """The same of a list of `count` elements: a tensor, a Buffer by its bytes, or an address."""
+    dtype = getattr(a, 'dtype', None)
+    if dtype is None:
+        if isinstance(a, Buffer) and a.nbytes < count * (8 if kind == 'int64' else 4):
+            raise ValueError(f'{name} has {a.nbytes} bytes, not {count} of {kind}')
+    elif _type_name(dtype) != kind or a.get_device() != gpu:
+        raise ValueError(f'{name} is a tensor of {_type_name(dtype)} on {a.device}, not of {kind} on GPU {gpu}')
+    elif a.numel() < count or not a.is_contiguous():
+        raise ValueError(f'{name} is not {count} elements in a row')
+
+
 class Heads(ctypes.Structure):
     """cpde_heads: a device tensor [batch][token][head][head_dim] by its element
-    strides, the last axis contiguous."""
+    strides, the last axis contiguous.  A view made by `of` keeps the tensor's type and
+    sizes, which calls check."""
     _fields_ = [('data', ctypes.c_void_p), ('batch', ctypes.c_int64), ('token', ctypes.c_int64),
                 ('head', ctypes.c_int64)]
+    held = None
 
     @classmethod
     def of(cls, tensor):
-        """The view of a tensor with data_ptr() and stride() (torch's), which the caller keeps."""
+        """The view of a tensor on a GPU (torch's), which the caller keeps."""
         batch, token, head, last = tensor.stride()
         if last != 1 and tensor.shape[-1] > 1:
             raise ValueError('the last axis is not contiguous')
-        return cls(tensor.data_ptr(), batch, token, head)
+        view = cls(tensor.data_ptr(), batch, token, head)
+        view.held = _held(tensor)
+        return view
 
 
 class Rows(ctypes.Structure):
-    """cpde_rows: a device matrix by its row stride in elements, columns contiguous."""
+    """cpde_rows: a device matrix by its row stride in elements, columns contiguous.  A
+    view made by `of` keeps the tensor's type and sizes, which calls check."""
     _fields_ = [('data', ctypes.c_void_p), ('stride', ctypes.c_int64)]
+    held = None
 
     @classmethod
     def of(cls, tensor):
         stride, last = tensor.stride()
         if last != 1 and tensor.shape[-1] > 1:
             raise ValueError('the last axis is not contiguous')
-        return cls(tensor.data_ptr(), stride)
+        view = cls(tensor.data_ptr(), stride)
+        view.held = _held(tensor)
+        return view
 
 
 class AttentionShape(ctypes.Structure):
@@ -74,6 +121,7 @@ heads_p = ctypes.POINTER(Heads)
 rows_p = ctypes.POINTER(Rows)
 
 F32, F16, BF16 = 0, 1, 2    # element types of the operators on sequences
+_element = ('float32', 'float16', 'bfloat16')
 
 SIGNATURES = {
     'cpde_last_error': (ctypes.c_char_p, []),
@@ -241,7 +289,7 @@ class Device:
             check(load().cpde_device_open(ordinal, ctypes.byref(h)))
         else:
             check(load().cpde_device_open_on(ordinal, stream, ctypes.byref(h)))
-        self.handle = h
+        self.handle, self.ordinal = h, ordinal
 
     def info(self):
         name = ctypes.create_string_buffer(256)
@@ -295,6 +343,14 @@ class Device:
     def dropout(self, dtype, rows, columns, x, y, probability, seed, offset=0, residual=None):
         """y = dropout(x) (+ residual), Rows of one type; the gradient is the same
         call on y's gradient with the same probability, seed and offset."""
+        if 0 <= dtype < len(_element):
+            want = (_element[dtype], self.ordinal, rows, columns)
+            if x and x.held != want:
+                _holds('x', x, want)
+            if y and y.held != want:
+                _holds('y', y, want)
+            if residual and residual.held != want:
+                _holds('residual', residual, want)
         check(load().cpde_dropout(self.handle, dtype, rows, columns, x, residual, y, probability, seed, offset))
 
     def capture_begin(self):
@@ -513,12 +569,32 @@ class Attention:
         h = vp()
         check(load().cpde_attention_create(device.handle, ctypes.byref(shape), ctypes.byref(h)))
         self.handle = h
+        self.query_side = (_element[dtype], device.ordinal, batch, query_tokens, heads, head_dim)
+        self.key_side = (_element[dtype], device.ordinal, batch, key_tokens, kv_heads, head_dim)
+        self.batch, self.rows = batch, batch * heads * query_tokens
+
+    def _check(self, queries, keys, lse, query_lengths, key_lengths):
+        """Tensors on the queries' and the keys' side, by name, and lists."""
+        for name, view in queries.items():
+            _holds(name, view, self.query_side)
+        for name, view in keys.items():
+            _holds(name, view, self.key_side)
+        gpu = self.query_side[1]
+        if lse is not None:
+            _list_holds('lse', lse, 'float32', gpu, self.rows)
+        if query_lengths is not None:
+            _list_holds('query_lengths', query_lengths, 'int32', gpu, self.batch)
+        if key_lengths is not None:
+            _list_holds('key_lengths', key_lengths, 'int32', gpu, self.batch)
 
     def forward(self, q, k, v, out, lse=None, query_lengths=None, key_lengths=None):
+        self._check({'q': q, 'out': out}, {'k': k, 'v': v}, lse, query_lengths, key_lengths)
         check(load().cpde_attention_forward(self.handle, q, k, v, out, _address(lse), _address(query_lengths),
                                             _address(key_lengths)))
 
     def backward(self, q, k, v, out, lse, dout, dq, dk, dv, query_lengths=None, key_lengths=None):
+        self._check({'q': q, 'out': out, 'dout': dout, 'dq': dq}, {'k': k, 'v': v, 'dk': dk, 'dv': dv}, lse, query_lengths,
+                    key_lengths)
         check(load().cpde_attention_backward(self.handle, q, k, v, out, _address(lse), dout, dq, dk, dv,
                                              _address(query_lengths), _address(key_lengths)))
 
@@ -537,11 +613,24 @@ class Embedding:
         h = vp()
         check(load().cpde_embedding_create(device.handle, dtype, rows, width, tokens, index_bytes, ctypes.byref(h)))
         self.handle = h
+        self.element, self.rows, self.width, self.tokens = _element[dtype], rows, width, tokens
+        self.index = 'int64' if index_bytes == 8 else 'int32'
+
+    def _check(self, ids, tokens, names, table, table_type, rows):
+        if tokens > self.tokens:
+            return  # (the library refuses it)
+        gpu = self.device.ordinal
+        if ids is not None:
+            _list_holds('ids', ids, self.index, gpu, tokens)
+        _holds(names[0], table, (table_type, gpu, self.rows, self.width))
+        _holds(names[1], rows, (self.element, gpu, tokens, self.width))
 
     def forward(self, ids, tokens, table, out, scale=1.0):
+        self._check(ids, tokens, ('table', 'out'), table, self.element, out)
         check(load().cpde_embedding_forward(self.handle, _address(ids), tokens, table, scale, out))
 
     def backward(self, ids, tokens, dout, dtable, scale=1.0, accumulate=False):
+        self._check(ids, tokens, ('dtable', 'dout'), dtable, 'float32', dout)
         check(load().cpde_embedding_backward(self.handle, _address(ids), tokens, dout, scale, dtable, int(accumulate)))
 
     def destroy(self):
