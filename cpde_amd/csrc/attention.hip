@@ -180,6 +180,7 @@ __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(Att
                 store_column(a.part + at * a.dim, out[d], 1.f, d, half, a.dim, a.dim % 4 == 0);
         return;
     }
+    if (sum == 0) clear(out);
     const float by = sum == 0 ? 0.f : 1.f / sum;
     T* to = head_row<T>(a.out, b, query, head);
 #pragma unroll
@@ -825,6 +826,10 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
     }
     const int end = fresh(lane), last_key = wave_first + (end & 31), last_half = end >> 5;
     if (last_key >= a.keys) return;
+    if (!seen(band, last_key)) {
+        clear(dk);
+        clear(dv);
+    }
     if (a.key_splits > 1) {
         // [which][split][pair][key][dim]
         const int64_t at = (int64_t(split) * a.pairs + pair) * a.keys + last_key;
@@ -920,6 +925,7 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
         step(t, lds[now][0], lds[now][1], lds[next][0], lds[next][1]);
     }
     if (row >= rows) return;
+    if (lo >= hi) clear(dq);
     if (a.splits > 1) {
         const int64_t at = (int64_t(split) * a.pairs + pair) * rows + row;
 #pragma unroll
@@ -995,6 +1001,10 @@ __device__ __attribute__((always_inline)) inline void few_keys_gradient(const At
     }
     float* const places[4] = {reinterpret_cast<float*>(shared.tiles[0]), reinterpret_cast<float*>(shared.tiles[1]),
                               reinterpret_cast<float*>(shared.tiles[2]), reinterpret_cast<float*>(shared.tiles[3])};
+    if (!seen(band, key)) {
+        clear(dk);
+        clear(dv);
+    }
     const int rows = min(kWaveRows, a.keys - first_key);
     join_waves<DP>(places, dk, wave, lane, rows, a.dim, [&](int r, int d, float x) {
         head_row<T>(a.dk, b, first_key + r, kv)[d] = T(x * a.scale);
@@ -1018,7 +1028,7 @@ __device__ __attribute__((always_inline)) inline void few_rows_gradient(const At
     const bool any = top_query < band.ql;
     const int last = min(last_query, band.ql - 1);
     const int from = any ? band.key_lo(top_query) : 0, to = any ? band.key_hi(last) : 0;
-    const int full_lo = any ? band.key_lo(last) : 0, full_hi = any ? band.key_hi(top_query) : 0;
+    const int full_lo = any ? band.key_lo(last) : 0, full_hi = any && last_query < band.ql ? band.key_hi(top_query) : 0;
 
     Frag<T> q[kSteps], dout[kSteps];
     load_fragments<T, DP>(q, head_row<const T>(a.q, b, query, head), a.dim, half, live, a.wide_in);
@@ -1042,6 +1052,7 @@ __device__ __attribute__((always_inline)) inline void few_rows_gradient(const At
         query_tile<T, DP>(a, dq, q, dout, tile, tile + kHalf, 0, first, lo, hi, first < full_lo || first + 32 > full_hi, lse,
                           delta, lane);
     }
+    if (lo >= hi) clear(dq);
     float* const places[4] = {reinterpret_cast<float*>(shared.tiles[0]), reinterpret_cast<float*>(shared.tiles[1]),
                               reinterpret_cast<float*>(shared.tiles[2]), reinterpret_cast<float*>(shared.tiles[3])};
     join_waves<DP>(places, dq, wave, lane, min(kWaveRows, rows - first_row), a.dim, [&](int r, int d, float x) {

@@ -326,6 +326,18 @@ __device__ inline void store_column(T* row, const Acc& c, float by, int block, i
     }
 }
 
+// Nothing in a lane's column: of a row or key without a part in the call, whose place in
+// the products a NaN or infinity of the others' may have reached (0 x NaN).
+template <int N>
+__device__ inline void clear(Acc (&c)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = Acc{};
+}
+// Whether any query sees a key.
+__device__ inline bool seen(const Band& band, int key) {
+    return key < band.kl && band.query_lo(key) < band.query_hi(key);
+}
+
 // The same over the two halves of a wave: lane l and lane l ^ 32 hold one column.
 __device__ inline float halves_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
