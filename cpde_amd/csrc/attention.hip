@@ -585,12 +585,13 @@ __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
 
 // ---- gradient ---------------------------------------------------------------------------
 // dout.out of every query row, and its lse in the scores' units (over the scale);
-// sixteen lanes a row.  Bound: HBM (2 x 4096 x 16 rows of 128, bf16: 67 MB in 16.6 us).
+// sixteen lanes a row, rows from `first` on.  Bound: HBM (2 x 4096 x 16 rows of 128, bf16:
+// 67 MB in 16.6 us).
 template <class T>
-__global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a) {
+__global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a, int64_t first) {
     const int heads = a.kv_heads * a.group;
     const int64_t count = int64_t(a.pairs / a.kv_heads) * a.queries * heads;
-    const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) / 16;
+    const int64_t i = first + (blockIdx.x * 256u + threadIdx.x) / 16;
     const int in = threadIdx.x & 15;
     const int64_t item = min(i, count - 1);  // (all lanes take part in the sum)
     const int head = int(item % heads), query = int(item / heads % a.queries), b = int(item / heads / a.queries);
@@ -1244,9 +1245,13 @@ AttentionArgs arguments(const Attention& p, const int* query_lengths, const int*
     return a;
 }
 
+int join_teams(int splits) {
+    int teams = 1;
+    while (teams < 8 && 2 * teams < splits) teams *= 2;
+    return teams;
+}
 Join join_of(const float* part, const HeadView& out, int pairs, int splits, int rows, int group, float scale) {
-    Join j{part, out, splits, rows, group, 0, 1, scale};
-    while (j.teams < 8 && 2 * j.teams < splits) j.teams *= 2;
+    Join j{part, out, splits, rows, group, 0, join_teams(splits), scale};
     j.blocks = splits > 1 ? ceil_div(int64_t(pairs) * rows, 8 / j.teams) : 0;
     return j;
 }
@@ -1331,13 +1336,16 @@ int cpde_attention_create(cpde_device* dev, const cpde_attention_shape* shape, c
         cut_launches(*p);
         const Cut& c = p->cut;
         const int64_t pairs = int64_t(s.batch) * s.kv_heads;
-        // workgroups of the largest launch: of rows, of keys, of joins
-        const int64_t rows = (c.few || c.few_gradient ? ceil_div(c.rows, kWaveRows) : c.row_tiles) * int64_t(std::max(c.forward, c.query));
-        const int64_t keys = (c.few_gradient ? ceil_div(s.key_tokens, kWaveRows) : c.key_tiles) * int64_t(c.key);
-        const int64_t joins = (c.forward > 1 || c.query > 1 ? int64_t(c.rows) : 0) + (c.key > 1 ? 2 * int64_t(s.key_tokens) : 0);
-        require(pairs <= kMost && pairs * std::max(rows + keys, joins) <= kMost &&
-                    int64_t(s.batch) * s.heads * s.query_tokens <= kMost * 8,
-                "too many workgroups: split the batch");
+        // lanes of the largest launch (the runtime takes fewer than 2^32): forward, gradient, joins
+        const int64_t forward = (c.step ? 1 : c.few ? ceil_div(c.rows, kWaveRows) : c.row_tiles) * int64_t(c.forward) *
+                                (c.step && c.brief ? 1024 : 256);
+        const int64_t gradient = c.few_gradient ? ceil_div(s.key_tokens, kWaveRows) + int64_t(ceil_div(c.rows, kWaveRows))
+                                                : c.key_tiles * int64_t(c.key) + c.row_tiles * int64_t(c.query);
+        const auto joined = [](int splits, int64_t rows) { return splits > 1 ? rows * 32 * join_teams(splits) : 0; };
+        const int64_t joins = std::max(joined(c.forward, c.rows), joined(c.query, c.rows) + 2 * joined(c.key, s.key_tokens));
+        const int64_t most = std::max({forward, s.backward ? gradient * 256 : 0, joins});
+        // (with room for the last workgroup of each join)
+        require(pairs <= kMost && (!pairs || most <= ((int64_t(1) << 32) - 1024) / pairs), "too many workgroups: split the batch");
         HIP_CHECK(hipMalloc(&p->work, std::max<size_t>(c.floats, 64) * sizeof(float)));
         *out = p.release();
     });
@@ -1439,8 +1447,10 @@ int cpde_attention_backward(cpde_attention* attention, const cpde_heads* q, cons
         with_type(s.dtype, [&](auto element) {
             using T = decltype(element);
             const int64_t count = int64_t(s.batch) * s.heads * s.query_tokens;
-            if (count)
-                hipLaunchKernelGGL((attention_delta_k<T>), unsigned((count * 16 + 255) / 256), 256, 0, d.stream, a);
+            constexpr int64_t kAtOnce = int64_t(1) << 27;  // (a launch takes fewer than 2^32 lanes)
+            for (int64_t first = 0; first < count; first += kAtOnce)
+                hipLaunchKernelGGL((attention_delta_k<T>), unsigned((std::min(count - first, kAtOnce) + 15) / 16), 256, 0,
+                                   d.stream, a, first);
             HIP_CHECK(hipGetLastError());
             a.tiles = c.row_tiles;
             a.splits = c.query;
