@@ -23,6 +23,7 @@ struct Attention {
     Device* dev = nullptr;
     cpde_attention_shape shape{};
     Cut cut;
+    double seen = 0;  // visible pairs at the full lengths, over the batch and the query heads
     float* work = nullptr;
 };
 
@@ -1195,6 +1196,20 @@ void cut_launches(Attention& p) {
     c.floats = c.stats + c.part + c.part_stats + c.key_part;
 }
 
+// Pairs of a query and a key that it sees, at the full lengths.
+double seen_pairs(const cpde_attention_shape& s) {
+    const int64_t n = s.query_tokens, m = s.key_tokens;
+    // x clamped to 0..m, summed over n values from `first` on
+    const auto clamped = [&](int64_t first) {
+        const auto below = [&](int64_t end) {
+            const int64_t ramp = std::clamp<int64_t>(end, 0, m);
+            return double(ramp) * double(ramp - 1) / 2 + double(std::max<int64_t>(end, 0) - ramp) * double(m);
+        };
+        return below(first + n) - below(first);
+    };
+    return (s.right < 0 ? double(n) * double(m) : clamped(m - n + s.right + 1)) - (s.left < 0 ? 0 : clamped(m - n - s.left));
+}
+
 HeadView view(const cpde_heads& h) { return {static_cast<char*>(h.data), h.batch, h.token, h.head}; }
 
 // Checks a tensor's address and strides; returns whether it takes 16-byte accesses.
@@ -1333,6 +1348,7 @@ int cpde_attention_create(cpde_device* dev, const cpde_attention_shape* shape, c
         auto p = std::make_unique<cpde_attention_s>();
         p->dev = dev;
         p->shape = s;
+        p->seen = double(s.batch) * s.heads * seen_pairs(s);
         cut_launches(*p);
         const Cut& c = p->cut;
         const int64_t pairs = int64_t(s.batch) * s.kv_heads;
@@ -1385,7 +1401,7 @@ int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const
         a.tiles = c.row_tiles;
         Device& d = *p.dev;
         flush_reduce(d);
-        TraceScope trace(d, kTraceAttention, 4.0 * s.batch * s.heads * double(s.query_tokens) * s.key_tokens * s.head_dim);
+        TraceScope trace(d, kTraceAttention, 4.0 * p.seen * s.head_dim);
         with_type(s.dtype, [&](auto element) {
             using T = decltype(element);
             if (c.step) step<T>(d, a, c.rows, c.brief);
@@ -1442,8 +1458,7 @@ int cpde_attention_backward(cpde_attention* attention, const cpde_heads* q, cons
         if (!a.pairs) return;
         Device& d = *p.dev;
         flush_reduce(d);
-        TraceScope trace(d, kTraceAttentionGradient,
-                         10.0 * s.batch * s.heads * double(s.query_tokens) * s.key_tokens * s.head_dim);
+        TraceScope trace(d, kTraceAttentionGradient, 10.0 * p.seen * s.head_dim);
         with_type(s.dtype, [&](auto element) {
             using T = decltype(element);
             const int64_t count = int64_t(s.batch) * s.heads * s.query_tokens;

@@ -502,7 +502,9 @@ int cpde_replay_destroy(cpde_replay* replay);
  * device stream and accounted to its kernel class.  Enabling (or disabling)
  * clears the totals.  cpde_trace_read synchronizes and returns a class's
  * launch count, summed device milliseconds and summed algorithmic work
- * (bytes for HBM-bound classes, flops for the matrix-core classes). */
+ * (bytes for HBM-bound classes, flops for the matrix-core classes; attention's
+ * two products, and its gradient's five, are counted over the pairs that the
+ * band shows at the plan's full lengths, as lengths lie on the device). */
 int cpde_trace_enable(cpde_device* dev, int on);
 int cpde_trace_read(cpde_device* dev, int kind, uint64_t* launches, double* total_ms, double* work);
 const char* cpde_trace_name(int kind);
