@@ -607,7 +607,8 @@ __global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a, int64_
     if (in == 0 && i < count) {
         const int64_t at = (int64_t(b) * heads + head) * a.queries + query;
         const float lse = live ? a.lse[at] : -INFINITY;
-        a.row_lse[at] = lse == -INFINITY ? INFINITY : lse / a.scale;  // (no key: every probability is 0)
+        // (no key: every probability is 0)
+        a.row_lse[at] = lse == -INFINITY ? INFINITY : (lse - kLift<T> * kLn2) / a.scale;
         a.row_delta[at] = dot;
     }
 }
@@ -626,8 +627,9 @@ __device__ __attribute__((always_inline)) inline void load_statistics(const Atte
 // queries of ONE key, and its probabilities and score gradients are, in place, the
 // fragments that multiply the transposed dout and queries into dv and dk.
 template <class T, int DP>
-__device__ __attribute__((always_inline)) inline void key_tile(const AttentionArgs& a, const Band& band, Acc* dk, Acc* dv,
-                                                               const Frag<T>* k, const Frag<T>* v, const char* queries,
+__device__ __attribute__((always_inline)) inline void key_tile(const AttentionArgs& a, const Band& band, Fit<T>& fit,
+                                                               Acc (&dk)[DP / 32], Acc* dv, const Frag<T>* k,
+                                                               const Frag<T>* v, const char* queries,
                                                                const char* douts, const float* statistics, int first,
                                                                int key, bool hidden, int lane) {
     using L = Tile<T, DP>;
@@ -676,6 +678,7 @@ __device__ __attribute__((always_inline)) inline void key_tile(const AttentionAr
         s[i] = p;
         dp[i] = ds;
     }
+    fit(dp, dk);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const Frag<T> p = as_fragment<T>(s, i), ds = as_fragment<T>(dp, i);
@@ -690,7 +693,8 @@ __device__ __attribute__((always_inline)) inline void key_tile(const AttentionAr
 // One tile of 32 keys of the gradient of a wave's 32 query rows: the forward's
 // shape, with queries and dout in registers.
 template <class T, int DP>
-__device__ __attribute__((always_inline)) inline void query_tile(const AttentionArgs& a, Acc* dq, const Frag<T>* q,
+__device__ __attribute__((always_inline)) inline void query_tile(const AttentionArgs& a, Fit<T>& fit, Acc (&dq)[DP / 32],
+                                                                 const Frag<T>* q,
                                                                  const Frag<T>* dout, const char* keys,
                                                                  const char* values, int at, int first, int lo, int hi,
                                                                  bool hidden, float lse, float delta, int lane) {
@@ -708,6 +712,7 @@ __device__ __attribute__((always_inline)) inline void query_tile(const Attention
         if (hidden) ds = key >= lo && key < hi ? ds : 0.f;
         s[i] = ds;
     }
+    fit(s, dq);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const Frag<T> ds = as_fragment<T>(s, i);
@@ -716,14 +721,15 @@ __device__ __attribute__((always_inline)) inline void query_tile(const Attention
     }
 }
 
-// A wave's gradient columns (32 rows of DP) into its place in LDS, and the four
+// A wave's gradient columns (32 rows of DP) times `by` into its place in LDS, and the four
 // waves' sums of it by all of them: column(row, d, value).
 template <int DP>
 constexpr int kPitch = DP + 4;  // floats of a row there
 template <int DP, class F>
-__device__ inline void join_waves(float* const (&places)[4], const Acc* c, int wave, int lane, int rows, int dim, F column) {
+__device__ inline void join_waves(float* const (&places)[4], const Acc* c, float by, int wave, int lane, int rows, int dim,
+                                  F column) {
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) store_column(places[wave] + (lane & 31) * kPitch<DP>, c[d], 1.f, d, lane >> 5, DP, true);
+    for (int d = 0; d < DP / 32; ++d) store_column(places[wave] + (lane & 31) * kPitch<DP>, c[d], by, d, lane >> 5, DP, true);
     __syncthreads();
     for (int i = threadIdx.x; i < rows * DP; i += 256) {
         const int row = i / DP, d = i % DP, at = row * kPitch<DP> + d;
@@ -801,6 +807,7 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
     };
 
     Acc dk[kBlocks] = {}, dv[kBlocks] = {};
+    Fit<T> fit;
     if (from < to) {
         for (int i = 0; i < 4; ++i) qload.clear(lds[i >> 1][i & 1]);
         if (qload.direct && a.dim < DP) __syncthreads();
@@ -817,7 +824,7 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
         if (++at == t1) at = t0;
         if (more) load(next_queries, next_douts, next_statistics);
         if (first >= wave_hi || first + kQueries <= wave_lo) return;
-        key_tile<T, DP>(a, band, dk, dv, k, v, queries, douts, statistics, first, key,
+        key_tile<T, DP>(a, band, fit, dk, dv, k, v, queries, douts, statistics, first, key,
                         first < full_lo || first + kQueries > full_hi, lane);
     };
     for (int i = from; i < to; ++i) {
@@ -828,6 +835,7 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
     }
     const int end = fresh(lane), last_key = wave_first + (end & 31), last_half = end >> 5;
     if (last_key >= a.keys) return;
+    const float off = fit.off();
     if (!seen(band, last_key)) {
         clear(dk);
         clear(dv);
@@ -838,16 +846,16 @@ __device__ __attribute__((always_inline)) inline void key_gradient(const Attenti
         const int64_t other = int64_t(a.key_splits) * a.pairs * a.keys;
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) {
-            store_column(a.key_part + at * a.dim, dk[d], 1.f, d, last_half, a.dim, a.dim % 4 == 0);
-            store_column(a.key_part + (other + at) * a.dim, dv[d], 1.f, d, last_half, a.dim, a.dim % 4 == 0);
+            store_column(a.key_part + at * a.dim, dk[d], off, d, last_half, a.dim, a.dim % 4 == 0);
+            store_column(a.key_part + (other + at) * a.dim, dv[d], fit.p_off(), d, last_half, a.dim, a.dim % 4 == 0);
         }
         return;
     }
     T *to_k = head_row<T>(a.dk, b, last_key, kv), *to_v = head_row<T>(a.dv, b, last_key, kv);
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d) {
-        store_column(to_k, dk[d], a.scale, d, last_half, a.dim, a.wide_out);
-        store_column(to_v, dv[d], 1.f, d, last_half, a.dim, a.wide_out);
+        store_column(to_k, dk[d], off * a.scale, d, last_half, a.dim, a.wide_out);
+        store_column(to_v, dv[d], fit.p_off(), d, last_half, a.dim, a.wide_out);
     }
 }
 
@@ -900,6 +908,7 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
     };
 
     Acc dq[kBlocks] = {};
+    Fit<T> fit;
     if (t0 < t1) {
         for (int i = 0; i < 4; ++i) kload.clear(lds[i >> 1][i & 1]);
         if (kload.direct && a.dim < DP) __syncthreads();
@@ -918,7 +927,7 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
         const bool hidden = first < full_lo || first + N > full_hi;
 #pragma unroll
         for (int u = 0; u < N; u += 32)
-            query_tile<T, DP>(a, dq, q, dout, keys, values, u, first + u, lo, hi, hidden, lse, delta, lane);
+            query_tile<T, DP>(a, fit, dq, q, dout, keys, values, u, first + u, lo, hi, hidden, lse, delta, lane);
     };
     for (int t = t0; t < t1; ++t) {
         const int now = (t - t0) & 1, next = now ^ 1;
@@ -928,16 +937,17 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
     }
     if (row >= rows) return;
     if (lo >= hi) clear(dq);
+    const float off = fit.off();
     if (a.splits > 1) {
         const int64_t at = (int64_t(split) * a.pairs + pair) * rows + row;
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d)
-            store_column(a.part + at * a.dim, dq[d], 1.f, d, half, a.dim, a.dim % 4 == 0);
+            store_column(a.part + at * a.dim, dq[d], off, d, half, a.dim, a.dim % 4 == 0);
         return;
     }
     T* to = head_row<T>(a.dq, b, query, head);
 #pragma unroll
-    for (int d = 0; d < kBlocks; ++d) store_column(to, dq[d], a.scale, d, half, a.dim, a.wide_out);
+    for (int d = 0; d < kBlocks; ++d) store_column(to, dq[d], off * a.scale, d, half, a.dim, a.wide_out);
 }
 
 // Both in one launch, the keys' workgroups first (four products to three): where
@@ -992,13 +1002,14 @@ __device__ __attribute__((always_inline)) inline void few_keys_gradient(const At
     qload.clear(tile, lane);
     oload.clear(tile + kHalf, lane);
     Acc dk[kBlocks] = {}, dv[kBlocks] = {};
+    Fit<T> fit;
     for (int i = wave; i < per_head * a.group; i += 4) {
         const int head = kv * a.group + i / per_head, first = (t0 + i % per_head) * kQueries, valid = band.ql - first;
         qload.load(tile, reinterpret_cast<const char*>(head_row<const T>(a.q, b, first, head)), valid, lane);
         oload.load(tile + kHalf, reinterpret_cast<const char*>(head_row<const T>(a.dout, b, first, head)), valid, lane);
         load_statistics(a, stats, (int64_t(b) * a.kv_heads * a.group + head) * a.queries + first, valid, lane);
         arrived();
-        key_tile<T, DP>(a, band, dk, dv, k, v, tile, tile + kHalf, stats, first, key,
+        key_tile<T, DP>(a, band, fit, dk, dv, k, v, tile, tile + kHalf, stats, first, key,
                         first < full_lo || first + kQueries > full_hi, lane);
     }
     float* const places[4] = {reinterpret_cast<float*>(shared.tiles[0]), reinterpret_cast<float*>(shared.tiles[1]),
@@ -1008,10 +1019,10 @@ __device__ __attribute__((always_inline)) inline void few_keys_gradient(const At
         clear(dv);
     }
     const int rows = min(kWaveRows, a.keys - first_key);
-    join_waves<DP>(places, dk, wave, lane, rows, a.dim, [&](int r, int d, float x) {
+    join_waves<DP>(places, dk, fit.off(), wave, lane, rows, a.dim, [&](int r, int d, float x) {
         head_row<T>(a.dk, b, first_key + r, kv)[d] = T(x * a.scale);
     });
-    join_waves<DP>(places, dv, wave, lane, rows, a.dim, [&](int r, int d, float x) {
+    join_waves<DP>(places, dv, fit.p_off(), wave, lane, rows, a.dim, [&](int r, int d, float x) {
         head_row<T>(a.dv, b, first_key + r, kv)[d] = T(x);
     });
 }
@@ -1046,18 +1057,19 @@ __device__ __attribute__((always_inline)) inline void few_rows_gradient(const At
     kload.clear(tile, lane);
     vload.clear(tile + kHalf, lane);
     Acc dq[kBlocks] = {};
+    Fit<T> fit;
     for (int t = from / 32 + wave; t * 32 < to; t += 4) {
         const int first = t * 32;
         kload.load(tile, kbase + int64_t(first) * kload.stride, band.kl - first, lane);
         vload.load(tile + kHalf, vbase + int64_t(first) * vload.stride, band.kl - first, lane);
         arrived();
-        query_tile<T, DP>(a, dq, q, dout, tile, tile + kHalf, 0, first, lo, hi, first < full_lo || first + 32 > full_hi, lse,
+        query_tile<T, DP>(a, fit, dq, q, dout, tile, tile + kHalf, 0, first, lo, hi, first < full_lo || first + 32 > full_hi, lse,
                           delta, lane);
     }
     if (lo >= hi) clear(dq);
     float* const places[4] = {reinterpret_cast<float*>(shared.tiles[0]), reinterpret_cast<float*>(shared.tiles[1]),
                               reinterpret_cast<float*>(shared.tiles[2]), reinterpret_cast<float*>(shared.tiles[3])};
-    join_waves<DP>(places, dq, wave, lane, min(kWaveRows, rows - first_row), a.dim, [&](int r, int d, float x) {
+    join_waves<DP>(places, dq, fit.off(), wave, lane, min(kWaveRows, rows - first_row), a.dim, [&](int r, int d, float x) {
         const int at = first_row + r;
         head_row<T>(a.dq, b, at / a.group, kv * a.group + at % a.group)[d] = T(x * a.scale);
     });

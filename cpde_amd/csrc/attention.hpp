@@ -31,7 +31,7 @@ struct AttentionArgs {
     int wide_in, wide_out;       // 16-byte loads and stores
     float *part, *part_stats;    // [split][pair][row][dim], [split][pair][row][2]
     float* key_part;             // dk, then dv: [split][pair][key][dim] each
-    float *row_lse, *row_delta;  // [batch][head][query]: lse over scale, dout.out
+    float *row_lse, *row_delta;  // [batch][head][query]: lse (less kLift) over scale, dout.out
 };
 
 // Lengths of a batch entry.
@@ -149,6 +149,10 @@ __device__ inline int fresh(int i) {
     return i;
 }
 
+// The power of two by which a gradient's probabilities are larger (Fit).
+template <class T>
+constexpr int kLift = std::is_same_v<T, _Float16> ? 14 : 0;
+
 // Brings ROWS rows of a tensor into a tile, 256 lanes.  Rows past `valid` repeat
 // the last valid one (the caller hides them): memory past the lengths is not read.
 template <class T, int DP, int ROWS>
@@ -158,6 +162,10 @@ struct TileLoader {
     // Where 256 slots are whole rows in eights, a lane's slots differ by whole rows:
     // one lane's offset and a step that is the same in every lane.
     static constexpr bool kRegular = 256 % (8 * L::kChunks) == 0;
+    // f16's gradients of 128-wide keys have no registers for addresses held ready: a
+    // spilled one, reloaded behind the loads under way, waits for them (2 x 4096 causal,
+    // 16 heads on 4, training: 893 us, 807 with addresses made anew).
+    static constexpr bool kAnew = kLift<T> != 0 && DP == 128 && ROWS == 32;
     static constexpr uint32_t kNone = ~0u;   // a column past the head's width
     uint32_t offset[kRegular ? 1 : kSteps];  // of a full tile
     int chunks;                              // that hold values
@@ -195,7 +203,7 @@ struct TileLoader {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 if (kSlots % 256 && i * 256 + wave * 64 >= kSlots) break;
-                const uint32_t at = offset[kRegular ? 0 : i];
+                const uint32_t at = kAnew ? fresh(offset[kRegular ? 0 : i]) : offset[kRegular ? 0 : i];
                 if (at != kNone) bring(i, base + (kRegular ? i * (256 / L::kChunks) * stride : 0) + at);
             }
         } else if (direct) {
@@ -347,6 +355,40 @@ __device__ inline float halves_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// Score gradients ds = p (dp - delta) of f16 tensors are rounded to f16, whose normal range
+// ends at 2^-14 and 2^16, and are about the output's gradient over the number of keys.  So
+// p, which is at most 1, comes 2^kLift times as large, and each column's ds (a key's, or a
+// query row's) times a power of two of its own, `by`: as large as can be at the start, and
+// down, with the column's sums so far, where its largest would pass 2^15, to leave that above
+// 2^11.  Roundings are relative down to 2^-25 of the largest so far, and 2^-36 of it below.
+// (bf16 and f32 need none of it.)
+template <class T>
+struct Fit {
+    float by = 0x1p100f;
+    template <int M>
+    __device__ __attribute__((always_inline)) void operator()(Acc& ds, Acc (&sum)[M]) {
+        if constexpr (kLift<T> != 0) {
+            float top = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
+            top = halves_max(top);
+            const bool grown = top * by > 0x1p15f;
+            if (__any(grown)) {
+                // 2^(11 - the exponent)
+                const float next = grown ? __uint_as_float((265 - (__float_as_uint(top) >> 23)) << 23) : by;
+                const float down = next / by;
+                by = next;
+#pragma unroll
+                for (int d = 0; d < M; ++d) sum[d] *= down;
+            }
+            ds *= by;
+        }
+    }
+    // What takes both factors, and p's alone, off again.
+    __device__ float off() const { return kLift<T> ? __builtin_ldexpf(1.f, -kLift<T>) / by : 1.f; }
+    __device__ static float p_off() { return kLift<T> ? __builtin_ldexpf(1.f, -kLift<T>) : 1.f; }
+};
 
 template <class T>
 __device__ inline T* head_row(const HeadView& v, int b, int64_t token, int head) {

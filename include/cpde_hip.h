@@ -433,8 +433,9 @@ int cpde_attention_destroy(cpde_attention* attention);
  * float (may be NULL).  query_lengths, key_lengths: int32 [batch] on the device, or
  * NULL; values outside 0..tokens count as the nearest of the two.  Keys and queries
  * at or past the lengths are not read.  A query that sees no key, or past its
- * length, gives zeros and lse = -inf.  Where matrix instructions multiply them,
- * probabilities are rounded to the tensors' type first.  A key that a query does
+ * length, gives zeros and lse = -inf.  Where matrix instructions multiply them (all
+ * calls but those of one or two query rows a key head), probabilities are rounded to the
+ * tensors' type first.  A key that a query does
  * not see has weight zero in it: finite values there leave no trace. */
 int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const cpde_heads* k, const cpde_heads* v,
                            const cpde_heads* out, float* lse, const int32_t* query_lengths,
@@ -442,7 +443,10 @@ int cpde_attention_forward(cpde_attention* attention, const cpde_heads* q, const
 /* The gradients of q, k and v from dout, with out and lse as the forward gave them
  * on the same inputs: the probabilities are recomputed.  Keys' gradients are summed
  * over the query heads that share them.  Rows at or past the lengths, queries that
- * see no key and keys that no query sees get zeros. */
+ * see no key and keys that no query sees get zeros, whatever stands in the others.
+ * With 16-bit tensors, probabilities and score gradients p (dout.v - dout.out) are
+ * rounded to their type, once each, before the products that sum them: relatively,
+ * also in f16, where powers of two keep them inside its normal range first. */
 int cpde_attention_backward(cpde_attention* attention, const cpde_heads* q, const cpde_heads* k, const cpde_heads* v,
                             const cpde_heads* out, const float* lse, const cpde_heads* dout, const cpde_heads* dq,
                             const cpde_heads* dk, const cpde_heads* dv, const int32_t* query_lengths,
