@@ -1,5 +1,6 @@
 // Attention over sets and sequences, and its gradient.
 #include <cmath>
+#include <cstdio>
 #include <initializer_list>
 
 #include "attention.hpp"
@@ -1386,6 +1387,19 @@ int cpde_attention_destroy(cpde_attention* attention) {
         ++attention->dev->layout;
         HIP_CHECK(hipFree(attention->work));
         delete attention;
+    });
+}
+
+int cpde_attention_info(cpde_attention* attention, char* text, size_t capacity) {
+    return guarded([&] {
+        require(attention && text && capacity, "null argument");
+        const Cut& c = attention->cut;
+        std::string s = std::string("forward attention_") + (c.step ? "step_k" : c.few ? "rows_k" : "forward_k") + " splits " +
+                        std::to_string(c.forward);
+        if (attention->shape.backward)
+            s += std::string(", gradient attention_") + (c.few_gradient ? "few_gradient_k" : "gradient_k") + " key splits " +
+                 std::to_string(c.key) + " query splits " + std::to_string(c.query);
+        std::snprintf(text, capacity, "%s", s.c_str());
     });
 }
 

@@ -182,6 +182,7 @@ SIGNATURES = {
     'cpde_epoch_expression': (i32, [vp, vp, vp, vp, i32, i32, i32, vp, vp, i32, i32, i32]),
     'cpde_attention_create': (i32, [vp, ctypes.POINTER(AttentionShape), ctypes.POINTER(vp)]),
     'cpde_attention_destroy': (i32, [vp]),
+    'cpde_attention_info': (i32, [vp, ctypes.c_char_p, ctypes.c_size_t]),
     'cpde_attention_forward': (i32, [vp, heads_p, heads_p, heads_p, heads_p, vp, vp, vp]),
     'cpde_attention_backward': (i32, [vp, heads_p, heads_p, heads_p, heads_p, vp, heads_p, heads_p, heads_p, heads_p,
                                       vp, vp]),
@@ -572,6 +573,12 @@ class Attention:
         self.query_side = (_element[dtype], device.ordinal, batch, query_tokens, heads, head_dim)
         self.key_side = (_element[dtype], device.ordinal, batch, key_tokens, kv_heads, head_dim)
         self.batch, self.rows = batch, batch * heads * query_tokens
+
+    def info(self):
+        """The kernels that the calls run, and over how many splits."""
+        text = ctypes.create_string_buffer(256)
+        check(load().cpde_attention_info(self.handle, text, 256))
+        return text.value.decode()
 
     def _check(self, queries, keys, lse, query_lengths, key_lengths):
         """Tensors on the queries' and the keys' side, by name, and lists."""

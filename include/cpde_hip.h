@@ -428,6 +428,10 @@ typedef struct {
 
 int cpde_attention_create(cpde_device* dev, const cpde_attention_shape* shape, cpde_attention** out);
 int cpde_attention_destroy(cpde_attention* attention);
+/* The kernels that the calls run, as chosen when the plan was made, and over how many
+ * splits of the other axis: "forward attention_rows_k splits 1" and, with a backward,
+ * ", gradient attention_gradient_k key splits 3 query splits 2". */
+int cpde_attention_info(cpde_attention* attention, char* text, size_t capacity);
 /* out_i = sum_j p_ij v_j with p_ij = exp(s_ij - lse_i) over the keys that i sees,
  * s_ij = scale q_i.k_j, lse_i = log sum_j exp(s_ij).  lse [batch][heads][query_tokens]
  * float (may be NULL).  query_lengths, key_lengths: int32 [batch] on the device, or
