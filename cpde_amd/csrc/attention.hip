@@ -49,9 +49,10 @@ constexpr int kGroups = DP * sizeof(T) <= 256 ? 2 : 1;
 // tensors' type for the second product (one rounding of each, of relative size
 // 2^-9 in bf16); their sum is of the unrounded ones.
 // A tile's keys and values go from memory to LDS without registers, one tile ahead.
-// Bound: matrix instructions, and LDS at the same rate (a wave reads a tile's 32 KB
-// for 1,024 cycles of products).  Measured: 2 x 8192 causal, 16 heads of 128, bf16:
-// 565 us, 973 TFLOP/s (a large library product on the same card: 1,144).
+// Bound: matrix instructions and LDS, each busy for 47% of the cycles (a wave reads a
+// tile's 32 KB for 1,024 cycles of products), one after the other at two waves a SIMD.
+// Measured: 2 x 8192 causal, 16 heads of 128, bf16: 561 us, 980 TFLOP/s (a large library
+// product on the same card: 1,144).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_forward_k(AttentionArgs a) {
     constexpr int N = kKeys<T>, kSub = N / 32, kBlocks = DP / 32, kSteps = DP / 16;
@@ -360,10 +361,11 @@ __global__ __launch_bounds__(64 * WAVES) void attention_step_k(AttentionArgs a) 
 // to its own part of LDS and computes on them in turn, with no barrier until their
 // outputs are joined.  For one token, or a few, on long lists eight such waves a CU
 // keep its share of memory busy (bound: HBM; 16 sequences of up to 32,768 keys, 4
-// heads of 128, bf16: 537 MB in 113 us of this kernel, 4.8 TB/s); small sets get four times the
+// heads of 128, bf16: 537 MB in 109 us of this kernel, 4.9 TB/s); small sets get four times the
 // workgroups of 128 rows, and waves that wait for different things (4 x 729 rows on
 // 729 keys, 32 wide, f32: 20.6 us, 31 with 128 rows a workgroup; bound: the float
-// instruction, 8.2 us, and the waves' own latencies).
+// instruction, 8.2 us, busy for 40% of the cycles, and the loads, which a wave waits for
+// tile by tile).
 template <class T, int DP>
 constexpr int kRowWaves = DP * sizeof(T) <= 256 ? 4 : 2;
 template <class T, int DP>
@@ -588,7 +590,7 @@ __global__ __launch_bounds__(256) void attention_join_k(JoinArgs a) {
 // ---- gradient ---------------------------------------------------------------------------
 // dout.out of every query row, and its lse in the scores' units (over the scale);
 // sixteen lanes a row, rows from `first` on.  Bound: HBM (2 x 4096 x 16 rows of 128, bf16:
-// 67 MB in 16.6 us).
+// 67 MB in 18 us).
 template <class T>
 __global__ __launch_bounds__(256) void attention_delta_k(AttentionArgs a, int64_t first) {
     const int heads = a.kv_heads * a.group;
@@ -954,9 +956,9 @@ __device__ __attribute__((always_inline)) inline void query_gradient(const Atten
 // Both in one launch, the keys' workgroups first (four products to three): where
 // either would leave the device short of workgroups the other fills it.  Score
 // gradients are rounded to the tensors' type for the products that sum them.  Bound:
-// as the forward's; at 128 columns of 16 bits a wave's keys, values and their
-// gradients leave 32 of its 256 registers.  Measured: 2 x 4096 causal, 16 heads on
-// 4, 128 wide, bf16: 560 us for seven products, 860 TFLOP/s.
+// as the forward's (busy 40% and 43%); at 128 columns of 16 bits a wave's keys, values and
+// their gradients leave 32 of its 256 registers.  Measured: 2 x 4096 causal, 16 heads on
+// 4, 128 wide, bf16: 531 us for seven products, 906 TFLOP/s.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (kGroups<T, DP>)) void attention_gradient_k(AttentionArgs a) {
     __shared__ __align__(16) union {
@@ -1089,8 +1091,8 @@ int step_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : 16; }
 
 // What a launch of `blocks` workgroups in `splits` each takes, in us: the longest
 // workgroup on a CU of its own, or all of them on the CUs they share, with their
-// starts; then the join, whose parts are written and read once.  Measured on 729 to
-// 8192 rows and keys, within about 15%.
+// starts; then the join, whose parts are written and read once.  Its constants were set
+// on calls of 729 to 8192 rows and keys.
 struct Work {
     int64_t blocks = 0;               // before splitting
     double longest = 0, mean = 0;     // steps of 32 keys (or queries) of a workgroup

@@ -577,9 +577,8 @@ __device__ inline void first_of(const uint32_t* keys, uint32_t tokens, uint32_t 
 // under way while one is added, whatever rows of the table they belong to.  Where a
 // whole run of kFan tokens, or of kFan such runs, belongs to one row, its partial
 // sum stands for it: the order of a sum depends on the tokens alone.  Bound: HBM
-// (131,072 uneven tokens of 65,536 rows x 512, bf16: 54 us, 218 MB, where
-// calls repeat on the same inputs; the sort's 33 us and the partial sums' 17 come before;
-// 116 the whole on changing inputs).
+// (131,072 uneven tokens of 65,536 rows x 512, bf16: 69 us, 114 MB read and 165 written;
+// the sort's 33 us and the partial sums' 20 come before; 115 the whole).
 template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void embedding_sum_k(SumArgs a) {
     constexpr int N = kLane<T>;

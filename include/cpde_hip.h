@@ -471,8 +471,8 @@ int cpde_embedding_backward(cpde_embedding* embedding, const void* ids, int64_t 
                             float scale, const cpde_rows* dtable, int accumulate);
 
 /* y = x / (1 - probability) where an element is kept, 0 where it is dropped, plus
- * residual (may be NULL); the gradient of x is the same call on y's gradient
- * without a residual.  Element e = row * columns + column takes word e % 4 of the
+ * residual (may be NULL), with the probability rounded to a multiple of 2^-32; the
+ * gradient of x is the same call on y's gradient without a residual.  Element e = row * columns + column takes word e % 4 of the
  * generator Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random
  * numbers: as easy as 1, 2, 3", 2011) at counter offset + e / 4 with key `seed`, and
  * is kept where the word is at least round(probability * 2^32): nothing of the
