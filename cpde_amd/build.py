@@ -53,7 +53,7 @@ def build_lib():
     embedded.write_text('namespace cpde {\nextern const char* const kFusedSource;\n'
                         'const char* const kFusedSource = R"CPDE_SRC(' + text + ')CPDE_SRC";\n}\n')
     sources = [CSRC / name for name in ('attention.hip', 'kernels.hip', 'api.hip', 'embedding.hip', 'dropout.hip',
-                                        'tables.cpp', 'jit.cpp')] + [embedded]
+                                        'linear.hip', 'rotation.hip', 'orthogonal.hip', 'tables.cpp', 'jit.cpp')] + [embedded]
     objs = [obj_dir / (src.name + '.o') for src in sources]
 
     def compile_one(pair):

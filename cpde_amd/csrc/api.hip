@@ -2420,7 +2420,7 @@ const char* cpde_trace_name(int kind) {
         "split_reduce",    "bias_grad",       "activate",       "cost",            "reduce",
         "optimizer",       "other",           "fused_input",    "fused_forward",   "fused_backward",
         "fused_output_backward", "network_forward", "network_backward", "network_epoch",
-        "attention", "attention_gradient", "embedding", "dropout"};
+        "attention", "attention_gradient", "embedding", "dropout", "linear", "linear_gradient", "rotation", "orthogonal"};
     return kind >= 0 && kind < kTraceKinds ? names[kind] : "";
 }
 

@@ -282,7 +282,8 @@ enum TraceKind {
     kTraceComposeForward, kTraceComposeAdjoint, kTraceGemm, kTraceGemmTransposed, kTraceWgrad, kTraceSplitReduce,
     kTraceBiasGrad, kTraceActivate, kTraceCost, kTraceReduce, kTraceOptimizer, kTraceOther, kTraceFusedInput,
     kTraceFusedForward, kTraceFusedBackward, kTraceFusedOutput, kTraceNetworkForward, kTraceNetworkBackward,
-    kTraceNetworkEpoch, kTraceAttention, kTraceAttentionGradient, kTraceEmbedding, kTraceDropout, kTraceKinds
+    kTraceNetworkEpoch, kTraceAttention, kTraceAttentionGradient, kTraceEmbedding, kTraceDropout, kTraceLinear,
+    kTraceLinearGradient, kTraceRotation, kTraceOrthogonal, kTraceKinds
 };
 // A one-pass epoch launch held back so that the next one can share it (api.hip).
 struct HeldEpoch;

@@ -1,0 +1,401 @@
+// A layer's product with its bias, activation and residual, and its gradient.
+#include <cmath>
+#include <cstdio>
+
+#include "product.hpp"
+
+namespace cpde {
+namespace {
+
+// ---- activations ------------------------------------------------------------------------
+__device__ inline float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+__device__ inline float sigmoid(float z) { return 1.f / (1.f + exp_fast(-z)); }
+// The normal distribution's integral up to z, (1 + erf(z / sqrt 2)) / 2.
+__device__ inline float normal_integral(float z) { return 0.5f * erfcf(z * -0.70710678118654752440f); }
+
+__device__ inline float activate(int kind, float z) {
+    switch (kind) {
+        case CPDE_SIGMOID: return sigmoid(z);
+        case CPDE_RELU: return z < 0 ? 0.f : z;  // (a NaN stays one)
+        case CPDE_SILU: return z * sigmoid(z);
+        case CPDE_GELU: return z * normal_integral(z);
+        default: return z;
+    }
+}
+// Its derivative.
+__device__ inline float slope(int kind, float z) {
+    switch (kind) {
+        case CPDE_SIGMOID: {
+            const float s = sigmoid(z);
+            return s * (1 - s);
+        }
+        case CPDE_RELU: return z > 0 ? 1.f : 0.f;
+        case CPDE_SILU: {
+            const float s = sigmoid(z);
+            return s * (1 + z * (1 - s));
+        }
+        case CPDE_GELU: return normal_integral(z) + z * 0.39894228040143267794f * exp_fast(-0.5f * z * z);
+        default: return 1.f;
+    }
+}
+
+// ---- rows of a product on their way out ----------------------------------------------------
+// y = activation(c + bias) + residual, and c + bias itself.  (Of a weight gradient: c, or
+// with residual = y, onto what is there.)
+template <class T>
+struct LinearEpilogue {
+    T *y, *pre;
+    const T *bias, *residual;
+    int64_t y_stride, pre_stride, residual_stride;
+    int activation, wide;  // wide: all rows and their addresses are whole 16-byte chunks
+    __device__ void row(int, int m, int n, int count, float (&v)[8]) const {
+        if (bias) {
+            float b[8];
+            read8(b, bias + n, count, wide);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += b[j];
+        }
+        if (pre) write8(pre + m * pre_stride + n, v, count, wide);
+        if (activation != CPDE_NONE)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = activate(activation, v[j]);
+        if (residual) {
+            float r[8];
+            read8(r, residual + m * residual_stride + n, count, wide);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += r[j];
+        }
+        write8(y + m * y_stride + n, v, count, wide);
+    }
+};
+
+// ---- floats as sums of three bf16 values -----------------------------------------------------
+// x = x0 + x1 + x2 to 24 bits, each the rounding of what the ones before leave.  Six of
+// the nine products of two such sums, to 2^-24 of the largest, run on the bf16 instruction
+// in less than half of the time that the float one takes.  Rows of the planes are padded
+// with zeros to whole 16-byte chunks.
+constexpr int kPlanes = 3;
+const Planes kFloatPlanes = {6, {0, 0, 1, 0, 1, 2}, {2, 1, 1, 0, 0, 0}};
+
+template <int>
+__global__ __launch_bounds__(256) void linear_split_k(const float* x, int64_t stride, int64_t rows, int columns, bf16* to,
+                                                      int pitch, int64_t plane) {
+    const int per_row = pitch / 8;
+    const int64_t all = rows * per_row, step = int64_t(gridDim.x) * 256;
+    for (int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x; at < all; at += step) {
+        const int64_t row = at / per_row;
+        const int first = int(at - row * per_row) * 8;
+        const float* from = x + row * stride + first;
+        vec<bf16, 8> out[kPlanes];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float v = first + j < columns ? from[j] : 0.f;
+#pragma unroll
+            for (int i = 0; i < kPlanes; ++i) {
+                out[i][j] = bf16(v);
+                v -= float(out[i][j]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kPlanes; ++i) *reinterpret_cast<vec<bf16, 8>*>(to + i * plane + row * pitch + first) = out[i];
+    }
+}
+
+// ---- dz = dy * slope(pre) and its sums over the rows -----------------------------------------
+// A workgroup takes 64 columns, eight a lane, of a strip of rows, 32 rows at a time; sums
+// of a strip go to `part` [strip][columns], which linear_bias_k adds up in order.
+struct SlopeArgs {
+    const void *dy, *pre;
+    void* dz;       // null: not wanted (no activation)
+    float* part;    // null: not wanted (no bias)
+    int64_t dy_stride, pre_stride, rows;
+    int columns, dz_stride, strip, activation, wide;
+};
+template <class T>
+__global__ __launch_bounds__(256) void linear_slope_k(SlopeArgs a) {
+    __shared__ float sums[32][64 + 8];
+    const int lane = threadIdx.x & 7, row_lane = threadIdx.x >> 3, n = blockIdx.x * 64 + lane * 8;
+    const int count = min(8, a.columns - n);
+    const int64_t first = int64_t(blockIdx.y) * a.strip, last = min(first + a.strip, a.rows);
+    float sum[8] = {};
+    if (count > 0)
+        for (int64_t m = first + row_lane; m < last; m += 32) {
+            float v[8], z[8];
+            read8(v, static_cast<const T*>(a.dy) + m * a.dy_stride + n, count, a.wide);
+            if (a.dz) {
+                read8(z, static_cast<const T*>(a.pre) + m * a.pre_stride + n, count, a.wide);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= slope(a.activation, z[j]);
+                write8(static_cast<T*>(a.dz) + m * a.dz_stride + n, v, count, true);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += v[j];
+        }
+    if (!a.part) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[row_lane][lane * 8 + j] = sum[j];
+    __syncthreads();
+    if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < unsigned(a.columns)) {
+        float total = 0;
+        for (int r = 0; r < 32; ++r) total += sums[r][threadIdx.x];
+        a.part[int64_t(blockIdx.y) * a.columns + blockIdx.x * 64 + threadIdx.x] = total;
+    }
+}
+template <class T>
+__global__ __launch_bounds__(64) void linear_bias_k(const float* part, int strips, int columns, T* dbias, int accumulate) {
+    const int n = blockIdx.x * 64 + threadIdx.x;
+    if (n >= columns) return;
+    float total = 0;
+    for (int s = 0; s < strips; ++s) total += part[int64_t(s) * columns + n];
+    dbias[n] = T(accumulate ? float(dbias[n]) + total : total);
+}
+
+// ---- plans ---------------------------------------------------------------------------------
+struct Linear {
+    Device* dev = nullptr;
+    int dtype = 0, inputs = 0, outputs = 0, activation = 0, backward = 0;
+    int64_t rows = 0;
+    char* work = nullptr;
+    size_t a_planes = 0, b_planes = 0, dz = 0, part = 0, bias_part = 0;  // places in the workspace
+};
+constexpr int64_t kMostRows = int64_t(1) << 30;
+constexpr int kMostWidth = 1 << 24;
+constexpr int kStrips = 256;  // of a bias's gradient
+
+
+int pitch_of(int64_t columns) { return int((columns + 7) / 8 * 8); }
+
+// Floats run on the float instruction up to here, as splitting them is two launches more.
+bool split_floats(const Linear& p, int64_t rows) {
+    return p.dtype == CPDE_F32 && double(rows) * p.inputs * p.outputs > 1e9;
+}
+
+// C[m][n] of a plan's product: operands by their rows, which AK and BK say the order of.
+struct Sides {
+    const void *a, *b;
+    int64_t a_stride, b_stride, m, k;
+    int n;
+};
+template <bool AK, bool BK, class T>
+void product(const Linear& p, const Sides& s, bool split, const LinearEpilogue<T>& e) {
+    Device& d = *p.dev;
+    ProductArgs args{};
+    args.m = int(s.m);
+    args.n = s.n;
+    args.k = int(s.k);
+    args.batch = 1;
+    args.planes = {1, {0}, {0}};
+    args.part = reinterpret_cast<float*>(p.work + p.part);
+    const int64_t a_rows = AK ? s.m : s.k, b_rows = BK ? s.n : s.k, a_columns = AK ? s.k : s.m, b_columns = BK ? s.k : s.n;
+    if (split) {
+        const auto planes = [&](const void* x, int64_t stride, int64_t rows, int64_t columns, char* to) {
+            const int pitch = pitch_of(columns);
+            const int64_t plane = rows * pitch;
+            const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>((plane / 8 + 255) / 256, int64_t(d.compute_units) * 32)));
+            hipLaunchKernelGGL((linear_split_k<0>), blocks, 256, 0, d.stream, static_cast<const float*>(x), stride, rows,
+                               int(columns), reinterpret_cast<bf16*>(to), pitch, plane);
+            HIP_CHECK(hipGetLastError());
+            Operand o = product_operand(to, pitch, pitch, 2);
+            o.plane = plane * 2;
+            return o;
+        };
+        args.a = planes(s.a, s.a_stride, a_rows, a_columns, p.work + p.a_planes);
+        args.b = planes(s.b, s.b_stride, b_rows, b_columns, p.work + p.b_planes);
+        args.planes = kFloatPlanes;
+        launch_product<bf16, AK, BK>(d, args, e);
+        return;
+    }
+    args.a = product_operand(s.a, s.a_stride, a_columns, sizeof(T));
+    args.b = product_operand(s.b, s.b_stride, b_columns, sizeof(T));
+    launch_product<T, AK, BK>(d, args, e);
+}
+
+// A matrix argument of `rows` x `columns`; an output's rows do not overlap.
+void check_rows(const cpde_rows* r, int64_t rows, int64_t columns, bool output) {
+    require(r, "null argument");
+    if (!rows || !columns) return;
+    require(r->data, "null tensor");
+    require(r->stride >= 0 && r->stride <= int64_t(1) << 40, "invalid stride");
+    require(!output || rows == 1 || r->stride >= columns, "output rows overlap");
+}
+bool wide_rows(const cpde_rows* r, size_t size) { return !r || wide(r->data, r->stride, size); }
+
+}  // namespace
+}  // namespace cpde
+
+struct cpde_linear_s : cpde::Linear {};
+using namespace cpde;
+
+extern "C" {
+
+int cpde_linear_create(cpde_device* dev, int dtype, int64_t rows, int inputs, int outputs, int activation, int backward,
+                       cpde_linear** out) {
+    return guarded([&] {
+        require(dev && out, "null argument");
+        *out = nullptr;
+        check_dtype(dtype);
+        require(activation >= CPDE_NONE && activation <= CPDE_GELU, "unknown activation");
+        require(rows >= 0 && inputs >= 0 && outputs >= 0, "negative size");
+        require(rows <= kMostRows && inputs <= kMostWidth && outputs <= kMostWidth, "too large a product");
+        require(!dev->capturing, "a capture is open on this device");
+        auto p = std::make_unique<cpde_linear_s>();
+        p->dev = dev;
+        p->dtype = dtype;
+        p->rows = rows;
+        p->inputs = inputs;
+        p->outputs = outputs;
+        p->activation = activation;
+        p->backward = backward != 0;
+        size_t at = 0;
+        const auto place = [&](size_t bytes) {
+            const size_t here = at;
+            at += (bytes + 255) / 256 * 256;
+            return here;
+        };
+        const int64_t in = pitch_of(inputs), o = pitch_of(outputs);
+        if (split_floats(*p, rows)) {
+            // planes of x and W, of dz and W, or of dz and x
+            p->a_planes = place(size_t(kPlanes) * 2 * rows * (backward ? std::max(in, o) : in));
+            p->b_planes = place(size_t(kPlanes) * 2 * in * (backward ? std::max<int64_t>(outputs, rows) : outputs));
+        }
+        if (backward && activation != CPDE_NONE) p->dz = place(type_bytes(dtype) * rows * o);
+        if (backward) p->bias_part = place(sizeof(float) * kStrips * outputs);
+        size_t part = product_part(dev->compute_units, 1, rows, outputs);
+        if (backward)
+            part = std::max({part, product_part(dev->compute_units, 1, rows, inputs),
+                             product_part(dev->compute_units, 1, outputs, inputs)});
+        p->part = place(sizeof(float) * part);
+        HIP_CHECK(hipMalloc(&p->work, std::max<size_t>(at, 256)));
+        *out = p.release();
+    });
+}
+
+int cpde_linear_destroy(cpde_linear* linear) {
+    return guarded([&] {
+        if (!linear) return;
+        sync_stream(*linear->dev, __LINE__);
+        ++linear->dev->layout;
+        HIP_CHECK(hipFree(linear->work));
+        delete linear;
+    });
+}
+
+int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, const cpde_rows* weight, const void* bias,
+                        const cpde_rows* residual, const cpde_rows* y, const cpde_rows* pre) {
+    return guarded([&] {
+        require(linear, "null argument");
+        const Linear& p = *linear;
+        require(rows >= 0 && rows <= p.rows, "more rows than the plan's");
+        check_rows(x, rows, p.inputs, false);
+        check_rows(weight, p.outputs, p.inputs, false);
+        check_rows(y, rows, p.outputs, true);
+        if (residual) check_rows(residual, rows, p.outputs, false);
+        if (pre) check_rows(pre, rows, p.outputs, true);
+        if (!rows || !p.outputs) return;
+        Device& d = *p.dev;
+        flush_reduce(d);
+        TraceScope trace(d, kTraceLinear, 2.0 * rows * p.inputs * p.outputs);
+        with_type(p.dtype, [&](auto element) {
+            using T = decltype(element);
+            LinearEpilogue<T> e{};
+            e.y = static_cast<T*>(y->data);
+            e.y_stride = y->stride;
+            e.bias = static_cast<const T*>(bias);
+            if (residual) {
+                e.residual = static_cast<const T*>(residual->data);
+                e.residual_stride = residual->stride;
+            }
+            if (pre) {
+                e.pre = static_cast<T*>(pre->data);
+                e.pre_stride = pre->stride;
+            }
+            e.activation = p.activation;
+            e.wide = wide_rows(y, sizeof(T)) && wide_rows(residual, sizeof(T)) && wide_rows(pre, sizeof(T)) && wide(bias, 0, sizeof(T));
+            product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs},
+                                   split_floats(p, rows), e);
+        });
+    });
+}
+
+int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, const cpde_rows* weight,
+                         const cpde_rows* pre, const cpde_rows* dy, const cpde_rows* dx, const cpde_rows* dweight,
+                         void* dbias, int accumulate) {
+    return guarded([&] {
+        require(linear, "null argument");
+        const Linear& p = *linear;
+        require(p.backward, "the plan was created without a backward");
+        require(rows >= 0 && rows <= p.rows, "more rows than the plan's");
+        const bool bent = p.activation != CPDE_NONE;
+        check_rows(dy, rows, p.outputs, false);
+        if (bent) check_rows(pre, rows, p.outputs, false);
+        if (dx) {
+            check_rows(weight, p.outputs, p.inputs, false);
+            check_rows(dx, rows, p.inputs, true);
+        }
+        if (dweight) {
+            check_rows(x, rows, p.inputs, false);
+            check_rows(dweight, p.outputs, p.inputs, true);
+        }
+        if (!dx && !dweight && !dbias) return;
+        Device& d = *p.dev;
+        flush_reduce(d);
+        TraceScope trace(d, kTraceLinearGradient, 2.0 * ((dx != nullptr) + (dweight != nullptr)) * rows * p.inputs * p.outputs);
+        with_type(p.dtype, [&](auto element) {
+            using T = decltype(element);
+            const void* dz = dy->data;
+            int64_t dz_stride = dy->stride;
+            if ((bent || dbias) && p.outputs) {
+                SlopeArgs a{};
+                a.dy = dy->data;
+                a.dy_stride = dy->stride;
+                a.rows = rows;
+                a.columns = p.outputs;
+                a.activation = p.activation;
+                a.wide = wide_rows(dy, sizeof(T));
+                if (bent) {
+                    a.pre = pre->data;
+                    a.pre_stride = pre->stride;
+                    a.dz = p.work + p.dz;
+                    a.dz_stride = pitch_of(p.outputs);
+                    a.wide = a.wide && wide_rows(pre, sizeof(T));
+                    dz = a.dz;
+                    dz_stride = a.dz_stride;
+                }
+                if (dbias) a.part = reinterpret_cast<float*>(p.work + p.bias_part);
+                // strips of 32 rows at least, and workgroups for the whole device
+                const int column_blocks = ceil_div(p.outputs, 64);
+                const int most = std::max(1, std::min<int>(kStrips, ceil_div(8 * d.compute_units, column_blocks)));
+                a.strip = std::max(32, ceil_div(rows, most));
+                const int strips = std::max(1, ceil_div(rows, a.strip));
+                hipLaunchKernelGGL((linear_slope_k<T>), dim3(column_blocks, strips), 256, 0, d.stream, a);
+                HIP_CHECK(hipGetLastError());
+                if (dbias) {
+                    hipLaunchKernelGGL((linear_bias_k<T>), column_blocks, 64, 0, d.stream, a.part, strips, p.outputs,
+                                       static_cast<T*>(dbias), accumulate);
+                    HIP_CHECK(hipGetLastError());
+                }
+            }
+            const bool split = split_floats(p, rows);
+            if (dx && rows) {
+                LinearEpilogue<T> e{};
+                e.y = static_cast<T*>(dx->data);
+                e.y_stride = dx->stride;
+                e.wide = wide_rows(dx, sizeof(T));
+                product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs}, split, e);
+            }
+            if (dweight) {
+                LinearEpilogue<T> e{};
+                e.y = static_cast<T*>(dweight->data);
+                e.y_stride = dweight->stride;
+                e.wide = wide_rows(dweight, sizeof(T));
+                if (accumulate) {
+                    e.residual = e.y;
+                    e.residual_stride = e.y_stride;
+                }
+                product<false, false, T>(p, {dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs}, split, e);
+            }
+        });
+    });
+}
+
+}  // extern "C"

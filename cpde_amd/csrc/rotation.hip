@@ -1,0 +1,540 @@
+// Queries and keys on their way from their products into attention: each head's vector
+// divided by its root mean square, times a weight a column, and its pairs of columns
+// turned by an angle that goes with the token's position.
+#include <cmath>
+
+#include "sequence.hpp"
+
+namespace cpde {
+namespace {
+
+constexpr int kMaxDim = 256;
+
+struct Rotation {
+    Device* dev = nullptr;
+    cpde_rotation_shape shape{};
+    double* rates = nullptr;  // turns a position of each pair
+    float* part = nullptr;    // weight gradients of the workgroups, [workgroup][queries, keys][dim]
+    int blocks = 0;           // of the gradient
+};
+
+// One side, queries or keys.
+struct Side {
+    const char* x;
+    char* y;         // forward: the result; gradient: dx
+    const char* dy;
+    const char* weight;
+    int64_t x_batch, x_token, x_head, y_batch, y_token, y_head, dy_batch, dy_token, dy_head;
+    int heads;
+};
+struct RotationArgs {
+    Side side[2];
+    const double* rates;
+    const int* positions;
+    float* part;
+    int64_t count;  // tokens of all entries
+    int tokens, dim, pairs, interleaved, norm;
+    int parts, span;  // groups of lanes that share a token's heads, and heads of each
+    float eps;
+};
+
+// Sum over groups of LANES neighbouring lanes, each the whole sum.
+template <int LANES>
+__device__ inline float sum_group(float x) {
+    const auto move = [](float v, auto control) {
+        return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(control)::value, 0xf, 0xf, true));
+    };
+    x += move(x, std::integral_constant<int, 0xB1>{});                    // quad_perm [1,0,3,2]
+    x += move(x, std::integral_constant<int, 0x4E>{});                    // quad_perm [2,3,0,1]
+    if (LANES >= 8) x += move(x, std::integral_constant<int, 0x141>{});   // row_half_mirror
+    if (LANES >= 16) x += move(x, std::integral_constant<int, 0x140>{});  // row_mirror
+    if (LANES >= 32) x += __shfl_xor(x, 16);
+    if (LANES >= 64) x += __shfl_xor(x, 32);
+    return x;
+}
+
+// What a lane holds of a head's vector: four pairs of columns.  WIDE: two runs of four
+// columns, from `first` and from `second` (interleaved: one run of eight); otherwise
+// single columns, -1 where there is none.  Columns that are not turned are pairs of an
+// angle of zero.
+template <bool WIDE>
+struct Columns {
+    int first[WIDE ? 1 : 4], second[WIDE ? 1 : 4];
+    int unit[4];  // number of the pair, -1 where it is not turned
+    bool live;
+    __device__ void start(const RotationArgs& a, int lane) {
+        if constexpr (WIDE) {
+            live = lane * 8 < a.dim;
+            const bool turned = lane * 4 < a.pairs;
+            first[0] = turned && !a.interleaved ? 4 * lane : 8 * lane;
+            second[0] = turned && !a.interleaved ? a.pairs + 4 * lane : 8 * lane + 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) unit[j] = turned ? 4 * lane + j : -1;
+        } else {
+            live = true;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int u = lane + 64 * j;
+                unit[j] = u < a.pairs ? u : -1;
+                first[j] = u < a.pairs ? (a.interleaved ? 2 * u : u) : 2 * u;  // (2 pairs + 2 (u - pairs))
+                second[j] = u < a.pairs ? (a.interleaved ? 2 * u + 1 : u + a.pairs) : 2 * u + 1;
+                if (first[j] >= a.dim) first[j] = -1;
+                if (second[j] >= a.dim) second[j] = -1;
+            }
+        }
+    }
+    template <class T>
+    __device__ void load(const T* p, const RotationArgs& a, float (&u)[4], float (&v)[4]) const {
+        if constexpr (WIDE) {
+            vec<T, 4> lo = {}, hi = {};
+            if (live) {
+                lo = *reinterpret_cast<const vec<T, 4>*>(p + first[0]);
+                hi = *reinterpret_cast<const vec<T, 4>*>(p + second[0]);
+            }
+            const bool across = a.interleaved && unit[0] >= 0;
+            u[0] = float(lo[0]);
+            u[1] = float(across ? lo[2] : lo[1]);
+            u[2] = float(across ? hi[0] : lo[2]);
+            u[3] = float(across ? hi[2] : lo[3]);
+            v[0] = float(across ? lo[1] : hi[0]);
+            v[1] = float(across ? lo[3] : hi[1]);
+            v[2] = float(across ? hi[1] : hi[2]);
+            v[3] = float(hi[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] = first[j] >= 0 ? float(p[first[j]]) : 0.f;
+                v[j] = second[j] >= 0 ? float(p[second[j]]) : 0.f;
+            }
+        }
+    }
+    template <class T>
+    __device__ void store(T* p, const RotationArgs& a, const float (&u)[4], const float (&v)[4]) const {
+        if constexpr (WIDE) {
+            if (!live) return;
+            const bool across = a.interleaved && unit[0] >= 0;
+            const vec<T, 4> lo = {T(u[0]), T(across ? v[0] : u[1]), T(across ? u[1] : u[2]), T(across ? v[1] : u[3])};
+            const vec<T, 4> hi = {T(across ? u[2] : v[0]), T(across ? v[2] : v[1]), T(across ? u[3] : v[2]), T(v[3])};
+            *reinterpret_cast<vec<T, 4>*>(p + first[0]) = lo;
+            *reinterpret_cast<vec<T, 4>*>(p + second[0]) = hi;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (first[j] >= 0) p[first[j]] = T(u[j]);
+                if (second[j] >= 0) p[second[j]] = T(v[j]);
+            }
+        }
+    }
+};
+
+// Cosine and sine of a lane's pairs at a position.  The turn is taken in double, whose
+// fraction is right for every position, and the fraction's sine in float.
+template <bool WIDE>
+__device__ inline void turn_of(const RotationArgs& a, const Columns<WIDE>& columns, int position, float (&c)[4], float (&s)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        c[j] = 1;
+        s[j] = 0;
+        if (columns.unit[j] >= 0) {
+            const double turns = position * a.rates[columns.unit[j]];
+            sincospif(2.f * float(turns - rint(turns)), &s[j], &c[j]);
+        }
+    }
+}
+
+// A group of LANES lanes takes one token and `span` of its heads, queries' then keys':
+// the angles are made once for all of them.
+template <class T, int LANES, bool WIDE>
+__global__ __launch_bounds__(256) void rotation_forward_k(RotationArgs a) {
+    const int lane = threadIdx.x % LANES;
+    const int64_t group = int64_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+    const int64_t at = group / a.parts;
+    if (at >= a.count) return;
+    const int64_t batch = at / a.tokens;
+    const int64_t token = at - batch * a.tokens;
+    const int position = a.positions ? a.positions[at] : int(token);
+    Columns<WIDE> columns;
+    columns.start(a, lane);
+    float c[4], s[4];
+    turn_of(a, columns, position, c, s);
+    const int part = int(group - at * a.parts), last = min((part + 1) * a.span, a.side[0].heads + a.side[1].heads);
+    for (int h = part * a.span; h < last; ++h) {
+        const bool keys = h >= a.side[0].heads;
+        const Side& side = a.side[keys];
+        const int head = keys ? h - a.side[0].heads : h;
+        T* y = reinterpret_cast<T*>(side.y) + batch * side.y_batch + token * side.y_token + head * side.y_head;
+        float u[4] = {}, v[4] = {};
+        if (position < 0) {  // (no token: a row of zeros)
+            columns.store(y, a, u, v);
+            continue;
+        }
+        columns.load(reinterpret_cast<const T*>(side.x) + batch * side.x_batch + token * side.x_token + head * side.x_head, a, u, v);
+        if (a.norm) {
+            float square = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) square += u[j] * u[j] + v[j] * v[j];
+            const float up = 1.f / sqrtf(sum_group<LANES>(square) / a.dim + a.eps);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] *= up;
+                v[j] *= up;
+            }
+        }
+        if (side.weight) {
+            float wu[4], wv[4];
+            columns.load(reinterpret_cast<const T*>(side.weight), a, wu, wv);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] *= wu[j];
+                v[j] *= wv[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float turned = u[j] * c[j] - v[j] * s[j];
+            v[j] = u[j] * s[j] + v[j] * c[j];
+            u[j] = turned;
+        }
+        columns.store(y, a, u, v);
+    }
+}
+
+// With n = x up, up = (mean x^2 + eps)^(-1/2) and g the gradient turned back: the
+// weight's gradient is the sum of g n, and x's up (g w - n mean(g w n)).  Groups of
+// lanes go through the tokens with a stride; their sums are joined in fixed order.
+template <class T, int LANES, bool WIDE>
+__global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
+    constexpr int kGroups = 256 / LANES;
+    __shared__ float sums[kGroups][LANES * 8 + 1];
+    const int lane = threadIdx.x % LANES;
+    Columns<WIDE> columns;
+    columns.start(a, lane);
+    float du[2][4] = {}, dv[2][4] = {};
+    const int64_t all = a.count * a.parts;
+    for (int64_t first = int64_t(blockIdx.x) * kGroups; first < all; first += int64_t(gridDim.x) * kGroups) {
+        const int64_t group = first + threadIdx.x / LANES, at = min(group, all - 1) / a.parts;
+        const int64_t batch = at / a.tokens, token = at - batch * a.tokens;
+        const int position = a.positions ? a.positions[at] : int(token);
+        float c[4], s[4];
+        turn_of(a, columns, position, c, s);
+        const int part = int(group - at * a.parts);
+        const int last = group < all ? min((part + 1) * a.span, a.side[0].heads + a.side[1].heads) : 0;
+        for (int h = part * a.span; h < last; ++h) {
+            const bool keys = h >= a.side[0].heads;
+            const Side& side = a.side[keys];
+            const int head = keys ? h - a.side[0].heads : h;
+            T* dx = reinterpret_cast<T*>(side.y) + batch * side.y_batch + token * side.y_token + head * side.y_head;
+            float u[4] = {}, v[4] = {}, gu[4], gv[4], wu[4], wv[4];
+            if (position < 0) {
+                columns.store(dx, a, u, v);
+                continue;
+            }
+            columns.load(reinterpret_cast<const T*>(side.x) + batch * side.x_batch + token * side.x_token + head * side.x_head, a, u, v);
+            columns.load(reinterpret_cast<const T*>(side.dy) + batch * side.dy_batch + token * side.dy_token + head * side.dy_head, a, gu, gv);
+            if (side.weight) columns.load(reinterpret_cast<const T*>(side.weight), a, wu, wv);
+            float square = 0, dot = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float back = gu[j] * c[j] + gv[j] * s[j];
+                gv[j] = gv[j] * c[j] - gu[j] * s[j];
+                gu[j] = back;
+                square += u[j] * u[j] + v[j] * v[j];
+            }
+            const float up = a.norm ? 1.f / sqrtf(sum_group<LANES>(square) / a.dim + a.eps) : 1.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] *= up;
+                v[j] *= up;
+                const float pu = gu[j] * u[j], pv = gv[j] * v[j];
+                du[0][j] += keys ? 0.f : pu;
+                dv[0][j] += keys ? 0.f : pv;
+                du[1][j] += keys ? pu : 0.f;
+                dv[1][j] += keys ? pv : 0.f;
+                if (side.weight) {
+                    gu[j] *= wu[j];
+                    gv[j] *= wv[j];
+                }
+                dot += gu[j] * u[j] + gv[j] * v[j];
+            }
+            const float mean = a.norm ? sum_group<LANES>(dot) / a.dim : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                gu[j] = up * (gu[j] - u[j] * mean);
+                gv[j] = up * (gv[j] - v[j] * mean);
+            }
+            columns.store(dx, a, gu, gv);
+        }
+    }
+    if (!a.part) return;
+    for (int keys = 0; keys < 2; ++keys) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            sums[threadIdx.x / LANES][lane * 8 + j] = du[keys][j];
+            sums[threadIdx.x / LANES][lane * 8 + 4 + j] = dv[keys][j];
+        }
+        __syncthreads();
+        // (in the order of the lanes' places; rotation_weights_k undoes it)
+        for (int i = threadIdx.x; i < LANES * 8; i += 256) {
+            float total = 0;
+            for (int g = 0; g < kGroups; ++g) total += sums[g][i];
+            a.part[(int64_t(blockIdx.x) * 2 + keys) * (LANES * 8) + i] = total;
+        }
+    }
+}
+
+// The workgroups' sums in order: 16 places and 16 runs of workgroups a workgroup.
+template <class T, int LANES, bool WIDE>
+__global__ __launch_bounds__(256) void rotation_weights_k(RotationArgs a, int blocks, T* dq_weight, T* dk_weight) {
+    __shared__ float sums[16][16];
+    const int keys = blockIdx.y, in = threadIdx.x & 15, run = threadIdx.x >> 4, place = blockIdx.x * 16 + in;
+    const int per = (blocks + 15) / 16;
+    float total = 0;
+    for (int b = run * per; b < min(blocks, (run + 1) * per); ++b) total += a.part[(int64_t(b) * 2 + keys) * (LANES * 8) + place];
+    sums[run][in] = total;
+    __syncthreads();
+    T* to = keys ? dk_weight : dq_weight;
+    if (run || !to) return;
+    for (int r = 1; r < 16; ++r) total += sums[r][in];
+    const int lane = place / 8, j = place & 3;
+    const bool second = place & 4;
+    Columns<WIDE> columns;
+    columns.start(a, lane);
+    int column;
+    if constexpr (WIDE) {
+        if (!columns.live) return;
+        if (a.interleaved && columns.unit[0] >= 0) column = columns.first[0] + 2 * j + second;
+        else column = (second ? columns.second[0] : columns.first[0]) + j;
+    } else {
+        column = second ? columns.second[j] : columns.first[j];
+        if (column < 0) return;
+    }
+    to[column] = T(total);
+}
+
+// ---- on the host ----------------------------------------------------------------------------
+// Checks a tensor [batch][tokens][heads][dim]; whether its rows are read four values at a time.
+bool check_view(const cpde_rotation_shape& s, const cpde_heads* h, int heads, bool output) {
+    require(h, "null argument");
+    if (!heads || !s.batch || !s.tokens) return true;
+    require(h->data, "null tensor");
+    require(h->batch >= 0 && h->token >= 0 && h->head >= 0, "negative stride");
+    constexpr int64_t kFar = int64_t(1) << 40;
+    require(h->batch <= kFar && h->token <= kFar && h->head <= kFar, "invalid stride");
+    if (output) {
+        std::pair<int64_t, int64_t> axes[] = {{h->batch, s.batch}, {h->token, s.tokens}, {h->head, heads}};
+        std::sort(std::begin(axes), std::end(axes));
+        int64_t extent = s.head_dim;
+        for (const auto& [stride, count] : axes) {
+            if (count == 1) continue;
+            require(stride >= extent, "output elements overlap");
+            extent = stride * (count - 1) + extent;
+        }
+    }
+    const int64_t size = int64_t(type_bytes(s.dtype));
+    const auto whole = [&](int64_t stride) { return stride * size % (4 * size) == 0; };
+    return reinterpret_cast<uintptr_t>(h->data) % (4 * size) == 0 && whole(h->batch) && whole(h->token) && whole(h->head);
+}
+bool whole_weight(const cpde_rotation_shape& s, const void* w) {
+    return reinterpret_cast<uintptr_t>(w) % (4 * type_bytes(s.dtype)) == 0;
+}
+
+RotationArgs arguments(const Rotation& p, const int32_t* positions) {
+    const auto& s = p.shape;
+    RotationArgs a{};
+    a.rates = p.rates;
+    a.positions = positions;
+    a.count = int64_t(s.batch) * s.tokens;
+    a.tokens = s.tokens;
+    a.dim = s.head_dim;
+    a.pairs = s.rotated / 2;
+    a.interleaved = s.interleaved;
+    a.norm = s.norm;
+    a.eps = s.eps;
+    a.side[0].heads = s.heads;
+    a.side[1].heads = s.kv_heads;
+    return a;
+}
+void set_side(Side& side, const cpde_heads* x, const cpde_heads* y, const cpde_heads* dy, const void* weight) {
+    side.x = static_cast<const char*>(x->data);
+    side.x_batch = x->batch;
+    side.x_token = x->token;
+    side.x_head = x->head;
+    side.y = static_cast<char*>(y->data);
+    side.y_batch = y->batch;
+    side.y_token = y->token;
+    side.y_head = y->head;
+    if (dy) {
+        side.dy = static_cast<const char*>(dy->data);
+        side.dy_batch = dy->batch;
+        side.dy_token = dy->token;
+        side.dy_head = dy->head;
+    }
+    side.weight = static_cast<const char*>(weight);
+}
+// Whether the columns come in whole fours (and, where not turned or interleaved, eights).
+bool whole_columns(const cpde_rotation_shape& s) {
+    return s.head_dim % 8 == 0 && s.rotated % 8 == 0;
+}
+template <class F>
+void with_lanes(const cpde_rotation_shape& s, bool wide_columns, F body) {
+    const std::true_type yes{};
+    if (!wide_columns) body(std::integral_constant<int, 64>{}, std::false_type{});
+    else if (s.head_dim <= 32) body(std::integral_constant<int, 4>{}, yes);
+    else if (s.head_dim <= 64) body(std::integral_constant<int, 8>{}, yes);
+    else if (s.head_dim <= 128) body(std::integral_constant<int, 16>{}, yes);
+    else body(std::integral_constant<int, 32>{}, yes);
+}
+// Heads a group of lanes takes: all of a token's, fewer where there are few tokens.
+void share_heads(const Device& d, RotationArgs& a, int lanes) {
+    const int heads = a.side[0].heads + a.side[1].heads;
+    const int64_t groups = int64_t(d.compute_units) * 8 * 64 / lanes;  // eight waves a unit
+    a.parts = int(std::min<int64_t>(heads, std::max<int64_t>(1, groups / std::max<int64_t>(1, a.count))));
+    a.span = (heads + a.parts - 1) / a.parts;
+    a.parts = (heads + a.span - 1) / a.span;
+}
+constexpr int kGradientBlocks = 8;  // of a unit, at most
+
+}  // namespace
+}  // namespace cpde
+
+struct cpde_rotation_s : cpde::Rotation {};
+using namespace cpde;
+
+extern "C" {
+
+int cpde_rotation_create(cpde_device* dev, const cpde_rotation_shape* shape, cpde_rotation** out) {
+    return guarded([&] {
+        require(dev && shape && out, "null argument");
+        *out = nullptr;
+        const cpde_rotation_shape s = *shape;
+        check_dtype(s.dtype);
+        require(s.batch >= 0 && s.tokens >= 0, "negative size");
+        require(s.heads >= 0 && s.kv_heads >= 0 && s.heads + int64_t(s.kv_heads) >= 1 && s.heads + int64_t(s.kv_heads) <= 1 << 16,
+                "1 to 65536 heads");
+        require(s.head_dim >= 1 && s.head_dim <= kMaxDim, "a head is 1 to 256 wide");
+        require(s.rotated >= 0 && s.rotated <= s.head_dim && s.rotated % 2 == 0, "an even number of a head's columns is rotated");
+        require(s.base > 0 && std::isfinite(s.base), "the base is positive");
+        require(s.eps >= 0 && std::isfinite(s.eps), "eps is not negative");
+        require(int64_t(s.batch) * s.tokens <= int64_t(1) << 30, "too many tokens");
+        require(!dev->capturing, "a capture is open on this device");
+        OnDevice on(*dev);
+        auto p = std::make_unique<cpde_rotation_s>();
+        p->dev = dev;
+        p->shape = s;
+        p->blocks = dev->compute_units * kGradientBlocks;
+        const size_t pairs = size_t(s.rotated / 2), part = s.backward ? size_t(p->blocks) * 2 * 64 * 8 : 0;
+        char* memory = nullptr;
+        HIP_CHECK(hipMalloc(&memory, kMaxDim * sizeof(double) + part * sizeof(float)));
+        p->rates = reinterpret_cast<double*>(memory);
+        p->part = part ? reinterpret_cast<float*>(memory + kMaxDim * sizeof(double)) : nullptr;
+        std::vector<double> rates(pairs);
+        for (size_t i = 0; i < pairs; ++i)
+            rates[i] = std::pow(double(s.base), -2.0 * double(i) / s.rotated) / 6.283185307179586476925;
+        const hipError_t copied = pairs ? hipMemcpy(p->rates, rates.data(), pairs * sizeof(double), hipMemcpyHostToDevice) : hipSuccess;
+        if (copied != hipSuccess) (void)hipFree(memory);
+        HIP_CHECK(copied);
+        *out = p.release();
+    });
+}
+
+int cpde_rotation_destroy(cpde_rotation* rotation) {
+    return guarded([&] {
+        if (!rotation) return;
+        OnDevice on(*rotation->dev);
+        sync_stream(*rotation->dev, __LINE__);
+        ++rotation->dev->layout;
+        HIP_CHECK(hipFree(rotation->rates));
+        delete rotation;
+    });
+}
+
+int cpde_rotation_forward(cpde_rotation* rotation, const cpde_heads* q, const cpde_heads* k, const void* q_weight,
+                          const void* k_weight, const int32_t* positions, const cpde_heads* q_out,
+                          const cpde_heads* k_out) {
+    return guarded([&] {
+        require(rotation, "null argument");
+        const Rotation& p = *rotation;
+        const auto& s = p.shape;
+        RotationArgs a = arguments(p, positions);
+        bool whole = whole_columns(s) && whole_weight(s, q_weight) && whole_weight(s, k_weight);
+        if (s.heads) {
+            whole = check_view(s, q, s.heads, false) && whole;
+            whole = check_view(s, q_out, s.heads, true) && whole;
+            set_side(a.side[0], q, q_out, nullptr, q_weight);
+        }
+        if (s.kv_heads) {
+            whole = check_view(s, k, s.kv_heads, false) && whole;
+            whole = check_view(s, k_out, s.kv_heads, true) && whole;
+            set_side(a.side[1], k, k_out, nullptr, k_weight);
+        }
+        if (!a.count) return;
+        Device& d = *p.dev;
+        OnDevice on(d);
+        flush_reduce(d);
+        TraceScope trace(d, kTraceRotation, 2.0 * a.count * (s.heads + s.kv_heads) * s.head_dim * type_bytes(s.dtype));
+        with_type(s.dtype, [&](auto element) {
+            using T = decltype(element);
+            with_lanes(s, whole, [&](auto lanes, auto whole_) {
+                constexpr int L = decltype(lanes)::value;
+                share_heads(d, a, L);
+                const int64_t blocks = (a.count * a.parts + 256 / L - 1) / (256 / L);
+                require(blocks < (int64_t(1) << 24), "too many workgroups: split the batch");
+                hipLaunchKernelGGL((rotation_forward_k<T, L, decltype(whole_)::value>), unsigned(blocks), 256, 0, d.stream, a);
+            });
+        });
+        HIP_CHECK(hipGetLastError());
+    });
+}
+
+int cpde_rotation_backward(cpde_rotation* rotation, const cpde_heads* q, const cpde_heads* k, const void* q_weight,
+                           const void* k_weight, const int32_t* positions, const cpde_heads* dq_out,
+                           const cpde_heads* dk_out, const cpde_heads* dq, const cpde_heads* dk, void* dq_weight,
+                           void* dk_weight) {
+    return guarded([&] {
+        require(rotation, "null argument");
+        const Rotation& p = *rotation;
+        const auto& s = p.shape;
+        require(s.backward, "the plan was created without a backward");
+        RotationArgs a = arguments(p, positions);
+        bool whole = whole_columns(s) && whole_weight(s, q_weight) && whole_weight(s, k_weight);
+        if (s.heads) {
+            whole = check_view(s, q, s.heads, false) && whole;
+            whole = check_view(s, dq_out, s.heads, false) && whole;
+            whole = check_view(s, dq, s.heads, true) && whole;
+            set_side(a.side[0], q, dq, dq_out, q_weight);
+        }
+        if (s.kv_heads) {
+            whole = check_view(s, k, s.kv_heads, false) && whole;
+            whole = check_view(s, dk_out, s.kv_heads, false) && whole;
+            whole = check_view(s, dk, s.kv_heads, true) && whole;
+            set_side(a.side[1], k, dk, dk_out, k_weight);
+        }
+        if (!s.kv_heads) dk_weight = nullptr;
+        if (!s.heads) dq_weight = nullptr;
+        if (dq_weight || dk_weight) a.part = p.part;
+        else if (!a.count) return;
+        Device& d = *p.dev;
+        OnDevice on(d);
+        flush_reduce(d);
+        TraceScope trace(d, kTraceRotation, 3.0 * a.count * (s.heads + s.kv_heads) * s.head_dim * type_bytes(s.dtype));
+        with_type(s.dtype, [&](auto element) {
+            using T = decltype(element);
+            with_lanes(s, whole, [&](auto lanes, auto whole_) {
+                constexpr int L = decltype(lanes)::value;
+                constexpr bool W = decltype(whole_)::value;
+                share_heads(d, a, L);
+                const int64_t want = (a.count * a.parts + 256 / L - 1) / (256 / L);
+                const int blocks = int(std::max<int64_t>(1, std::min<int64_t>(want, p.blocks)));
+                hipLaunchKernelGGL((rotation_gradient_k<T, L, W>), blocks, 256, 0, d.stream, a);
+                HIP_CHECK(hipGetLastError());
+                if (a.part)
+                    hipLaunchKernelGGL((rotation_weights_k<T, L, W>), dim3(L * 8 / 16, 2), 256, 0, d.stream, a, blocks,
+                                       static_cast<T*>(dq_weight), static_cast<T*>(dk_weight));
+            });
+        });
+        HIP_CHECK(hipGetLastError());
+    });
+}
+
+}  // extern "C"

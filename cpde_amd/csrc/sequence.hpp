@@ -28,5 +28,20 @@ inline bool wide(const void* p, int64_t stride, size_t size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * int64_t(size) % 16 == 0;
 }
 
+// The caller's current GPU is set back at the end of a scope that works on the library's.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(const Device& d) {
+        int now = 0;
+        HIP_CHECK(hipGetDevice(&now));
+        if (now == d.ordinal) return;
+        HIP_CHECK(hipSetDevice(d.ordinal));
+        before = now;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    OnDevice(const OnDevice&) = delete;
+};
 
 }  // namespace cpde

@@ -100,9 +100,32 @@ class Rows(ctypes.Structure):
         return view
 
 
+class Matrices(ctypes.Structure):
+    """cpde_matrices: matrices [count][rows][columns] on a device by their element strides,
+    columns contiguous.  A view made by `of` keeps the tensor's type and sizes, which calls
+    check."""
+    _fields_ = [('data', ctypes.c_void_p), ('matrix', ctypes.c_int64), ('row', ctypes.c_int64)]
+    held = None
+
+    @classmethod
+    def of(cls, tensor):
+        matrix, row, last = tensor.stride()
+        if last != 1 and tensor.shape[-1] > 1:
+            raise ValueError('the last axis is not contiguous')
+        view = cls(tensor.data_ptr(), matrix, row)
+        view.held = _held(tensor)
+        return view
+
+
 class AttentionShape(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ('dtype', 'batch', 'query_tokens', 'key_tokens', 'heads', 'kv_heads',
                                               'head_dim', 'left', 'right', 'backward')] + [('scale', ctypes.c_float)]
+
+
+class RotationShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ('dtype', 'batch', 'tokens', 'heads', 'kv_heads', 'head_dim', 'rotated',
+                                              'interleaved', 'norm', 'backward')] + \
+               [('eps', ctypes.c_float), ('base', ctypes.c_double)]
 
 
 class CpdeError(RuntimeError):
@@ -119,9 +142,11 @@ i64 = ctypes.c_int64
 u64 = ctypes.c_uint64
 heads_p = ctypes.POINTER(Heads)
 rows_p = ctypes.POINTER(Rows)
+matrices_p = ctypes.POINTER(Matrices)
 
 F32, F16, BF16 = 0, 1, 2    # element types of the operators on sequences
 _element = ('float32', 'float16', 'bfloat16')
+NONE, SIGMOID, RELU, SILU, GELU = range(5)    # activations
 
 SIGNATURES = {
     'cpde_last_error': (ctypes.c_char_p, []),
@@ -191,6 +216,18 @@ SIGNATURES = {
     'cpde_embedding_forward': (i32, [vp, vp, i64, rows_p, f32, rows_p]),
     'cpde_embedding_backward': (i32, [vp, vp, i64, rows_p, f32, rows_p, i32]),
     'cpde_dropout': (i32, [vp, i32, i64, i64, rows_p, rows_p, rows_p, ctypes.c_double, u64, u64]),
+    'cpde_linear_create': (i32, [vp, i32, i64, i32, i32, i32, i32, ctypes.POINTER(vp)]),
+    'cpde_linear_destroy': (i32, [vp]),
+    'cpde_linear_forward': (i32, [vp, i64, rows_p, rows_p, vp, rows_p, rows_p, rows_p]),
+    'cpde_linear_backward': (i32, [vp, i64, rows_p, rows_p, rows_p, rows_p, rows_p, rows_p, vp, i32]),
+    'cpde_rotation_create': (i32, [vp, ctypes.POINTER(RotationShape), ctypes.POINTER(vp)]),
+    'cpde_rotation_destroy': (i32, [vp]),
+    'cpde_rotation_forward': (i32, [vp, heads_p, heads_p, vp, vp, vp, heads_p, heads_p]),
+    'cpde_rotation_backward': (i32, [vp, heads_p, heads_p, vp, vp, vp, heads_p, heads_p, heads_p, heads_p, vp, vp]),
+    'cpde_orthogonal_create': (i32, [vp, i32, i32, i32, i32, i32, ctypes.POINTER(vp)]),
+    'cpde_orthogonal_destroy': (i32, [vp]),
+    'cpde_orthogonal_forward': (i32, [vp, matrices_p, matrices_p]),
+    'cpde_orthogonal_update': (i32, [vp, matrices_p, matrices_p, matrices_p, f32, f32, f32, i32]),
     'cpde_capture_begin': (i32, [vp]),
     'cpde_capture_end': (i32, [vp, i32, vp]),
     'cpde_replay_launch': (i32, [vp]),
@@ -643,6 +680,125 @@ class Embedding:
     def destroy(self):
         if self.handle:
             check(load().cpde_embedding_destroy(self.handle))
+            self.handle = None
+
+
+class Linear:
+    """y = activation(x W^T + bias) + residual of at most `rows` rows a call, and its
+    gradient; W is [outputs][inputs].  Matrices are Rows, biases device addresses (or
+    tensors, or Buffers) of `outputs` values of the plan's type."""
+
+    def __init__(self, device, dtype, rows, inputs, outputs, activation=NONE, backward=True):
+        self.device = device
+        h = vp()
+        check(load().cpde_linear_create(device.handle, dtype, rows, inputs, outputs, activation, int(backward),
+                                        ctypes.byref(h)))
+        self.handle = h
+        self.element, self.rows, self.inputs, self.outputs = _element[dtype], rows, inputs, outputs
+
+    def _check(self, rows, inputs, outputs, weights, bias):
+        """Matrices by name: as wide as the inputs, as the outputs, and of the weights' sizes."""
+        if rows > self.rows:
+            return  # (the library refuses it)
+        gpu = self.device.ordinal
+        for views, want in ((inputs, (rows, self.inputs)), (outputs, (rows, self.outputs)),
+                            (weights, (self.outputs, self.inputs))):
+            for name, view in views.items():
+                _holds(name, view, (self.element, gpu, *want))
+        for name, a in bias.items():
+            if a is not None:
+                _list_holds(name, a, self.element, gpu, self.outputs)
+
+    def forward(self, rows, x, weight, y, bias=None, residual=None, pre=None):
+        self._check(rows, {'x': x}, {'y': y, 'residual': residual, 'pre': pre}, {'weight': weight}, {'bias': bias})
+        check(load().cpde_linear_forward(self.handle, rows, x, weight, _address(bias), residual, y, pre))
+
+    def backward(self, rows, x, weight, dy, pre=None, dx=None, dweight=None, dbias=None, accumulate=False):
+        self._check(rows, {'x': x, 'dx': dx}, {'pre': pre, 'dy': dy}, {'weight': weight, 'dweight': dweight},
+                    {'dbias': dbias})
+        check(load().cpde_linear_backward(self.handle, rows, x, weight, pre, dy, dx, dweight, _address(dbias),
+                                          int(accumulate)))
+
+    def destroy(self):
+        if self.handle:
+            check(load().cpde_linear_destroy(self.handle))
+            self.handle = None
+
+
+class Rotation:
+    """Each head's norm and its rotation by the token's position, of queries and keys
+    (cpde_rotation_shape; rotated: None for whole heads), and their gradients.  Tensors are
+    Heads, weights and positions device addresses (or tensors, or Buffers)."""
+
+    def __init__(self, device, dtype, batch, tokens, heads, kv_heads, head_dim, rotated=None, interleaved=False,
+                 base=10000.0, eps=1e-6, norm=True, backward=True):
+        self.device = device
+        shape = RotationShape(dtype, batch, tokens, heads, kv_heads, head_dim, head_dim if rotated is None else rotated,
+                              int(interleaved), int(norm), int(backward), eps, base)
+        h = vp()
+        check(load().cpde_rotation_create(device.handle, ctypes.byref(shape), ctypes.byref(h)))
+        self.handle = h
+        gpu = device.ordinal
+        self.query_side = (_element[dtype], gpu, batch, tokens, heads, head_dim)
+        self.key_side = (_element[dtype], gpu, batch, tokens, kv_heads, head_dim)
+
+    def _check(self, queries, keys, weights, positions):
+        for views, want in ((queries, self.query_side), (keys, self.key_side)):
+            for name, view in views.items():
+                if want[4]:
+                    _holds(name, view, want)
+        element, gpu, batch, tokens, _, dim = self.query_side
+        for name, a in weights.items():
+            if a is not None:
+                _list_holds(name, a, element, gpu, dim)
+        if positions is not None:
+            _list_holds('positions', positions, 'int32', gpu, batch * tokens)
+
+    def forward(self, q, k, q_out, k_out, q_weight=None, k_weight=None, positions=None):
+        self._check({'q': q, 'q_out': q_out}, {'k': k, 'k_out': k_out}, {'q_weight': q_weight, 'k_weight': k_weight}, positions)
+        check(load().cpde_rotation_forward(self.handle, q, k, _address(q_weight), _address(k_weight), _address(positions),
+                                           q_out, k_out))
+
+    def backward(self, q, k, dq_out, dk_out, dq, dk, q_weight=None, k_weight=None, dq_weight=None, dk_weight=None,
+                 positions=None):
+        self._check({'q': q, 'dq_out': dq_out, 'dq': dq}, {'k': k, 'dk_out': dk_out, 'dk': dk},
+                    {'q_weight': q_weight, 'k_weight': k_weight, 'dq_weight': dq_weight, 'dk_weight': dk_weight}, positions)
+        check(load().cpde_rotation_backward(self.handle, q, k, _address(q_weight), _address(k_weight), _address(positions),
+                                            dq_out, dk_out, dq, dk, _address(dq_weight), _address(dk_weight)))
+
+    def destroy(self):
+        if self.handle:
+            check(load().cpde_rotation_destroy(self.handle))
+            self.handle = None
+
+
+class Orthogonal:
+    """`count` matrices of rows x columns brought near the orthogonal ones of their singular
+    vectors, and an optimizer's step along them.  Tensors are Matrices."""
+
+    def __init__(self, device, dtype, count, rows, columns, steps=5):
+        self.device = device
+        h = vp()
+        check(load().cpde_orthogonal_create(device.handle, dtype, count, rows, columns, steps, ctypes.byref(h)))
+        self.handle = h
+        self.side = (_element[dtype], device.ordinal, count, rows, columns)
+
+    def forward(self, x, out):
+        _holds('x', x, self.side)
+        _holds('out', out, self.side)
+        check(load().cpde_orthogonal_forward(self.handle, x, out))
+
+    def update(self, gradient, momentum, weight, rate, momentum_factor=0.95, decay=0.0, nesterov=True):
+        """One step of the weights, in place, and of their (float) momentum."""
+        _holds('gradient', gradient, self.side)
+        _holds('momentum', momentum, ('float32', *self.side[1:]))
+        _holds('weight', weight, self.side)
+        check(load().cpde_orthogonal_update(self.handle, gradient, momentum, weight, rate, momentum_factor, decay,
+                                            int(nesterov)))
+
+    def destroy(self):
+        if self.handle:
+            check(load().cpde_orthogonal_destroy(self.handle))
             self.handle = None
 
 

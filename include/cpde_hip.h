@@ -45,6 +45,9 @@ typedef struct cpde_stacks_s cpde_stacks;
 typedef struct cpde_replay_s cpde_replay;
 typedef struct cpde_attention_s cpde_attention;
 typedef struct cpde_embedding_s cpde_embedding;
+typedef struct cpde_linear_s cpde_linear;
+typedef struct cpde_rotation_s cpde_rotation;
+typedef struct cpde_orthogonal_s cpde_orthogonal;
 
 /* Per-cost reduction result: signed double sum and the first bad (sample,
  * component); component -1 means the objective itself
@@ -480,6 +483,91 @@ int cpde_embedding_backward(cpde_embedding* embedding, const void* ids, int64_t 
  * probability 1 drops everything. */
 int cpde_dropout(cpde_device* dev, int dtype, int64_t rows, int64_t columns, const cpde_rows* x,
                  const cpde_rows* residual, const cpde_rows* y, double probability, uint64_t seed, uint64_t offset);
+
+/* y = activation(x W^T + bias) + residual for at most `rows` rows a call: x
+ * [rows][inputs], W [outputs][inputs] (a row an output), bias [outputs], residual and y
+ * [rows][outputs], all of one type.  GELU is z (1 + erf(z / sqrt 2)) / 2, SILU
+ * z / (1 + exp(-z)).  Products are summed in 32 bits.  Floats of large products are taken
+ * as sums of three bf16 values (24 bits; products to 2^-24 of a row's and a column's
+ * largest) on the bf16 instruction: as exact as the float one, but an infinity, or a
+ * product of more than about 3.39e38, gives NaN there.  backward = 0:
+ * cpde_linear_backward will not be called. */
+#define CPDE_NONE 0
+#define CPDE_SIGMOID 1
+#define CPDE_RELU 2
+#define CPDE_SILU 3
+#define CPDE_GELU 4
+int cpde_linear_create(cpde_device* dev, int dtype, int64_t rows, int inputs, int outputs, int activation, int backward,
+                       cpde_linear** out);
+int cpde_linear_destroy(cpde_linear* linear);
+/* bias and residual may be NULL, and residual may be y.  pre (may be NULL) gets
+ * x W^T + bias, rounded to the type, which the backward of a plan with an activation
+ * needs. */
+int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, const cpde_rows* weight, const void* bias,
+                        const cpde_rows* residual, const cpde_rows* y, const cpde_rows* pre);
+/* The gradients of x, W and bias from y's (the residual's is y's own): with
+ * dz = dy activation'(pre), dx = dz W, dW = dz^T x, dbias = the sum of dz's rows.  Any of
+ * dx, dweight and dbias may be NULL, and is then not computed; x is read for dweight only,
+ * weight for dx only, pre (else NULL) where there is an activation.  With 16-bit tensors dz
+ * is rounded to their type, once, before the two products.  accumulate=1 adds dweight and
+ * dbias onto what is there, 0 overwrites them. */
+int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, const cpde_rows* weight,
+                         const cpde_rows* pre, const cpde_rows* dy, const cpde_rows* dx, const cpde_rows* dweight,
+                         void* dbias, int accumulate);
+
+/* Queries and keys between their products and attention: each head's vector x becomes
+ * w x / sqrt(mean x^2 + eps) (norm = 0: w x), and then its first `rotated` columns (even)
+ * are turned in pairs, pair i of a token at position p by the angle p base^(-2 i / rotated):
+ * (a, b) -> (a cos - b sin, a sin + b cos).  Pair i is columns i and i + rotated / 2,
+ * interleaved = 1: 2 i and 2 i + 1.  heads or kv_heads may be 0: no queries, no keys.
+ * head_dim at most 256.  backward = 0: cpde_rotation_backward will not be called. */
+typedef struct {
+    int32_t dtype, batch, tokens, heads, kv_heads, head_dim;
+    int32_t rotated, interleaved, norm, backward;
+    float eps;
+    double base;
+} cpde_rotation_shape;
+
+int cpde_rotation_create(cpde_device* dev, const cpde_rotation_shape* shape, cpde_rotation** out);
+int cpde_rotation_destroy(cpde_rotation* rotation);
+/* q, q_out [batch][tokens][heads][head_dim], k, k_out with kv_heads; weights [head_dim] of
+ * the tensors' type, NULL for ones.  positions: int32 [batch][tokens] on the device, NULL
+ * for the token's number; a negative one marks a place without a token, whose results are
+ * zeros whatever stands there.  q_out may be q, and k_out k.  Angles are taken in 64 bits
+ * at every position. */
+int cpde_rotation_forward(cpde_rotation* rotation, const cpde_heads* q, const cpde_heads* k, const void* q_weight,
+                          const void* k_weight, const int32_t* positions, const cpde_heads* q_out,
+                          const cpde_heads* k_out);
+/* The gradients of q, k and both weights from those of q_out and k_out, with q and k as the
+ * forward got them.  dq_weight and dk_weight [head_dim] may be NULL (not wanted); dq may be
+ * dq_out, and dk dk_out. */
+int cpde_rotation_backward(cpde_rotation* rotation, const cpde_heads* q, const cpde_heads* k, const void* q_weight,
+                           const void* k_weight, const int32_t* positions, const cpde_heads* dq_out,
+                           const cpde_heads* dk_out, const cpde_heads* dq, const cpde_heads* dk, void* dq_weight,
+                           void* dk_weight);
+
+/* `count` matrices [rows][columns] by their strides in elements, columns contiguous. */
+typedef struct {
+    void* data;
+    int64_t matrix, row;
+} cpde_matrices;
+
+/* O(x): x / |x| (the root of the sum of its squares), then `steps` times
+ * X <- a X + b (X X^T) X + c (X X^T)^2 X with (a, b, c) = (3.4445, -4.7750, 2.0315), which
+ * keeps the singular vectors and takes the singular values into 0.68..1.13 (five steps: those
+ * above about 0.003 of |x|).  The products run on f16 operands: f32 and f16 matrices as sums of two
+ * (22 bits), bf16 ones as one.  A matrix of zeros gives zeros. */
+int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int columns, int steps, cpde_orthogonal** out);
+int cpde_orthogonal_destroy(cpde_orthogonal* orthogonal);
+/* out = O(x); out may be x. */
+int cpde_orthogonal_forward(cpde_orthogonal* orthogonal, const cpde_matrices* x, const cpde_matrices* out);
+/* One step of an optimizer (beside cpde_rprop and cpde_adam) on weights of any layers of
+ * one shape: momentum <- factor momentum + gradient, u = momentum (nesterov = 1:
+ * gradient + factor momentum), weight <- (1 - rate decay) weight -
+ * rate sqrt(max(1, rows / columns)) O(u).  gradient and weight are of the plan's type, the
+ * momentum is float whatever that is. */
+int cpde_orthogonal_update(cpde_orthogonal* orthogonal, const cpde_matrices* gradient, const cpde_matrices* momentum,
+                           const cpde_matrices* weight, float rate, float factor, float decay, int nesterov);
 
 /* ---- captured epochs ------------------------------------------------------------- */
 /* No counterpart in the reference, whose server issues every launch of every
