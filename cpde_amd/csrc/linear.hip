@@ -10,19 +10,33 @@ namespace {
 // ---- activations ------------------------------------------------------------------------
 __device__ inline float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 __device__ inline float sigmoid(float z) { return 1.f / (1.f + exp_fast(-z)); }
-// The normal distribution's integral up to z, (1 + erf(z / sqrt 2)) / 2.
-__device__ inline float normal_integral(float z) { return 0.5f * erfcf(z * -0.70710678118654752440f); }
+// The normal distribution's integral up to z, (1 + erf(z / sqrt 2)) / 2.  For 16-bit tensors
+// by the formula 7.1.26 of M. Abramowitz, I. Stegun, "Handbook of mathematical functions"
+// (1964), off by at most 1.5e-7, which takes a third of the instructions.
+template <class T>
+__device__ inline float normal_integral(float z) {
+    if (sizeof(T) == 4) return 0.5f * erfcf(z * -0.70710678118654752440f);
+    const float x = fabsf(z) * 0.70710678118654752440f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    q *= 0.5f * t * exp_fast(-x * x);
+    return z < 0 ? q : 1 - q;
+}
 
+template <class T>
 __device__ inline float activate(int kind, float z) {
     switch (kind) {
         case CPDE_SIGMOID: return sigmoid(z);
         case CPDE_RELU: return z < 0 ? 0.f : z;  // (a NaN stays one)
         case CPDE_SILU: return z * sigmoid(z);
-        case CPDE_GELU: return z * normal_integral(z);
+        case CPDE_GELU: return z * normal_integral<T>(z);
         default: return z;
     }
 }
 // Its derivative.
+template <class T>
 __device__ inline float slope(int kind, float z) {
     switch (kind) {
         case CPDE_SIGMOID: {
@@ -34,7 +48,7 @@ __device__ inline float slope(int kind, float z) {
             const float s = sigmoid(z);
             return s * (1 + z * (1 - s));
         }
-        case CPDE_GELU: return normal_integral(z) + z * 0.39894228040143267794f * exp_fast(-0.5f * z * z);
+        case CPDE_GELU: return normal_integral<T>(z) + z * 0.39894228040143267794f * exp_fast(-0.5f * z * z);
         default: return 1.f;
     }
 }
@@ -58,7 +72,7 @@ struct LinearEpilogue {
         if (pre) write8(pre + m * pre_stride + n, v, count, wide);
         if (activation != CPDE_NONE)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = activate(activation, v[j]);
+            for (int j = 0; j < 8; ++j) v[j] = activate<T>(activation, v[j]);
         if (residual) {
             float r[8];
             read8(r, residual + m * residual_stride + n, count, wide);
@@ -75,7 +89,8 @@ struct LinearEpilogue {
 // in less than half of the time that the float one takes.  Rows of the planes are padded
 // with zeros to whole 16-byte chunks.
 constexpr int kPlanes = 3;
-const Planes kFloatPlanes = {6, {0, 0, 1, 0, 1, 2}, {2, 1, 1, 0, 0, 0}};
+// (the smallest first: a 2, b 0; 0, 2; 1, 1; 1, 0; 0, 1; 0, 0)
+const Planes kFloatPlanes = {6, 0b00'00'01'01'00'10, 0b00'01'00'01'10'00};
 
 template <int>
 __global__ __launch_bounds__(256) void linear_split_k(const float* x, int64_t stride, int64_t rows, int columns, bf16* to,
@@ -125,7 +140,7 @@ __global__ __launch_bounds__(256) void linear_slope_k(SlopeArgs a) {
             if (a.dz) {
                 read8(z, static_cast<const T*>(a.pre) + m * a.pre_stride + n, count, a.wide);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= slope(a.activation, z[j]);
+                for (int j = 0; j < 8; ++j) v[j] *= slope<T>(a.activation, z[j]);
                 write8(static_cast<T*>(a.dz) + m * a.dz_stride + n, v, count, true);
             }
 #pragma unroll
@@ -184,7 +199,7 @@ void product(const Linear& p, const Sides& s, bool split, const LinearEpilogue<T
     args.n = s.n;
     args.k = int(s.k);
     args.batch = 1;
-    args.planes = {1, {0}, {0}};
+    args.planes = {1, 0, 0};
     args.part = reinterpret_cast<float*>(p.work + p.part);
     const int64_t a_rows = AK ? s.m : s.k, b_rows = BK ? s.n : s.k, a_columns = AK ? s.k : s.m, b_columns = BK ? s.k : s.n;
     if (split) {

@@ -199,8 +199,8 @@ struct StepEpilogue {
 };
 
 // ---- on the host ----------------------------------------------------------------------------
-const Planes kOne = {1, {0}, {0}};
-const Planes kTwo = {3, {0, 1, 0}, {1, 0, 0}};
+const Planes kOne = {1, 0, 0};
+const Planes kTwo = {3, 0b00'01'00, 0b00'00'01};  // (high and low, low and high, high and high)
 
 void check_matrices(const Orthogonal& p, const cpde_matrices* x, bool output) {
     require(x, "null argument");
