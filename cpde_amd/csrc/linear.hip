@@ -83,39 +83,6 @@ struct LinearEpilogue {
     }
 };
 
-// ---- floats as sums of three bf16 values -----------------------------------------------------
-// x = x0 + x1 + x2 to 24 bits, each the rounding of what the ones before leave.  Six of
-// the nine products of two such sums, to 2^-24 of the largest, run on the bf16 instruction
-// in less than half of the time that the float one takes.  Rows of the planes are padded
-// with zeros to whole 16-byte chunks.
-constexpr int kPlanes = 3;
-// (the smallest first: a 2, b 0; 0, 2; 1, 1; 1, 0; 0, 1; 0, 0)
-const Planes kFloatPlanes = {6, 0b00'00'01'01'00'10, 0b00'01'00'01'10'00};
-
-template <int>
-__global__ __launch_bounds__(256) void linear_split_k(const float* x, int64_t stride, int64_t rows, int columns, bf16* to,
-                                                      int pitch, int64_t plane) {
-    const int per_row = pitch / 8;
-    const int64_t all = rows * per_row, step = int64_t(gridDim.x) * 256;
-    for (int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x; at < all; at += step) {
-        const int64_t row = at / per_row;
-        const int first = int(at - row * per_row) * 8;
-        const float* from = x + row * stride + first;
-        vec<bf16, 8> out[kPlanes];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float v = first + j < columns ? from[j] : 0.f;
-#pragma unroll
-            for (int i = 0; i < kPlanes; ++i) {
-                out[i][j] = bf16(v);
-                v -= float(out[i][j]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kPlanes; ++i) *reinterpret_cast<vec<bf16, 8>*>(to + i * plane + row * pitch + first) = out[i];
-    }
-}
-
 // ---- dz = dy * slope(pre) and its sums over the rows -----------------------------------------
 // A workgroup takes 64 columns, eight a lane, of a strip of rows, 32 rows at a time; sums
 // of a strip go to `part` [strip][columns], which linear_bias_k adds up in order.
@@ -156,12 +123,19 @@ __global__ __launch_bounds__(256) void linear_slope_k(SlopeArgs a) {
         a.part[int64_t(blockIdx.y) * a.columns + blockIdx.x * 64 + threadIdx.x] = total;
     }
 }
+// The strips' sums in order: 16 columns and 64 runs of strips a workgroup.
 template <class T>
-__global__ __launch_bounds__(64) void linear_bias_k(const float* part, int strips, int columns, T* dbias, int accumulate) {
-    const int n = blockIdx.x * 64 + threadIdx.x;
-    if (n >= columns) return;
+__global__ __launch_bounds__(1024) void linear_bias_k(const float* part, int strips, int columns, T* dbias, int accumulate) {
+    __shared__ float sums[64][17];
+    const int in = threadIdx.x & 15, run = threadIdx.x >> 4, n = blockIdx.x * 16 + in;
+    const int per = (strips + 63) / 64;
     float total = 0;
-    for (int s = 0; s < strips; ++s) total += part[int64_t(s) * columns + n];
+    if (n < columns)
+        for (int s = run * per; s < min(strips, (run + 1) * per); ++s) total += part[int64_t(s) * columns + n];
+    sums[run][in] = total;
+    __syncthreads();
+    if (run || n >= columns) return;
+    for (int r = 1; r < 64; ++r) total += sums[r][in];
     dbias[n] = T(accumulate ? float(dbias[n]) + total : total);
 }
 
@@ -171,7 +145,7 @@ struct Linear {
     int dtype = 0, inputs = 0, outputs = 0, activation = 0, backward = 0;
     int64_t rows = 0;
     char* work = nullptr;
-    size_t a_planes = 0, b_planes = 0, dz = 0, part = 0, bias_part = 0;  // places in the workspace
+    size_t dz = 0, part = 0, bias_part = 0;  // places in the workspace
 };
 constexpr int64_t kMostRows = int64_t(1) << 30;
 constexpr int kMostWidth = 1 << 24;
@@ -180,11 +154,6 @@ constexpr int kStrips = 256;  // of a bias's gradient
 
 int pitch_of(int64_t columns) { return int((columns + 7) / 8 * 8); }
 
-// Floats run on the float instruction up to here, as splitting them is two launches more.
-bool split_floats(const Linear& p, int64_t rows) {
-    return p.dtype == CPDE_F32 && double(rows) * p.inputs * p.outputs > 1e9;
-}
-
 // C[m][n] of a plan's product: operands by their rows, which AK and BK say the order of.
 struct Sides {
     const void *a, *b;
@@ -192,7 +161,7 @@ struct Sides {
     int n;
 };
 template <bool AK, bool BK, class T>
-void product(const Linear& p, const Sides& s, bool split, const LinearEpilogue<T>& e) {
+void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
     Device& d = *p.dev;
     ProductArgs args{};
     args.m = int(s.m);
@@ -201,27 +170,8 @@ void product(const Linear& p, const Sides& s, bool split, const LinearEpilogue<T
     args.batch = 1;
     args.planes = {1, 0, 0};
     args.part = reinterpret_cast<float*>(p.work + p.part);
-    const int64_t a_rows = AK ? s.m : s.k, b_rows = BK ? s.n : s.k, a_columns = AK ? s.k : s.m, b_columns = BK ? s.k : s.n;
-    if (split) {
-        const auto planes = [&](const void* x, int64_t stride, int64_t rows, int64_t columns, char* to) {
-            const int pitch = pitch_of(columns);
-            const int64_t plane = rows * pitch;
-            const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>((plane / 8 + 255) / 256, int64_t(d.compute_units) * 32)));
-            hipLaunchKernelGGL((linear_split_k<0>), blocks, 256, 0, d.stream, static_cast<const float*>(x), stride, rows,
-                               int(columns), reinterpret_cast<bf16*>(to), pitch, plane);
-            HIP_CHECK(hipGetLastError());
-            Operand o = product_operand(to, pitch, pitch, 2);
-            o.plane = plane * 2;
-            return o;
-        };
-        args.a = planes(s.a, s.a_stride, a_rows, a_columns, p.work + p.a_planes);
-        args.b = planes(s.b, s.b_stride, b_rows, b_columns, p.work + p.b_planes);
-        args.planes = kFloatPlanes;
-        launch_product<bf16, AK, BK>(d, args, e);
-        return;
-    }
-    args.a = product_operand(s.a, s.a_stride, a_columns, sizeof(T));
-    args.b = product_operand(s.b, s.b_stride, b_columns, sizeof(T));
+    args.a = product_operand(s.a, s.a_stride, AK ? s.k : s.m, sizeof(T));
+    args.b = product_operand(s.b, s.b_stride, BK ? s.k : s.n, sizeof(T));
     launch_product<T, AK, BK>(d, args, e);
 }
 
@@ -267,13 +217,7 @@ int cpde_linear_create(cpde_device* dev, int dtype, int64_t rows, int inputs, in
             at += (bytes + 255) / 256 * 256;
             return here;
         };
-        const int64_t in = pitch_of(inputs), o = pitch_of(outputs);
-        if (split_floats(*p, rows)) {
-            // planes of x and W, of dz and W, or of dz and x
-            p->a_planes = place(size_t(kPlanes) * 2 * rows * (backward ? std::max(in, o) : in));
-            p->b_planes = place(size_t(kPlanes) * 2 * in * (backward ? std::max<int64_t>(outputs, rows) : outputs));
-        }
-        if (backward && activation != CPDE_NONE) p->dz = place(type_bytes(dtype) * rows * o);
+        if (backward && activation != CPDE_NONE) p->dz = place(type_bytes(dtype) * rows * pitch_of(outputs));
         if (backward) p->bias_part = place(sizeof(float) * kStrips * outputs);
         size_t part = product_part(dev->compute_units, 1, rows, outputs);
         if (backward)
@@ -326,8 +270,7 @@ int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, c
             }
             e.activation = p.activation;
             e.wide = wide_rows(y, sizeof(T)) && wide_rows(residual, sizeof(T)) && wide_rows(pre, sizeof(T)) && wide(bias, 0, sizeof(T));
-            product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs},
-                                   split_floats(p, rows), e);
+            product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs}, e);
         });
     });
 }
@@ -385,18 +328,17 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                 hipLaunchKernelGGL((linear_slope_k<T>), dim3(column_blocks, strips), 256, 0, d.stream, a);
                 HIP_CHECK(hipGetLastError());
                 if (dbias) {
-                    hipLaunchKernelGGL((linear_bias_k<T>), column_blocks, 64, 0, d.stream, a.part, strips, p.outputs,
+                    hipLaunchKernelGGL((linear_bias_k<T>), ceil_div(p.outputs, 16), 1024, 0, d.stream, a.part, strips, p.outputs,
                                        static_cast<T*>(dbias), accumulate);
                     HIP_CHECK(hipGetLastError());
                 }
             }
-            const bool split = split_floats(p, rows);
             if (dx && rows) {
                 LinearEpilogue<T> e{};
                 e.y = static_cast<T*>(dx->data);
                 e.y_stride = dx->stride;
                 e.wide = wide_rows(dx, sizeof(T));
-                product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs}, split, e);
+                product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs}, e);
             }
             if (dweight) {
                 LinearEpilogue<T> e{};
@@ -407,7 +349,7 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     e.residual = e.y;
                     e.residual_stride = e.y_stride;
                 }
-                product<false, false, T>(p, {dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs}, split, e);
+                product<false, false, T>(p, {dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs}, e);
             }
         });
     });

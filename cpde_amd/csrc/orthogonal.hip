@@ -321,7 +321,7 @@ int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int
         p->columns = columns;
         p->steps = steps;
         const size_t pitch = pitch_of(columns), side = p->side(), side_pitch = pitch_of(p->side()), n = count;
-        p->blocks = int(std::max<int64_t>(1, std::min<int64_t>(256, int64_t(rows) * (pitch / 8) / 512)));
+        p->blocks = int(std::max<int64_t>(1, std::min<int64_t>(2048, int64_t(rows) * (pitch / 8) / 256)));
         size_t at = 0;
         const auto place = [&](size_t bytes) {
             const size_t here = at;

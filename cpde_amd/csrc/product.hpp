@@ -49,6 +49,38 @@ __device__ inline Acc multiply(Frag<float> a, Frag<float> b, Acc c) {
     return c;
 }
 
+// A fragment of floats as three of bf16 values whose sums they are: x0 + x1 + x2 to 24 bits,
+// each the rounding of what the ones before leave.  Six of the nine products of two such
+// sums are exact to 2^-23 of the factors' and take 192 cycles where the float
+// instruction takes 512; what is split is shared by the products of a wave's tile.
+struct Split {
+    Frag<bf16> part[3];
+};
+__device__ inline Split split(Frag<float> x) {
+    Split s;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        s.part[i] = __builtin_convertvector(x, Frag<bf16>);
+        x -= __builtin_convertvector(s.part[i], Frag<float>);
+    }
+    return s;
+}
+__device__ inline Acc multiply(const Split& a, const Split& b, Acc c) {
+    c = multiply(a.part[2], b.part[0], c);  // (the smallest first)
+    c = multiply(a.part[0], b.part[2], c);
+    c = multiply(a.part[1], b.part[1], c);
+    c = multiply(a.part[1], b.part[0], c);
+    c = multiply(a.part[0], b.part[1], c);
+    return multiply(a.part[0], b.part[0], c);
+}
+template <class T, bool Exact>
+using Part = std::conditional_t<std::is_same_v<T, float> && !Exact, Split, Frag<T>>;
+template <class T, bool Exact>
+__device__ inline Part<T, Exact> part(Frag<T> f) {
+    if constexpr (std::is_same_v<T, float> && !Exact) return split(f);
+    else return f;
+}
+
 // A value that is the same in every lane, where the compiler cannot see it.
 __device__ inline int uniform(int i) { return __builtin_amdgcn_readfirstlane(i); }
 
@@ -114,26 +146,31 @@ struct TileSide {
     }
 
     // ---- bringing tiles: rows first..first + N of the operand, inner indices from kDeep t
-    uint32_t low, high;  // the address of the workgroup's first row (column), the same in every lane
+    uint32_t low, high;  // the address of the next tile, the same in every lane
     int64_t stride;
-    int rows, k;         // rows (columns) from there on, inner indices in all
+    int rows, left;      // rows (columns) from there on, inner indices
 
-    __device__ void start(const Operand& o, int batch, int first, int all, int k_) {
+    __device__ void start(const Operand& o, int batch, int first, int all, int k, int t) {
         const uint64_t at = reinterpret_cast<uint64_t>(o.data) + batch * o.batch +
-                            (K ? int64_t(first) * o.stride : int64_t(first) * int64_t(sizeof(T)));
+                            (K ? int64_t(first) * o.stride : int64_t(first) * int64_t(sizeof(T))) + t * step(o.stride);
         low = uniform(int(uint32_t(at)));
         high = uniform(int(uint32_t(at >> 32)));
         stride = o.stride;
         rows = all - first;
-        k = k_;
+        left = k - t * kDeep;
     }
-    __device__ uint64_t base(int64_t plane, int t) const {
-        return ((uint64_t(high) << 32) | low) + plane + t * (K ? int64_t(kTileBytes) : kDeep * stride);
+    __device__ static int64_t step(int64_t stride) { return K ? kTileBytes : kDeep * stride; }  // from tile to tile
+    __device__ uint64_t base() const { return (uint64_t(high) << 32) | low; }
+    __device__ __attribute__((always_inline)) void next() {
+        const uint64_t at = base() + step(stride);
+        low = uint32_t(at);
+        high = uint32_t(at >> 32);
+        left -= kDeep;
     }
     // Byte offset of a lane's chunk i of a tile with `left` inner indices.  Rows past the
     // last repeat it (their results are not stored); inner indices past the end are zeros.
     __device__ uint32_t place(int i, int left) const {
-        const int slot = i * Threads + threadIdx.x, row = slot / kChunks, chunk = (slot % kChunks) ^ turn(row);
+        const int slot = i * Threads + threadIdx.x % Threads, row = slot / kChunks, chunk = (slot % kChunks) ^ turn(row);
         if (K) return chunk * kChunk < left ? uint32_t(min(row, rows - 1)) * uint32_t(stride) + (chunk << 4) : kNone;
         return row < left ? uint32_t(row) * uint32_t(stride) + (min(chunk, (rows + kChunk - 1) / kChunk - 1) << 4) : kNone;
     }
@@ -143,11 +180,10 @@ struct TileSide {
     }
     // From memory to LDS without registers, for operands of whole 16-byte chunks.  The
     // loads have arrived after loads_arrived() and a barrier.
-    __device__ __attribute__((always_inline)) void load(char* tile, const uint32_t (&offset)[kSteps], int64_t plane, int t,
+    __device__ __attribute__((always_inline)) void load(char* tile, const uint32_t (&offset)[kSteps], int64_t plane,
                                                         int wave) const {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's compiler does not know a buffer's type)
-        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base(plane, t)), 0, 0x7ffffff0, 0x00020000);
-        const int left = k - t * kDeep;
+        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base() + plane), 0, 0x7ffffff0, 0x00020000);
         const auto bring = [&](int i, uint32_t at) __attribute__((always_inline)) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 buffer, (__attribute__((address_space(3))) void*)(tile + (i * Threads + wave * 64) * 16), 16, at, 0, 0, 0);
@@ -162,11 +198,10 @@ struct TileSide {
 #endif
     }
     // Value by value, for any other.
-    __device__ void load_any(char* tile, int64_t plane, int t) const {
-        const int left = k - t * kDeep;
+    __device__ void load_any(char* tile, int64_t plane) const {
         for (int i = 0; i < kSteps; ++i) {
-            const int slot = i * Threads + threadIdx.x, row = slot / kChunks, first = ((slot % kChunks) ^ turn(row)) * kChunk;
-            const T* p = reinterpret_cast<const T*>(base(plane, t) + int64_t(K ? min(row, rows - 1) : row) * stride);
+            const int slot = i * Threads + threadIdx.x % Threads, row = slot / kChunks, first = ((slot % kChunks) ^ turn(row)) * kChunk;
+            const T* p = reinterpret_cast<const T*>(base() + plane + int64_t(K ? min(row, rows - 1) : row) * stride);
             vec<T, kChunk> v;
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
@@ -179,6 +214,10 @@ struct TileSide {
 };
 
 __device__ inline void loads_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0), the other counters open
+
+// All but the last N loads have arrived (the other counters stay open).
+template <int N>
+__device__ inline void arrived_but() { __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14)); }
 
 // Where a workgroup's tile lies.  Workgroups go to the 8 XCDs in turn, each with an L2 of
 // its own: an XCD takes a run of neighbouring tiles, in bands of 8 tiles of m, so that
@@ -227,19 +266,22 @@ __device__ inline void write8(T* p, const float (&v)[8], int count, bool wide) {
 
 // What the kernels of products share: C's tile [BM][BN] by waves of [WM][WN] each, two
 // tiles of either operand in LDS.
-template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN>
+template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN, int Stages = 2, bool Exact = false>
 struct Tiles {
     static constexpr int kThreads = (BM / WM) * (BN / WN) * 64, kMB = WM / 32, kNB = WN / 32, kS = kDepth<T> / 16;
     using A = TileSide<T, AK, BM, kThreads>;
     using B = TileSide<T, BK, BN, kThreads>;
     static constexpr int kPitch = WN + 4, kStage = 32 * kPitch * 4;  // a wave's rows of C on their way out
     static constexpr int kTile = A::kBytes + B::kBytes, kOut = kThreads / 64 * kStage;
-    static constexpr int kLds = 2 * kTile > kOut ? 2 * kTile : kOut;
+    static constexpr int kLds = Stages * kTile > kOut ? Stages * kTile : kOut;
+    static constexpr int kLoads = A::kSteps + B::kSteps;  // of a tile, by each lane
+
+    using P = Part<T, Exact>;  // of a fragment, as it is multiplied
 
     A a;
     B b;
     uint32_t a_offset[A::kSteps], b_offset[B::kSteps];
-    int lane, wave, wm, wn, split, batch, m0, n0, t, t1, plane, steps;
+    int lane, wave, wm, wn, split, batch, m0, n0, plane, steps;
     Acc acc[kMB][kNB];
 
     __device__ __attribute__((always_inline)) void start(const ProductArgs& p) {
@@ -253,14 +295,13 @@ struct Tiles {
         tile_of(blockIdx.x, p.m_tiles * p.n_tiles, p.m_tiles, p.n_tiles, tm, tn);
         m0 = tm * BM;
         n0 = tn * BN;
-        a.start(p.a, batch, m0, p.m, p.k);
-        b.start(p.b, batch, n0, p.n, p.k);
+        const int t = split * p.span;
+        a.start(p.a, batch, m0, p.m, p.k, t);
+        b.start(p.b, batch, n0, p.n, p.k, t);
         a.places(a_offset);
         b.places(b_offset);
-        t = split * p.span;
-        t1 = min((p.k + kDepth<T> - 1) / kDepth<T>, t + p.span);
         plane = 0;
-        steps = max(0, t1 - t) * p.planes.count;
+        steps = max(0, min((p.k + kDepth<T> - 1) / kDepth<T> - t, p.span)) * p.planes.count;
 #pragma unroll
         for (int i = 0; i < kMB; ++i)
 #pragma unroll
@@ -269,23 +310,28 @@ struct Tiles {
     // The next tile's loads.
     template <bool Any>
     __device__ __attribute__((always_inline)) void load(const ProductArgs& p, char* tile) {
-        const int64_t pa = int64_t((p.planes.a >> (2 * plane)) & 3) * p.a.plane, pb = int64_t((p.planes.b >> (2 * plane)) & 3) * p.b.plane;
-        if (Any && !p.a.wide) a.load_any(tile, pa, t);
-        else a.load(tile, a_offset, pa, t, wave);
-        if (Any && !p.b.wide) b.load_any(tile + A::kBytes, pb, t);
-        else b.load(tile + A::kBytes, b_offset, pb, t, wave);
-        if (++plane == p.planes.count) {
+        int64_t pa = 0, pb = 0;
+        if (p.planes.count > 1) {
+            pa = int64_t((p.planes.a >> (2 * plane)) & 3) * p.a.plane;
+            pb = int64_t((p.planes.b >> (2 * plane)) & 3) * p.b.plane;
+        }
+        if (Any && !p.a.wide) a.load_any(tile, pa);
+        else a.load(tile, a_offset, pa, wave);
+        if (Any && !p.b.wide) b.load_any(tile + A::kBytes, pb);
+        else b.load(tile + A::kBytes, b_offset, pb, wave);
+        if (++plane >= p.planes.count) {
             plane = 0;
-            ++t;
+            a.next();
+            b.next();
         }
     }
-    __device__ __attribute__((always_inline)) void fragments(const char* tile, int s, Frag<T> (&fa)[kMB], Frag<T> (&fb)[kNB]) const {
+    __device__ __attribute__((always_inline)) void fragments(const char* tile, int s, P (&fa)[kMB], P (&fb)[kNB]) const {
 #pragma unroll
-        for (int i = 0; i < kMB; ++i) fa[i] = A::fragment(tile, wm * kMB + i, s, lane);
+        for (int i = 0; i < kMB; ++i) fa[i] = part<T, Exact>(A::fragment(tile, wm * kMB + i, s, lane));
 #pragma unroll
-        for (int i = 0; i < kNB; ++i) fb[i] = B::fragment(tile + A::kBytes, wn * kNB + i, s, lane);
+        for (int i = 0; i < kNB; ++i) fb[i] = part<T, Exact>(B::fragment(tile + A::kBytes, wn * kNB + i, s, lane));
     }
-    __device__ __attribute__((always_inline)) void products(const Frag<T> (&fa)[kMB], const Frag<T> (&fb)[kNB]) {
+    __device__ __attribute__((always_inline)) void products(const P (&fa)[kMB], const P (&fb)[kNB]) {
 #pragma unroll
         for (int i = 0; i < kMB; ++i)
 #pragma unroll
@@ -325,30 +371,51 @@ struct Tiles {
     }
 };
 
-// The next tile's loads are under way while one is multiplied.  Any: operands of any
-// alignment.
-template <class T, bool AK, bool BK, int Side, int Wave, int PerSimd, bool Any, class Epilogue>
+// The loads of the next Stages - 1 tiles are under way while one is multiplied.  Any:
+// operands of any alignment.
+template <class T, bool AK, bool BK, int Side, int Wave, int Stages, int PerSimd, bool Any, class Epilogue>
 __global__ __launch_bounds__((Side / Wave) * (Side / Wave) * 64, PerSimd) void product_k(ProductArgs p, Epilogue e) {
-    using C = Tiles<T, AK, BK, Side, Side, Wave, Wave>;
+    using C = Tiles<T, AK, BK, Side, Side, Wave, Wave, Stages, (Side < 128)>;
     __shared__ __align__(16) char lds[C::kLds];
     C c;
     c.start(p);
     // (the tiles read and written do not overlap, which the compiler has to know so as
     // not to wait for the loads under way before it reads)
-    const auto step = [&](const char* __restrict__ tile) __attribute__((always_inline)) {
+    const auto step = [&](const char* __restrict__ tile, auto load) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < C::kS; ++s) {
-            Frag<T> fa[C::kMB], fb[C::kNB];
+            typename C::P fa[C::kMB], fb[C::kNB];
             c.fragments(tile, s, fa, fb);
+            if (s == 0) load();
             c.products(fa, fb);
         }
     };
-    if (c.steps) c.template load<Any>(p, lds);
-    for (int i = 0; i < c.steps; ++i) {
-        loads_arrived();
-        __syncthreads();
-        if (i + 1 < c.steps) c.template load<Any>(p, lds + ((i + 1) & 1) * C::kTile);
-        step(lds + (i & 1) * C::kTile);
+    if constexpr (Any) {
+        for (int i = 0; i < c.steps; ++i) {
+            c.template load<true>(p, lds);
+            loads_arrived();
+            __syncthreads();
+            step(lds, [] {});
+            __syncthreads();
+        }
+    } else {
+        int to = 0;  // the place of the next loads
+        const auto load = [&](int i) __attribute__((always_inline)) {
+            if (i < c.steps) c.template load<false>(p, lds + to * C::kTile);
+            to = to + 1 == Stages ? 0 : to + 1;
+        };
+        int from = 0;
+#pragma unroll
+        for (int i = 0; i < Stages - 1; ++i) load(i);
+        for (int i = 0; i < c.steps; ++i) {
+            if (c.steps - i >= Stages - 1) arrived_but<(Stages - 2) * C::kLoads>();
+            else loads_arrived();
+            // (every wave's reads of the tile before, whose place is written next, are done)
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+            asm volatile("s_barrier" ::: "memory");
+            step(lds + from * C::kTile, [&]() __attribute__((always_inline)) { load(i + Stages - 1); });
+            from = from + 1 == Stages ? 0 : from + 1;
+        }
     }
     __syncthreads();
     c.finish(p, e, lds);
@@ -382,7 +449,7 @@ __global__ __launch_bounds__(512, 2) void product_large_k(ProductArgs p, Epilogu
         const char* tile = lds + (i & 1) * C::kTile;
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-            Frag<T> fa[2][C::kMB], fb[2][C::kNB];
+            typename C::P fa[2][C::kMB], fb[2][C::kNB];
             c.fragments(tile, 2 * part, fa[0], fb[0]);
             c.fragments(tile, 2 * part + 1, fa[1], fb[1]);
             __builtin_amdgcn_sched_barrier(0);
@@ -403,6 +470,79 @@ __global__ __launch_bounds__(512, 2) void product_large_k(ProductArgs p, Epilogu
     __syncthreads();
     c.finish(p, e, lds);
 }
+
+// Small products and few rows: a workgroup makes a tile of 32 x 32, its waves sharing the
+// inner axis, each with tiles of its own in LDS, two at a time and no barrier until
+// their sums are joined.  Bound: the latency of a launch and of a round or two of loads; with
+// few rows and a large matrix, HBM.
+template <class T, bool AK, bool BK, bool Any, class Epilogue>
+__global__ __launch_bounds__(512) void product_run_k(ProductArgs p, Epilogue e) {
+    extern __shared__ __align__(16) char lds[];  // [wave][2][A, B], then [wave][32][36] sums
+    using A = TileSide<T, AK, 32, 64>;
+    using B = TileSide<T, BK, 32, 64>;
+    constexpr int kTile = A::kBytes + B::kBytes, kPitch = 36;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), waves = blockDim.x / 64, half = lane >> 5;
+    int tm, tn;
+    tile_of(blockIdx.x, p.m_tiles * p.n_tiles, p.m_tiles, p.n_tiles, tm, tn);
+    const int m0 = tm * 32, n0 = tn * 32, batch = blockIdx.y;
+    const int deep = (p.k + A::kDeep - 1) / A::kDeep, share = (deep + waves - 1) / waves;
+    const int first = wave * share, steps = min(deep - first, share);
+    A a;
+    B b;
+    a.start(p.a, batch, m0, p.m, p.k, first);
+    b.start(p.b, batch, n0, p.n, p.k, first);
+    uint32_t a_offset[A::kSteps], b_offset[B::kSteps];
+    a.places(a_offset);
+    b.places(b_offset);
+    char* mine = lds + wave * 2 * kTile;
+    const auto load = [&](int i) __attribute__((always_inline)) {
+        char* tile = mine + (i & 1) * kTile;
+        if (Any && !p.a.wide) a.load_any(tile, 0);
+        else a.load(tile, a_offset, 0, 0);
+        if (Any && !p.b.wide) b.load_any(tile + A::kBytes, 0);
+        else b.load(tile + A::kBytes, b_offset, 0, 0);
+        a.next();
+        b.next();
+    };
+    Acc acc = {};
+    if (steps > 0) load(0);
+    for (int i = 0; i < steps; ++i) {
+        if (i + 1 < steps) load(i + 1);
+        if (i + 1 < steps && !Any) arrived_but<A::kSteps + B::kSteps>();
+        else loads_arrived();
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): stores to LDS, and the reads of the tile before
+        asm volatile("" ::: "memory");
+        const char* tile = mine + (i & 1) * kTile;
+#pragma unroll
+        for (int s = 0; s < kDepth<T> / 16; ++s)
+            acc = multiply(B::fragment(tile + A::kBytes, 0, s, lane), A::fragment(tile, 0, s, lane), acc);
+        // (the next loads write where these reads were)
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        asm volatile("" ::: "memory");
+    }
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(lds);
+    float* to = sums + (wave * 32 + (lane & 31)) * kPitch;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const Quad v = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+        *reinterpret_cast<Quad*>(to + 8 * g + 4 * half) = v;
+    }
+    __syncthreads();
+    // eight columns of a row a lane
+    for (int at = threadIdx.x; at < 128; at += blockDim.x) {
+        const int row = at / 4, column = at % 4 * 8;
+        float v[8] = {};
+        for (int w = 0; w < waves; ++w) {
+            const float* from = sums + (w * 32 + row) * kPitch + column;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += from[j];
+        }
+        if (m0 + row < p.m && n0 + column < p.n) e.row(batch, m0 + row, n0 + column, min(8, p.n - n0 - column), v);
+    }
+}
+template <class T>
+constexpr size_t kRunBytes = 2 * 2 * 32 * kTileBytes;  // of LDS for each wave
 
 // The splits of a product summed in order, eight columns a lane, and its epilogue.
 template <class Epilogue>
@@ -425,24 +565,63 @@ __global__ __launch_bounds__(256) void product_join_k(ProductArgs p, Epilogue e)
 // ---- on the host --------------------------------------------------------------------------
 inline int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
-// How a product is cut: the side of its tiles, and splits of its inner axis.
+// How a product is cut: the side of its tiles (32: product_run_k, of `waves` waves), and
+// splits of its inner axis.
 struct ProductCut {
-    int side = 64, splits = 1, span = 1;
+    int side = 64, splits = 1, waves = 4;
 };
-constexpr int kMostSplits = 64;
-// depth: inner indices of all products of planes together.
-inline ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t depth, int size, bool wide) {
-    ProductCut c;
-    const auto tiles = [&](int side) { return batch * ceil_div(m, side) * int64_t(ceil_div(n, side)); };
-    if (wide && size == 2 && tiles(256) >= compute_units) c.side = 256;
-    else if (wide && tiles(128) >= compute_units) c.side = 128;
-    const int64_t have = std::max<int64_t>(1, tiles(c.side)), deep = (depth + kTileBytes / size - 1) / (kTileBytes / size);
-    if (c.side < 256) c.splits = int(std::max<int64_t>(1, std::min<int64_t>({2 * compute_units / have, deep / 4, kMostSplits})));
-    return c;
+constexpr int kMostSplits = 32;
+constexpr int64_t kPartTiles = 4;  // 128 x 128 tiles of partial sums a unit, at most
+
+// By the times that the kernels take (microseconds, 256 CUs), measured with 128 to 1,024
+// workgroups and inner axes of 256 to 4,096: what a launch takes with its first loads
+// and its last stores, and a tile of the inner axis with one and with several
+// workgroups a CU.
+struct ProductTime {
+    int side;
+    double start, alone, shared;
+};
+constexpr ProductTime kTimes16[] = {{64, 3.8, 0.30, 0.195}, {128, 5.0, 0.63, 0.48}, {256, 11.5, 1.50, 1.50}};
+constexpr ProductTime kTimes32[] = {{64, 4.5, 0.65, 0.53}, {128, 8.0, 1.60, 1.43}};
+// planes: products of planes.
+inline ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, int planes, int size, bool wide) {
+    ProductCut best;
+    double least = 1e30;
+    const int64_t deep = std::max<int64_t>(1, (k + kTileBytes / size - 1) / (kTileBytes / size)) * planes;
+    const auto consider = [&](const ProductTime& t) {
+        const int64_t tiles = batch * ceil_div(m, t.side) * int64_t(ceil_div(n, t.side));
+        for (int splits = 1; splits <= kMostSplits && (splits == 1 || (splits * 2 <= deep && t.side < 256)); ++splits) {
+            if (splits > 1 && splits * batch * m * n > kPartTiles * compute_units * 128 * 128) break;
+            const int64_t each = (tiles * splits + compute_units - 1) / compute_units;
+            double time = t.start + double((deep + splits - 1) / splits) * (each == 1 ? t.alone : std::max(t.alone, each * t.shared));
+            if (splits > 1) time += 3.5 + double(batch) * m * n * splits * 8 / 4e6;
+            if (time < least) {
+                least = time;
+                best.side = t.side;
+                best.splits = splits;
+            }
+        }
+    };
+    for (const auto& t : kTimes16)
+        if (size == 2 && (wide || t.side == 64)) consider(t);
+    for (const auto& t : kTimes32)
+        if (size == 4 && (wide || t.side == 64)) consider(t);
+    // a workgroup of 32 x 32, one or two on a CU at once
+    const int64_t tiles = batch * ceil_div(m, 32) * int64_t(ceil_div(n, 32));
+    if (planes == 1 && tiles <= 2 * compute_units) {
+        const int waves = int(std::min<int64_t>(tiles <= compute_units ? 8 : 4, deep));
+        const double time = 3.6 + double((deep + waves - 1) / waves) * (size == 2 ? 0.5 : 0.8);
+        if (time < least) {
+            best.side = 32;
+            best.splits = 1;
+            best.waves = waves;
+        }
+    }
+    return best;
 }
 // Floats of ProductArgs::part that no call with up to `m` rows passes.
 inline size_t product_part(int compute_units, int64_t batch, int64_t m, int64_t n) {
-    return size_t(std::min<int64_t>(int64_t(2) * compute_units * 128 * 128, kMostSplits * batch * m * n));
+    return size_t(std::min<int64_t>(kPartTiles * compute_units * 128 * 128, kMostSplits * batch * m * n));
 }
 
 // An operand of rows of `columns` values of `size` bytes.
@@ -456,12 +635,12 @@ inline Operand product_operand(const void* data, int64_t stride, int64_t columns
 
 // A launch of one of the kernels of tiles of `side`.
 template <class K, class E>
-void launch_tiles(Device& d, K kernel, int side, int threads, ProductArgs p, const E& e) {
+void launch_tiles(Device& d, K kernel, int side, int threads, ProductArgs p, const E& e, size_t lds = 0) {
     p.m_tiles = ceil_div(p.m, side);
     p.n_tiles = ceil_div(p.n, side);
     require(int64_t(p.m_tiles) * p.n_tiles * threads < (int64_t(1) << 31) && int64_t(p.splits) * p.batch < 65536,
             "too many workgroups");
-    hipLaunchKernelGGL(kernel, dim3(unsigned(p.m_tiles) * p.n_tiles, unsigned(p.splits) * p.batch), threads, 0, d.stream, p, e);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(p.m_tiles) * p.n_tiles, unsigned(p.splits) * p.batch), threads, lds, d.stream, p, e);
     HIP_CHECK(hipGetLastError());
 }
 
@@ -469,14 +648,24 @@ void launch_tiles(Device& d, K kernel, int side, int threads, ProductArgs p, con
 template <class T, bool AK, bool BK, class E>
 void launch_product(Device& d, ProductArgs p, const E& e) {
     if (!p.m || !p.n || !p.batch) return;
-    const ProductCut c = cut_product(d.compute_units, p.batch, p.m, p.n, int64_t(p.k) * p.planes.count, sizeof(T), p.a.wide && p.b.wide);
+    const bool wide = p.a.wide && p.b.wide;
+    const ProductCut c = cut_product(d.compute_units, p.batch, p.m, p.n, p.k, p.planes.count, sizeof(T), wide);
     const int deep = std::max(1, ceil_div(p.k, kDepth<T>));
     p.span = ceil_div(deep, std::min(c.splits, deep));
     p.splits = ceil_div(deep, p.span);
-    if (!p.a.wide || !p.b.wide) launch_tiles(d, product_k<T, AK, BK, 64, 32, 2, true, E>, 64, 256, p, e);
-    else if (c.side == 64) launch_tiles(d, product_k<T, AK, BK, 64, 32, 2, false, E>, 64, 256, p, e);
-    else if (c.side == 128) launch_tiles(d, product_k<T, AK, BK, 128, 64, 2, false, E>, 128, 256, p, e);
-    else if constexpr (sizeof(T) == 2) launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
+    if (c.side == 32) {
+        const size_t lds = c.waves * kRunBytes<T>;
+        if (wide) launch_tiles(d, product_run_k<T, AK, BK, false, E>, 32, 64 * c.waves, p, e, lds);
+        else launch_tiles(d, product_run_k<T, AK, BK, true, E>, 32, 64 * c.waves, p, e, lds);
+    } else if (!wide) {
+        launch_tiles(d, product_k<T, AK, BK, 64, 32, 1, 2, true, E>, 64, 256, p, e);
+    } else if (c.side == 64) {
+        launch_tiles(d, product_k<T, AK, BK, 64, 32, 4, 2, false, E>, 64, 256, p, e);
+    } else if (c.side == 128) {
+        launch_tiles(d, product_k<T, AK, BK, 128, 64, 2, 2, false, E>, 128, 256, p, e);
+    } else {
+        if constexpr (sizeof(T) == 2) launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
+    }
     if (p.splits > 1) {
         const int64_t lanes = int64_t(p.batch) * p.m * ((p.n + 7) / 8);
         hipLaunchKernelGGL((product_join_k<E>), unsigned((lanes + 255) / 256), 256, 0, d.stream, p, e);

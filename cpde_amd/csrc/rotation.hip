@@ -283,19 +283,19 @@ __global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
     }
 }
 
-// The workgroups' sums in order: 16 places and 16 runs of workgroups a workgroup.
+// The workgroups' sums in order: 16 places and 64 runs of workgroups a workgroup.
 template <class T, int LANES, bool WIDE>
-__global__ __launch_bounds__(256) void rotation_weights_k(RotationArgs a, int blocks, T* dq_weight, T* dk_weight) {
-    __shared__ float sums[16][16];
+__global__ __launch_bounds__(1024) void rotation_weights_k(RotationArgs a, int blocks, T* dq_weight, T* dk_weight) {
+    __shared__ float sums[64][17];
     const int keys = blockIdx.y, in = threadIdx.x & 15, run = threadIdx.x >> 4, place = blockIdx.x * 16 + in;
-    const int per = (blocks + 15) / 16;
+    const int per = (blocks + 63) / 64;
     float total = 0;
     for (int b = run * per; b < min(blocks, (run + 1) * per); ++b) total += a.part[(int64_t(b) * 2 + keys) * (LANES * 8) + place];
     sums[run][in] = total;
     __syncthreads();
     T* to = keys ? dk_weight : dq_weight;
     if (run || !to) return;
-    for (int r = 1; r < 16; ++r) total += sums[r][in];
+    for (int r = 1; r < 64; ++r) total += sums[r][in];
     const int lane = place / 8, j = place & 3;
     const bool second = place & 4;
     Columns<WIDE> columns;
@@ -529,7 +529,7 @@ int cpde_rotation_backward(cpde_rotation* rotation, const cpde_heads* q, const c
                 hipLaunchKernelGGL((rotation_gradient_k<T, L, W>), blocks, 256, 0, d.stream, a);
                 HIP_CHECK(hipGetLastError());
                 if (a.part)
-                    hipLaunchKernelGGL((rotation_weights_k<T, L, W>), dim3(L * 8 / 16, 2), 256, 0, d.stream, a, blocks,
+                    hipLaunchKernelGGL((rotation_weights_k<T, L, W>), dim3(L * 8 / 16, 2), 1024, 0, d.stream, a, blocks,
                                        static_cast<T*>(dq_weight), static_cast<T*>(dk_weight));
             });
         });
