@@ -14,10 +14,20 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 // The products' operands are f16, times 2^12: entries of X, A and b A + c A^2 lie below 4,
 // and those down to 2^-26 stay in the type's normal range.  f32 and f16 matrices go as sums
 // of two f16 values (22 bits; three of the four products, to 2^-22), so that the products
-// stay as exact as the type; bf16 ones as one.  X itself is kept in floats: its
-// roundings would pass through all later steps, which multiply small singular values by
+// stay as exact as the type; bf16 ones as one.  X itself is kept as a sum of two whatever the
+// type: its roundings pass through all later steps, which multiply small singular values by
 // up to 485.
 constexpr float kUp = 4096.f, kDown = 1.f / (4096.f * 4096.f);
+
+// b A + c A^2 from a = A - one (one: the diagonal, or zero) and a's square.
+template <int PLANES>
+__device__ inline float poly_of(float a, float square, float one) {
+    if (PLANES == 1) {
+        square += 2 * a + one;  // A^2 = (A - 1)^2 + 2 (A - 1) + 1
+        a += one;
+    }
+    return kB * a + kC * square;
+}
 
 struct Orthogonal {
     Device* dev = nullptr;
@@ -27,7 +37,7 @@ struct Orthogonal {
     int side() const { return std::min(rows, columns); }
     int planes() const { return dtype == CPDE_BF16 ? 1 : 2; }
     char* work = nullptr;
-    size_t sums = 0, x = 0, x_half[2] = {}, gram = 0, gram_half = 0, poly = 0, part = 0;  // places in the workspace
+    size_t sums = 0, x[2] = {}, gram = 0, poly = 0, part = 0;  // places in the workspace
 };
 int pitch_of(int columns) { return (columns + 7) / 8 * 8; }
 
@@ -106,11 +116,18 @@ __device__ inline void write_halves(_Float16* to, int64_t plane, const float (&v
     *reinterpret_cast<vec<_Float16, 8>*>(to) = hi;
     if (PLANES == 2) *reinterpret_cast<vec<_Float16, 8>*>(to + plane) = lo;
 }
+template <int PLANES>
+__device__ inline void read_halves(float (&v)[8], const _Float16* from, int64_t plane) {
+    const auto hi = *reinterpret_cast<const vec<_Float16, 8>*>(from);
+    vec<_Float16, 8> lo = {};
+    if (PLANES == 2) lo = *reinterpret_cast<const vec<_Float16, 8>*>(from + plane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float(hi[j]) + float(lo[j])) * (1.f / kUp);
+}
 
-// X = x / |x|, in floats and as the products' operand; columns past the last are zeros.
-template <class T, int PLANES>
-__global__ __launch_bounds__(256) void orthogonal_scale_k(Source<T> s, Shape p, const double* sums, float* x, _Float16* half,
-                                                          int64_t plane) {
+// X = x / |x|; columns past the last are zeros.
+template <class T>
+__global__ __launch_bounds__(256) void orthogonal_scale_k(Source<T> s, Shape p, const double* sums, _Float16* x, int64_t plane) {
     double total = 0;
     for (int i = threadIdx.x; i < p.blocks; i += 256) total += sums[blockIdx.y * p.blocks + i];
     total = sum_block(total);
@@ -122,69 +139,66 @@ __global__ __launch_bounds__(256) void orthogonal_scale_k(Source<T> s, Shape p, 
         float v[8];
         s.template read<false>(v, blockIdx.y, row, first, min(8, p.columns - first));
         for (int j = 0; j < 8; ++j) v[j] = first + j < p.columns ? float(v[j] * down) : 0.f;
-        const int64_t to = (int64_t(blockIdx.y) * p.rows + row) * p.pitch + first;
-        write8(x + to, v, 8, true);
-        write_halves<PLANES>(half + to, plane, v);
+        write_halves<2>(x + (int64_t(blockIdx.y) * p.rows + row) * p.pitch + first, plane, v);
     }
 }
 
-// A from its product.  With one plane an operand, what is squared is A - 1: near the end A
-// is, and the rounding of what differs from it is the smaller by as much.
+// A from its product.  With one plane an operand, what is kept and squared is A - 1: near the
+// end A is, and the rounding of what differs from it is the smaller by as much.
 template <int PLANES>
 struct GramEpilogue {
-    float* gram;
-    _Float16* half;
+    static constexpr bool kSymmetric = true;
+    _Float16* gram;
     int64_t plane;
     int side, pitch;
-    __device__ void row(int batch, int m, int n, int count, float (&v)[8]) const {
-        const int64_t at = (int64_t(batch) * side + m) * pitch + n;
+    __device__ int columns(int, int) const { return 0; }
+    __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < count ? v[j] * kDown : 0.f;
-        write8(gram + at, v, 8, true);
-        if (PLANES == 1)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] -= m == n + j ? 1.f : 0.f;
-        write_halves<PLANES>(half + at, plane, v);
+        for (int j = 0; j < 8; ++j)
+            v[j] = j < count ? v[j] * kDown - (PLANES == 1 && m == n + j ? 1.f : 0.f) : 0.f;
+        write_halves<PLANES>(gram + (int64_t(batch) * side + m) * pitch + n, plane, v);
     }
 };
 // b A + c A^2 from the square of A (or of A - 1, less 1 - 2 A).
 template <int PLANES>
 struct PolyEpilogue {
-    const float* gram;
-    _Float16* half;
+    static constexpr bool kSymmetric = true;
+    const _Float16* gram;
+    _Float16* poly;
     int64_t plane;
     int side, pitch;
-    __device__ void row(int batch, int m, int n, int count, float (&v)[8]) const {
+    __device__ int columns(int, int) const { return 0; }
+    __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
         const int64_t at = (int64_t(batch) * side + m) * pitch + n;
         float a[8];
-        read8(a, gram + at, 8, true);
+        read_halves<PLANES>(a, gram + at, plane);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float square = v[j] * kDown;
-            if (PLANES == 1) square += 2 * a[j] - (m == n + j ? 1.f : 0.f);
-            v[j] = j < count ? kB * a[j] + kC * square : 0.f;
+            const float one = PLANES == 1 && m == n + j ? 1.f : 0.f, square = v[j] * kDown;
+            v[j] = j < count ? poly_of<PLANES>(a[j], square, one) : 0.f;
         }
-        write_halves<PLANES>(half + at, plane, v);
+        write_halves<PLANES>(poly + at, plane, v);
     }
 };
 // The next X; after the last step out, or the weights' step along it.
-template <class T, int PLANES>
+template <class T>
 struct StepEpilogue {
-    float* x;
-    _Float16* half;  // null: the last step
+    static constexpr bool kSymmetric = false;
+    const _Float16* x;
+    _Float16* next;  // null: the last step
     int64_t plane;
     int rows, pitch, wide, update;
     Matrices<T> out;
     float keep, rate;  // weights <- keep weights - rate X
-    __device__ void row(int batch, int m, int n, int count, float (&v)[8]) const {
+    __device__ int columns(int, int) const { return 0; }
+    __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
         const int64_t at = (int64_t(batch) * rows + m) * pitch + n;
         float old[8];
-        read8(old, x + at, 8, true);
+        read_halves<2>(old, x + at, plane);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = j < count ? kA * old[j] + v[j] * kDown : 0.f;
-        if (half) {
-            write8(x + at, v, 8, true);
-            write_halves<PLANES>(half + at, plane, v);
+        if (next) {
+            write_halves<2>(next + at, plane, v);
             return;
         }
         T* to = out.at(batch, m) + n;
@@ -197,6 +211,195 @@ struct StepEpilogue {
         write8(to, v, count, wide);
     }
 };
+
+// ---- small matrices in one launch -----------------------------------------------------------
+// A workgroup takes a matrix of at most 128 x 128 through all steps: X and A (then
+// b A + c A^2) stay in LDS as the products' operands, the matrix lying so that it is at
+// least as wide as high, a wave's 64 x 32 of X and A in registers besides.  Bound: the products of
+// one CU (128 x 128 f32: 1.2 us each at the matrix unit's rate) and the barriers between them.
+constexpr int kSmall = 128;
+struct SmallArgs {
+    int rows, columns, steps;  // as the caller has them
+    int wide, update;
+    float keep, rate;
+};
+// Chunk `chunk` of row `row` of a [128][128] f16 matrix in LDS, turned so that both 16 rows'
+// same chunk and four rows' 64 bytes lie in different banks.
+__device__ inline int small_at(int row, int chunk) {
+    return row * 256 + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
+}
+__device__ inline Frag<_Float16> small_row(const char* matrix, int block, int s, int lane) {
+    return *reinterpret_cast<const Frag<_Float16>*>(matrix + small_at(32 * block + (lane & 31), 2 * s + (lane >> 5)));
+}
+__device__ inline Frag<_Float16> small_column(const char* matrix, int block, int s, int lane) {
+    const int row = 16 * s + 8 * (lane >> 5) + ((lane & 15) >> 2), chunk = 4 * block + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4* at;
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(matrix + small_at(row, chunk) + (lane & 1) * 8));
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(matrix + small_at(row + 4, chunk) + (lane & 1) * 8));
+    return __builtin_bit_cast(Frag<_Float16>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <class T, int PLANES>
+__global__ __launch_bounds__(512, 2) void orthogonal_small_k(Source<T> s, SmallArgs p, Matrices<T> out) {
+    constexpr int kPlane = kSmall * 256;  // bytes
+    __shared__ __align__(16) char x_lds[2 * kPlane];
+    __shared__ __align__(16) char g_lds[PLANES * kPlane];
+    __shared__ double sums[8];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, matrix = blockIdx.x;
+    const bool tall = p.rows > p.columns;
+    const int high = min(p.rows, p.columns), wide = max(p.rows, p.columns);
+    // the matrix, its size, and X in LDS (its transpose where it is tall), zeros around it
+    for (int i = threadIdx.x; i < 2 * kPlane / 16; i += 512) *reinterpret_cast<u32x4*>(x_lds + i * 16) = u32x4{0, 0, 0, 0};
+    const int per_row = (p.columns + 7) / 8, all = p.rows * per_row;
+    constexpr int kMost = kSmall * kSmall / 8 / 512;  // (128 rows of 16 chunks)
+    float v[kMost][8];
+    double total = 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int at = i * 512 + threadIdx.x, row = at / per_row, first = at % per_row * 8;
+        const int count = at < all ? min(8, p.columns - first) : 0;
+        if (count > 0) s.template read<true>(v[i], matrix, row, first, count);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[i][j] = j < count ? v[i][j] : 0.f;
+            total += double(v[i][j]) * double(v[i][j]);
+        }
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+    if (lane == 0) sums[wave] = total;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < 8; ++w) total += sums[w];
+    const double down = total > 0 ? double(kUp) / sqrt(total) : total;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int at = i * 512 + threadIdx.x, row = at / per_row, first = at % per_row * 8;
+        if (at < all)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (first + j >= p.columns) continue;
+                const float up = float(v[i][j] * down);
+                const _Float16 hi = _Float16(up), lo = _Float16(up - float(hi));
+                const int r = tall ? first + j : row, c = tall ? row : first + j;
+                char* to = x_lds + small_at(r, c / 8) + (c & 7) * 2;
+                *reinterpret_cast<_Float16*>(to) = hi;
+                *reinterpret_cast<_Float16*>(to + kPlane) = lo;
+            }
+    }
+    __syncthreads();
+    // this wave's part: rows 64 wm.., columns 32 wn..
+    const int wm = wave & 1, wn = wave >> 1;
+    const auto busy = [&](int i, int columns) { return 64 * wm + 32 * i < high && 32 * wn < columns; };
+    const auto put = [&](char* to, int planes, int i, const Acc& c) __attribute__((always_inline)) {
+        const int row = 64 * wm + 32 * i + (lane & 31);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            vec<_Float16, 4> hi, lo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float up = c[4 * g + j] * kUp;
+                hi[j] = _Float16(up);
+                lo[j] = _Float16(up - float(hi[j]));
+            }
+            char* at = to + small_at(row, 4 * wn + g) + 8 * half;
+            *reinterpret_cast<vec<_Float16, 4>*>(at) = hi;
+            if (planes == 2) *reinterpret_cast<vec<_Float16, 4>*>(at + kPlane) = lo;
+        }
+    };
+    // sum over k of A(m, k) B(n, k): rows of `a`, rows or columns of `b`
+    const auto product = [&](Acc (&c)[2], const char* a, const char* b, int steps, auto rows) __attribute__((always_inline)) {
+        c[0] = c[1] = Acc{};
+        for (int k = 0; k < steps; ++k) {
+            Frag<_Float16> fb[PLANES], fa[2][PLANES];
+#pragma unroll
+            for (int q = 0; q < PLANES; ++q) {
+                fb[q] = decltype(rows)::value ? small_row(b + q * kPlane, wn, k, lane) : small_column(b + q * kPlane, wn, k, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) fa[i][q] = small_row(a + q * kPlane, 2 * wm + i, k, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (PLANES == 2) {
+                    c[i] = multiply(fb[1 % PLANES], fa[i][0], c[i]);
+                    c[i] = multiply(fb[0], fa[i][1 % PLANES], c[i]);
+                }
+                c[i] = multiply(fb[0], fa[i][0], c[i]);
+            }
+        }
+    };
+    Acc x[2], a[2], c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = 64 * wm + 32 * i + (lane & 31);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const char* at = x_lds + small_at(row, 4 * wn + g) + 8 * half;
+            const auto hi = *reinterpret_cast<const vec<_Float16, 4>*>(at), lo = *reinterpret_cast<const vec<_Float16, 4>*>(at + kPlane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][4 * g + j] = (float(hi[j]) + float(lo[j])) * (1.f / kUp);
+        }
+    }
+    const int side_steps = (high + 15) / 16, wide_steps = (wide + 15) / 16;
+    const std::true_type by_rows{};
+    const std::false_type by_columns{};
+    for (int step = 0; step < p.steps; ++step) {
+        if (busy(0, high)) product(a, x_lds, x_lds, wide_steps, by_rows);
+        else a[0] = a[1] = Acc{};
+        // (with one plane A - 1 is what is squared; the diagonal outside the matrix stays zero)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = 64 * wm + 32 * i + (lane & 31), n = 32 * wn + 8 * (e >> 2) + 4 * half + (e & 3);
+                a[i][e] = a[i][e] * kDown - (PLANES == 1 && m == n && m < high ? 1.f : 0.f);
+            }
+        put(g_lds, PLANES, 0, a[0]);
+        put(g_lds, PLANES, 1, a[1]);
+        __syncthreads();
+        if (busy(0, high)) product(c, g_lds, g_lds, side_steps, by_rows);
+        else c[0] = c[1] = Acc{};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = 64 * wm + 32 * i + (lane & 31), n = 32 * wn + 8 * (e >> 2) + 4 * half + (e & 3);
+                c[i][e] = poly_of<PLANES>(a[i][e], c[i][e] * kDown, PLANES == 1 && m == n && m < high ? 1.f : 0.f);
+            }
+        __syncthreads();
+        put(g_lds, PLANES, 0, c[0]);
+        put(g_lds, PLANES, 1, c[1]);
+        __syncthreads();
+        if (busy(0, wide)) product(c, g_lds, x_lds, side_steps, by_columns);
+        else c[0] = c[1] = Acc{};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = kA * x[i] + kDown * c[i];
+        __syncthreads();
+        if (step + 1 < p.steps) {
+            put(x_lds, 2, 0, x[0]);
+            put(x_lds, 2, 1, x[1]);
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int m = 64 * wm + 32 * i + (lane & 31);
+        if (m >= high) continue;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int n = 32 * wn + 8 * g + 4 * half;
+            if (n >= wide) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (n + j >= wide) continue;
+                T* to = tall ? out.at(matrix, n + j) + m : out.at(matrix, m) + n + j;
+                const float y = x[i][4 * g + j];
+                *to = T(p.update ? p.keep * float(*to) - p.rate * y : y);
+            }
+        }
+    }
+}
 
 // ---- on the host ----------------------------------------------------------------------------
 const Planes kOne = {1, 0, 0};
@@ -221,20 +424,24 @@ bool wide_matrices(const cpde_matrices* x, size_t size) {
 }
 
 template <class T, int PLANES>
-void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> last) {
+void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T> last) {
     Device& d = *p.dev;
+    if (p.rows <= kSmall && p.columns <= kSmall) {
+        const SmallArgs a{p.rows, p.columns, p.steps, last.wide, last.update, last.keep, last.rate};
+        hipLaunchKernelGGL((orthogonal_small_k<T, PLANES>), unsigned(p.count), 512, 0, d.stream, source, a, last.out);
+        HIP_CHECK(hipGetLastError());
+        return;
+    }
     const int pitch = pitch_of(p.columns), side = p.side(), side_pitch = pitch_of(side);
     const int64_t plane = int64_t(p.count) * p.rows * pitch, side_plane = int64_t(p.count) * side * side_pitch;
     const auto at = [&](size_t place) { return p.work + place; };
     double* sums = reinterpret_cast<double*>(at(p.sums));
-    float *x = reinterpret_cast<float*>(at(p.x)), *gram = reinterpret_cast<float*>(at(p.gram));
-    _Float16 *x_half[2] = {reinterpret_cast<_Float16*>(at(p.x_half[0])), reinterpret_cast<_Float16*>(at(p.x_half[1]))};
-    _Float16 *gram_half = reinterpret_cast<_Float16*>(at(p.gram_half)), *poly = reinterpret_cast<_Float16*>(at(p.poly));
+    _Float16 *x[2] = {reinterpret_cast<_Float16*>(at(p.x[0])), reinterpret_cast<_Float16*>(at(p.x[1]))};
+    _Float16 *gram = reinterpret_cast<_Float16*>(at(p.gram)), *poly = reinterpret_cast<_Float16*>(at(p.poly));
     const Shape shape{p.rows, p.columns, pitch, p.blocks};
     hipLaunchKernelGGL((orthogonal_sums_k<T>), dim3(p.blocks, p.count), 256, 0, d.stream, source, shape, sums);
     HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((orthogonal_scale_k<T, PLANES>), dim3(p.blocks, p.count), 256, 0, d.stream, source, shape, sums, x,
-                       x_half[0], plane);
+    hipLaunchKernelGGL((orthogonal_scale_k<T>), dim3(p.blocks, p.count), 256, 0, d.stream, source, shape, sums, x[0], plane);
     HIP_CHECK(hipGetLastError());
     const auto operand = [&](const _Float16* data, int rows, int columns, int64_t plane_) {
         Operand o = product_operand(data, columns, columns, 2);
@@ -247,23 +454,25 @@ void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> l
     g.planes = PLANES == 2 ? kTwo : kOne;
     g.part = reinterpret_cast<float*>(at(p.part));
     for (int step = 0; step < p.steps; ++step) {
-        const Operand xs = operand(x_half[step & 1], p.rows, pitch, plane);
-        const Operand as = operand(gram_half, side, side_pitch, side_plane), ps = operand(poly, side, side_pitch, side_plane);
+        const Operand xs = operand(x[step & 1], p.rows, pitch, plane);
+        const Operand as = operand(gram, side, side_pitch, side_plane), ps = operand(poly, side, side_pitch, side_plane);
         ProductArgs q = g;
+        q.symmetric = 1;
         q.m = q.n = side;
         q.a = q.b = xs;
         q.k = p.tall() ? p.rows : p.columns;
-        const GramEpilogue<PLANES> ge{gram, gram_half, side_plane, side, side_pitch};
+        const GramEpilogue<PLANES> ge{gram, side_plane, side, side_pitch};
         if (p.tall()) launch_product<_Float16, false, false>(d, q, ge);
         else launch_product<_Float16, true, true>(d, q, ge);
         q.a = q.b = as;
         q.k = side;
         launch_product<_Float16, true, true>(d, q, PolyEpilogue<PLANES>{gram, poly, side_plane, side, side_pitch});
+        q.symmetric = 0;
         q.m = p.rows;
         q.n = p.columns;
-        StepEpilogue<T, PLANES> se = last;
-        se.x = x;
-        se.half = step + 1 < p.steps ? x_half[(step + 1) & 1] : nullptr;
+        StepEpilogue<T> se = last;
+        se.x = x[step & 1];
+        se.next = step + 1 < p.steps ? x[(step + 1) & 1] : nullptr;
         se.plane = plane;
         se.rows = p.rows;
         se.pitch = pitch;
@@ -280,14 +489,13 @@ void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> l
 }
 template <class T>
 void run_typed(const Orthogonal& p, const Source<T>& source, const cpde_matrices* out, bool update, float keep, float rate) {
-    constexpr int kPlanes = std::is_same_v<T, bf16> ? 1 : 2;
-    StepEpilogue<T, kPlanes> last{};
+    StepEpilogue<T> last{};
     last.out = matrices<T>(out);
     last.wide = wide_matrices(out, sizeof(T));
     last.update = update;
     last.keep = keep;
     last.rate = rate;
-    run<T, kPlanes>(p, source, last);
+    run<T, std::is_same_v<T, bf16> ? 1 : 2>(p, source, last);
 }
 // Operations of a call: three products a step, the symmetric two by halves.
 double flops(const Orthogonal& p) {
@@ -328,14 +536,15 @@ int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int
             at += (bytes + 255) / 256 * 256;
             return here;
         };
-        p->sums = place(sizeof(double) * n * p->blocks);
-        p->x = place(sizeof(float) * n * rows * pitch);
-        for (auto& half : p->x_half) half = place(2 * p->planes() * n * rows * pitch);
-        p->gram = place(sizeof(float) * n * side * side_pitch);
-        p->gram_half = place(2 * p->planes() * n * side * side_pitch);
-        p->poly = place(2 * p->planes() * n * side * side_pitch);
-        p->part = place(sizeof(float) * std::max(product_part(dev->compute_units, count, side, side),
+        const bool small = rows <= kSmall && columns <= kSmall;
+        if (!small) {
+            p->sums = place(sizeof(double) * n * p->blocks);
+            for (auto& x : p->x) x = place(2 * 2 * n * rows * pitch);
+            p->gram = place(2 * p->planes() * n * side * side_pitch);
+            p->poly = place(2 * p->planes() * n * side * side_pitch);
+            p->part = place(sizeof(float) * std::max(product_part(dev->compute_units, count, side, side),
                                                  product_part(dev->compute_units, count, rows, columns)));
+        }
         HIP_CHECK(hipMalloc(&p->work, std::max<size_t>(at, 256)));
         *out = p.release();
     });

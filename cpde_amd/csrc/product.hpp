@@ -24,6 +24,7 @@ struct Planes {
 struct ProductArgs {
     Operand a, b;
     int m, n, k, batch;
+    int symmetric;     // C is symmetric: tiles on and below its diagonal, mirrored as they are stored
     int m_tiles, n_tiles;
     int splits, span;  // of the inner axis, and a split's tiles of it
     float* part;       // [split][batch][m][n] where there are several
@@ -230,6 +231,14 @@ __device__ inline void tile_of(int at, int count, int m_tiles, int n_tiles, int&
     tn = in / height;
 }
 
+// The tiles on and below the diagonal, row by row.
+__device__ inline void triangle_of(int at, int& tm, int& tn) {
+    tm = int((sqrtf(8.f * at + 1.f) - 1.f) * 0.5f);
+    while (tm * (tm + 1) / 2 > at) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= at) ++tm;
+    tn = at - tm * (tm + 1) / 2;
+}
+
 // Up to eight neighbouring values of a row, as floats.
 template <class T>
 __device__ inline void read8(float (&v)[8], const T* p, int count, bool wide) {
@@ -237,9 +246,9 @@ __device__ inline void read8(float (&v)[8], const T* p, int count, bool wide) {
     if (wide && count == 8) {
 #pragma unroll
         for (int part = 0; part < 8; part += N) {
-            const auto in = *reinterpret_cast<const vec<T, N>*>(p + part);
+            const auto in = __builtin_convertvector(*reinterpret_cast<const vec<T, N>*>(p + part), vec<float, N>);
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[part + j] = float(in[j]);
+            for (int j = 0; j < N; ++j) v[part + j] = in[j];
         }
     } else {
 #pragma unroll
@@ -252,10 +261,10 @@ __device__ inline void write8(T* p, const float (&v)[8], int count, bool wide) {
     if (wide && count == 8) {
 #pragma unroll
         for (int part = 0; part < 8; part += N) {
-            vec<T, N> out;
+            vec<float, N> out;
 #pragma unroll
-            for (int j = 0; j < N; ++j) out[j] = T(v[part + j]);
-            *reinterpret_cast<vec<T, N>*>(p + part) = out;
+            for (int j = 0; j < N; ++j) out[j] = v[part + j];
+            *reinterpret_cast<vec<T, N>*>(p + part) = __builtin_convertvector(out, vec<T, N>);
         }
     } else {
 #pragma unroll
@@ -281,7 +290,7 @@ struct Tiles {
     A a;
     B b;
     uint32_t a_offset[A::kSteps], b_offset[B::kSteps];
-    int lane, wave, wm, wn, split, batch, m0, n0, plane, steps;
+    int lane, wave, wm, wn, split, batch, m0, n0, plane, steps, mirrored;
     Acc acc[kMB][kNB];
 
     __device__ __attribute__((always_inline)) void start(const ProductArgs& p) {
@@ -292,7 +301,9 @@ struct Tiles {
         split = blockIdx.y % p.splits;
         batch = blockIdx.y / p.splits;
         int tm, tn;
-        tile_of(blockIdx.x, p.m_tiles * p.n_tiles, p.m_tiles, p.n_tiles, tm, tn);
+        if (p.symmetric) triangle_of(blockIdx.x, tm, tn);
+        else tile_of(blockIdx.x, p.m_tiles * p.n_tiles, p.m_tiles, p.n_tiles, tm, tn);
+        mirrored = p.symmetric && tm != tn;
         m0 = tm * BM;
         n0 = tn * BN;
         const int t = split * p.span;
@@ -342,7 +353,8 @@ struct Tiles {
     __device__ __attribute__((always_inline)) void finish(const ProductArgs& p, const Epilogue& e, char* lds) {
         float* stage = reinterpret_cast<float*>(lds + wave * kStage);
         constexpr int kLanes = WN / 8, kAtOnce = 64 / kLanes;
-        const int half = lane >> 5;
+        const int half = lane >> 5, column = (lane % kLanes) * 8, n = n0 + wn * WN + column;
+        const auto columns = e.columns(n, min(8, p.n - n));
 #pragma unroll
         for (int i = 0; i < kMB; ++i) {
 #pragma unroll
@@ -355,8 +367,7 @@ struct Tiles {
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int r = 0; r < 32 / kAtOnce; ++r) {
-                const int row = r * kAtOnce + lane / kLanes, column = (lane % kLanes) * 8;
-                const int m = m0 + wm * WM + 32 * i + row, n = n0 + wn * WN + column;
+                const int row = r * kAtOnce + lane / kLanes, m = m0 + wm * WM + 32 * i + row;
                 float v[8];
                 *reinterpret_cast<Quad*>(v) = *reinterpret_cast<const Quad*>(stage + row * kPitch + column);
                 *reinterpret_cast<Quad*>(v + 4) = *reinterpret_cast<const Quad*>(stage + row * kPitch + column + 4);
@@ -364,7 +375,20 @@ struct Tiles {
                 if (p.splits > 1)
                     write8(p.part + ((int64_t(split) * p.batch + batch) * p.m + m) * p.n + n, v, min(8, p.n - n), p.n % 4 == 0);
                 else
-                    e.row(batch, m, n, min(8, p.n - n), v);
+                    e.row(columns, batch, m, n, min(8, p.n - n), v);
+            }
+            if constexpr (Epilogue::kSymmetric) {
+                // the same with rows and columns exchanged: eight rows of a column a lane
+                if (mirrored && p.splits == 1)
+#pragma unroll
+                    for (int r = 0; r < WN / 16; ++r) {
+                        const int to = r * 16 + lane / 4, from = 8 * (lane % 4);
+                        const int m = n0 + wn * WN + to, n = m0 + wm * WM + 32 * i + from;
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = stage[(from + j) * kPitch + to];
+                        if (m < p.n && n < p.m) e.row(e.columns(n, min(8, p.m - n)), batch, m, n, min(8, p.m - n), v);
+                    }
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -538,7 +562,8 @@ __global__ __launch_bounds__(512) void product_run_k(ProductArgs p, Epilogue e) 
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += from[j];
         }
-        if (m0 + row < p.m && n0 + column < p.n) e.row(batch, m0 + row, n0 + column, min(8, p.n - n0 - column), v);
+        const int n = n0 + column, count = min(8, p.n - n);
+        if (m0 + row < p.m && n < p.n) e.row(e.columns(n, count), batch, m0 + row, n, count, v);
     }
 }
 template <class T>
@@ -559,7 +584,43 @@ __global__ __launch_bounds__(256) void product_join_k(ProductArgs p, Epilogue e)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += one[j];
     }
-    e.row(batch, int(row - int64_t(batch) * p.m), n, count, v);
+    e.row(e.columns(n, count), batch, int(row - int64_t(batch) * p.m), n, count, v);
+}
+
+// The same of a symmetric product: 64 x 64 on and below the diagonal a workgroup, stored
+// twice.
+template <class Epilogue>
+__global__ __launch_bounds__(256) void product_join_symmetric_k(ProductArgs p, Epilogue e) {
+    __shared__ float stage[64][65];
+    int tm, tn;
+    triangle_of(blockIdx.x, tm, tn);
+    const int batch = blockIdx.y, row = threadIdx.x / 4, column = threadIdx.x % 4 * 16;
+#pragma unroll
+    for (int part = 0; part < 16; part += 8) {
+        const int m = tm * 64 + row, n = tn * 64 + column + part, count = min(8, p.n - n);
+        float v[8] = {};
+        if (m < p.m && n < p.n) {
+            for (int s = 0; s < p.splits; ++s) {
+                float one[8];
+                read8(one, p.part + ((int64_t(s) * p.batch + batch) * p.m + m) * p.n + n, count, p.n % 4 == 0);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += one[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) stage[row][column + part + j] = v[j];
+        if (m < p.m && n < p.n) e.row(e.columns(n, count), batch, m, n, count, v);
+    }
+    __syncthreads();
+    if (tm == tn) return;
+#pragma unroll
+    for (int part = 0; part < 16; part += 8) {
+        const int m = tn * 64 + row, n = tm * 64 + column + part, count = min(8, p.m - n);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = stage[column + part + j][row];
+        if (m < p.n && n < p.m) e.row(e.columns(n, count), batch, m, n, count, v);
+    }
 }
 
 // ---- on the host --------------------------------------------------------------------------
@@ -584,12 +645,13 @@ struct ProductTime {
 constexpr ProductTime kTimes16[] = {{64, 3.8, 0.30, 0.195}, {128, 5.0, 0.63, 0.48}, {256, 11.5, 1.50, 1.50}};
 constexpr ProductTime kTimes32[] = {{64, 4.5, 0.65, 0.53}, {128, 8.0, 1.60, 1.43}};
 // planes: products of planes.
-inline ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, int planes, int size, bool wide) {
+inline ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, int planes, int size, bool wide,
+                              bool symmetric) {
     ProductCut best;
     double least = 1e30;
     const int64_t deep = std::max<int64_t>(1, (k + kTileBytes / size - 1) / (kTileBytes / size)) * planes;
     const auto consider = [&](const ProductTime& t) {
-        const int64_t tiles = batch * ceil_div(m, t.side) * int64_t(ceil_div(n, t.side));
+        const int64_t rows = ceil_div(m, t.side), tiles = batch * (symmetric ? rows * (rows + 1) / 2 : rows * ceil_div(n, t.side));
         for (int splits = 1; splits <= kMostSplits && (splits == 1 || (splits * 2 <= deep && t.side < 256)); ++splits) {
             if (splits > 1 && splits * batch * m * n > kPartTiles * compute_units * 128 * 128) break;
             const int64_t each = (tiles * splits + compute_units - 1) / compute_units;
@@ -638,9 +700,10 @@ template <class K, class E>
 void launch_tiles(Device& d, K kernel, int side, int threads, ProductArgs p, const E& e, size_t lds = 0) {
     p.m_tiles = ceil_div(p.m, side);
     p.n_tiles = ceil_div(p.n, side);
-    require(int64_t(p.m_tiles) * p.n_tiles * threads < (int64_t(1) << 31) && int64_t(p.splits) * p.batch < 65536,
+    const int64_t tiles = p.symmetric ? int64_t(p.m_tiles) * (p.m_tiles + 1) / 2 : int64_t(p.m_tiles) * p.n_tiles;
+    require(tiles * threads < (int64_t(1) << 31) && int64_t(p.splits) * p.batch < 65536,
             "too many workgroups");
-    hipLaunchKernelGGL(kernel, dim3(unsigned(p.m_tiles) * p.n_tiles, unsigned(p.splits) * p.batch), threads, lds, d.stream, p, e);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(tiles), unsigned(p.splits) * p.batch), threads, lds, d.stream, p, e);
     HIP_CHECK(hipGetLastError());
 }
 
@@ -649,12 +712,13 @@ template <class T, bool AK, bool BK, class E>
 void launch_product(Device& d, ProductArgs p, const E& e) {
     if (!p.m || !p.n || !p.batch) return;
     const bool wide = p.a.wide && p.b.wide;
-    const ProductCut c = cut_product(d.compute_units, p.batch, p.m, p.n, p.k, p.planes.count, sizeof(T), wide);
+    const ProductCut c = cut_product(d.compute_units, p.batch, p.m, p.n, p.k, p.planes.count, sizeof(T), wide, p.symmetric);
     const int deep = std::max(1, ceil_div(p.k, kDepth<T>));
     p.span = ceil_div(deep, std::min(c.splits, deep));
     p.splits = ceil_div(deep, p.span);
     if (c.side == 32) {
         const size_t lds = c.waves * kRunBytes<T>;
+        p.symmetric = 0;  // (whole tiles of both halves)
         if (wide) launch_tiles(d, product_run_k<T, AK, BK, false, E>, 32, 64 * c.waves, p, e, lds);
         else launch_tiles(d, product_run_k<T, AK, BK, true, E>, 32, 64 * c.waves, p, e, lds);
     } else if (!wide) {
@@ -667,6 +731,14 @@ void launch_product(Device& d, ProductArgs p, const E& e) {
         if constexpr (sizeof(T) == 2) launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
     }
     if (p.splits > 1) {
+        if constexpr (E::kSymmetric)
+            if (p.symmetric) {
+                const int64_t rows = ceil_div(p.m, 64);
+                hipLaunchKernelGGL((product_join_symmetric_k<E>), dim3(unsigned(rows * (rows + 1) / 2), unsigned(p.batch)), 256, 0,
+                                   d.stream, p, e);
+                HIP_CHECK(hipGetLastError());
+                return;
+            }
         const int64_t lanes = int64_t(p.batch) * p.m * ((p.n + 7) / 8);
         hipLaunchKernelGGL((product_join_k<E>), unsigned((lanes + 255) / 256), 256, 0, d.stream, p, e);
         HIP_CHECK(hipGetLastError());

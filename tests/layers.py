@@ -159,7 +159,8 @@ def orthogonal_first(x, dtype):
     poly_off = abs(b) * gram_off + c * (square_off + (2 * gram_off if dtype == 'bf16' else 0)) + 8 * E * (1 + gram.abs())
     poly_off = poly_off + h * (poly.abs() + poly_off) + least
     y = a * x + poly @ x
-    y_off = (poly_off @ x.abs() + (poly.abs() + poly_off) @ (h * x.abs() + least)
+    # (X itself is a sum of two f16 values, to `least` where it is small)
+    y_off = (a * (PAIR * x.abs() + least) + poly_off @ x.abs() + (poly.abs() + poly_off) @ (h * x.abs() + least)
              + (3 * r + 16) * E * (poly.abs() @ x.abs()) + 8 * E * (a * x.abs() + y.abs()))
     y_off = y_off + UNIT[dtype] * (y.abs() + y_off) + TINY[dtype]
     return tuple((t.transpose(1, 2) if tall else t).contiguous() for t in (y, y_off))
