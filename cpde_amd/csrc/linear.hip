@@ -57,7 +57,7 @@ __device__ inline float slope(float z) {
 // with residual = y, onto what is there.)
 template <class T>
 struct LinearEpilogue {
-    static constexpr bool kSymmetric = false;
+    static constexpr bool kSymmetric = false, kAny = true;
     T *y, *pre;
     const T *bias, *residual;
     int64_t y_stride, pre_stride, residual_stride;
@@ -176,7 +176,6 @@ void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
     args.n = s.n;
     args.k = int(s.k);
     args.batch = 1;
-    args.planes = {1, 0, 0};
     args.part = reinterpret_cast<float*>(p.work + p.part);
     args.a = product_operand(s.a, s.a_stride, AK ? s.k : s.m, sizeof(T));
     args.b = product_operand(s.b, s.b_stride, BK ? s.k : s.n, sizeof(T));

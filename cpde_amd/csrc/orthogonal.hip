@@ -39,7 +39,7 @@ struct Orthogonal {
     char* work = nullptr;
     size_t sums = 0, x[2] = {}, gram = 0, poly = 0, part = 0;  // places in the workspace
 };
-int pitch_of(int columns) { return (columns + 7) / 8 * 8; }
+int pitch_of(int columns) { return (columns + 31) / 32 * 32; }  // (whole groups of pairs)
 
 template <class T>
 struct Matrices {
@@ -103,9 +103,16 @@ __global__ __launch_bounds__(256) void orthogonal_sums_k(Source<T> s, Shape p, d
     if (threadIdx.x == 0) sums[blockIdx.y * p.blocks + blockIdx.x] = total;
 }
 
-// Eight values as f16, or as the sums of two, times 2^12.
+// Where eight values of a matrix of f16 (PLANES 1: and a second one, `plane` on, of what they
+// leave) or of pairs stand, and how far on their second parts.
 template <int PLANES>
-__device__ inline void write_halves(_Float16* to, int64_t plane, const float (&v)[8]) {
+__device__ inline int64_t half_at(int64_t row, int pitch, int n) {
+    return PLANES == 1 ? row * pitch + n : 2 * row * pitch + (n / 32) * 64 + n % 32;
+}
+template <int PLANES>
+__device__ inline int64_t second_of(int64_t plane) { return PLANES == 1 ? plane : 32; }
+// Eight values as f16, times 2^12, and what they leave.
+__device__ inline void write_halves(_Float16* to, int64_t second, bool both, const float (&v)[8]) {
     vec<_Float16, 8> hi, lo;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -114,19 +121,18 @@ __device__ inline void write_halves(_Float16* to, int64_t plane, const float (&v
         lo[j] = _Float16(up - float(hi[j]));
     }
     *reinterpret_cast<vec<_Float16, 8>*>(to) = hi;
-    if (PLANES == 2) *reinterpret_cast<vec<_Float16, 8>*>(to + plane) = lo;
+    if (both) *reinterpret_cast<vec<_Float16, 8>*>(to + second) = lo;
 }
-template <int PLANES>
-__device__ inline void read_halves(float (&v)[8], const _Float16* from, int64_t plane) {
+__device__ inline void read_halves(float (&v)[8], const _Float16* from, int64_t second, bool both) {
     const auto hi = *reinterpret_cast<const vec<_Float16, 8>*>(from);
     vec<_Float16, 8> lo = {};
-    if (PLANES == 2) lo = *reinterpret_cast<const vec<_Float16, 8>*>(from + plane);
+    if (both) lo = *reinterpret_cast<const vec<_Float16, 8>*>(from + second);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (float(hi[j]) + float(lo[j])) * (1.f / kUp);
 }
 
 // X = x / |x|; columns past the last are zeros.
-template <class T>
+template <class T, int PLANES>
 __global__ __launch_bounds__(256) void orthogonal_scale_k(Source<T> s, Shape p, const double* sums, _Float16* x, int64_t plane) {
     double total = 0;
     for (int i = threadIdx.x; i < p.blocks; i += 256) total += sums[blockIdx.y * p.blocks + i];
@@ -139,7 +145,7 @@ __global__ __launch_bounds__(256) void orthogonal_scale_k(Source<T> s, Shape p, 
         float v[8];
         s.template read<false>(v, blockIdx.y, row, first, min(8, p.columns - first));
         for (int j = 0; j < 8; ++j) v[j] = first + j < p.columns ? float(v[j] * down) : 0.f;
-        write_halves<2>(x + (int64_t(blockIdx.y) * p.rows + row) * p.pitch + first, plane, v);
+        write_halves(x + half_at<PLANES>(int64_t(blockIdx.y) * p.rows + row, p.pitch, first), second_of<PLANES>(plane), true, v);
     }
 }
 
@@ -147,43 +153,41 @@ __global__ __launch_bounds__(256) void orthogonal_scale_k(Source<T> s, Shape p, 
 // end A is, and the rounding of what differs from it is the smaller by as much.
 template <int PLANES>
 struct GramEpilogue {
-    static constexpr bool kSymmetric = true;
+    static constexpr bool kSymmetric = true, kAny = false;
     _Float16* gram;
-    int64_t plane;
     int side, pitch;
     __device__ int columns(int, int) const { return 0; }
     __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             v[j] = j < count ? v[j] * kDown - (PLANES == 1 && m == n + j ? 1.f : 0.f) : 0.f;
-        write_halves<PLANES>(gram + (int64_t(batch) * side + m) * pitch + n, plane, v);
+        write_halves(gram + half_at<PLANES>(int64_t(batch) * side + m, pitch, n), 32, PLANES == 2, v);
     }
 };
 // b A + c A^2 from the square of A (or of A - 1, less 1 - 2 A).
 template <int PLANES>
 struct PolyEpilogue {
-    static constexpr bool kSymmetric = true;
+    static constexpr bool kSymmetric = true, kAny = false;
     const _Float16* gram;
     _Float16* poly;
-    int64_t plane;
     int side, pitch;
     __device__ int columns(int, int) const { return 0; }
     __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
-        const int64_t at = (int64_t(batch) * side + m) * pitch + n;
+        const int64_t at = half_at<PLANES>(int64_t(batch) * side + m, pitch, n);
         float a[8];
-        read_halves<PLANES>(a, gram + at, plane);
+        read_halves(a, gram + at, 32, PLANES == 2);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float one = PLANES == 1 && m == n + j ? 1.f : 0.f, square = v[j] * kDown;
             v[j] = j < count ? poly_of<PLANES>(a[j], square, one) : 0.f;
         }
-        write_halves<PLANES>(poly + at, plane, v);
+        write_halves(poly + at, 32, PLANES == 2, v);
     }
 };
 // The next X; after the last step out, or the weights' step along it.
-template <class T>
+template <class T, int PLANES>
 struct StepEpilogue {
-    static constexpr bool kSymmetric = false;
+    static constexpr bool kSymmetric = false, kAny = false;
     const _Float16* x;
     _Float16* next;  // null: the last step
     int64_t plane;
@@ -192,13 +196,13 @@ struct StepEpilogue {
     float keep, rate;  // weights <- keep weights - rate X
     __device__ int columns(int, int) const { return 0; }
     __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
-        const int64_t at = (int64_t(batch) * rows + m) * pitch + n;
+        const int64_t at = half_at<PLANES>(int64_t(batch) * rows + m, pitch, n), second = second_of<PLANES>(plane);
         float old[8];
-        read_halves<2>(old, x + at, plane);
+        read_halves(old, x + at, second, true);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = j < count ? kA * old[j] + v[j] * kDown : 0.f;
         if (next) {
-            write_halves<2>(next + at, plane, v);
+            write_halves(next + at, second, true, v);
             return;
         }
         T* to = out.at(batch, m) + n;
@@ -311,22 +315,32 @@ __global__ __launch_bounds__(512, 2) void orthogonal_small_k(Source<T> s, SmallA
     // sum over k of A(m, k) B(n, k): rows of `a`, rows or columns of `b`
     const auto product = [&](Acc (&c)[2], const char* a, const char* b, int steps, auto rows) __attribute__((always_inline)) {
         c[0] = c[1] = Acc{};
-        for (int k = 0; k < steps; ++k) {
-            Frag<_Float16> fb[PLANES], fa[2][PLANES];
+        // (a step's fragments are read while the one before is multiplied; the last one reads its own again)
+        Frag<_Float16> fb[2][PLANES], fa[2][2][PLANES];
+        const auto read = [&](int k, int to) __attribute__((always_inline)) {
 #pragma unroll
             for (int q = 0; q < PLANES; ++q) {
-                fb[q] = decltype(rows)::value ? small_row(b + q * kPlane, wn, k, lane) : small_column(b + q * kPlane, wn, k, lane);
+                fb[to][q] = decltype(rows)::value ? small_row(b + q * kPlane, wn, k, lane) : small_column(b + q * kPlane, wn, k, lane);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) fa[i][q] = small_row(a + q * kPlane, 2 * wm + i, k, lane);
+                for (int i = 0; i < 2; ++i) fa[to][i][q] = small_row(a + q * kPlane, 2 * wm + i, k, lane);
             }
+        };
+        const auto multiply_step = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (PLANES == 2) {
-                    c[i] = multiply(fb[1 % PLANES], fa[i][0], c[i]);
-                    c[i] = multiply(fb[0], fa[i][1 % PLANES], c[i]);
+                    c[i] = multiply(fb[from][1 % PLANES], fa[from][i][0], c[i]);
+                    c[i] = multiply(fb[from][0], fa[from][i][1 % PLANES], c[i]);
                 }
-                c[i] = multiply(fb[0], fa[i][0], c[i]);
+                c[i] = multiply(fb[from][0], fa[from][i][0], c[i]);
             }
+        };
+        read(0, 0);
+        for (int k = 0; k < steps; k += 2) {
+            read(min(k + 1, steps - 1), 1);
+            multiply_step(0);
+            read(min(k + 2, steps - 1), 0);
+            if (k + 1 < steps) multiply_step(1);
         }
     };
     Acc x[2], a[2], c[2];
@@ -402,9 +416,6 @@ __global__ __launch_bounds__(512, 2) void orthogonal_small_k(Source<T> s, SmallA
 }
 
 // ---- on the host ----------------------------------------------------------------------------
-const Planes kOne = {1, 0, 0};
-const Planes kTwo = {3, 0b00'01'00, 0b00'00'01};  // (high and low, low and high, high and high)
-
 void check_matrices(const Orthogonal& p, const cpde_matrices* x, bool output) {
     require(x, "null argument");
     if (!p.count || !p.rows || !p.columns) return;
@@ -424,7 +435,7 @@ bool wide_matrices(const cpde_matrices* x, size_t size) {
 }
 
 template <class T, int PLANES>
-void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T> last) {
+void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> last) {
     Device& d = *p.dev;
     if (p.rows <= kSmall && p.columns <= kSmall) {
         const SmallArgs a{p.rows, p.columns, p.steps, last.wide, last.update, last.keep, last.rate};
@@ -432,45 +443,43 @@ void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T> last) {
         HIP_CHECK(hipGetLastError());
         return;
     }
+    using Value = std::conditional_t<PLANES == 2, Pair, _Float16>;  // of the operands
     const int pitch = pitch_of(p.columns), side = p.side(), side_pitch = pitch_of(side);
-    const int64_t plane = int64_t(p.count) * p.rows * pitch, side_plane = int64_t(p.count) * side * side_pitch;
-    const auto at = [&](size_t place) { return p.work + place; };
-    double* sums = reinterpret_cast<double*>(at(p.sums));
-    _Float16 *x[2] = {reinterpret_cast<_Float16*>(at(p.x[0])), reinterpret_cast<_Float16*>(at(p.x[1]))};
-    _Float16 *gram = reinterpret_cast<_Float16*>(at(p.gram)), *poly = reinterpret_cast<_Float16*>(at(p.poly));
+    const auto at = [&](size_t place) { return reinterpret_cast<_Float16*>(p.work + place); };
+    double* sums = reinterpret_cast<double*>(p.work + p.sums);
+    _Float16 *x[2] = {at(p.x[0]), at(p.x[1])}, *gram = at(p.gram), *poly = at(p.poly);
     const Shape shape{p.rows, p.columns, pitch, p.blocks};
+    const int64_t plane = int64_t(p.count) * p.rows * pitch;
     hipLaunchKernelGGL((orthogonal_sums_k<T>), dim3(p.blocks, p.count), 256, 0, d.stream, source, shape, sums);
     HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((orthogonal_scale_k<T>), dim3(p.blocks, p.count), 256, 0, d.stream, source, shape, sums, x[0], plane);
+    hipLaunchKernelGGL((orthogonal_scale_k<T, PLANES>), dim3(p.blocks, p.count), 256, 0, d.stream, source, shape, sums, x[0], plane);
     HIP_CHECK(hipGetLastError());
-    const auto operand = [&](const _Float16* data, int rows, int columns, int64_t plane_) {
-        Operand o = product_operand(data, columns, columns, 2);
-        o.plane = 2 * plane_;
-        o.batch = int64_t(2) * rows * columns;
+    const auto operand = [&](const _Float16* data, int rows, int columns) {
+        Operand o = product_operand(data, columns, columns, sizeof(Value));
+        o.batch = int64_t(sizeof(Value)) * rows * columns;
         return o;
     };
+    // (an inner axis along rows goes to the end of their zeros)
     ProductArgs g{};
     g.batch = p.count;
-    g.planes = PLANES == 2 ? kTwo : kOne;
-    g.part = reinterpret_cast<float*>(at(p.part));
+    g.part = reinterpret_cast<float*>(p.work + p.part);
     for (int step = 0; step < p.steps; ++step) {
-        const Operand xs = operand(x[step & 1], p.rows, pitch, plane);
-        const Operand as = operand(gram, side, side_pitch, side_plane), ps = operand(poly, side, side_pitch, side_plane);
+        const Operand xs = operand(x[step & 1], p.rows, pitch), as = operand(gram, side, side_pitch), ps = operand(poly, side, side_pitch);
         ProductArgs q = g;
         q.symmetric = 1;
         q.m = q.n = side;
         q.a = q.b = xs;
-        q.k = p.tall() ? p.rows : p.columns;
-        const GramEpilogue<PLANES> ge{gram, side_plane, side, side_pitch};
-        if (p.tall()) launch_product<_Float16, false, false>(d, q, ge);
-        else launch_product<_Float16, true, true>(d, q, ge);
+        q.k = p.tall() ? p.rows : pitch;
+        const GramEpilogue<PLANES> ge{gram, side, side_pitch};
+        if (p.tall()) launch_product<Value, false, false>(d, q, ge);
+        else launch_product<Value, true, true>(d, q, ge);
         q.a = q.b = as;
-        q.k = side;
-        launch_product<_Float16, true, true>(d, q, PolyEpilogue<PLANES>{gram, poly, side_plane, side, side_pitch});
+        q.k = side_pitch;
+        launch_product<Value, true, true>(d, q, PolyEpilogue<PLANES>{gram, poly, side, side_pitch});
         q.symmetric = 0;
         q.m = p.rows;
         q.n = p.columns;
-        StepEpilogue<T> se = last;
+        StepEpilogue<T, PLANES> se = last;
         se.x = x[step & 1];
         se.next = step + 1 < p.steps ? x[(step + 1) & 1] : nullptr;
         se.plane = plane;
@@ -479,23 +488,26 @@ void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T> last) {
         if (p.tall()) {
             q.a = xs;
             q.b = ps;
-            launch_product<_Float16, true, true>(d, q, se);
+            launch_product<Value, true, true>(d, q, se);
         } else {
+            // (the last columns of b A + c A^2 meet rows of X that there are not: k ends with them)
             q.a = ps;
             q.b = xs;
-            launch_product<_Float16, true, false>(d, q, se);
+            q.k = side;
+            launch_product<Value, true, false>(d, q, se);
         }
     }
 }
 template <class T>
 void run_typed(const Orthogonal& p, const Source<T>& source, const cpde_matrices* out, bool update, float keep, float rate) {
-    StepEpilogue<T> last{};
+    constexpr int kPlanes = std::is_same_v<T, bf16> ? 1 : 2;
+    StepEpilogue<T, kPlanes> last{};
     last.out = matrices<T>(out);
     last.wide = wide_matrices(out, sizeof(T));
     last.update = update;
     last.keep = keep;
     last.rate = rate;
-    run<T, std::is_same_v<T, bf16> ? 1 : 2>(p, source, last);
+    run<T, kPlanes>(p, source, last);
 }
 // Operations of a call: three products a step, the symmetric two by halves.
 double flops(const Orthogonal& p) {
@@ -546,6 +558,8 @@ int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int
                                                  product_part(dev->compute_units, count, rows, columns)));
         }
         HIP_CHECK(hipMalloc(&p->work, std::max<size_t>(at, 256)));
+        // (what stands behind the matrices' columns is never written: zeros)
+        if (!small) launch_fill(*dev, reinterpret_cast<float*>(p->work), at / sizeof(float), 0.f);
         *out = p.release();
     });
 }

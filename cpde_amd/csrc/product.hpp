@@ -7,19 +7,13 @@ namespace cpde {
 namespace {
 
 // A matrix of a product: `stride` bytes from row to row.  Rows are m (or n) where k is
-// contiguous, and k where m (or n) is.  A matrix may stand as several planes whose sum
-// it is, `plane` bytes apart, and be one of a batch, `batch` bytes apart.  wide: its
-// rows are read in whole 16-byte chunks, and its stride leaves a tile's offsets in 31 bits.
+// contiguous, and k where m (or n) is.  It may be one of a batch, `batch` bytes apart.
+// wide: its rows are read in whole 16-byte chunks, and its stride leaves a tile's offsets in
+// 31 bits.
 struct Operand {
     const char* data;
-    int64_t stride, plane, batch;
+    int64_t stride, batch;
     int wide;
-};
-// Products of planes that make up one of the matrices: A's and B's plane numbers, two bits
-// a product from the lowest.
-struct Planes {
-    int count;
-    uint32_t a, b;
 };
 struct ProductArgs {
     Operand a, b;
@@ -28,7 +22,6 @@ struct ProductArgs {
     int m_tiles, n_tiles;
     int splits, span;  // of the inner axis, and a split's tiles of it
     float* part;       // [split][batch][m][n] where there are several
-    Planes planes;
 };
 
 typedef float Acc __attribute__((ext_vector_type(16)));
@@ -74,12 +67,26 @@ __device__ inline Acc multiply(const Split& a, const Split& b, Acc c) {
     c = multiply(a.part[0], b.part[1], c);
     return multiply(a.part[0], b.part[0], c);
 }
-template <class T, bool Exact>
-using Part = std::conditional_t<std::is_same_v<T, float> && !Exact, Split, Frag<T>>;
-template <class T, bool Exact>
-__device__ inline Part<T, Exact> part(Frag<T> f) {
-    if constexpr (std::is_same_v<T, float> && !Exact) return split(f);
+// A fragment as it is multiplied.
+template <bool Exact, class F>
+__device__ inline auto part(const F& f) {
+    if constexpr (std::is_same_v<F, Frag<float>> && !Exact) return split(f);
     else return f;
+}
+
+// A sum of two f16 values, 22 bits together.  Matrices of them hold 32 first parts and then
+// the 32 second ones, and so on, in rows of whole such groups.  Three of the four products
+// are exact to 2^-21 of the factors'.
+struct Pair {
+    _Float16 part[2];
+};
+struct PairFragment {
+    Frag<_Float16> part[2];
+};
+__device__ inline Acc multiply(const PairFragment& a, const PairFragment& b, Acc c) {
+    c = multiply(a.part[1], b.part[0], c);
+    c = multiply(a.part[0], b.part[1], c);
+    return multiply(a.part[0], b.part[0], c);
 }
 
 // A value that is the same in every lane, where the compiler cannot see it.
@@ -107,13 +114,37 @@ struct TileSide {
 
     __device__ static int turn(int row) {
         if (K) return (row >> 1) & 7;
-        if (sizeof(T) == 4) return (((row >> 3) & 1) << 3) & (kChunks - 1);
+        if (std::is_same_v<T, float>) return (((row >> 3) & 1) << 3) & (kChunks - 1);
         return ((row & 3) << 2) & (kChunks - 1);
     }
+    // Of 32 columns from a chunk on: sixteen lanes read four k-rows of sixteen values (four lanes a
+    // row) and get them back transposed, a column each.
+    template <class V>
+    __device__ static Frag<V> transposed(const char* tile, int first, int s, int lane) {
+        const int row = 16 * s + 8 * (lane >> 5) + ((lane & 15) >> 2), chunk = first + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4* at;
+        // (four rows on, the turn is the same)
+        const char* p = tile + row * kRowBytes + ((chunk ^ turn(row)) << 4) + (lane & 1) * 8;
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(p));
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(p + 4 * kRowBytes));
+        return __builtin_bit_cast(Frag<V>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
     // Fragment of rows 32 block + lane % 32, inner indices 16 s + 8 (lane / 32) + j.
-    __device__ static Frag<T> fragment(const char* tile, int block, int s, int lane) {
+    __device__ static auto fragment(const char* tile, int block, int s, int lane) {
         const int half = lane >> 5;
-        if constexpr (K && sizeof(T) == 2) {
+        if constexpr (std::is_same_v<T, Pair>) {
+            PairFragment f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if constexpr (K) {
+                    const int row = 32 * block + (lane & 31);
+                    f.part[i] = *reinterpret_cast<const Frag<_Float16>*>(tile + row * kRowBytes + (((4 * i + 2 * s + half) ^ turn(row)) << 4));
+                } else {
+                    f.part[i] = transposed<_Float16>(tile, 8 * block + 4 * i, s, lane);
+                }
+            return f;
+        } else if constexpr (K && sizeof(T) == 2) {
             const int row = 32 * block + (lane & 31);
             return *reinterpret_cast<const Frag<T>*>(tile + row * kRowBytes + (((2 * s + half) ^ turn(row)) << 4));
         } else if constexpr (K) {
@@ -121,19 +152,9 @@ struct TileSide {
             const char* p = tile + row * kRowBytes;
             const auto lo = *reinterpret_cast<const vec<T, 4>*>(p + (((4 * s + 2 * half) ^ turn(row)) << 4));
             const auto hi = *reinterpret_cast<const vec<T, 4>*>(p + (((4 * s + 2 * half + 1) ^ turn(row)) << 4));
-            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return Frag<T>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else if constexpr (sizeof(T) == 2) {
-            // Sixteen lanes read four k-rows of sixteen values (four lanes a row) and get
-            // them back transposed, a column each.
-            const int row = 16 * s + 8 * half + ((lane & 15) >> 2);
-            const int chunk = 4 * block + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-            typedef short s4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) s4* at;
-            // (four rows on, the turn is the same)
-            const char* p = tile + row * kRowBytes + ((chunk ^ turn(row)) << 4) + (lane & 1) * 8;
-            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(p));
-            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(p + 4 * kRowBytes));
-            return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            return transposed<T>(tile, 4 * block, s, lane);
         } else {
             const int column = 32 * block + (lane & 31);
             Frag<T> f;
@@ -172,8 +193,11 @@ struct TileSide {
     // last repeat it (their results are not stored); inner indices past the end are zeros.
     __device__ uint32_t place(int i, int left) const {
         const int slot = i * Threads + threadIdx.x % Threads, row = slot / kChunks, chunk = (slot % kChunks) ^ turn(row);
-        if (K) return chunk * kChunk < left ? uint32_t(min(row, rows - 1)) * uint32_t(stride) + (chunk << 4) : kNone;
-        return row < left ? uint32_t(row) * uint32_t(stride) + (min(chunk, (rows + kChunk - 1) / kChunk - 1) << 4) : kNone;
+        // (a group of pairs is eight chunks, four of either part)
+        constexpr bool pairs = std::is_same_v<T, Pair>;
+        if (K) return (pairs ? 8 * (chunk & 3) : chunk * kChunk) < left ? uint32_t(min(row, rows - 1)) * uint32_t(stride) + (chunk << 4) : kNone;
+        const int chunks = pairs ? (rows + 31) / 32 * 8 : (rows + kChunk - 1) / kChunk;
+        return row < left ? uint32_t(row) * uint32_t(stride) + (min(chunk, chunks - 1) << 4) : kNone;
     }
     __device__ void places(uint32_t (&offset)[kSteps]) const {
 #pragma unroll
@@ -181,10 +205,9 @@ struct TileSide {
     }
     // From memory to LDS without registers, for operands of whole 16-byte chunks.  The
     // loads have arrived after loads_arrived() and a barrier.
-    __device__ __attribute__((always_inline)) void load(char* tile, const uint32_t (&offset)[kSteps], int64_t plane,
-                                                        int wave) const {
+    __device__ __attribute__((always_inline)) void load(char* tile, const uint32_t (&offset)[kSteps], int wave) const {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's compiler does not know a buffer's type)
-        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base() + plane), 0, 0x7ffffff0, 0x00020000);
+        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base()), 0, 0x7ffffff0, 0x00020000);
         const auto bring = [&](int i, uint32_t at) __attribute__((always_inline)) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 buffer, (__attribute__((address_space(3))) void*)(tile + (i * Threads + wave * 64) * 16), 16, at, 0, 0, 0);
@@ -199,10 +222,11 @@ struct TileSide {
 #endif
     }
     // Value by value, for any other.
-    __device__ void load_any(char* tile, int64_t plane) const {
+    __device__ void load_any(char* tile) const {
+        if constexpr (std::is_arithmetic_v<T> || sizeof(T) == 2)
         for (int i = 0; i < kSteps; ++i) {
             const int slot = i * Threads + threadIdx.x % Threads, row = slot / kChunks, first = ((slot % kChunks) ^ turn(row)) * kChunk;
-            const T* p = reinterpret_cast<const T*>(base() + plane + int64_t(K ? min(row, rows - 1) : row) * stride);
+            const T* p = reinterpret_cast<const T*>(base() + int64_t(K ? min(row, rows - 1) : row) * stride);
             vec<T, kChunk> v;
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
@@ -285,12 +309,12 @@ struct Tiles {
     static constexpr int kLds = Stages * kTile > kOut ? Stages * kTile : kOut;
     static constexpr int kLoads = A::kSteps + B::kSteps;  // of a tile, by each lane
 
-    using P = Part<T, Exact>;  // of a fragment, as it is multiplied
+    using P = decltype(part<Exact>(A::fragment(nullptr, 0, 0, 0)));
 
     A a;
     B b;
     uint32_t a_offset[A::kSteps], b_offset[B::kSteps];
-    int lane, wave, wm, wn, split, batch, m0, n0, plane, steps, mirrored;
+    int lane, wave, wm, wn, split, batch, m0, n0, steps, mirrored;
     Acc acc[kMB][kNB];
 
     __device__ __attribute__((always_inline)) void start(const ProductArgs& p) {
@@ -311,8 +335,7 @@ struct Tiles {
         b.start(p.b, batch, n0, p.n, p.k, t);
         a.places(a_offset);
         b.places(b_offset);
-        plane = 0;
-        steps = max(0, min((p.k + kDepth<T> - 1) / kDepth<T> - t, p.span)) * p.planes.count;
+        steps = max(0, min((p.k + kDepth<T> - 1) / kDepth<T> - t, p.span));
 #pragma unroll
         for (int i = 0; i < kMB; ++i)
 #pragma unroll
@@ -321,26 +344,18 @@ struct Tiles {
     // The next tile's loads.
     template <bool Any>
     __device__ __attribute__((always_inline)) void load(const ProductArgs& p, char* tile) {
-        int64_t pa = 0, pb = 0;
-        if (p.planes.count > 1) {
-            pa = int64_t((p.planes.a >> (2 * plane)) & 3) * p.a.plane;
-            pb = int64_t((p.planes.b >> (2 * plane)) & 3) * p.b.plane;
-        }
-        if (Any && !p.a.wide) a.load_any(tile, pa);
-        else a.load(tile, a_offset, pa, wave);
-        if (Any && !p.b.wide) b.load_any(tile + A::kBytes, pb);
-        else b.load(tile + A::kBytes, b_offset, pb, wave);
-        if (++plane >= p.planes.count) {
-            plane = 0;
-            a.next();
-            b.next();
-        }
+        if (Any && !p.a.wide) a.load_any(tile);
+        else a.load(tile, a_offset, wave);
+        if (Any && !p.b.wide) b.load_any(tile + A::kBytes);
+        else b.load(tile + A::kBytes, b_offset, wave);
+        a.next();
+        b.next();
     }
     __device__ __attribute__((always_inline)) void fragments(const char* tile, int s, P (&fa)[kMB], P (&fb)[kNB]) const {
 #pragma unroll
-        for (int i = 0; i < kMB; ++i) fa[i] = part<T, Exact>(A::fragment(tile, wm * kMB + i, s, lane));
+        for (int i = 0; i < kMB; ++i) fa[i] = part<Exact>(A::fragment(tile, wm * kMB + i, s, lane));
 #pragma unroll
-        for (int i = 0; i < kNB; ++i) fb[i] = part<T, Exact>(B::fragment(tile + A::kBytes, wn * kNB + i, s, lane));
+        for (int i = 0; i < kNB; ++i) fb[i] = part<Exact>(B::fragment(tile + A::kBytes, wn * kNB + i, s, lane));
     }
     __device__ __attribute__((always_inline)) void products(const P (&fa)[kMB], const P (&fb)[kNB]) {
 #pragma unroll
@@ -473,17 +488,18 @@ __global__ __launch_bounds__(512, 2) void product_large_k(ProductArgs p, Epilogu
         const char* tile = lds + (i & 1) * C::kTile;
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-            typename C::P fa[2][C::kMB], fb[2][C::kNB];
-            c.fragments(tile, 2 * part, fa[0], fb[0]);
-            c.fragments(tile, 2 * part + 1, fa[1], fb[1]);
+            constexpr int kSteps = C::kS / 2;
+            typename C::P fa[kSteps][C::kMB], fb[kSteps][C::kNB];
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) c.fragments(tile, kSteps * part + s, fa[s], fb[s]);
             __builtin_amdgcn_sched_barrier(0);
             if (part == 0 && i + 1 < c.steps) c.template load<false>(p, lds + ((i + 1) & 1) * C::kTile);
             if (part == 1 && second) loads_arrived();
             __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the reads
             barrier();
             __builtin_amdgcn_s_setprio(1);
-            c.products(fa[0], fb[0]);
-            c.products(fa[1], fb[1]);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) c.products(fa[s], fb[s]);
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
             if (part == 1 && !second) loads_arrived();
@@ -521,10 +537,10 @@ __global__ __launch_bounds__(512) void product_run_k(ProductArgs p, Epilogue e) 
     char* mine = lds + wave * 2 * kTile;
     const auto load = [&](int i) __attribute__((always_inline)) {
         char* tile = mine + (i & 1) * kTile;
-        if (Any && !p.a.wide) a.load_any(tile, 0);
-        else a.load(tile, a_offset, 0, 0);
-        if (Any && !p.b.wide) b.load_any(tile + A::kBytes, 0);
-        else b.load(tile + A::kBytes, b_offset, 0, 0);
+        if (Any && !p.a.wide) a.load_any(tile);
+        else a.load(tile, a_offset, 0);
+        if (Any && !p.b.wide) b.load_any(tile + A::kBytes);
+        else b.load(tile + A::kBytes, b_offset, 0);
         a.next();
         b.next();
     };
@@ -644,12 +660,14 @@ struct ProductTime {
 };
 constexpr ProductTime kTimes16[] = {{64, 3.8, 0.30, 0.195}, {128, 5.0, 0.63, 0.48}, {256, 11.5, 1.50, 1.50}};
 constexpr ProductTime kTimes32[] = {{64, 4.5, 0.65, 0.53}, {128, 8.0, 1.60, 1.43}};
-// planes: products of planes.
-inline ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, int planes, int size, bool wide,
+constexpr ProductTime kTimesPair[] = {{64, 4.0, 0.33, 0.22}, {128, 5.5, 0.75, 0.62}, {256, 12.0, 2.0, 2.0}};
+template <class T>
+ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, bool wide,
                               bool symmetric) {
+    constexpr int size = sizeof(T);
     ProductCut best;
     double least = 1e30;
-    const int64_t deep = std::max<int64_t>(1, (k + kTileBytes / size - 1) / (kTileBytes / size)) * planes;
+    const int64_t deep = std::max<int64_t>(1, (k + kTileBytes / size - 1) / (kTileBytes / size));
     const auto consider = [&](const ProductTime& t) {
         const int64_t rows = ceil_div(m, t.side), tiles = batch * (symmetric ? rows * (rows + 1) / 2 : rows * ceil_div(n, t.side));
         for (int splits = 1; splits <= kMostSplits && (splits == 1 || (splits * 2 <= deep && t.side < 256)); ++splits) {
@@ -664,13 +682,16 @@ inline ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64
             }
         }
     };
-    for (const auto& t : kTimes16)
-        if (size == 2 && (wide || t.side == 64)) consider(t);
-    for (const auto& t : kTimes32)
-        if (size == 4 && (wide || t.side == 64)) consider(t);
+    const auto consider_all = [&](const auto& times) {
+        for (const auto& t : times)
+            if (wide || t.side == 64) consider(t);
+    };
+    if constexpr (std::is_same_v<T, Pair>) consider_all(kTimesPair);
+    else if constexpr (size == 2) consider_all(kTimes16);
+    else consider_all(kTimes32);
     // a workgroup of 32 x 32, one or two on a CU at once
     const int64_t tiles = batch * ceil_div(m, 32) * int64_t(ceil_div(n, 32));
-    if (planes == 1 && tiles <= 2 * compute_units) {
+    if (tiles <= 2 * compute_units) {
         const int waves = int(std::min<int64_t>(tiles <= compute_units ? 8 : 4, deep));
         const double time = 3.6 + double((deep + waves - 1) / waves) * (size == 2 ? 0.5 : 0.8);
         if (time < least) {
@@ -711,24 +732,29 @@ void launch_tiles(Device& d, K kernel, int side, int threads, ProductArgs p, con
 template <class T, bool AK, bool BK, class E>
 void launch_product(Device& d, ProductArgs p, const E& e) {
     if (!p.m || !p.n || !p.batch) return;
+    constexpr bool kAny = E::kAny;  // (whether operands may be of any alignment)
     const bool wide = p.a.wide && p.b.wide;
-    const ProductCut c = cut_product(d.compute_units, p.batch, p.m, p.n, p.k, p.planes.count, sizeof(T), wide, p.symmetric);
+    require(wide || kAny, "operands of products are aligned");
+    const ProductCut c = cut_product<T>(d.compute_units, p.batch, p.m, p.n, p.k, wide, p.symmetric);
     const int deep = std::max(1, ceil_div(p.k, kDepth<T>));
     p.span = ceil_div(deep, std::min(c.splits, deep));
     p.splits = ceil_div(deep, p.span);
     if (c.side == 32) {
         const size_t lds = c.waves * kRunBytes<T>;
         p.symmetric = 0;  // (whole tiles of both halves)
-        if (wide) launch_tiles(d, product_run_k<T, AK, BK, false, E>, 32, 64 * c.waves, p, e, lds);
-        else launch_tiles(d, product_run_k<T, AK, BK, true, E>, 32, 64 * c.waves, p, e, lds);
+        if (wide) {
+            launch_tiles(d, product_run_k<T, AK, BK, false, E>, 32, 64 * c.waves, p, e, lds);
+        } else {
+            if constexpr (kAny) launch_tiles(d, product_run_k<T, AK, BK, true, E>, 32, 64 * c.waves, p, e, lds);
+        }
     } else if (!wide) {
-        launch_tiles(d, product_k<T, AK, BK, 64, 32, 1, 2, true, E>, 64, 256, p, e);
+        if constexpr (kAny) launch_tiles(d, product_k<T, AK, BK, 64, 32, 1, 2, true, E>, 64, 256, p, e);
     } else if (c.side == 64) {
         launch_tiles(d, product_k<T, AK, BK, 64, 32, 4, 2, false, E>, 64, 256, p, e);
     } else if (c.side == 128) {
         launch_tiles(d, product_k<T, AK, BK, 128, 64, 2, 2, false, E>, 128, 256, p, e);
     } else {
-        if constexpr (sizeof(T) == 2) launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
+        if constexpr (!std::is_same_v<T, float>) launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
     }
     if (p.splits > 1) {
         if constexpr (E::kSymmetric)
