@@ -219,8 +219,10 @@ struct StepEpilogue {
 // ---- small matrices in one launch -----------------------------------------------------------
 // A workgroup takes a matrix of at most 128 x 128 through all steps: X and A (then
 // b A + c A^2) stay in LDS as the products' operands, the matrix lying so that it is at
-// least as wide as high, a wave's 64 x 32 of X and A in registers besides.  Bound: the products of
-// one CU (128 x 128 f32: 1.2 us each at the matrix unit's rate) and the barriers between them.
+// least as wide as high; its sixteen waves hold a 32 x 32 of X and of A in registers.
+// Symmetric products are made by the ten on and below the diagonal and stored twice.
+// Bound: the products of one CU (128 x 128 f32: 1.3 us each at the matrix unit's rate) and
+// the barriers between them.
 constexpr int kSmall = 128;
 struct SmallArgs {
     int rows, columns, steps;  // as the caller has them
@@ -245,24 +247,25 @@ __device__ inline Frag<_Float16> small_column(const char* matrix, int block, int
 }
 
 template <class T, int PLANES>
-__global__ __launch_bounds__(512, 2) void orthogonal_small_k(Source<T> s, SmallArgs p, Matrices<T> out) {
-    constexpr int kPlane = kSmall * 256;  // bytes
-    __shared__ __align__(16) char x_lds[2 * kPlane];
+__global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArgs p, Matrices<T> out) {
+    constexpr int kPlane = kSmall * 256, kThreads = 1024;  // bytes of a plane
+    __shared__ __align__(16) char x_lds[2 * kPlane];       // X; at the end the result in floats
     __shared__ __align__(16) char g_lds[PLANES * kPlane];
-    __shared__ double sums[8];
+    __shared__ double sums[16];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, matrix = blockIdx.x;
     const bool tall = p.rows > p.columns;
     const int high = min(p.rows, p.columns), wide = max(p.rows, p.columns);
     // the matrix, its size, and X in LDS (its transpose where it is tall), zeros around it
-    for (int i = threadIdx.x; i < 2 * kPlane / 16; i += 512) *reinterpret_cast<u32x4*>(x_lds + i * 16) = u32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < 2 * kPlane / 16; i += kThreads) *reinterpret_cast<u32x4*>(x_lds + i * 16) = u32x4{0, 0, 0, 0};
     const int per_row = (p.columns + 7) / 8, all = p.rows * per_row;
-    constexpr int kMost = kSmall * kSmall / 8 / 512;  // (128 rows of 16 chunks)
+    constexpr int kMost = kSmall * kSmall / 8 / kThreads;  // (128 rows of 16 chunks)
     float v[kMost][8];
     double total = 0;
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
-        const int at = i * 512 + threadIdx.x, row = at / per_row, first = at % per_row * 8;
+        const int at = i * kThreads + threadIdx.x, row = at / per_row, first = at % per_row * 8;
         const int count = at < all ? min(8, p.columns - first) : 0;
+        for (int j = 0; j < 8; ++j) v[i][j] = 0;
         if (count > 0) s.template read<true>(v[i], matrix, row, first, count);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -275,29 +278,45 @@ __global__ __launch_bounds__(512, 2) void orthogonal_small_k(Source<T> s, SmallA
     if (lane == 0) sums[wave] = total;
     __syncthreads();
     total = 0;
-    for (int w = 0; w < 8; ++w) total += sums[w];
+    for (int w = 0; w < 16; ++w) total += sums[w];
     const double down = total > 0 ? double(kUp) / sqrt(total) : total;
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
-        const int at = i * 512 + threadIdx.x, row = at / per_row, first = at % per_row * 8;
-        if (at < all)
+        const int at = i * kThreads + threadIdx.x, row = at / per_row, first = at % per_row * 8;
+        if (at >= all) continue;
+        vec<_Float16, 8> hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float up = float(v[i][j] * down);
+            hi[j] = _Float16(up);
+            lo[j] = _Float16(up - float(hi[j]));
+        }
+        if (!tall) {
+            char* to = x_lds + small_at(row, first / 8);
+            *reinterpret_cast<vec<_Float16, 8>*>(to) = hi;
+            *reinterpret_cast<vec<_Float16, 8>*>(to + kPlane) = lo;
+        } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (first + j >= p.columns) continue;
-                const float up = float(v[i][j] * down);
-                const _Float16 hi = _Float16(up), lo = _Float16(up - float(hi));
-                const int r = tall ? first + j : row, c = tall ? row : first + j;
-                char* to = x_lds + small_at(r, c / 8) + (c & 7) * 2;
-                *reinterpret_cast<_Float16*>(to) = hi;
-                *reinterpret_cast<_Float16*>(to + kPlane) = lo;
+                char* to = x_lds + small_at(first + j, row / 8) + (row & 7) * 2;
+                *reinterpret_cast<_Float16*>(to) = hi[j];
+                *reinterpret_cast<_Float16*>(to + kPlane) = lo[j];
             }
+        }
     }
     __syncthreads();
-    // this wave's part: rows 64 wm.., columns 32 wn..
-    const int wm = wave & 1, wn = wave >> 1;
-    const auto busy = [&](int i, int columns) { return 64 * wm + 32 * i < high && 32 * wn < columns; };
-    const auto put = [&](char* to, int planes, int i, const Acc& c) __attribute__((always_inline)) {
-        const int row = 64 * wm + 32 * i + (lane & 31);
+    // this wave's block: the first ten lie on and below the diagonal, row by row
+    int bm, bn;
+    if (wave < 10) {
+        triangle_of(wave, bm, bn);
+    } else {
+        triangle_of(wave - 10, bn, bm);  // 0 0, 1 0, 1 1, ... exchanged, a column further
+        ++bn;
+    }
+    const int m = 32 * bm + (lane & 31), n = 32 * bn + 4 * half;  // element e: row m, column n + 8 (e / 4) + e % 4
+    const bool square = wave < 10 && 32 * bm < high, live = 32 * bm < high && 32 * bn < wide;
+    // a block as f16 into LDS; turned: its transpose as well
+    const auto put = [&](char* to, int planes, bool turned, const Acc& c) __attribute__((always_inline)) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             vec<_Float16, 4> hi, lo;
@@ -307,33 +326,36 @@ __global__ __launch_bounds__(512, 2) void orthogonal_small_k(Source<T> s, SmallA
                 hi[j] = _Float16(up);
                 lo[j] = _Float16(up - float(hi[j]));
             }
-            char* at = to + small_at(row, 4 * wn + g) + 8 * half;
+            char* at = to + small_at(m, 4 * bn + g) + 8 * half;
             *reinterpret_cast<vec<_Float16, 4>*>(at) = hi;
             if (planes == 2) *reinterpret_cast<vec<_Float16, 4>*>(at + kPlane) = lo;
+            if (turned)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    char* other = to + small_at(n + 8 * g + j, m / 8) + (m & 7) * 2;
+                    *reinterpret_cast<_Float16*>(other) = hi[j];
+                    if (planes == 2) *reinterpret_cast<_Float16*>(other + kPlane) = lo[j];
+                }
         }
     };
     // sum over k of A(m, k) B(n, k): rows of `a`, rows or columns of `b`
-    const auto product = [&](Acc (&c)[2], const char* a, const char* b, int steps, auto rows) __attribute__((always_inline)) {
-        c[0] = c[1] = Acc{};
+    const auto product = [&](const char* a, const char* b, int steps, auto rows) __attribute__((always_inline)) {
+        Acc c = {};
         // (a step's fragments are read while the one before is multiplied; the last one reads its own again)
-        Frag<_Float16> fb[2][PLANES], fa[2][2][PLANES];
+        Frag<_Float16> fb[2][PLANES], fa[2][PLANES];
         const auto read = [&](int k, int to) __attribute__((always_inline)) {
 #pragma unroll
             for (int q = 0; q < PLANES; ++q) {
-                fb[to][q] = decltype(rows)::value ? small_row(b + q * kPlane, wn, k, lane) : small_column(b + q * kPlane, wn, k, lane);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) fa[to][i][q] = small_row(a + q * kPlane, 2 * wm + i, k, lane);
+                fb[to][q] = decltype(rows)::value ? small_row(b + q * kPlane, bn, k, lane) : small_column(b + q * kPlane, bn, k, lane);
+                fa[to][q] = small_row(a + q * kPlane, bm, k, lane);
             }
         };
         const auto multiply_step = [&](int from) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (PLANES == 2) {
-                    c[i] = multiply(fb[from][1 % PLANES], fa[from][i][0], c[i]);
-                    c[i] = multiply(fb[from][0], fa[from][i][1 % PLANES], c[i]);
-                }
-                c[i] = multiply(fb[from][0], fa[from][i][0], c[i]);
+            if (PLANES == 2) {
+                c = multiply(fb[from][1 % PLANES], fa[from][0], c);
+                c = multiply(fb[from][0], fa[from][1 % PLANES], c);
             }
+            c = multiply(fb[from][0], fa[from][0], c);
         };
         read(0, 0);
         for (int k = 0; k < steps; k += 2) {
@@ -342,76 +364,70 @@ __global__ __launch_bounds__(512, 2) void orthogonal_small_k(Source<T> s, SmallA
             read(min(k + 2, steps - 1), 0);
             if (k + 1 < steps) multiply_step(1);
         }
+        return c;
     };
-    Acc x[2], a[2], c[2];
+    Acc x, a, c;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = 64 * wm + 32 * i + (lane & 31);
+    for (int g = 0; g < 4; ++g) {
+        const char* at = x_lds + small_at(m, 4 * bn + g) + 8 * half;
+        const auto hi = *reinterpret_cast<const vec<_Float16, 4>*>(at), lo = *reinterpret_cast<const vec<_Float16, 4>*>(at + kPlane);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const char* at = x_lds + small_at(row, 4 * wn + g) + 8 * half;
-            const auto hi = *reinterpret_cast<const vec<_Float16, 4>*>(at), lo = *reinterpret_cast<const vec<_Float16, 4>*>(at + kPlane);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[i][4 * g + j] = (float(hi[j]) + float(lo[j])) * (1.f / kUp);
-        }
+        for (int j = 0; j < 4; ++j) x[4 * g + j] = (float(hi[j]) + float(lo[j])) * (1.f / kUp);
     }
     const int side_steps = (high + 15) / 16, wide_steps = (wide + 15) / 16;
-    const std::true_type by_rows{};
-    const std::false_type by_columns{};
+    const auto one = [&](int e) { return PLANES == 1 && m == n + 8 * (e >> 2) + (e & 3) && m < high ? 1.f : 0.f; };
     for (int step = 0; step < p.steps; ++step) {
-        if (busy(0, high)) product(a, x_lds, x_lds, wide_steps, by_rows);
-        else a[0] = a[1] = Acc{};
-        // (with one plane A - 1 is what is squared; the diagonal outside the matrix stays zero)
+        if (square) {
+            // (with one plane A - 1 is what is squared; the diagonal outside the matrix stays zero)
+            a = product(x_lds, x_lds, wide_steps, std::true_type{});
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = 64 * wm + 32 * i + (lane & 31), n = 32 * wn + 8 * (e >> 2) + 4 * half + (e & 3);
-                a[i][e] = a[i][e] * kDown - (PLANES == 1 && m == n && m < high ? 1.f : 0.f);
-            }
-        put(g_lds, PLANES, 0, a[0]);
-        put(g_lds, PLANES, 1, a[1]);
+            for (int e = 0; e < 16; ++e) a[e] = a[e] * kDown - one(e);
+            put(g_lds, PLANES, bm != bn, a);
+        }
         __syncthreads();
-        if (busy(0, high)) product(c, g_lds, g_lds, side_steps, by_rows);
-        else c[0] = c[1] = Acc{};
+        if (square) {
+            c = product(g_lds, g_lds, side_steps, std::true_type{});
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = 64 * wm + 32 * i + (lane & 31), n = 32 * wn + 8 * (e >> 2) + 4 * half + (e & 3);
-                c[i][e] = poly_of<PLANES>(a[i][e], c[i][e] * kDown, PLANES == 1 && m == n && m < high ? 1.f : 0.f);
-            }
+            for (int e = 0; e < 16; ++e) c[e] = poly_of<PLANES>(a[e], c[e] * kDown, one(e));
+        }
         __syncthreads();
-        put(g_lds, PLANES, 0, c[0]);
-        put(g_lds, PLANES, 1, c[1]);
+        if (square) put(g_lds, PLANES, bm != bn, c);
         __syncthreads();
-        if (busy(0, wide)) product(c, g_lds, x_lds, side_steps, by_columns);
-        else c[0] = c[1] = Acc{};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) x[i] = kA * x[i] + kDown * c[i];
+        if (live) {
+            c = product(g_lds, x_lds, side_steps, std::false_type{});
+            x = kA * x + kDown * c;
+        }
         __syncthreads();
         if (step + 1 < p.steps) {
-            put(x_lds, 2, 0, x[0]);
-            put(x_lds, 2, 1, x[1]);
+            if (live) put(x_lds, 2, false, x);
             __syncthreads();
         }
     }
+    // out by whole rows, through LDS: 16-byte chunks turned with the row
+    const auto float_at = [&](int row, int column) { return x_lds + row * 512 + ((((column >> 2) ^ row) & 31) << 4) + (column & 3) * 4; };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int m = 64 * wm + 32 * i + (lane & 31);
-        if (m >= high) continue;
+    for (int g = 0; g < 4; ++g) {
+        const Quad four = {x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+        *reinterpret_cast<Quad*>(float_at(m, n + 8 * g)) = four;
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < all; at += kThreads) {
+        const int row = at / per_row, first = at % per_row * 8, count = min(8, p.columns - first);
+        float y[8], w[8] = {};
+        if (!tall) {
+            *reinterpret_cast<Quad*>(y) = *reinterpret_cast<const Quad*>(float_at(row, first));
+            *reinterpret_cast<Quad*>(y + 4) = *reinterpret_cast<const Quad*>(float_at(row, first + 4));
+        } else {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int n = 32 * wn + 8 * g + 4 * half;
-            if (n >= wide) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (n + j >= wide) continue;
-                T* to = tall ? out.at(matrix, n + j) + m : out.at(matrix, m) + n + j;
-                const float y = x[i][4 * g + j];
-                *to = T(p.update ? p.keep * float(*to) - p.rate * y : y);
-            }
+            for (int j = 0; j < 8; ++j) y[j] = *reinterpret_cast<const float*>(float_at(first + j, row));
         }
+        T* to = out.at(matrix, row) + first;
+        if (p.update) {
+            read8(w, to, count, p.wide);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = p.keep * w[j] - p.rate * y[j];
+        }
+        write8(to, y, count, p.wide);
     }
 }
 
@@ -439,7 +455,7 @@ void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> l
     Device& d = *p.dev;
     if (p.rows <= kSmall && p.columns <= kSmall) {
         const SmallArgs a{p.rows, p.columns, p.steps, last.wide, last.update, last.keep, last.rate};
-        hipLaunchKernelGGL((orthogonal_small_k<T, PLANES>), unsigned(p.count), 512, 0, d.stream, source, a, last.out);
+        hipLaunchKernelGGL((orthogonal_small_k<T, PLANES>), unsigned(p.count), 1024, 0, d.stream, source, a, last.out);
         HIP_CHECK(hipGetLastError());
         return;
     }
