@@ -153,7 +153,7 @@ struct Linear {
     int dtype = 0, inputs = 0, outputs = 0, activation = 0, backward = 0;
     int64_t rows = 0;
     char* work = nullptr;
-    size_t dz = 0, part = 0, bias_part = 0;  // places in the workspace
+    size_t a_copy = 0, b_copy = 0, dz = 0, part = 0, bias_part = 0;  // places in the workspace
 };
 constexpr int64_t kMostRows = int64_t(1) << 30;
 constexpr int kMostWidth = 1 << 24;
@@ -162,11 +162,26 @@ constexpr int kStrips = 256;  // of a bias's gradient
 
 int pitch_of(int64_t columns) { return int((columns + 7) / 8 * 8); }
 
+// Rows copied to whole 16-byte chunks, zeros behind their columns.
+template <class T>
+__global__ __launch_bounds__(256) void linear_copy_k(const T* x, int64_t stride, int64_t rows, int columns, T* to, int pitch) {
+    const int per_row = pitch / 8;
+    const int64_t all = rows * per_row, step = int64_t(gridDim.x) * 256;
+    for (int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x; at < all; at += step) {
+        const int64_t row = at / per_row;
+        const int first = int(at - row * per_row) * 8;
+        float v[8];
+        read8(v, x + row * stride + first, min(8, columns - first), false);
+        write8(to + row * pitch + first, v, 8, true);
+    }
+}
+
 // C[m][n] of a plan's product: operands by their rows, which AK and BK say the order of.
 struct Sides {
     const void *a, *b;
     int64_t a_stride, b_stride, m, k;
     int n;
+    bool a_whole;  // a's rows go on in zeros to whole chunks
 };
 template <bool AK, bool BK, class T>
 void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
@@ -177,8 +192,26 @@ void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
     args.k = int(s.k);
     args.batch = 1;
     args.part = reinterpret_cast<float*>(p.work + p.part);
-    args.a = product_operand(s.a, s.a_stride, AK ? s.k : s.m, sizeof(T));
+    args.a = product_operand(s.a, s.a_stride, s.a_whole ? s.a_stride : AK ? s.k : s.m, sizeof(T));
     args.b = product_operand(s.b, s.b_stride, BK ? s.k : s.n, sizeof(T));
+    // Operands that are not whole chunks are read value by value, tile by tile, where that is a
+    // few tiles; more are copied to whole chunks first (a plan whose widths are not whole
+    // eights has room for it).  8,190 -> 4,093 over 4,000 rows, bf16: LINEAR_COPY.
+    const int64_t tiles = int64_t(ceil_div(s.m, 64)) * ceil_div(s.n, 64), deep = ceil_div(s.k, kDepth<T>);
+    if ((!args.a.wide || !args.b.wide) && p.a_copy && deep * std::max<int64_t>(1, tiles / (4 * d.compute_units)) > 6) {
+        const auto copy = [&](Operand& o, const void* x, int64_t stride, int64_t rows, int64_t columns, size_t place) {
+            if (o.wide) return;
+            const int pitch = pitch_of(columns);
+            T* to = reinterpret_cast<T*>(p.work + place);
+            const int64_t chunks = rows * (pitch / 8);
+            const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>((chunks + 255) / 256, int64_t(d.compute_units) * 32)));
+            hipLaunchKernelGGL((linear_copy_k<T>), blocks, 256, 0, d.stream, static_cast<const T*>(x), stride, rows, int(columns), to, pitch);
+            HIP_CHECK(hipGetLastError());
+            o = product_operand(to, pitch, pitch, sizeof(T));
+        };
+        copy(args.a, s.a, s.a_stride, AK ? s.m : s.k, AK ? s.k : s.m, p.a_copy);
+        copy(args.b, s.b, s.b_stride, BK ? s.n : s.k, BK ? s.k : s.n, p.b_copy);
+    }
     launch_product<T, AK, BK>(d, args, e);
 }
 
@@ -210,6 +243,7 @@ int cpde_linear_create(cpde_device* dev, int dtype, int64_t rows, int inputs, in
         require(rows >= 0 && inputs >= 0 && outputs >= 0, "negative size");
         require(rows <= kMostRows && inputs <= kMostWidth && outputs <= kMostWidth, "too large a product");
         require(!dev->capturing, "a capture is open on this device");
+        OnDevice on(*dev);
         auto p = std::make_unique<cpde_linear_s>();
         p->dev = dev;
         p->dtype = dtype;
@@ -224,6 +258,13 @@ int cpde_linear_create(cpde_device* dev, int dtype, int64_t rows, int inputs, in
             at += (bytes + 255) / 256 * 256;
             return here;
         };
+        if (inputs % 8 || outputs % 8) {
+            // x or dy, and W or x, in whole chunks (the first place is never 0)
+            const size_t size = type_bytes(dtype), in = pitch_of(inputs), o = pitch_of(outputs);
+            place(256);
+            p->a_copy = place(size * rows * (backward ? std::max(in, o) : in));
+            p->b_copy = place(size * std::max(size_t(outputs) * in, backward ? size_t(rows) * in : 0));
+        }
         if (backward && activation != CPDE_NONE) p->dz = place(type_bytes(dtype) * rows * pitch_of(outputs));
         if (backward) p->bias_part = place(sizeof(float) * kStrips * outputs);
         size_t part = product_part(dev->compute_units, 1, rows, outputs);
@@ -239,6 +280,7 @@ int cpde_linear_create(cpde_device* dev, int dtype, int64_t rows, int inputs, in
 int cpde_linear_destroy(cpde_linear* linear) {
     return guarded([&] {
         if (!linear) return;
+        OnDevice on(*linear->dev);
         sync_stream(*linear->dev, __LINE__);
         ++linear->dev->layout;
         HIP_CHECK(hipFree(linear->work));
@@ -259,6 +301,7 @@ int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, c
         if (pre) check_rows(pre, rows, p.outputs, true);
         if (!rows || !p.outputs) return;
         Device& d = *p.dev;
+        OnDevice on(d);
         flush_reduce(d);
         TraceScope trace(d, kTraceLinear, 2.0 * rows * p.inputs * p.outputs);
         with_type(p.dtype, [&](auto element) {
@@ -277,7 +320,7 @@ int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, c
             }
             e.activation = p.activation;
             e.wide = wide_rows(y, sizeof(T)) && wide_rows(residual, sizeof(T)) && wide_rows(pre, sizeof(T)) && wide(bias, 0, sizeof(T));
-            product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs}, e);
+            product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs, false}, e);
         });
     });
 }
@@ -303,12 +346,13 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
         }
         if (!dx && !dweight && !dbias) return;
         Device& d = *p.dev;
+        OnDevice on(d);
         flush_reduce(d);
         TraceScope trace(d, kTraceLinearGradient, 2.0 * ((dx != nullptr) + (dweight != nullptr)) * rows * p.inputs * p.outputs);
         with_type(p.dtype, [&](auto element) {
             using T = decltype(element);
             const void* dz = dy->data;
-            int64_t dz_stride = dy->stride;
+            int64_t dz_stride = dy->stride;  // (of the plan's own: whole chunks, zeros behind the columns)
             if ((bent || dbias) && p.outputs) {
                 SlopeArgs a{};
                 a.dy = dy->data;
@@ -345,7 +389,7 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                 e.y = static_cast<T*>(dx->data);
                 e.y_stride = dx->stride;
                 e.wide = wide_rows(dx, sizeof(T));
-                product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs}, e);
+                product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs, bent}, e);
             }
             if (dweight) {
                 LinearEpilogue<T> e{};
@@ -356,7 +400,7 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     e.residual = e.y;
                     e.residual_stride = e.y_stride;
                 }
-                product<false, false, T>(p, {dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs}, e);
+                product<false, false, T>(p, {dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs, bent}, e);
             }
         });
     });

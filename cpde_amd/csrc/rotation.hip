@@ -34,9 +34,10 @@ struct RotationArgs {
     float* part;
     int64_t count;  // tokens of all entries
     int tokens, dim, pairs, interleaved, norm;
-    int parts, span;  // groups of lanes that share a token's heads, and heads of each
+    int most;  // tokens of a workgroup at once, at most kTokens
     float eps;
 };
+constexpr int kTokens = 16;
 
 // Sum over groups of LANES neighbouring lanes, each the whole sum.
 template <int LANES>
@@ -127,142 +128,186 @@ struct Columns {
     }
 };
 
-// Cosine and sine of a lane's pairs at a position.  The turn is taken in double, whose
-// fraction is right for every position, and the fraction's sine in float.
-template <bool WIDE>
-__device__ inline void turn_of(const RotationArgs& a, const Columns<WIDE>& columns, int position, float (&c)[4], float (&s)[4]) {
+// What a workgroup keeps in LDS of its tokens: positions, cosines and sines, made once for
+// all heads, and how far each token stands from a tensor's start.
+struct Tokens {
+    float cos[kTokens][kMaxDim / 2], sin[kTokens][kMaxDim / 2];
+    int position[kTokens];
+    int64_t x[2][kTokens], y[2][kTokens], dy[2][kTokens];
+};
+// Tokens first..first + count.  The turn is taken in double, whose fraction is right for
+// every position, and the fraction's sine in float.
+__device__ inline void start_tokens(const RotationArgs& a, Tokens& t, int64_t first, int count) {
+    for (int i = threadIdx.x; i < count; i += 256) {
+        const int64_t at = first + i, batch = at / a.tokens, token = at - batch * a.tokens;
+        t.position[i] = a.positions ? a.positions[at] : int(token);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        c[j] = 1;
-        s[j] = 0;
-        if (columns.unit[j] >= 0) {
-            const double turns = position * a.rates[columns.unit[j]];
-            sincospif(2.f * float(turns - rint(turns)), &s[j], &c[j]);
+        for (int side = 0; side < 2; ++side) {
+            const Side& s = a.side[side];
+            t.x[side][i] = batch * s.x_batch + token * s.x_token;
+            t.y[side][i] = batch * s.y_batch + token * s.y_token;
+            t.dy[side][i] = batch * s.dy_batch + token * s.dy_token;
         }
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < count * a.pairs; i += 256) {
+        const int token = i / a.pairs, pair = i - token * a.pairs;
+        const double turns = t.position[token] * a.rates[pair];
+        sincospif(2.f * float(turns - rint(turns)), &t.sin[token][pair], &t.cos[token][pair]);
+    }
+    __syncthreads();
 }
-
-// A group of LANES lanes takes one token and `span` of its heads, queries' then keys':
-// the angles are made once for all of them.
-template <class T, int LANES, bool WIDE>
-__global__ __launch_bounds__(256) void rotation_forward_k(RotationArgs a) {
-    const int lane = threadIdx.x % LANES;
-    const int64_t group = int64_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
-    const int64_t at = group / a.parts;
-    if (at >= a.count) return;
-    const int64_t batch = at / a.tokens;
-    const int64_t token = at - batch * a.tokens;
-    const int position = a.positions ? a.positions[at] : int(token);
-    Columns<WIDE> columns;
-    columns.start(a, lane);
-    float c[4], s[4];
-    turn_of(a, columns, position, c, s);
-    const int part = int(group - at * a.parts), last = min((part + 1) * a.span, a.side[0].heads + a.side[1].heads);
-    for (int h = part * a.span; h < last; ++h) {
-        const bool keys = h >= a.side[0].heads;
-        const Side& side = a.side[keys];
-        const int head = keys ? h - a.side[0].heads : h;
-        T* y = reinterpret_cast<T*>(side.y) + batch * side.y_batch + token * side.y_token + head * side.y_head;
-        float u[4] = {}, v[4] = {};
-        if (position < 0) {  // (no token: a row of zeros)
-            columns.store(y, a, u, v);
-            continue;
-        }
-        columns.load(reinterpret_cast<const T*>(side.x) + batch * side.x_batch + token * side.x_token + head * side.x_head, a, u, v);
-        if (a.norm) {
-            float square = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) square += u[j] * u[j] + v[j] * v[j];
-            const float up = 1.f / sqrtf(sum_group<LANES>(square) / a.dim + a.eps);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u[j] *= up;
-                v[j] *= up;
-            }
-        }
-        if (side.weight) {
-            float wu[4], wv[4];
-            columns.load(reinterpret_cast<const T*>(side.weight), a, wu, wv);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u[j] *= wu[j];
-                v[j] *= wv[j];
-            }
+// A lane's cosines and sines of a token.
+template <bool WIDE>
+__device__ inline void turn_of(const Tokens& t, int token, const Columns<WIDE>& columns, float (&c)[4], float (&s)[4]) {
+    if constexpr (WIDE) {
+        typedef float Quad __attribute__((ext_vector_type(4)));
+        Quad cos = {1, 1, 1, 1}, sin = {};
+        if (columns.unit[0] >= 0) {
+            cos = *reinterpret_cast<const Quad*>(&t.cos[token][columns.unit[0]]);
+            sin = *reinterpret_cast<const Quad*>(&t.sin[token][columns.unit[0]]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float turned = u[j] * c[j] - v[j] * s[j];
-            v[j] = u[j] * s[j] + v[j] * c[j];
-            u[j] = turned;
+            c[j] = cos[j];
+            s[j] = sin[j];
         }
-        columns.store(y, a, u, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            c[j] = columns.unit[j] >= 0 ? t.cos[token][columns.unit[j]] : 1.f;
+            s[j] = columns.unit[j] >= 0 ? t.sin[token][columns.unit[j]] : 0.f;
+        }
+    }
+}
+// Calls body(token, head) for every head of the workgroup's tokens, a group of lanes each, in
+// the order in which they stand in memory.
+template <int LANES, class F>
+__device__ __attribute__((always_inline)) inline void each_head(const Side& side, int tokens, F body) {
+    constexpr int kGroups = 256 / LANES;
+    const bool heads_first = side.x_head <= side.x_token;  // neighbours are a token's heads
+    const int inner = heads_first ? side.heads : tokens, outer = heads_first ? tokens : side.heads;
+    const int group = threadIdx.x / LANES;
+    int o = group / inner, i = group - o * inner;
+    const int step_o = kGroups / inner, step_i = kGroups - step_o * inner;
+    while (o < outer) {
+        body(heads_first ? o : i, heads_first ? i : o);
+        o += step_o;
+        i += step_i;
+        if (i >= inner) {
+            i -= inner;
+            ++o;
+        }
+    }
+}
+// A side's weights in a lane's columns; ones where there are none.
+template <class T, bool WIDE>
+__device__ inline void weights_of(const RotationArgs& a, const Side& side, const Columns<WIDE>& columns, float (&u)[4], float (&v)[4]) {
+    if (side.weight) columns.load(reinterpret_cast<const T*>(side.weight), a, u, v);
+    else
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = v[j] = 1;
+}
+
+// A workgroup takes a few tokens, a group of LANES lanes one head's vector after another.
+// Bound: HBM (2 x 8192 tokens, 16 + 4 heads of 128, bf16: 168 MB in 38 us, 4.4 TB/s; the
+// gradient's 252 MB in 61, 4.1 TB/s; a copy 5.1).  Neighbouring groups read neighbouring
+// vectors: with a token each, and so a token's heads apart, they met on the same few
+// channels of memory (54 and 69 us).
+template <class T, int LANES, bool WIDE>
+__global__ __launch_bounds__(256) void rotation_forward_k(RotationArgs a) {
+    __shared__ __align__(16) Tokens t;
+    const int64_t first = int64_t(blockIdx.x) * a.most;
+    const int count = int(min(int64_t(a.most), a.count - first));
+    start_tokens(a, t, first, count);
+    Columns<WIDE> columns;
+    columns.start(a, threadIdx.x % LANES);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const Side& side = a.side[k];
+        if (!side.heads) continue;
+        float wu[4], wv[4];
+        weights_of<T>(a, side, columns, wu, wv);
+        each_head<LANES>(side, count, [&](int token, int head) __attribute__((always_inline)) {
+            float u[4] = {}, v[4] = {};
+            if (t.position[token] >= 0) {  // (a place without a token, whose row is zeros, is not read)
+                columns.load(reinterpret_cast<const T*>(side.x) + t.x[k][token] + head * side.x_head, a, u, v);
+                float up = 1, c[4], s[4];
+                if (a.norm) {
+                    float square = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) square += u[j] * u[j] + v[j] * v[j];
+                    up = 1.f / sqrtf(sum_group<LANES>(square) / a.dim + a.eps);
+                }
+                turn_of(t, token, columns, c, s);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = u[j] * up * wu[j], y = v[j] * up * wv[j];
+                    u[j] = x * c[j] - y * s[j];
+                    v[j] = x * s[j] + y * c[j];
+                }
+            }
+            columns.store(reinterpret_cast<T*>(side.y) + t.y[k][token] + head * side.y_head, a, u, v);
+        });
     }
 }
 
 // With n = x up, up = (mean x^2 + eps)^(-1/2) and g the gradient turned back: the
-// weight's gradient is the sum of g n, and x's up (g w - n mean(g w n)).  Groups of
-// lanes go through the tokens with a stride; their sums are joined in fixed order.
+// weight's gradient is the sum of g n, and x's up (g w - n mean(g w n)).  Workgroups go
+// through the tokens with a stride; their sums are joined in fixed order.
 template <class T, int LANES, bool WIDE>
 __global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
     constexpr int kGroups = 256 / LANES;
+    __shared__ __align__(16) Tokens t;
     __shared__ float sums[kGroups][LANES * 8 + 1];
     const int lane = threadIdx.x % LANES;
     Columns<WIDE> columns;
     columns.start(a, lane);
     float du[2][4] = {}, dv[2][4] = {};
-    const int64_t all = a.count * a.parts;
-    for (int64_t first = int64_t(blockIdx.x) * kGroups; first < all; first += int64_t(gridDim.x) * kGroups) {
-        const int64_t group = first + threadIdx.x / LANES, at = min(group, all - 1) / a.parts;
-        const int64_t batch = at / a.tokens, token = at - batch * a.tokens;
-        const int position = a.positions ? a.positions[at] : int(token);
-        float c[4], s[4];
-        turn_of(a, columns, position, c, s);
-        const int part = int(group - at * a.parts);
-        const int last = group < all ? min((part + 1) * a.span, a.side[0].heads + a.side[1].heads) : 0;
-        for (int h = part * a.span; h < last; ++h) {
-            const bool keys = h >= a.side[0].heads;
-            const Side& side = a.side[keys];
-            const int head = keys ? h - a.side[0].heads : h;
-            T* dx = reinterpret_cast<T*>(side.y) + batch * side.y_batch + token * side.y_token + head * side.y_head;
-            float u[4] = {}, v[4] = {}, gu[4], gv[4], wu[4], wv[4];
-            if (position < 0) {
-                columns.store(dx, a, u, v);
-                continue;
-            }
-            columns.load(reinterpret_cast<const T*>(side.x) + batch * side.x_batch + token * side.x_token + head * side.x_head, a, u, v);
-            columns.load(reinterpret_cast<const T*>(side.dy) + batch * side.dy_batch + token * side.dy_token + head * side.dy_head, a, gu, gv);
-            if (side.weight) columns.load(reinterpret_cast<const T*>(side.weight), a, wu, wv);
-            float square = 0, dot = 0;
+    for (int64_t first = int64_t(blockIdx.x) * a.most; first < a.count; first += int64_t(gridDim.x) * a.most) {
+        const int count = int(min(int64_t(a.most), a.count - first));
+        __syncthreads();
+        start_tokens(a, t, first, count);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float back = gu[j] * c[j] + gv[j] * s[j];
-                gv[j] = gv[j] * c[j] - gu[j] * s[j];
-                gu[j] = back;
-                square += u[j] * u[j] + v[j] * v[j];
-            }
-            const float up = a.norm ? 1.f / sqrtf(sum_group<LANES>(square) / a.dim + a.eps) : 1.f;
+        for (int k = 0; k < 2; ++k) {
+            const Side& side = a.side[k];
+            if (!side.heads) continue;
+            float wu[4], wv[4];
+            weights_of<T>(a, side, columns, wu, wv);
+            each_head<LANES>(side, count, [&](int token, int head) __attribute__((always_inline)) {
+                float u[4] = {}, v[4] = {}, gu[4] = {}, gv[4] = {};
+                if (t.position[token] >= 0) {
+                    columns.load(reinterpret_cast<const T*>(side.x) + t.x[k][token] + head * side.x_head, a, u, v);
+                    columns.load(reinterpret_cast<const T*>(side.dy) + t.dy[k][token] + head * side.dy_head, a, gu, gv);
+                    float c[4], s[4], square = 0, dot = 0;
+                    turn_of(t, token, columns, c, s);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u[j] *= up;
-                v[j] *= up;
-                const float pu = gu[j] * u[j], pv = gv[j] * v[j];
-                du[0][j] += keys ? 0.f : pu;
-                dv[0][j] += keys ? 0.f : pv;
-                du[1][j] += keys ? pu : 0.f;
-                dv[1][j] += keys ? pv : 0.f;
-                if (side.weight) {
-                    gu[j] *= wu[j];
-                    gv[j] *= wv[j];
+                    for (int j = 0; j < 4; ++j) {
+                        const float back = gu[j] * c[j] + gv[j] * s[j];
+                        gv[j] = gv[j] * c[j] - gu[j] * s[j];
+                        gu[j] = back;
+                        square += u[j] * u[j] + v[j] * v[j];
+                    }
+                    const float up = a.norm ? 1.f / sqrtf(sum_group<LANES>(square) / a.dim + a.eps) : 1.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        u[j] *= up;
+                        v[j] *= up;
+                        du[k][j] += gu[j] * u[j];
+                        dv[k][j] += gv[j] * v[j];
+                        gu[j] *= wu[j];
+                        gv[j] *= wv[j];
+                        dot += gu[j] * u[j] + gv[j] * v[j];
+                    }
+                    const float mean = a.norm ? sum_group<LANES>(dot) / a.dim : 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        gu[j] = up * (gu[j] - u[j] * mean);
+                        gv[j] = up * (gv[j] - v[j] * mean);
+                    }
                 }
-                dot += gu[j] * u[j] + gv[j] * v[j];
-            }
-            const float mean = a.norm ? sum_group<LANES>(dot) / a.dim : 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                gu[j] = up * (gu[j] - u[j] * mean);
-                gv[j] = up * (gv[j] - v[j] * mean);
-            }
-            columns.store(dx, a, gu, gv);
+                columns.store(reinterpret_cast<T*>(side.y) + t.y[k][token] + head * side.y_head, a, gu, gv);
+            });
         }
     }
     if (!a.part) return;
@@ -385,13 +430,13 @@ void with_lanes(const cpde_rotation_shape& s, bool wide_columns, F body) {
     else if (s.head_dim <= 128) body(std::integral_constant<int, 16>{}, yes);
     else body(std::integral_constant<int, 32>{}, yes);
 }
-// Heads a group of lanes takes: all of a token's, fewer where there are few tokens.
-void share_heads(const Device& d, RotationArgs& a, int lanes) {
-    const int heads = a.side[0].heads + a.side[1].heads;
-    const int64_t groups = int64_t(d.compute_units) * 8 * 64 / lanes;  // eight waves a unit
-    a.parts = int(std::min<int64_t>(heads, std::max<int64_t>(1, groups / std::max<int64_t>(1, a.count))));
-    a.span = (heads + a.parts - 1) / a.parts;
-    a.parts = (heads + a.span - 1) / a.span;
+// Tokens a workgroup takes at once: as many as leave `blocks` workgroups a unit (forward eight,
+// gradient four; the other way round 41 and 66 us for 38 and 61), but as many as give each
+// group of lanes a vector (4 x 729 tokens, 4 + 4 heads of 32, with the gradient: 31 us without).
+void share_tokens(const Device& d, RotationArgs& a, int blocks, int lanes) {
+    const int heads = std::max(a.side[0].heads, a.side[1].heads), groups = 256 / lanes;
+    const int64_t most = std::max<int64_t>(a.count / (int64_t(blocks) * d.compute_units), (groups + heads - 1) / heads);
+    a.most = int(std::max<int64_t>(1, std::min<int64_t>(kTokens, most)));
 }
 constexpr int kGradientBlocks = 8;  // of a unit, at most
 
@@ -416,7 +461,7 @@ int cpde_rotation_create(cpde_device* dev, const cpde_rotation_shape* shape, cpd
         require(s.rotated >= 0 && s.rotated <= s.head_dim && s.rotated % 2 == 0, "an even number of a head's columns is rotated");
         require(s.base > 0 && std::isfinite(s.base), "the base is positive");
         require(s.eps >= 0 && std::isfinite(s.eps), "eps is not negative");
-        require(int64_t(s.batch) * s.tokens <= int64_t(1) << 30, "too many tokens");
+        require(int64_t(s.batch) * s.tokens <= int64_t(1) << 27, "too many tokens");
         require(!dev->capturing, "a capture is open on this device");
         OnDevice on(*dev);
         auto p = std::make_unique<cpde_rotation_s>();
@@ -477,9 +522,8 @@ int cpde_rotation_forward(cpde_rotation* rotation, const cpde_heads* q, const cp
             using T = decltype(element);
             with_lanes(s, whole, [&](auto lanes, auto whole_) {
                 constexpr int L = decltype(lanes)::value;
-                share_heads(d, a, L);
-                const int64_t blocks = (a.count * a.parts + 256 / L - 1) / (256 / L);
-                require(blocks < (int64_t(1) << 24), "too many workgroups: split the batch");
+                share_tokens(d, a, 8, L);
+                const int64_t blocks = (a.count + a.most - 1) / a.most;
                 hipLaunchKernelGGL((rotation_forward_k<T, L, decltype(whole_)::value>), unsigned(blocks), 256, 0, d.stream, a);
             });
         });
@@ -523,8 +567,8 @@ int cpde_rotation_backward(cpde_rotation* rotation, const cpde_heads* q, const c
             with_lanes(s, whole, [&](auto lanes, auto whole_) {
                 constexpr int L = decltype(lanes)::value;
                 constexpr bool W = decltype(whole_)::value;
-                share_heads(d, a, L);
-                const int64_t want = (a.count * a.parts + 256 / L - 1) / (256 / L);
+                share_tokens(d, a, 4, L);
+                const int64_t want = (a.count + a.most - 1) / a.most;
                 const int blocks = int(std::max<int64_t>(1, std::min<int64_t>(want, p.blocks)));
                 hipLaunchKernelGGL((rotation_gradient_k<T, L, W>), blocks, 256, 0, d.stream, a);
                 HIP_CHECK(hipGetLastError());

@@ -239,6 +239,24 @@ def test_large_products(device):
         plan.destroy()
 
 
+@pytest.mark.parametrize('dtype,rows,inputs,outputs', [
+    ('bf16', 300, 1001, 515), ('f16', 515, 520, 1030), ('f32', 203, 515, 333), ('f32', 1031, 264, 250), ('bf16', 3, 4100, 1003)])
+@pytest.mark.parametrize('kind', ['none', 'silu'])
+def test_odd_widths(device, dtype, rows, inputs, outputs, kind):
+    """Widths that are not whole eights, over many tiles; a smaller call of the same plan."""
+    print(f'[case] linear {dtype} {rows}x{inputs}x{outputs} {kind}', flush=True)
+    x, w, b, r = operands(dtype, rows, inputs, outputs, True, True)
+    plan = plan_of(device, dtype, rows, inputs, outputs, kind)
+    dy = matrix(rows, outputs, dtype, seed=5, scale=0.1)
+    for n in (rows, max(1, rows // 3)):
+        y, z = forward(device, plan, x[:n], w, b, r[:n])
+        want = linear(x[:n].cpu(), w.cpu(), b.cpu(), r[:n].cpu(), kind, dtype)
+        check(y, *want['y'], 'y')
+        check(z, *want['pre'], 'pre')
+        gradient(device, plan, x[:n], w, z, dy[:n], kind, dtype, True)
+    plan.destroy()
+
+
 def test_gradient_is_that_of_differences(device):
     """Along a random direction of x, W and bias, in float: central differences of the sum of
     dy y.  With step h their truncation is h^2 / 6 of third derivatives (of order one a
