@@ -61,31 +61,31 @@ struct LinearEpilogue {
     T *y, *pre;
     const T *bias, *residual;
     int64_t y_stride, pre_stride, residual_stride;
-    int activation, wide;  // wide: all rows and their addresses are whole 16-byte chunks
+    int activation;
     // What a lane's columns have in common for all of its rows.
     struct Columns {
         float bias[8];
     };
     __device__ Columns columns(int n, int count) const {
         Columns c{};
-        if (bias) read8(c.bias, bias + n, count, wide);
+        if (bias) read8(c.bias, bias + n, count);
         return c;
     }
     __device__ void row(const Columns& c, int, int m, int n, int count, float (&v)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += c.bias[j];
-        if (pre) write8(pre + m * pre_stride + n, v, count, wide);
+        if (pre) write8(pre + m * pre_stride + n, v, count);
         with_activation(activation, [&](auto kind) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = activate<T, decltype(kind)::value>(v[j]);
         });
         if (residual) {
             float r[8];
-            read8(r, residual + m * residual_stride + n, count, wide);
+            read8(r, residual + m * residual_stride + n, count);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += r[j];
         }
-        write8(y + m * y_stride + n, v, count, wide);
+        write8(y + m * y_stride + n, v, count);
     }
 };
 
@@ -97,7 +97,7 @@ struct SlopeArgs {
     void* dz;       // null: not wanted (no activation)
     float* part;    // null: not wanted (no bias)
     int64_t dy_stride, pre_stride, rows;
-    int columns, dz_stride, strip, activation, wide;
+    int columns, dz_stride, strip, activation;
 };
 template <class T>
 __global__ __launch_bounds__(256) void linear_slope_k(SlopeArgs a) {
@@ -109,14 +109,14 @@ __global__ __launch_bounds__(256) void linear_slope_k(SlopeArgs a) {
     if (count > 0)
         for (int64_t m = first + row_lane; m < last; m += 32) {
             float v[8], z[8];
-            read8(v, static_cast<const T*>(a.dy) + m * a.dy_stride + n, count, a.wide);
+            read8(v, static_cast<const T*>(a.dy) + m * a.dy_stride + n, count);
             if (a.dz) {
-                read8(z, static_cast<const T*>(a.pre) + m * a.pre_stride + n, count, a.wide);
+                read8(z, static_cast<const T*>(a.pre) + m * a.pre_stride + n, count);
                 with_activation(a.activation, [&](auto kind) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] *= slope<T, decltype(kind)::value>(z[j]);
                 });
-                write8(static_cast<T*>(a.dz) + m * a.dz_stride + n, v, count, true);
+                write8(static_cast<T*>(a.dz) + m * a.dz_stride + n, v, count);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += v[j];
@@ -171,8 +171,8 @@ __global__ __launch_bounds__(256) void linear_copy_k(const T* x, int64_t stride,
         const int64_t row = at / per_row;
         const int first = int(at - row * per_row) * 8;
         float v[8];
-        read8(v, x + row * stride + first, min(8, columns - first), false);
-        write8(to + row * pitch + first, v, 8, true);
+        read8(v, x + row * stride + first, min(8, columns - first));
+        write8(to + row * pitch + first, v, 8);
     }
 }
 
@@ -223,7 +223,6 @@ void check_rows(const cpde_rows* r, int64_t rows, int64_t columns, bool output) 
     require(r->stride >= 0 && r->stride <= int64_t(1) << 40, "invalid stride");
     require(!output || rows == 1 || r->stride >= columns, "output rows overlap");
 }
-bool wide_rows(const cpde_rows* r, size_t size) { return !r || wide(r->data, r->stride, size); }
 
 }  // namespace
 }  // namespace cpde
@@ -319,7 +318,6 @@ int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, c
                 e.pre_stride = pre->stride;
             }
             e.activation = p.activation;
-            e.wide = wide_rows(y, sizeof(T)) && wide_rows(residual, sizeof(T)) && wide_rows(pre, sizeof(T)) && wide(bias, 0, sizeof(T));
             product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs, false}, e);
         });
     });
@@ -360,13 +358,11 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                 a.rows = rows;
                 a.columns = p.outputs;
                 a.activation = p.activation;
-                a.wide = wide_rows(dy, sizeof(T));
                 if (bent) {
                     a.pre = pre->data;
                     a.pre_stride = pre->stride;
                     a.dz = p.work + p.dz;
                     a.dz_stride = pitch_of(p.outputs);
-                    a.wide = a.wide && wide_rows(pre, sizeof(T));
                     dz = a.dz;
                     dz_stride = a.dz_stride;
                 }
@@ -388,14 +384,12 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                 LinearEpilogue<T> e{};
                 e.y = static_cast<T*>(dx->data);
                 e.y_stride = dx->stride;
-                e.wide = wide_rows(dx, sizeof(T));
                 product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs, bent}, e);
             }
             if (dweight) {
                 LinearEpilogue<T> e{};
                 e.y = static_cast<T*>(dweight->data);
                 e.y_stride = dweight->stride;
-                e.wide = wide_rows(dweight, sizeof(T));
                 if (accumulate) {
                     e.residual = e.y;
                     e.residual_stride = e.y_stride;

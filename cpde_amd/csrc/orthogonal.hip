@@ -55,18 +55,18 @@ struct Source {
     Matrices<const T> x;
     Matrices<float> momentum;  // (data null: none)
     float factor;
-    int nesterov, wide;
+    int nesterov;
     template <bool Move>
     __device__ void read(float (&v)[8], int matrix, int row, int first, int count) const {
-        read8(v, x.at(matrix, row) + first, count, wide);
+        read8(v, x.at(matrix, row) + first, count);
         if (!momentum.data) return;
         float m[8];
         float* at = momentum.at(matrix, row) + first;
-        read8(m, at, count, wide);
+        read8(m, at, count);
         if (Move) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) m[j] = fmaf(factor, m[j], v[j]);
-            write8(at, m, count, wide);
+            write8(at, m, count);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = nesterov ? fmaf(factor, m[j], v[j]) : m[j];
@@ -191,7 +191,7 @@ struct StepEpilogue {
     const _Float16* x;
     _Float16* next;  // null: the last step
     int64_t plane;
-    int rows, pitch, wide, update;
+    int rows, pitch, update;
     Matrices<T> out;
     float keep, rate;  // weights <- keep weights - rate X
     __device__ int columns(int, int) const { return 0; }
@@ -208,11 +208,11 @@ struct StepEpilogue {
         T* to = out.at(batch, m) + n;
         if (update) {
             float w[8];
-            read8(w, to, count, wide);
+            read8(w, to, count);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = keep * w[j] - rate * v[j];
         }
-        write8(to, v, count, wide);
+        write8(to, v, count);
     }
 };
 
@@ -226,7 +226,7 @@ struct StepEpilogue {
 constexpr int kSmall = 128;
 struct SmallArgs {
     int rows, columns, steps;  // as the caller has them
-    int wide, update;
+    int update;
     float keep, rate;
 };
 // Chunk `chunk` of row `row` of a [128][128] f16 matrix in LDS, turned so that both 16 rows'
@@ -423,11 +423,11 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
         }
         T* to = out.at(matrix, row) + first;
         if (p.update) {
-            read8(w, to, count, p.wide);
+            read8(w, to, count);
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = p.keep * w[j] - p.rate * y[j];
         }
-        write8(to, y, count, p.wide);
+        write8(to, y, count);
     }
 }
 
@@ -446,15 +446,11 @@ template <class T>
 Matrices<T> matrices(const cpde_matrices* x) {
     return {static_cast<T*>(x->data), x->matrix, x->row};
 }
-bool wide_matrices(const cpde_matrices* x, size_t size) {
-    return wide(x->data, x->row, size) && wide(x->data, x->matrix, size);
-}
-
 template <class T, int PLANES>
 void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> last) {
     Device& d = *p.dev;
     if (p.rows <= kSmall && p.columns <= kSmall) {
-        const SmallArgs a{p.rows, p.columns, p.steps, last.wide, last.update, last.keep, last.rate};
+        const SmallArgs a{p.rows, p.columns, p.steps, last.update, last.keep, last.rate};
         hipLaunchKernelGGL((orthogonal_small_k<T, PLANES>), unsigned(p.count), 1024, 0, d.stream, source, a, last.out);
         HIP_CHECK(hipGetLastError());
         return;
@@ -519,7 +515,6 @@ void run_typed(const Orthogonal& p, const Source<T>& source, const cpde_matrices
     constexpr int kPlanes = std::is_same_v<T, bf16> ? 1 : 2;
     StepEpilogue<T, kPlanes> last{};
     last.out = matrices<T>(out);
-    last.wide = wide_matrices(out, sizeof(T));
     last.update = update;
     last.keep = keep;
     last.rate = rate;
@@ -605,7 +600,6 @@ int cpde_orthogonal_forward(cpde_orthogonal* orthogonal, const cpde_matrices* x,
             using T = decltype(element);
             Source<T> s{};
             s.x = matrices<const T>(x);
-            s.wide = wide_matrices(x, sizeof(T));
             run_typed<T>(p, s, out, false, 0, 0);
         });
     });
@@ -631,7 +625,6 @@ int cpde_orthogonal_update(cpde_orthogonal* orthogonal, const cpde_matrices* gra
             s.momentum = matrices<float>(momentum);
             s.factor = factor;
             s.nesterov = nesterov;
-            s.wide = wide_matrices(gradient, sizeof(T)) && wide_matrices(momentum, sizeof(float));
             const double size = double(rate) * std::sqrt(std::max(1.0, double(p.rows) / p.columns));
             run_typed<T>(p, s, weight, true, float(1 - double(rate) * decay), float(size));
         });

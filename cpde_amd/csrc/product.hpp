@@ -21,7 +21,7 @@ struct ProductArgs {
     int symmetric;     // C is symmetric: tiles on and below its diagonal, mirrored as they are stored
     int m_tiles, n_tiles;
     int splits, span;  // of the inner axis, and a split's tiles of it
-    float* part;       // [split][batch][m][n] where there are several
+    float* part;       // [split][batch][m][n, to whole eights] where there are several
 };
 
 typedef float Acc __attribute__((ext_vector_type(16)));
@@ -43,10 +43,11 @@ __device__ inline Acc multiply(Frag<float> a, Frag<float> b, Acc c) {
     return c;
 }
 
-// A fragment of floats as three of bf16 values whose sums they are: x0 + x1 + x2 to 24 bits,
-// each the rounding of what the ones before leave.  Six of the nine products of two such
-// sums are exact to 2^-23 of the factors' and take 192 cycles where the float
-// instruction takes 512; what is split is shared by the products of a wave's tile.
+// A fragment of floats as three of bf16 values whose sums they are, exactly: the leading
+// 8 of the 24 bits, the next 8 and the rest, cut off by masks (rounding each took a third
+// more instructions).  Six of the nine products of two such sums leave out 2^-21 of the
+// factors' at most and take 192 cycles where the float instruction takes 512; what is
+// split is shared by the products of a wave's tile.
 struct Split {
     Frag<bf16> part[3];
 };
@@ -54,8 +55,14 @@ __device__ inline Split split(Frag<float> x) {
     Split s;
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-        s.part[i] = __builtin_convertvector(x, Frag<bf16>);
-        x -= __builtin_convertvector(s.part[i], Frag<float>);
+        vec<uint32_t, 4> two;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)  // the upper halves of two floats
+            two[j] = __builtin_amdgcn_perm(__float_as_uint(x[2 * j + 1]), __float_as_uint(x[2 * j]), 0x07060302u);
+        s.part[i] = __builtin_bit_cast(Frag<bf16>, two);
+        if (i < 2)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] -= __uint_as_float(__float_as_uint(x[j]) & 0xffff0000u);
     }
     return s;
 }
@@ -228,10 +235,12 @@ struct TileSide {
             const int slot = i * Threads + threadIdx.x % Threads, row = slot / kChunks, first = ((slot % kChunks) ^ turn(row)) * kChunk;
             const T* p = reinterpret_cast<const T*>(base() + int64_t(K ? min(row, rows - 1) : row) * stride);
             vec<T, kChunk> v;
+            const int count = K ? left - first : row < left ? rows - first : 0;
+            if (count >= kChunk) {
+                __builtin_memcpy(&v, p + first, sizeof(v));
+            } else {
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                const bool there = K ? first + j < left : row < left && first + j < rows;
-                v[j] = there ? p[first + j] : T(0.f);
+                for (int j = 0; j < kChunk; ++j) v[j] = j < count ? p[first + j] : T(0.f);
             }
             *reinterpret_cast<vec<T, kChunk>*>(tile + slot * 16) = v;
         }
@@ -255,6 +264,11 @@ __device__ inline void tile_of(int at, int count, int m_tiles, int n_tiles, int&
     tn = in / height;
 }
 
+// Where a split's sums of row m from column n on stand: rows of whole eights.
+__device__ inline int64_t part_at(const ProductArgs& p, int split, int64_t batch, int64_t m, int n) {
+    return ((int64_t(split) * p.batch + batch) * p.m + m) * ((p.n + 7) & ~7) + n;
+}
+
 // The tiles on and below the diagonal, row by row.
 __device__ inline void triangle_of(int at, int& tm, int& tn) {
     tm = int((sqrtf(8.f * at + 1.f) - 1.f) * 0.5f);
@@ -263,33 +277,29 @@ __device__ inline void triangle_of(int at, int& tm, int& tn) {
     tn = at - tm * (tm + 1) / 2;
 }
 
-// Up to eight neighbouring values of a row, as floats.
+// Up to eight neighbouring values of a row, as floats; eight by 16-byte accesses of any
+// alignment.
 template <class T>
-__device__ inline void read8(float (&v)[8], const T* p, int count, bool wide) {
-    constexpr int N = 16 / int(sizeof(T));
-    if (wide && count == 8) {
+__device__ inline void read8(float (&v)[8], const T* p, int count) {
+    if (count == 8) {
+        vec<T, 8> in;
+        __builtin_memcpy(&in, p, sizeof(in));
+        const auto wide = __builtin_convertvector(in, vec<float, 8>);
 #pragma unroll
-        for (int part = 0; part < 8; part += N) {
-            const auto in = __builtin_convertvector(*reinterpret_cast<const vec<T, N>*>(p + part), vec<float, N>);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[part + j] = in[j];
-        }
+        for (int j = 0; j < 8; ++j) v[j] = wide[j];
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = j < count ? float(p[j]) : 0.f;
     }
 }
 template <class T>
-__device__ inline void write8(T* p, const float (&v)[8], int count, bool wide) {
-    constexpr int N = 16 / int(sizeof(T));
-    if (wide && count == 8) {
+__device__ inline void write8(T* p, const float (&v)[8], int count) {
+    if (count == 8) {
+        vec<float, 8> wide;
 #pragma unroll
-        for (int part = 0; part < 8; part += N) {
-            vec<float, N> out;
-#pragma unroll
-            for (int j = 0; j < N; ++j) out[j] = v[part + j];
-            *reinterpret_cast<vec<T, N>*>(p + part) = __builtin_convertvector(out, vec<T, N>);
-        }
+        for (int j = 0; j < 8; ++j) wide[j] = v[j];
+        const vec<T, 8> out = __builtin_convertvector(wide, vec<T, 8>);
+        __builtin_memcpy(p, &out, sizeof(out));
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -388,7 +398,7 @@ struct Tiles {
                 *reinterpret_cast<Quad*>(v + 4) = *reinterpret_cast<const Quad*>(stage + row * kPitch + column + 4);
                 if (m >= p.m || n >= p.n) continue;
                 if (p.splits > 1)
-                    write8(p.part + ((int64_t(split) * p.batch + batch) * p.m + m) * p.n + n, v, min(8, p.n - n), p.n % 4 == 0);
+                    write8(p.part + part_at(p, split, batch, m, n), v, 8);
                 else
                     e.row(columns, batch, m, n, min(8, p.n - n), v);
             }
@@ -596,7 +606,7 @@ __global__ __launch_bounds__(256) void product_join_k(ProductArgs p, Epilogue e)
     float v[8] = {};
     for (int s = 0; s < p.splits; ++s) {
         float one[8];
-        read8(one, p.part + (int64_t(s) * p.batch * p.m + row) * p.n + n, count, p.n % 4 == 0);
+        read8(one, p.part + part_at(p, s, 0, row, n), 8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += one[j];
     }
@@ -618,7 +628,7 @@ __global__ __launch_bounds__(256) void product_join_symmetric_k(ProductArgs p, E
         if (m < p.m && n < p.n) {
             for (int s = 0; s < p.splits; ++s) {
                 float one[8];
-                read8(one, p.part + ((int64_t(s) * p.batch + batch) * p.m + m) * p.n + n, count, p.n % 4 == 0);
+                read8(one, p.part + part_at(p, s, batch, m, n), 8);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] += one[j];
             }
@@ -659,7 +669,7 @@ struct ProductTime {
     double start, alone, shared;
 };
 constexpr ProductTime kTimes16[] = {{64, 3.8, 0.30, 0.195}, {128, 5.0, 0.63, 0.48}, {256, 11.5, 1.50, 1.50}};
-constexpr ProductTime kTimes32[] = {{64, 4.5, 0.65, 0.53}, {128, 8.0, 1.60, 1.43}};
+constexpr ProductTime kTimes32[] = {{64, 4.5, 0.65, 0.53}, {128, 8.0, 1.55, 1.43}, {256, 14.0, 4.7, 4.7}};
 constexpr ProductTime kTimesPair[] = {{64, 4.0, 0.33, 0.22}, {128, 5.5, 0.75, 0.62}, {256, 12.0, 2.0, 2.0}};
 template <class T>
 ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, bool wide,
@@ -671,7 +681,7 @@ ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, i
     const auto consider = [&](const ProductTime& t) {
         const int64_t rows = ceil_div(m, t.side), tiles = batch * (symmetric ? rows * (rows + 1) / 2 : rows * ceil_div(n, t.side));
         for (int splits = 1; splits <= kMostSplits && (splits == 1 || (splits * 2 <= deep && t.side < 256)); ++splits) {
-            if (splits > 1 && splits * batch * m * n > kPartTiles * compute_units * 128 * 128) break;
+            if (splits > 1 && splits * batch * m * ((n + 7) / 8 * 8) > kPartTiles * compute_units * 128 * 128) break;
             const int64_t each = (tiles * splits + compute_units - 1) / compute_units;
             double time = t.start + double((deep + splits - 1) / splits) * (each == 1 ? t.alone : std::max(t.alone, each * t.shared));
             if (splits > 1) time += 3.5 + double(batch) * m * n * splits * 8 / 4e6;
@@ -704,7 +714,7 @@ ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, i
 }
 // Floats of ProductArgs::part that no call with up to `m` rows passes.
 inline size_t product_part(int compute_units, int64_t batch, int64_t m, int64_t n) {
-    return size_t(std::min<int64_t>(kPartTiles * compute_units * 128 * 128, kMostSplits * batch * m * n));
+    return size_t(std::min<int64_t>(kPartTiles * compute_units * 128 * 128, kMostSplits * batch * m * ((n + 7) / 8 * 8)));
 }
 
 // An operand of rows of `columns` values of `size` bytes.
@@ -750,11 +760,11 @@ void launch_product(Device& d, ProductArgs p, const E& e) {
     } else if (!wide) {
         if constexpr (kAny) launch_tiles(d, product_k<T, AK, BK, 64, 32, 1, 2, true, E>, 64, 256, p, e);
     } else if (c.side == 64) {
-        launch_tiles(d, product_k<T, AK, BK, 64, 32, 4, 2, false, E>, 64, 256, p, e);
+        launch_tiles(d, product_k<T, AK, BK, 64, 32, 3, 2, false, E>, 64, 256, p, e);
     } else if (c.side == 128) {
         launch_tiles(d, product_k<T, AK, BK, 128, 64, 2, 2, false, E>, 128, 256, p, e);
     } else {
-        if constexpr (!std::is_same_v<T, float>) launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
+        launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
     }
     if (p.splits > 1) {
         if constexpr (E::kSymmetric)

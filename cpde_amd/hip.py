@@ -57,7 +57,7 @@ def _list_holds(name, a, kind, gpu, count):
     """The same of a list of `count` elements: a tensor, a Buffer by its bytes, or an address."""
     dtype = getattr(a, 'dtype', None)
     if dtype is None:
-        if isinstance(a, Buffer) and a.nbytes < count * (8 if kind == 'int64' else 4):
+        if isinstance(a, Buffer) and a.nbytes < count * {'int64': 8, 'float16': 2, 'bfloat16': 2}.get(kind, 4):
             raise ValueError(f'{name} has {a.nbytes} bytes, not {count} of {kind}')
     elif _type_name(dtype) != kind or a.get_device() != gpu:
         raise ValueError(f'{name} is a tensor of {_type_name(dtype)} on {a.device}, not of {kind} on GPU {gpu}')
