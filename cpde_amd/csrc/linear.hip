@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void linear_slope_k(SlopeArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] *= slope<T, decltype(kind)::value>(z[j]);
                 });
-                write8(static_cast<T*>(a.dz) + m * a.dz_stride + n, v, count);
+                write8(static_cast<T*>(a.dz) + m * a.dz_stride + n, v, 8);  // (zeros behind the columns)
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += v[j];

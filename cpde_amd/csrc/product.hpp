@@ -422,9 +422,9 @@ struct Tiles {
 
 // The loads of the next Stages - 1 tiles are under way while one is multiplied.  Any:
 // operands of any alignment.
-template <class T, bool AK, bool BK, int Side, int Wave, int Stages, int PerSimd, bool Any, class Epilogue>
-__global__ __launch_bounds__((Side / Wave) * (Side / Wave) * 64, PerSimd) void product_k(ProductArgs p, Epilogue e) {
-    using C = Tiles<T, AK, BK, Side, Side, Wave, Wave, Stages, (Side < 128)>;
+template <class T, bool AK, bool BK, int Side, int WM, int WN, int Stages, int PerSimd, bool Any, class Epilogue>
+__global__ __launch_bounds__((Side / WM) * (Side / WN) * 64, PerSimd) void product_k(ProductArgs p, Epilogue e) {
+    using C = Tiles<T, AK, BK, Side, Side, WM, WN, Stages, (Side < 128)>;
     __shared__ __align__(16) char lds[C::kLds];
     C c;
     c.start(p);
@@ -668,9 +668,9 @@ struct ProductTime {
     int side;
     double start, alone, shared;
 };
-constexpr ProductTime kTimes16[] = {{64, 3.8, 0.30, 0.195}, {128, 5.0, 0.63, 0.48}, {256, 11.5, 1.50, 1.50}};
+constexpr ProductTime kTimes16[] = {{64, 3.8, 0.30, 0.195}, {128, 4.2, 0.62, 0.47}, {256, 11.5, 1.50, 1.50}};
 constexpr ProductTime kTimes32[] = {{64, 4.5, 0.65, 0.53}, {128, 8.0, 1.55, 1.43}, {256, 14.0, 4.7, 4.7}};
-constexpr ProductTime kTimesPair[] = {{64, 4.0, 0.33, 0.22}, {128, 5.5, 0.75, 0.62}, {256, 12.0, 2.0, 2.0}};
+constexpr ProductTime kTimesPair[] = {{64, 4.0, 0.40, 0.27}, {128, 5.0, 0.95, 0.75}, {256, 12.0, 2.2, 2.2}};
 template <class T>
 ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, bool wide,
                               bool symmetric) {
@@ -758,11 +758,14 @@ void launch_product(Device& d, ProductArgs p, const E& e) {
             if constexpr (kAny) launch_tiles(d, product_run_k<T, AK, BK, true, E>, 32, 64 * c.waves, p, e, lds);
         }
     } else if (!wide) {
-        if constexpr (kAny) launch_tiles(d, product_k<T, AK, BK, 64, 32, 1, 2, true, E>, 64, 256, p, e);
+        if constexpr (kAny) launch_tiles(d, product_k<T, AK, BK, 64, 32, 32, 1, 2, true, E>, 64, 256, p, e);
     } else if (c.side == 64) {
-        launch_tiles(d, product_k<T, AK, BK, 64, 32, 3, 2, false, E>, 64, 256, p, e);
+        launch_tiles(d, product_k<T, AK, BK, 64, 32, 32, 3, 2, false, E>, 64, 256, p, e);
     } else if (c.side == 128) {
-        launch_tiles(d, product_k<T, AK, BK, 128, 64, 2, 2, false, E>, 128, 256, p, e);
+        // eight waves where a fragment costs a read (16 bits: 128 tiles, k = 1024, 11.9 us for 13.7), four where
+        // splitting it costs more (floats, 1,024 tiles, k = 1024: 185 us for 199)
+        constexpr int kWave = std::is_same_v<T, float> ? 64 : 32;
+        launch_tiles(d, product_k<T, AK, BK, 128, 64, kWave, 2, 128 / kWave, false, E>, 128, 256 * 64 / kWave, p, e);
     } else {
         launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
     }

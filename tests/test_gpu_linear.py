@@ -257,6 +257,22 @@ def test_odd_widths(device, dtype, rows, inputs, outputs, kind):
     plan.destroy()
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_workspaces_start_with_anything(device, dtype):
+    """Plans on memory that held NaN: what stands behind a width in them reaches no result."""
+    held = [torch.full((size,), math.nan, device='cuda') for size in (1 << 10, 1 << 14, 1 << 18, 1 << 22) for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+    torch.cuda.empty_cache()
+    for rows, inputs, outputs in ((9, 130, 33), (70, 41, 77), (300, 515, 203)):
+        x, w, b, r = operands(dtype, rows, inputs, outputs, True, True)
+        plan = plan_of(device, dtype, rows, inputs, outputs, 'silu')
+        y, z = forward(device, plan, x, w, b, r)
+        check(y, *linear(x.cpu(), w.cpu(), b.cpu(), r.cpu(), 'silu', dtype)['y'], 'y')
+        gradient(device, plan, x, w, z, matrix(rows, outputs, dtype, seed=5), 'silu', dtype, True)
+        plan.destroy()
+
+
 def test_gradient_is_that_of_differences(device):
     """Along a random direction of x, W and bias, in float: central differences of the sum of
     dy y.  With step h their truncation is h^2 / 6 of third derivatives (of order one a

@@ -93,6 +93,19 @@ def test_strides_and_alignment(device, dtype, pad, offset):
     assert torch.equal(forward(device, x, dtype, 3, x), want)     # in place
 
 
+def test_workspaces_start_with_anything(device):
+    """Plans on memory that held NaN: what stands behind a width in them reaches no result."""
+    held = [torch.full((size,), math.nan, device='cuda') for size in (1 << 16, 1 << 18, 1 << 20, 1 << 22) for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+    torch.cuda.empty_cache()
+    for dtype in ('f32', 'bf16'):
+        for rows, columns in ((150, 33), (41, 300), (203, 515)):
+            x = matrices(1, rows, columns, dtype)
+            assert torch.equal(forward(device, x, dtype, 5), forward(device, x, dtype, 5))
+            check(forward(device, x, dtype, 1), *orthogonal_first(x.cpu(), dtype), 'out')
+
+
 def test_scale_and_zeros(device):
     """The size of a matrix does not count, from the type's smallest values to its largest; zeros give zeros."""
     x = matrices(1, 40, 56, 'f32')
