@@ -217,32 +217,39 @@ struct StepEpilogue {
 };
 
 // ---- small matrices in one launch -----------------------------------------------------------
-// A workgroup takes a matrix of at most 128 x 128 through all steps: X and A (then
-// b A + c A^2) stay in LDS as the products' operands, the matrix lying so that it is at
-// least as wide as high; its sixteen waves hold a 32 x 32 of X and of A in registers.
-// Symmetric products are made by the ten on and below the diagonal and stored twice.
-// Bound: the products of one CU (128 x 128 f32: 1.3 us each at the matrix unit's rate) and
-// the barriers between them.
+// A workgroup takes a matrix of at most 128 x 128, 64 x 256 or 32 x 512 (or higher than
+// wide) through all steps: X and A (then b A + c A^2) stay in LDS as the products' operands,
+// the matrix lying so that it is at least as wide as high; its sixteen waves hold a 32 x 32
+// of X and of A in registers.  Symmetric products are made by the waves of the blocks on and
+// below the diagonal and stored twice.  Bound: the products of one CU (128 x 128 f32: 1.3 us
+// each at the matrix unit's rate) and the barriers between them: 7 us a step; in launches
+// of their own the three products of a step take 13.
 constexpr int kSmall = 128;
+// X's row in LDS, in columns.
+__host__ __device__ inline int small_width(int wide) { return wide <= 128 ? 128 : wide <= 256 ? 256 : 512; }
+__host__ __device__ inline bool is_small(int rows, int columns) {
+    const int high = rows < columns ? rows : columns, wide = rows < columns ? columns : rows;
+    return wide <= 512 && high <= kSmall * kSmall / small_width(wide);
+}
 struct SmallArgs {
     int rows, columns, steps;  // as the caller has them
     int update;
     float keep, rate;
 };
-// Chunk `chunk` of row `row` of a [128][128] f16 matrix in LDS, turned so that both 16 rows'
-// same chunk and four rows' 64 bytes lie in different banks.
-__device__ inline int small_at(int row, int chunk) {
-    return row * 256 + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
+// Chunk `chunk` of row `row` of an f16 matrix in LDS whose rows are `pitch` bytes (whole
+// 256s), turned so that both 16 rows' same chunk and four rows' 64 bytes lie in different banks.
+__device__ inline int small_at(int pitch, int row, int chunk) {
+    return row * pitch + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
 }
-__device__ inline Frag<_Float16> small_row(const char* matrix, int block, int s, int lane) {
-    return *reinterpret_cast<const Frag<_Float16>*>(matrix + small_at(32 * block + (lane & 31), 2 * s + (lane >> 5)));
+__device__ inline Frag<_Float16> small_row(const char* matrix, int pitch, int block, int s, int lane) {
+    return *reinterpret_cast<const Frag<_Float16>*>(matrix + small_at(pitch, 32 * block + (lane & 31), 2 * s + (lane >> 5)));
 }
-__device__ inline Frag<_Float16> small_column(const char* matrix, int block, int s, int lane) {
+__device__ inline Frag<_Float16> small_column(const char* matrix, int pitch, int block, int s, int lane) {
     const int row = 16 * s + 8 * (lane >> 5) + ((lane & 15) >> 2), chunk = 4 * block + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s4* at;
-    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(matrix + small_at(row, chunk) + (lane & 1) * 8));
-    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(matrix + small_at(row + 4, chunk) + (lane & 1) * 8));
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(matrix + small_at(pitch, row, chunk) + (lane & 1) * 8));
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(matrix + small_at(pitch, row + 4, chunk) + (lane & 1) * 8));
     return __builtin_bit_cast(Frag<_Float16>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
@@ -255,10 +262,12 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, matrix = blockIdx.x;
     const bool tall = p.rows > p.columns;
     const int high = min(p.rows, p.columns), wide = max(p.rows, p.columns);
+    constexpr int kG = 2 * kSmall;                    // bytes of a row of A
+    const int width = small_width(wide), kX = 2 * width;  // X's
     // the matrix, its size, and X in LDS (its transpose where it is tall), zeros around it
     for (int i = threadIdx.x; i < 2 * kPlane / 16; i += kThreads) *reinterpret_cast<u32x4*>(x_lds + i * 16) = u32x4{0, 0, 0, 0};
     const int per_row = (p.columns + 7) / 8, all = p.rows * per_row;
-    constexpr int kMost = kSmall * kSmall / 8 / kThreads;  // (128 rows of 16 chunks)
+    constexpr int kMost = kSmall * kSmall / 8 / kThreads;
     float v[kMost][8];
     double total = 0;
 #pragma unroll
@@ -292,31 +301,31 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
             lo[j] = _Float16(up - float(hi[j]));
         }
         if (!tall) {
-            char* to = x_lds + small_at(row, first / 8);
+            char* to = x_lds + small_at(kX, row, first / 8);
             *reinterpret_cast<vec<_Float16, 8>*>(to) = hi;
             *reinterpret_cast<vec<_Float16, 8>*>(to + kPlane) = lo;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                char* to = x_lds + small_at(first + j, row / 8) + (row & 7) * 2;
+                if (first + j >= high) continue;
+                char* to = x_lds + small_at(kX, first + j, row / 8) + (row & 7) * 2;
                 *reinterpret_cast<_Float16*>(to) = hi[j];
                 *reinterpret_cast<_Float16*>(to + kPlane) = lo[j];
             }
         }
     }
     __syncthreads();
-    // this wave's block: the first ten lie on and below the diagonal, row by row
-    int bm, bn;
-    if (wave < 10) {
-        triangle_of(wave, bm, bn);
-    } else {
-        triangle_of(wave - 10, bn, bm);  // 0 0, 1 0, 1 1, ... exchanged, a column further
-        ++bn;
-    }
-    const int m = 32 * bm + (lane & 31), n = 32 * bn + 4 * half;  // element e: row m, column n + 8 (e / 4) + e % 4
-    const bool square = wave < 10 && 32 * bm < high, live = 32 * bm < high && 32 * bn < wide;
+    // this wave's block of X, and of A: the first ten waves have one on or below the diagonal
+    struct Block {
+        int m, n, row, column;  // element e: this row, column + 8 (e / 4) + e % 4
+    };
+    const auto block = [&](int m, int n) { return Block{m, n, 32 * m + (lane & 31), 32 * n + 4 * half}; };
+    int am, an;
+    triangle_of(wave, am, an);
+    const Block bx = block(wave / (width / 32), wave % (width / 32)), ba = block(am, an);
+    const bool square = wave < 10 && 32 * am < high, live = 32 * bx.m < high && 32 * bx.n < wide;
     // a block as f16 into LDS; turned: its transpose as well
-    const auto put = [&](char* to, int planes, bool turned, const Acc& c) __attribute__((always_inline)) {
+    const auto put = [&](char* to, int pitch, int planes, const Block& b, bool turned, const Acc& c) __attribute__((always_inline)) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             vec<_Float16, 4> hi, lo;
@@ -326,28 +335,29 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
                 hi[j] = _Float16(up);
                 lo[j] = _Float16(up - float(hi[j]));
             }
-            char* at = to + small_at(m, 4 * bn + g) + 8 * half;
+            char* at = to + small_at(pitch, b.row, 4 * b.n + g) + 8 * half;
             *reinterpret_cast<vec<_Float16, 4>*>(at) = hi;
             if (planes == 2) *reinterpret_cast<vec<_Float16, 4>*>(at + kPlane) = lo;
             if (turned)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    char* other = to + small_at(n + 8 * g + j, m / 8) + (m & 7) * 2;
+                    char* other = to + small_at(pitch, b.column + 8 * g + j, b.row / 8) + (b.row & 7) * 2;
                     *reinterpret_cast<_Float16*>(other) = hi[j];
                     if (planes == 2) *reinterpret_cast<_Float16*>(other + kPlane) = lo[j];
                 }
         }
     };
     // sum over k of A(m, k) B(n, k): rows of `a`, rows or columns of `b`
-    const auto product = [&](const char* a, const char* b, int steps, auto rows) __attribute__((always_inline)) {
+    const auto product = [&](const char* a, int a_pitch, const char* b, int b_pitch, const Block& at, int steps, auto rows) __attribute__((always_inline)) {
         Acc c = {};
         // (a step's fragments are read while the one before is multiplied; the last one reads its own again)
         Frag<_Float16> fb[2][PLANES], fa[2][PLANES];
         const auto read = [&](int k, int to) __attribute__((always_inline)) {
 #pragma unroll
             for (int q = 0; q < PLANES; ++q) {
-                fb[to][q] = decltype(rows)::value ? small_row(b + q * kPlane, bn, k, lane) : small_column(b + q * kPlane, bn, k, lane);
-                fa[to][q] = small_row(a + q * kPlane, bm, k, lane);
+                fb[to][q] = decltype(rows)::value ? small_row(b + q * kPlane, b_pitch, at.n, k, lane)
+                                                  : small_column(b + q * kPlane, b_pitch, at.n, k, lane);
+                fa[to][q] = small_row(a + q * kPlane, a_pitch, at.m, k, lane);
             }
         };
         const auto multiply_step = [&](int from) __attribute__((always_inline)) {
@@ -369,46 +379,46 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
     Acc x, a, c;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const char* at = x_lds + small_at(m, 4 * bn + g) + 8 * half;
+        const char* at = x_lds + small_at(kX, bx.row, 4 * bx.n + g) + 8 * half;
         const auto hi = *reinterpret_cast<const vec<_Float16, 4>*>(at), lo = *reinterpret_cast<const vec<_Float16, 4>*>(at + kPlane);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[4 * g + j] = (float(hi[j]) + float(lo[j])) * (1.f / kUp);
     }
     const int side_steps = (high + 15) / 16, wide_steps = (wide + 15) / 16;
-    const auto one = [&](int e) { return PLANES == 1 && m == n + 8 * (e >> 2) + (e & 3) && m < high ? 1.f : 0.f; };
+    const auto one = [&](int e) { return PLANES == 1 && ba.row == ba.column + 8 * (e >> 2) + (e & 3) && ba.row < high ? 1.f : 0.f; };
     for (int step = 0; step < p.steps; ++step) {
         if (square) {
             // (with one plane A - 1 is what is squared; the diagonal outside the matrix stays zero)
-            a = product(x_lds, x_lds, wide_steps, std::true_type{});
+            a = product(x_lds, kX, x_lds, kX, ba, wide_steps, std::true_type{});
 #pragma unroll
             for (int e = 0; e < 16; ++e) a[e] = a[e] * kDown - one(e);
-            put(g_lds, PLANES, bm != bn, a);
+            put(g_lds, kG, PLANES, ba, am != an, a);
         }
         __syncthreads();
         if (square) {
-            c = product(g_lds, g_lds, side_steps, std::true_type{});
+            c = product(g_lds, kG, g_lds, kG, ba, side_steps, std::true_type{});
 #pragma unroll
             for (int e = 0; e < 16; ++e) c[e] = poly_of<PLANES>(a[e], c[e] * kDown, one(e));
         }
         __syncthreads();
-        if (square) put(g_lds, PLANES, bm != bn, c);
+        if (square) put(g_lds, kG, PLANES, ba, am != an, c);
         __syncthreads();
         if (live) {
-            c = product(g_lds, x_lds, side_steps, std::false_type{});
+            c = product(g_lds, kG, x_lds, kX, bx, side_steps, std::false_type{});
             x = kA * x + kDown * c;
         }
         __syncthreads();
         if (step + 1 < p.steps) {
-            if (live) put(x_lds, 2, false, x);
+            if (live) put(x_lds, kX, 2, bx, false, x);
             __syncthreads();
         }
     }
     // out by whole rows, through LDS: 16-byte chunks turned with the row
-    const auto float_at = [&](int row, int column) { return x_lds + row * 512 + ((((column >> 2) ^ row) & 31) << 4) + (column & 3) * 4; };
+    const auto float_at = [&](int row, int column) { return x_lds + row * 4 * width + (((column >> 2) ^ (row & 31)) << 4) + (column & 3) * 4; };
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         const Quad four = {x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
-        *reinterpret_cast<Quad*>(float_at(m, n + 8 * g)) = four;
+        *reinterpret_cast<Quad*>(float_at(bx.row, bx.column + 8 * g)) = four;
     }
     __syncthreads();
     for (int at = threadIdx.x; at < all; at += kThreads) {
@@ -449,7 +459,7 @@ Matrices<T> matrices(const cpde_matrices* x) {
 template <class T, int PLANES>
 void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> last) {
     Device& d = *p.dev;
-    if (p.rows <= kSmall && p.columns <= kSmall) {
+    if (is_small(p.rows, p.columns)) {
         const SmallArgs a{p.rows, p.columns, p.steps, last.update, last.keep, last.rate};
         hipLaunchKernelGGL((orthogonal_small_k<T, PLANES>), unsigned(p.count), 1024, 0, d.stream, source, a, last.out);
         HIP_CHECK(hipGetLastError());
@@ -559,7 +569,7 @@ int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int
             at += (bytes + 255) / 256 * 256;
             return here;
         };
-        const bool small = rows <= kSmall && columns <= kSmall;
+        const bool small = is_small(rows, columns);
         if (!small) {
             p->sums = place(sizeof(double) * n * p->blocks);
             for (auto& x : p->x) x = place(2 * 2 * n * rows * pitch);

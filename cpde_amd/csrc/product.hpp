@@ -762,9 +762,10 @@ void launch_product(Device& d, ProductArgs p, const E& e) {
     } else if (c.side == 64) {
         launch_tiles(d, product_k<T, AK, BK, 64, 32, 32, 3, 2, false, E>, 64, 256, p, e);
     } else if (c.side == 128) {
-        // eight waves where a fragment costs a read (16 bits: 128 tiles, k = 1024, 11.9 us for 13.7), four where
-        // splitting it costs more (floats, 1,024 tiles, k = 1024: 185 us for 199)
-        constexpr int kWave = std::is_same_v<T, float> ? 64 : 32;
+        // eight waves, or four where a fragment costs more: floats' splits (1,024 tiles, k = 1024:
+        // 185 us for 199), transposing reads of both operands (4096 x 2048, k = 8192, bf16: 133 for 156;
+        // of neither, 128 tiles, k = 1024: 13.7, and 11.9 by eight)
+        constexpr int kWave = std::is_same_v<T, float> || (!AK && !BK) ? 64 : 32;
         launch_tiles(d, product_k<T, AK, BK, 128, 64, kWave, 2, 128 / kWave, false, E>, 128, 256 * 64 / kWave, p, e);
     } else {
         launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);

@@ -487,11 +487,11 @@ int cpde_dropout(cpde_device* dev, int dtype, int64_t rows, int64_t columns, con
 /* y = activation(x W^T + bias) + residual for at most `rows` rows a call: x
  * [rows][inputs], W [outputs][inputs] (a row an output), bias [outputs], residual and y
  * [rows][outputs], all of one type.  GELU is z (1 + erf(z / sqrt 2)) / 2, SILU
- * z / (1 + exp(-z)).  Products are summed in 32 bits.  Floats of large products are taken
- * as sums of three bf16 values (24 bits; products to 2^-24 of a row's and a column's
- * largest) on the bf16 instruction: as exact as the float one, but an infinity, or a
- * product of more than about 3.39e38, gives NaN there.  backward = 0:
- * cpde_linear_backward will not be called. */
+ * z / (1 + exp(-z)).  Products are summed in 32 bits.  Floats may be multiplied as exact
+ * sums of three bf16 values, whose least products (2^-21 of the factors' at most) are left
+ * out: about as exact as rounded floats, but an infinity in x, W or dz may give NaN where
+ * the float instruction would give an infinity.  A call of more than 2^31 / 256 tiles of
+ * 64 x 64 results is refused.  backward = 0: cpde_linear_backward will not be called. */
 #define CPDE_NONE 0
 #define CPDE_SIGMOID 1
 #define CPDE_RELU 2
