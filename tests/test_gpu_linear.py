@@ -354,6 +354,28 @@ def test_callers_stream(device):
     other.close()
 
 
+def test_past_32_bits(device):
+    """Rows more than 2^32 bytes from the first, on both sides and in the gradients."""
+    rows, inputs, outputs, stride = 70000, 64, 40, 32768
+    big = torch.empty(rows * stride, device='cuda', dtype=torch.bfloat16).view(rows, stride)
+    x, y, dy = big[:, :inputs], big[:, 128:128 + outputs], big[:, 256:256 + outputs]
+    for t, seed in ((x, 1), (dy, 2)):
+        t.copy_(matrix(rows, t.shape[1], 'bf16', seed=seed))
+    w = matrix(outputs, inputs, 'bf16', seed=3, scale=0.125)
+    plan = plan_of(device, 'bf16', rows, inputs, outputs, 'none')
+    forward(device, plan, x, w, None, None, pre=False, y=y)
+    last = slice(rows - 100, rows)
+    check(y[last], *linear(x[last].cpu(), w.cpu(), None, None, 'none', 'bf16')['y'], 'y')
+    dx, dw = torch.empty(rows, inputs, device='cuda', dtype=torch.bfloat16), torch.empty_like(w)
+    torch.cuda.synchronize()
+    plan.backward(rows, rows_of(x), rows_of(w), rows_of(dy), dx=rows_of(dx), dweight=rows_of(dw))
+    device.synchronize()
+    want = linear_gradient(x, w, None, dy, 'none', 'bf16')
+    check(dx[last], *(t[last].cpu() for t in want['dx']), 'dx')
+    check(dw, *(t.cpu() for t in want['dweight']), 'dweight')
+    plan.destroy()
+
+
 def refused(match, call):
     with pytest.raises(hip.CpdeError, match=match) as err:
         call()

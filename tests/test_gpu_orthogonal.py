@@ -60,6 +60,19 @@ def test_five_steps(device, dtype, count, rows, columns):
         assert far < orthogonal_far(dtype, max(rows, columns)), (i, far)
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('rows,columns', [(1500, 2056), (2100, 1030), (9000, 9016)])
+def test_large_matrices(device, dtype, rows, columns):
+    """One step on tiles of every size, against double on the GPU."""
+    print(f'[case] orthogonal {dtype} 1x{rows}x{columns}, one step', flush=True)
+    x = matrices(1, rows, columns, dtype)
+    got = forward(device, x, dtype, 1).double()
+    want, far = orthogonal_first(x, dtype)
+    assert ((got - want).abs() <= far).all()
+    # and no further than roundings of both signs leave sums
+    assert float((got - want).norm() / want.norm()) < orthogonal_far(dtype, columns) / 4 + UNIT[dtype]
+
+
 def test_singular_values(device):
     """What it is for: singular vectors stay, values come into 0.68..1.13 (and the type's rounding)."""
     for dtype in ('f32', 'bf16'):

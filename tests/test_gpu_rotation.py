@@ -159,6 +159,21 @@ def test_many_tokens(device):
     run(device, 'bf16', 3, 3001, 4, 1, 32)
 
 
+def test_past_32_bits(device):
+    """Entries of a cache more than 2^32 bytes apart."""
+    stride = (1 << 31) + 64
+    cache = torch.empty(2 * stride, device='cuda', dtype=torch.bfloat16)
+    k = cache.as_strided((2, 9, 2, 64), (stride, 128, 64, 1), 16)
+    k.copy_(tensor((2, 9, 2, 64), 'bf16', seed=2))
+    before = k.clone()
+    plan = hip.Rotation(device, hip.BF16, 2, 9, 0, 2, 64, backward=False)
+    torch.cuda.synchronize()
+    plan.forward(None, hip.Heads.of(k), None, hip.Heads.of(k))
+    device.synchronize()
+    plan.destroy()
+    check(k, *rotation(before.cpu(), None, torch.arange(9).expand(2, 9), 64, False, 10000.0, 1e-6, True, 'bf16')['out'], 'k_out')
+
+
 @pytest.mark.parametrize('batch,tokens', [(0, 4), (3, 0)])
 def test_no_tokens(device, batch, tokens):
     plan = hip.Rotation(device, hip.F32, batch, tokens, 2, 1, 16)
