@@ -524,7 +524,8 @@ __global__ __launch_bounds__(512, 2) void product_large_k(ProductArgs p, Epilogu
 // Small products and few rows: a workgroup makes a tile of 32 x 32, its waves sharing the
 // inner axis, each with tiles of its own in LDS, two at a time and no barrier until
 // their sums are joined.  Bound: the latency of a launch and of a round or two of loads; with
-// few rows and a large matrix, HBM.
+// few rows and a large matrix, HBM (16 rows, 2048 -> 8192, bf16: 34 MB in 7.9 us, 4.3 TB/s; 11.8 by
+// split 64 x 64 tiles and a join; fragments straight from memory, 32 bytes a row, 11.3).
 template <class T, bool AK, bool BK, bool Any, class Epilogue>
 __global__ __launch_bounds__(512) void product_run_k(ProductArgs p, Epilogue e) {
     extern __shared__ __align__(16) char lds[];  // [wave][2][A, B], then [wave][32][36] sums
@@ -672,8 +673,7 @@ constexpr ProductTime kTimes16[] = {{64, 3.8, 0.30, 0.195}, {128, 4.2, 0.62, 0.4
 constexpr ProductTime kTimes32[] = {{64, 4.5, 0.65, 0.53}, {128, 8.0, 1.55, 1.43}, {256, 14.0, 4.7, 4.7}};
 constexpr ProductTime kTimesPair[] = {{64, 4.0, 0.40, 0.27}, {128, 5.0, 0.95, 0.75}, {256, 12.0, 2.2, 2.2}};
 template <class T>
-ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, bool wide,
-                              bool symmetric) {
+ProductCut cut_product(int compute_units, int64_t batch, int64_t m, int64_t n, int64_t k, bool wide, bool symmetric) {
     constexpr int size = sizeof(T);
     ProductCut best;
     double least = 1e30;
@@ -732,8 +732,7 @@ void launch_tiles(Device& d, K kernel, int side, int threads, ProductArgs p, con
     p.m_tiles = ceil_div(p.m, side);
     p.n_tiles = ceil_div(p.n, side);
     const int64_t tiles = p.symmetric ? int64_t(p.m_tiles) * (p.m_tiles + 1) / 2 : int64_t(p.m_tiles) * p.n_tiles;
-    require(tiles * threads < (int64_t(1) << 31) && int64_t(p.splits) * p.batch < 65536,
-            "too many workgroups");
+    require(tiles * threads < (int64_t(1) << 31) && int64_t(p.splits) * p.batch < 65536, "too many workgroups");
     hipLaunchKernelGGL(kernel, dim3(unsigned(tiles), unsigned(p.splits) * p.batch), threads, lds, d.stream, p, e);
     HIP_CHECK(hipGetLastError());
 }
