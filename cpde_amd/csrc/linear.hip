@@ -194,12 +194,13 @@ void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
     args.part = reinterpret_cast<float*>(p.work + p.part);
     args.a = product_operand(s.a, s.a_stride, s.a_whole ? s.a_stride : AK ? s.k : s.m, sizeof(T));
     args.b = product_operand(s.b, s.b_stride, BK ? s.k : s.n, sizeof(T));
-    // Operands that are not whole chunks are read value by value, tile by tile, where that is a
-    // few tiles; more are copied to whole chunks first (a plan whose widths are not whole
-    // eights has room for it).  2,748 -> 4,776 over 3,962 rows in training, bf16: 2,545 us value by
-    // value, 497 with copies of x and W.
-    const int64_t tiles = int64_t(ceil_div(s.m, 64)) * ceil_div(s.n, 64), deep = ceil_div(s.k, kDepth<T>);
-    if ((!args.a.wide || !args.b.wide) && p.a_copy && deep * std::max<int64_t>(1, tiles / (4 * d.compute_units)) > 6) {
+    // Operands that are not whole chunks are read by registers, a tile at a time, where few tiles
+    // share them; else they are copied to whole chunks first (a plan whose widths are not whole
+    // eights has room for it).  2,047 -> 2,047, bf16: 128 rows 16.2 us by registers, 17.2 copied, 256
+    // rows 27.2 and 20.6, 1,024 rows 54.9 and 29.9.
+    const int64_t m_tiles = ceil_div(s.m, 64), n_tiles = ceil_div(s.n, 64), deep = ceil_div(s.k, kDepth<T>);
+    const bool shared = std::min(m_tiles, n_tiles) > 2 && deep * std::max<int64_t>(1, m_tiles * n_tiles / (4 * d.compute_units)) > 12;
+    if ((!args.a.wide || !args.b.wide) && p.a_copy && shared) {
         const auto copy = [&](Operand& o, const void* x, int64_t stride, int64_t rows, int64_t columns, size_t place) {
             if (o.wide) return;
             const int pitch = pitch_of(columns);

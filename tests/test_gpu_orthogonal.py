@@ -38,7 +38,7 @@ def forward(device, x, dtype, steps, out=None):
 
 SIZES = [(1, 1, 1), (1, 1, 40), (3, 7, 5), (2, 16, 16), (1, 33, 70), (2, 64, 64), (1, 100, 257), (4, 128, 128), (1, 130, 129),
          (2, 300, 72), (1, 40, 600), (1, 260, 512),
-         (2, 64, 256), (1, 65, 256), (3, 32, 512), (2, 500, 17), (1, 33, 512), (2, 200, 61), (1, 16, 513), (4, 8, 129)]
+         (2, 64, 256), (1, 65, 256), (3, 32, 512), (2, 500, 17), (1, 33, 512), (2, 200, 61), (1, 16, 513), (4, 8, 129), (1, 1, 1000), (2, 700, 1)]
 
 
 @pytest.mark.parametrize('dtype', ['f32', 'f16', 'bf16'])
