@@ -66,7 +66,7 @@ struct LinearEpilogue {
     struct Columns {
         float bias[8];
     };
-    __device__ Columns columns(int n, int count) const {
+    __device__ Columns columns(int, int n, int count) const {
         Columns c{};
         if (bias) read8(c.bias, bias + n, count);
         return c;

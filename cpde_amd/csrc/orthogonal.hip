@@ -16,16 +16,17 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 // of two f16 values (22 bits; three of the four products, to 2^-22), so that the products
 // stay as exact as the type; bf16 ones as one.  X itself is kept as a sum of two whatever the
 // type: its roundings pass through all later steps, which multiply small singular values by
-// up to 485.
+// up to 485.  With one value an operand the diagonals D of A and of b A + c A^2 stay apart in
+// 32 bits, and the operands hold zeros there: a row's diagonal is the largest of it, and
+// alike in all rows of a matrix with even singular values, so that its rounding would move
+// all of them one way (4 x 15 x 526: 0.0026 from the exact values for 0.0017, which is the
+// type's own rounding).  With A = D + O: A^2 = D^2 + D O + O D + O^2.
 constexpr float kUp = 4096.f, kDown = 1.f / (4096.f * 4096.f);
 
-// b A + c A^2 from a = A - one (one: the diagonal, or zero) and a's square.
+// b A + c A^2 of an entry from A and A^2; with one plane from O^2, less the diagonal's share.
 template <int PLANES>
-__device__ inline float poly_of(float a, float square, float one) {
-    if (PLANES == 1) {
-        square += 2 * a + one;  // A^2 = (A - 1)^2 + 2 (A - 1) + 1
-        a += one;
-    }
+__device__ inline float poly_of(float a, float square, bool diagonal, float row, float column) {
+    if (PLANES == 1) square += a * (diagonal ? a : row + column);
     return kB * a + kC * square;
 }
 
@@ -37,7 +38,8 @@ struct Orthogonal {
     int side() const { return std::min(rows, columns); }
     int planes() const { return dtype == CPDE_BF16 ? 1 : 2; }
     char* work = nullptr;
-    size_t sums = 0, x[2] = {}, gram = 0, poly = 0, part = 0;  // places in the workspace
+    // places in the workspace (diagonal: of A, then of b A + c A^2)
+    size_t sums = 0, x[2] = {}, gram = 0, poly = 0, diagonal = 0, part = 0;
 };
 int pitch_of(int columns) { return (columns + 31) / 32 * 32; }  // (whole groups of pairs)
 
@@ -149,37 +151,57 @@ __global__ __launch_bounds__(256) void orthogonal_scale_k(Source<T> s, Shape p, 
     }
 }
 
-// A from its product.  With one plane an operand, what is kept and squared is A - 1: near the
-// end A is, and the rounding of what differs from it is the smaller by as much.
+// What stands on the diagonal at a lane's eight columns.
+struct Diagonal {
+    float d[8];
+};
+// A from its product.
 template <int PLANES>
 struct GramEpilogue {
     static constexpr bool kSymmetric = true, kAny = false;
     _Float16* gram;
+    float* diagonal;  // (of one plane)
     int side, pitch;
-    __device__ int columns(int, int) const { return 0; }
+    __device__ int columns(int, int, int) const { return 0; }
     __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = j < count ? v[j] * kDown - (PLANES == 1 && m == n + j ? 1.f : 0.f) : 0.f;
+        for (int j = 0; j < 8; ++j) {
+            v[j] = j < count ? v[j] * kDown : 0.f;
+            if (PLANES == 1 && m == n + j) {
+                diagonal[batch * side + m] = v[j];
+                v[j] = 0;
+            }
+        }
         write_halves(gram + half_at<PLANES>(int64_t(batch) * side + m, pitch, n), 32, PLANES == 2, v);
     }
 };
-// b A + c A^2 from the square of A (or of A - 1, less 1 - 2 A).
+// b A + c A^2 from the square of A (or of O).
 template <int PLANES>
 struct PolyEpilogue {
     static constexpr bool kSymmetric = true, kAny = false;
     const _Float16* gram;
     _Float16* poly;
+    const float* diagonal;
+    float* poly_diagonal;
     int side, pitch;
-    __device__ int columns(int, int) const { return 0; }
-    __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
+    __device__ Diagonal columns(int batch, int n, int count) const {
+        Diagonal c = {};
+        if (PLANES == 1 && count > 0) read8(c.d, diagonal + batch * side + n, count);
+        return c;
+    }
+    __device__ void row(const Diagonal& column, int batch, int m, int n, int count, float (&v)[8]) const {
         const int64_t at = half_at<PLANES>(int64_t(batch) * side + m, pitch, n);
         float a[8];
         read_halves(a, gram + at, 32, PLANES == 2);
+        const float row = PLANES == 1 ? diagonal[batch * side + m] : 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float one = PLANES == 1 && m == n + j ? 1.f : 0.f, square = v[j] * kDown;
-            v[j] = j < count ? poly_of<PLANES>(a[j], square, one) : 0.f;
+            const bool one = PLANES == 1 && m == n + j;
+            v[j] = j < count ? poly_of<PLANES>(one ? row : a[j], v[j] * kDown, one, row, column.d[j]) : 0.f;
+            if (one) {
+                poly_diagonal[batch * side + m] = v[j];
+                v[j] = 0;
+            }
         }
         write_halves(poly + at, 32, PLANES == 2, v);
     }
@@ -190,17 +212,24 @@ struct StepEpilogue {
     static constexpr bool kSymmetric = false, kAny = false;
     const _Float16* x;
     _Float16* next;  // null: the last step
+    const float* diagonal;  // of b A + c A^2, with one plane
     int64_t plane;
-    int rows, pitch, update;
+    int rows, side, pitch, update;
+    bool tall;  // (A stands on the right)
     Matrices<T> out;
     float keep, rate;  // weights <- keep weights - rate X
-    __device__ int columns(int, int) const { return 0; }
-    __device__ void row(int, int batch, int m, int n, int count, float (&v)[8]) const {
+    __device__ Diagonal columns(int batch, int n, int count) const {
+        Diagonal c = {};
+        if (PLANES == 1 && tall && count > 0) read8(c.d, diagonal + batch * side + n, count);
+        return c;
+    }
+    __device__ void row(const Diagonal& column, int batch, int m, int n, int count, float (&v)[8]) const {
         const int64_t at = half_at<PLANES>(int64_t(batch) * rows + m, pitch, n), second = second_of<PLANES>(plane);
         float old[8];
         read_halves(old, x + at, second, true);
+        const float row = PLANES == 1 && !tall ? diagonal[batch * side + m] : 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < count ? kA * old[j] + v[j] * kDown : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = j < count ? (kA + (row + column.d[j])) * old[j] + v[j] * kDown : 0.f;
         if (next) {
             write_halves(next + at, second, true, v);
             return;
@@ -259,6 +288,7 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
     __shared__ __align__(16) char x_lds[2 * kPlane];       // X; at the end the result in floats
     __shared__ __align__(16) char g_lds[PLANES * kPlane];
     __shared__ double sums[16];
+    __shared__ float diagonal[kSmall];  // with one plane: of A, then of b A + c A^2
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, matrix = blockIdx.x;
     const bool tall = p.rows > p.columns;
     const int high = min(p.rows, p.columns), wide = max(p.rows, p.columns);
@@ -385,27 +415,39 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
         for (int j = 0; j < 4; ++j) x[4 * g + j] = (float(hi[j]) + float(lo[j])) * (1.f / kUp);
     }
     const int side_steps = (high + 15) / 16, wide_steps = (wide + 15) / 16;
-    const auto one = [&](int e) { return PLANES == 1 && ba.row == ba.column + 8 * (e >> 2) + (e & 3) && ba.row < high ? 1.f : 0.f; };
+    const auto on_diagonal = [&](int e) { return PLANES == 1 && ba.row == ba.column + 8 * (e >> 2) + (e & 3); };
+    // a symmetric matrix's block into LDS; with one plane its diagonal apart, zeros in its place
+    const auto put_square = [&](Acc v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (on_diagonal(e)) {
+                diagonal[ba.row] = v[e];
+                v[e] = 0;
+            }
+        put(g_lds, kG, PLANES, ba, am != an, v);
+    };
     for (int step = 0; step < p.steps; ++step) {
         if (square) {
-            // (with one plane A - 1 is what is squared; the diagonal outside the matrix stays zero)
             a = product(x_lds, kX, x_lds, kX, ba, wide_steps, std::true_type{});
-#pragma unroll
-            for (int e = 0; e < 16; ++e) a[e] = a[e] * kDown - one(e);
-            put(g_lds, kG, PLANES, ba, am != an, a);
+            a *= kDown;
+            put_square(a);
         }
         __syncthreads();
         if (square) {
             c = product(g_lds, kG, g_lds, kG, ba, side_steps, std::true_type{});
+            const float row = PLANES == 1 ? diagonal[ba.row] : 0;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) c[e] = poly_of<PLANES>(a[e], c[e] * kDown, one(e));
+            for (int e = 0; e < 16; ++e) {
+                const float column = PLANES == 1 ? diagonal[ba.column + 8 * (e >> 2) + (e & 3)] : 0;
+                c[e] = poly_of<PLANES>(a[e], c[e] * kDown, on_diagonal(e), row, column);
+            }
         }
         __syncthreads();
-        if (square) put(g_lds, kG, PLANES, ba, am != an, c);
+        if (square) put_square(c);
         __syncthreads();
         if (live) {
             c = product(g_lds, kG, x_lds, kX, bx, side_steps, std::false_type{});
-            x = kA * x + kDown * c;
+            x = (kA + (PLANES == 1 ? diagonal[bx.row] : 0.f)) * x + kDown * c;
         }
         __syncthreads();
         if (step + 1 < p.steps) {
@@ -469,6 +511,7 @@ void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> l
     const int pitch = pitch_of(p.columns), side = p.side(), side_pitch = pitch_of(side);
     const auto at = [&](size_t place) { return reinterpret_cast<_Float16*>(p.work + place); };
     double* sums = reinterpret_cast<double*>(p.work + p.sums);
+    float *diagonal = reinterpret_cast<float*>(p.work + p.diagonal), *poly_diagonal = diagonal + int64_t(p.count) * side;
     _Float16 *x[2] = {at(p.x[0]), at(p.x[1])}, *gram = at(p.gram), *poly = at(p.poly);
     const Shape shape{p.rows, p.columns, pitch, p.blocks};
     const int64_t plane = int64_t(p.count) * p.rows * pitch;
@@ -492,18 +535,21 @@ void run(const Orthogonal& p, const Source<T>& source, StepEpilogue<T, PLANES> l
         q.m = q.n = side;
         q.a = q.b = xs;
         q.k = p.tall() ? p.rows : pitch;
-        const GramEpilogue<PLANES> ge{gram, side, side_pitch};
+        const GramEpilogue<PLANES> ge{gram, diagonal, side, side_pitch};
         if (p.tall()) launch_product<Value, false, false>(d, q, ge);
         else launch_product<Value, true, true>(d, q, ge);
         q.a = q.b = as;
         q.k = side_pitch;
-        launch_product<Value, true, true>(d, q, PolyEpilogue<PLANES>{gram, poly, side, side_pitch});
+        launch_product<Value, true, true>(d, q, PolyEpilogue<PLANES>{gram, poly, diagonal, poly_diagonal, side, side_pitch});
         q.symmetric = 0;
         q.m = p.rows;
         q.n = p.columns;
         StepEpilogue<T, PLANES> se = last;
         se.x = x[step & 1];
         se.next = step + 1 < p.steps ? x[(step + 1) & 1] : nullptr;
+        se.diagonal = poly_diagonal;
+        se.side = side;
+        se.tall = p.tall();
         se.plane = plane;
         se.rows = p.rows;
         se.pitch = pitch;
@@ -575,6 +621,7 @@ int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int
             for (auto& x : p->x) x = place(2 * 2 * n * rows * pitch);
             p->gram = place(2 * p->planes() * n * side * side_pitch);
             p->poly = place(2 * p->planes() * n * side * side_pitch);
+            p->diagonal = place(sizeof(float) * 2 * n * side);
             p->part = place(sizeof(float) * std::max(product_part(dev->compute_units, count, side, side),
                                                  product_part(dev->compute_units, count, rows, columns)));
         }

@@ -379,7 +379,7 @@ struct Tiles {
         float* stage = reinterpret_cast<float*>(lds + wave * kStage);
         constexpr int kLanes = WN / 8, kAtOnce = 64 / kLanes;
         const int half = lane >> 5, column = (lane % kLanes) * 8, n = n0 + wn * WN + column;
-        const auto columns = e.columns(n, min(8, p.n - n));
+        const auto columns = e.columns(batch, n, min(8, p.n - n));
 #pragma unroll
         for (int i = 0; i < kMB; ++i) {
 #pragma unroll
@@ -412,7 +412,7 @@ struct Tiles {
                         float v[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = stage[(from + j) * kPitch + to];
-                        if (m < p.n && n < p.m) e.row(e.columns(n, min(8, p.m - n)), batch, m, n, min(8, p.m - n), v);
+                        if (m < p.n && n < p.m) e.row(e.columns(batch, n, min(8, p.m - n)), batch, m, n, min(8, p.m - n), v);
                     }
             }
             __builtin_amdgcn_wave_barrier();
@@ -590,7 +590,7 @@ __global__ __launch_bounds__(512) void product_run_k(ProductArgs p, Epilogue e) 
             for (int j = 0; j < 8; ++j) v[j] += from[j];
         }
         const int n = n0 + column, count = min(8, p.n - n);
-        if (m0 + row < p.m && n < p.n) e.row(e.columns(n, count), batch, m0 + row, n, count, v);
+        if (m0 + row < p.m && n < p.n) e.row(e.columns(batch, n, count), batch, m0 + row, n, count, v);
     }
 }
 template <class T>
@@ -611,7 +611,7 @@ __global__ __launch_bounds__(256) void product_join_k(ProductArgs p, Epilogue e)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += one[j];
     }
-    e.row(e.columns(n, count), batch, int(row - int64_t(batch) * p.m), n, count, v);
+    e.row(e.columns(batch, n, count), batch, int(row - int64_t(batch) * p.m), n, count, v);
 }
 
 // The same of a symmetric product: 64 x 64 on and below the diagonal a workgroup, stored
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(256) void product_join_symmetric_k(ProductArgs p, E
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) stage[row][column + part + j] = v[j];
-        if (m < p.m && n < p.n) e.row(e.columns(n, count), batch, m, n, count, v);
+        if (m < p.m && n < p.n) e.row(e.columns(batch, n, count), batch, m, n, count, v);
     }
     __syncthreads();
     if (tm == tn) return;
@@ -646,7 +646,7 @@ __global__ __launch_bounds__(256) void product_join_symmetric_k(ProductArgs p, E
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = stage[column + part + j][row];
-        if (m < p.n && n < p.m) e.row(e.columns(n, count), batch, m, n, count, v);
+        if (m < p.n && n < p.m) e.row(e.columns(batch, n, count), batch, m, n, count, v);
     }
 }
 

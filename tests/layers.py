@@ -137,7 +137,8 @@ def orthogonal(x, steps):
 
 def orthogonal_first(x, dtype):
     """(values, bounds) of one step.  Operands of the products are off by half a unit of f16
-    (bf16 matrices) or of a sum of two of them; in the first case A - 1 is what is squared."""
+    (bf16 matrices) or of a sum of two of them; in the first case without the diagonals of A and
+    of b A + c A^2, which stay as they are."""
     a, b, c = QUINTIC
     h = 2.0 ** -11 if dtype == 'bf16' else PAIR
     least = 2.0 ** -24 / 4096      # of an operand times 2^12
@@ -151,16 +152,17 @@ def orthogonal_first(x, dtype):
     gram = x @ x.transpose(1, 2).contiguous()
     spread = x.abs().sum(2)
     gram_off = (2 * h + (3 * k + 16) * E) * size + least * (spread[:, :, None] + spread[:, None, :])
-    eye = torch.eye(r, dtype=torch.float64, device=x.device)
-    inner = (gram - eye if dtype == 'bf16' else gram).abs() + gram_off
-    inner_off = gram_off + h * inner + least
-    square_off = inner @ inner_off + inner_off @ inner + (3 * r + 16) * E * (inner @ inner)
+    off = torch.ones_like(gram[0]) - (torch.eye(r, dtype=torch.float64, device=x.device) if dtype == 'bf16' else 0)
+    gram_off = gram_off + off * (h * (gram.abs() + gram_off) + least)
+    inner = gram.abs() + gram_off
+    square_off = inner @ gram_off + gram_off @ inner + (3 * r + 16) * E * (inner @ inner)
     poly = b * gram + c * (gram @ gram)
-    poly_off = abs(b) * gram_off + c * (square_off + (2 * gram_off if dtype == 'bf16' else 0)) + 8 * E * (1 + gram.abs())
-    poly_off = poly_off + h * (poly.abs() + poly_off) + least
+    poly_off = abs(b) * gram_off + c * square_off + 8 * E * (1 + gram.abs())
+    poly_off = poly_off + off * (h * (poly.abs() + poly_off) + least)
     y = a * x + poly @ x
-    # (X itself is a sum of two f16 values, to `least` where it is small)
-    y_off = (a * (PAIR * x.abs() + least) + poly_off @ x.abs() + (poly.abs() + poly_off) @ (h * x.abs() + least)
+    # (X itself is a sum of two f16 values, to `least` where it is small; in products one)
+    y_off = (a * (PAIR * x.abs() + least) + ((1 - off) * poly.abs()) @ (PAIR * x.abs() + least) + poly_off @ x.abs()
+             + (off * (poly.abs() + poly_off)) @ (h * x.abs() + least)
              + (3 * r + 16) * E * (poly.abs() @ x.abs()) + 8 * E * (a * x.abs() + y.abs()))
     y_off = y_off + UNIT[dtype] * (y.abs() + y_off) + TINY[dtype]
     return tuple((t.transpose(1, 2) if tall else t).contiguous() for t in (y, y_off))

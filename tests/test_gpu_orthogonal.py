@@ -73,6 +73,22 @@ def test_large_matrices(device, dtype, rows, columns):
     assert float((got - want).norm() / want.norm()) < orthogonal_far(dtype, columns) / 4 + UNIT[dtype]
 
 
+@pytest.mark.parametrize('count,rows,columns', [(4, 15, 526), (1, 40, 700), (3, 8, 200), (2, 1100, 64), (1, 24, 480), (1, 1, 600),
+                                                (1, 140, 2600)])
+def test_even_singular_values(device, count, rows, columns):
+    """Where A is nearly one number times the unit matrix, five steps of bf16 matrices are as
+    exact as the type: what is rounded inside is off the diagonal only, a row of it at most
+    0.3 of the diagonal (sqrt(rows / columns)), each to rms 2^-12 and weighed by 1.4 at most
+    (4.775 of 3.44), independently in five steps whose errors later ones raise by 5 at most:
+    under 0.3 * 1.4 * 2^-12 * sqrt(5) * 5 = 0.0011.  Rounding the result leaves 0.0017."""
+    print(f'[case] orthogonal bf16 {count}x{rows}x{columns}, even', flush=True)
+    x = matrices(count, rows, columns, 'bf16')
+    got, want = forward(device, x, 'bf16', 5).double(), orthogonal(x, 5)
+    least = float((want.bfloat16().double() - want).norm() / want.norm())
+    far = float((got - want).norm() / want.norm())
+    assert far < 1.25 * least, (far, least)
+
+
 def test_singular_values(device):
     """What it is for: singular vectors stay, values come into 0.68..1.13 (and the type's rounding)."""
     for dtype in ('f32', 'bf16'):
