@@ -89,19 +89,52 @@ struct LinearEpilogue {
     }
 };
 
+// Rows copied to whole 16-byte chunks, zeros behind their columns.  Where `again` is not 0:
+// row r goes to rows r * every and r * every + again, and zeros follow the last one up to `all_rows`.
+struct CopyArgs {
+    int64_t stride, rows, all_rows;
+    int columns, pitch, every, again;
+};
+template <class T>
+__device__ inline void copy_chunks(const T* x, T* to, const CopyArgs& c, int64_t first_chunk, int64_t step) {
+    const int per_row = c.pitch / 8;
+    const int64_t all = c.all_rows * per_row;
+    for (int64_t at = first_chunk; at < all; at += step) {
+        const int64_t row = at / per_row;
+        const int first = int(at - row * per_row) * 8;
+        float v[8] = {};
+        if (row < c.rows) read8(v, x + row * c.stride + first, min(8, c.columns - first));
+        T* at_row = to + row * c.every * c.pitch + first;
+        write8(at_row, v, 8);
+        if (c.again) write8(at_row + int64_t(c.again) * c.pitch, v, 8);
+    }
+}
+
 // ---- dz = dy * slope(pre) and its sums over the rows -----------------------------------------
 // A workgroup takes 64 columns, eight a lane, of a strip of rows, 32 rows at a time; sums
-// of a strip go to `part` [strip][columns], which linear_bias_k adds up in order.
+// of a strip go to `part` [strip][columns], which linear_bias_k adds up in order.  Workgroups
+// behind the last strip write what a dz of two values meets twice: weights, then x.
 struct SlopeArgs {
     const void *dy, *pre;
     void* dz;       // null: not wanted (no activation)
+    int64_t low;    // of what dz's rounding leaves, behind dz (0: not wanted)
     float* part;    // null: not wanted (no bias)
     int64_t dy_stride, pre_stride, rows;
-    int columns, dz_stride, strip, activation;
+    int columns, dz_stride, strip, strips, activation;
+    const void* from[2];
+    void* to[2];
+    CopyArgs copy[2];
 };
 template <class T>
 __global__ __launch_bounds__(256) void linear_slope_k(SlopeArgs a) {
     __shared__ float sums[32][64 + 8];
+    if (int(blockIdx.y) >= a.strips) {
+        const int64_t at = (int64_t(blockIdx.y - a.strips) * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+        const int64_t step = int64_t(gridDim.y - a.strips) * gridDim.x * 256;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) copy_chunks(static_cast<const T*>(a.from[i]), static_cast<T*>(a.to[i]), a.copy[i], at, step);
+        return;
+    }
     const int lane = threadIdx.x & 7, row_lane = threadIdx.x >> 3, n = blockIdx.x * 64 + lane * 8;
     const int count = min(8, a.columns - n);
     const int64_t first = int64_t(blockIdx.y) * a.strip, last = min(first + a.strip, a.rows);
@@ -116,7 +149,17 @@ __global__ __launch_bounds__(256) void linear_slope_k(SlopeArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] *= slope<T, decltype(kind)::value>(z[j]);
                 });
-                write8(static_cast<T*>(a.dz) + m * a.dz_stride + n, v, 8);  // (zeros behind the columns)
+                T* to = static_cast<T*>(a.dz) + m * a.dz_stride + n;
+                write8(to, v, 8);  // (zeros behind the columns)
+                if (a.low) {
+                    float left[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float high = float(T(v[j]));
+                        left[j] = isfinite(high) ? v[j] - high : 0.f;
+                    }
+                    write8(to + a.low, left, 8);
+                }
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += v[j];
@@ -153,27 +196,31 @@ struct Linear {
     int dtype = 0, inputs = 0, outputs = 0, activation = 0, backward = 0;
     int64_t rows = 0;
     char* work = nullptr;
-    size_t a_copy = 0, b_copy = 0, dz = 0, part = 0, bias_part = 0;  // places in the workspace
+    size_t a_copy = 0, b_copy = 0, dz = 0, twice[2] = {}, part = 0, bias_part = 0;  // places in the workspace
 };
 constexpr int64_t kMostRows = int64_t(1) << 30;
 constexpr int kMostWidth = 1 << 24;
 constexpr int kStrips = 256;  // of a bias's gradient
-
+// Gradients of at most kFew values, from matrices of at most kFewInner, take a 16-bit dz as a
+// sum of two values (the inner axis twice as long, its other operand written twice by
+// linear_slope_k), and are as exact as the type.  Such calls wait for launches more than for
+// products (256 -> 256, 256 rows: 13.5 us with and without; 128 -> 128, 1,000 rows: 16.4 for
+// 13.5; 64 -> 64, 16,384 rows: 33 for 27).  Beyond, dz is rounded once and the products run at
+// the matrix units' rate: the results lie 1.4 times as far from the exact ones.
+constexpr int64_t kFew = 1 << 17, kFewInner = 1 << 20;
 
 int pitch_of(int64_t columns) { return int((columns + 7) / 8 * 8); }
 
-// Rows copied to whole 16-byte chunks, zeros behind their columns.
 template <class T>
-__global__ __launch_bounds__(256) void linear_copy_k(const T* x, int64_t stride, int64_t rows, int columns, T* to, int pitch) {
-    const int per_row = pitch / 8;
-    const int64_t all = rows * per_row, step = int64_t(gridDim.x) * 256;
-    for (int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x; at < all; at += step) {
-        const int64_t row = at / per_row;
-        const int first = int(at - row * per_row) * 8;
-        float v[8];
-        read8(v, x + row * stride + first, min(8, columns - first));
-        write8(to + row * pitch + first, v, 8);
-    }
+__global__ __launch_bounds__(256) void linear_copy_k(const T* x, T* to, CopyArgs c) {
+    copy_chunks(x, to, c, int64_t(blockIdx.x) * 256 + threadIdx.x, int64_t(gridDim.x) * 256);
+}
+template <class T>
+void copy_rows(Device& d, const void* x, T* to, const CopyArgs& c) {
+    const int64_t chunks = c.all_rows * (c.pitch / 8);
+    const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>((chunks + 255) / 256, int64_t(d.compute_units) * 32)));
+    hipLaunchKernelGGL((linear_copy_k<T>), blocks, 256, 0, d.stream, static_cast<const T*>(x), to, c);
+    HIP_CHECK(hipGetLastError());
 }
 
 // C[m][n] of a plan's product: operands by their rows, which AK and BK say the order of.
@@ -181,7 +228,7 @@ struct Sides {
     const void *a, *b;
     int64_t a_stride, b_stride, m, k;
     int n;
-    bool a_whole;  // a's rows go on in zeros to whole chunks
+    bool a_whole, b_whole;  // its rows go on in zeros to whole chunks
 };
 template <bool AK, bool BK, class T>
 void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
@@ -193,7 +240,7 @@ void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
     args.batch = 1;
     args.part = reinterpret_cast<float*>(p.work + p.part);
     args.a = product_operand(s.a, s.a_stride, s.a_whole ? s.a_stride : AK ? s.k : s.m, sizeof(T));
-    args.b = product_operand(s.b, s.b_stride, BK ? s.k : s.n, sizeof(T));
+    args.b = product_operand(s.b, s.b_stride, s.b_whole ? s.b_stride : BK ? s.k : s.n, sizeof(T));
     // Operands that are not whole chunks are read by registers, a tile at a time, where few tiles
     // share them; else they are copied to whole chunks first (a plan whose widths are not whole
     // eights has room for it).  2,047 -> 2,047, bf16: 128 rows 16.2 us by registers, 17.2 copied, 256
@@ -205,10 +252,7 @@ void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
             if (o.wide) return;
             const int pitch = pitch_of(columns);
             T* to = reinterpret_cast<T*>(p.work + place);
-            const int64_t chunks = rows * (pitch / 8);
-            const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>((chunks + 255) / 256, int64_t(d.compute_units) * 32)));
-            hipLaunchKernelGGL((linear_copy_k<T>), blocks, 256, 0, d.stream, static_cast<const T*>(x), stride, rows, int(columns), to, pitch);
-            HIP_CHECK(hipGetLastError());
+            copy_rows<T>(d, x, to, {stride, rows, rows, int(columns), pitch, 1, 0});
             o = product_operand(to, pitch, pitch, sizeof(T));
         };
         copy(args.a, s.a, s.a_stride, AK ? s.m : s.k, AK ? s.k : s.m, p.a_copy);
@@ -266,7 +310,13 @@ int cpde_linear_create(cpde_device* dev, int dtype, int64_t rows, int inputs, in
             p->a_copy = place(size * rows * (backward ? std::max(in, o) : in));
             p->b_copy = place(size * std::max(size_t(outputs) * in, backward ? size_t(rows) * in : 0));
         }
-        if (backward && activation != CPDE_NONE) p->dz = place(type_bytes(dtype) * rows * pitch_of(outputs));
+        if (backward && activation != CPDE_NONE) {
+            const int64_t in = pitch_of(inputs), o = pitch_of(outputs);
+            const bool short_type = dtype != CPDE_F32;  // (dz as two values, and what they meet written twice)
+            p->dz = place(type_bytes(dtype) * (short_type ? std::max(rows * o, std::min(2 * rows * o, 2 * kFewInner)) : rows * o));
+            if (short_type)
+                for (int i = 0; i < 2; ++i) p->twice[i] = place(type_bytes(dtype) * std::min(2 * (i ? rows : o) * in, 2 * kFewInner));
+        }
         if (backward) p->bias_part = place(sizeof(float) * kStrips * outputs);
         size_t part = product_part(dev->compute_units, 1, rows, outputs);
         if (backward)
@@ -320,7 +370,7 @@ int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, c
                 e.pre_stride = pre->stride;
             }
             e.activation = p.activation;
-            product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs, false}, e);
+            product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs, false, false}, e);
         });
     });
 }
@@ -353,6 +403,11 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
             using T = decltype(element);
             const void* dz = dy->data;
             int64_t dz_stride = dy->stride;  // (of the plan's own: whole chunks, zeros behind the columns)
+            const int in = pitch_of(p.inputs), o = pitch_of(p.outputs);
+            // (rows and widths to whole chunks are what is written)
+            const bool two = bent && sizeof(T) == 2 && rows * o <= kFewInner;
+            const bool two_x = two && dx && rows * in <= kFew && int64_t(o) * in <= kFewInner;
+            const bool two_w = two && dweight && int64_t(o) * in <= kFew && rows * in <= kFewInner;
             if ((bent || dbias) && p.outputs) {
                 SlopeArgs a{};
                 a.dy = dy->data;
@@ -364,7 +419,8 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     a.pre = pre->data;
                     a.pre_stride = pre->stride;
                     a.dz = p.work + p.dz;
-                    a.dz_stride = pitch_of(p.outputs);
+                    a.dz_stride = two_x || two_w ? 2 * o : o;
+                    a.low = two_x || two_w ? o : 0;
                     dz = a.dz;
                     dz_stride = a.dz_stride;
                 }
@@ -373,8 +429,22 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                 const int column_blocks = ceil_div(p.outputs, 64);
                 const int most = std::max(1, std::min<int>(kStrips, ceil_div(8 * d.compute_units, column_blocks)));
                 a.strip = std::max(32, ceil_div(rows, most));
-                const int strips = std::max(1, ceil_div(rows, a.strip));
-                hipLaunchKernelGGL((linear_slope_k<T>), dim3(column_blocks, strips), 256, 0, d.stream, a);
+                const int strips = a.strips = std::max(1, ceil_div(rows, a.strip));
+                // weights again below themselves, where dz and what it leaves stand side by side; rows of
+                // x in turn with themselves, where those are rows of o
+                if (two_x) {
+                    a.from[0] = weight->data;
+                    a.to[0] = p.work + p.twice[0];
+                    a.copy[0] = {weight->stride, p.outputs, o, p.inputs, in, 1, o};
+                }
+                if (two_w) {
+                    a.from[1] = x->data;
+                    a.to[1] = p.work + p.twice[1];
+                    a.copy[1] = {x->stride, rows, rows, p.inputs, in, 2, 1};
+                }
+                const int64_t chunks = std::max(two_x ? int64_t(o) * in : 0, two_w ? rows * in : 0) / 8;
+                const int copiers = int(std::min<int64_t>(ceil_div(chunks, 256 * column_blocks), most));
+                hipLaunchKernelGGL((linear_slope_k<T>), dim3(column_blocks, strips + copiers), 256, 0, d.stream, a);
                 HIP_CHECK(hipGetLastError());
                 if (dbias) {
                     hipLaunchKernelGGL((linear_bias_k<T>), ceil_div(p.outputs, 16), 1024, 0, d.stream, a.part, strips, p.outputs,
@@ -386,7 +456,10 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                 LinearEpilogue<T> e{};
                 e.y = static_cast<T*>(dx->data);
                 e.y_stride = dx->stride;
-                product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs, bent}, e);
+                if (two_x)
+                    product<true, false, T>(p, {dz, p.work + p.twice[0], dz_stride, in, rows, 2 * o, p.inputs, true, true}, e);
+                else
+                    product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs, bent, false}, e);
             }
             if (dweight) {
                 LinearEpilogue<T> e{};
@@ -396,7 +469,10 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     e.residual = e.y;
                     e.residual_stride = e.y_stride;
                 }
-                product<false, false, T>(p, {dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs, bent}, e);
+                if (two_w)
+                    product<false, false, T>(p, {dz, p.work + p.twice[1], o, in, p.outputs, 2 * rows, p.inputs, true, true}, e);
+                else
+                    product<false, false, T>(p, {dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs, bent, false}, e);
             }
         });
     });

@@ -257,6 +257,34 @@ def test_odd_widths(device, dtype, rows, inputs, outputs, kind):
     plan.destroy()
 
 
+@pytest.mark.parametrize('dtype', ['f16', 'bf16'])
+@pytest.mark.parametrize('plan_rows,rows,inputs,outputs,kind,few', [
+    (63, 63, 31, 61, 'gelu', 'both'), (400, 300, 40, 16, 'silu', 'both'), (16, 16, 2000, 24, 'relu', 'both'),
+    (5000, 5000, 16, 32, 'sigmoid', 'both'), (20, 20, 100, 3000, 'gelu', 'dx'), (900, 900, 600, 100, 'silu', 'dweight'),
+    (4000, 100, 600, 900, 'gelu', 'dx'), (64, 33, 257, 65, 'sigmoid', 'both')])
+def test_few_gradients_are_rounded_once(device, dtype, plan_rows, rows, inputs, outputs, kind, few):
+    """Gradients of few values are as far from those of `pre` as it stands as the exact ones
+    rounded once: dz is a sum of two values (2^-17 of it left out, 2^-9 of half the result's rounding;
+    f16: 2^-22), sums in 32 bits leave 2^-24 sqrt(5000) = 4e-6, slopes 16 * 2^-24 = 1e-6 where dz is of
+    size one."""
+    print(f'[case] linear gradient {dtype} {rows}x{inputs}x{outputs} {kind}, few', flush=True)
+    x, w, b, _ = operands(dtype, rows, inputs, outputs, True, False)
+    plan = plan_of(device, dtype, plan_rows, inputs, outputs, kind)
+    _, z = forward(device, plan, x, w, b, None)
+    dy = matrix(rows, outputs, dtype, seed=5)
+    got = gradient(device, plan, x, w, z, dy, kind, dtype, True)
+    want = linear_gradient(x, w, z, dy, kind, dtype)
+    for n in ('dx', 'dweight'):
+        if few in (n, 'both'):
+            exact = want[n][0]
+            least = float((exact.to(x.dtype).double() - exact).norm() / exact.norm())
+            far = float((got[n].double() - exact).norm() / exact.norm())
+            assert far < 1.01 * least + 1e-5, (n, far, least)
+    again = gradient(device, plan, x, w, z, dy, kind, dtype, True, accumulate=True)
+    assert torch.equal(again['dx'], got['dx'])
+    plan.destroy()
+
+
 @pytest.mark.parametrize('dtype', ['f32', 'bf16'])
 def test_workspaces_start_with_anything(device, dtype):
     """Plans on memory that held NaN: what stands behind a width in them reaches no result."""
