@@ -228,22 +228,37 @@ struct TileSide {
         }
 #endif
     }
-    // Value by value, for any other.
-    __device__ void load_any(char* tile) const {
-        if constexpr (std::is_arithmetic_v<T> || sizeof(T) == 2)
-        for (int i = 0; i < kSteps; ++i) {
-            const int slot = i * Threads + threadIdx.x % Threads, row = slot / kChunks, first = ((slot % kChunks) ^ turn(row)) * kChunk;
-            const T* p = reinterpret_cast<const T*>(base() + int64_t(K ? min(row, rows - 1) : row) * stride);
-            vec<T, kChunk> v;
-            const int count = K ? left - first : row < left ? rows - first : 0;
-            if (count >= kChunk) {
-                __builtin_memcpy(&v, p + first, sizeof(v));
-            } else {
+    // Through registers, for any other: whole tiles by 16-byte loads of any alignment, all under
+    // way at once; ends of the inner axis (and of columns) value by value.
+    using Chunk = vec<std::conditional_t<std::is_same_v<T, Pair>, float, T>, kChunk>;
+    using Held = Chunk[kSteps];
+    __device__ __attribute__((always_inline)) void fetch(Held& held) const {
+        if constexpr (std::is_arithmetic_v<T> || sizeof(T) == 2) {
+            const auto slot_of = [&](int i, int& row, int& first) __attribute__((always_inline)) {
+                const int slot = i * Threads + threadIdx.x % Threads;
+                row = slot / kChunks;
+                first = ((slot % kChunks) ^ turn(row)) * kChunk;
+                return reinterpret_cast<const T*>(base() + int64_t(K ? min(row, rows - 1) : row) * stride) + first;
+            };
+            int row, first;
+            if (left >= kDeep && (K || rows >= N)) {
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) v[j] = j < count ? p[first + j] : T(0.f);
+                for (int i = 0; i < kSteps; ++i) __builtin_memcpy(&held[i], slot_of(i, row, first), 16);
+                return;
             }
-            *reinterpret_cast<vec<T, kChunk>*>(tile + slot * 16) = v;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const T* p = slot_of(i, row, first);
+                const int count = K ? left - first : row < left ? rows - first : 0;
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) held[i][j] = j < count ? p[j] : T(0.f);
+            }
         }
+    }
+    __device__ __attribute__((always_inline)) void put(char* tile, const Held& held) const {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+            *reinterpret_cast<Chunk*>(tile + (i * Threads + threadIdx.x % Threads) * 16) = held[i];
     }
 };
 
@@ -352,12 +367,9 @@ struct Tiles {
             for (int j = 0; j < kNB; ++j) acc[i][j] = Acc{};
     }
     // The next tile's loads.
-    template <bool Any>
-    __device__ __attribute__((always_inline)) void load(const ProductArgs& p, char* tile) {
-        if (Any && !p.a.wide) a.load_any(tile);
-        else a.load(tile, a_offset, wave);
-        if (Any && !p.b.wide) b.load_any(tile + A::kBytes);
-        else b.load(tile + A::kBytes, b_offset, wave);
+    __device__ __attribute__((always_inline)) void load(char* tile) {
+        a.load(tile, a_offset, wave);
+        b.load(tile + A::kBytes, b_offset, wave);
         a.next();
         b.next();
     }
@@ -440,17 +452,43 @@ __global__ __launch_bounds__((Side / WM) * (Side / WN) * 64, PerSimd) void produ
         }
     };
     if constexpr (Any) {
+        // (what goes through registers is under way while the tile before is multiplied)
+        typename C::A::Held ha;
+        typename C::B::Held hb;
+        const auto fetch = [&]() __attribute__((always_inline)) {
+            if (!p.a.wide) {
+                c.a.fetch(ha);
+                c.a.next();
+            }
+            if (!p.b.wide) {
+                c.b.fetch(hb);
+                c.b.next();
+            }
+        };
+        if (c.steps > 0) fetch();
         for (int i = 0; i < c.steps; ++i) {
-            c.template load<true>(p, lds);
+            if (p.a.wide) {
+                c.a.load(lds, c.a_offset, c.wave);
+                c.a.next();
+            } else {
+                c.a.put(lds, ha);
+            }
+            if (p.b.wide) {
+                c.b.load(lds + C::A::kBytes, c.b_offset, c.wave);
+                c.b.next();
+            } else {
+                c.b.put(lds + C::A::kBytes, hb);
+            }
             loads_arrived();
             __syncthreads();
+            if (i + 1 < c.steps) fetch();
             step(lds, [] {});
             __syncthreads();
         }
     } else {
         int to = 0;  // the place of the next loads
         const auto load = [&](int i) __attribute__((always_inline)) {
-            if (i < c.steps) c.template load<false>(p, lds + to * C::kTile);
+            if (i < c.steps) c.load(lds + to * C::kTile);
             to = to + 1 == Stages ? 0 : to + 1;
         };
         int from = 0;
@@ -490,7 +528,7 @@ __global__ __launch_bounds__(512, 2) void product_large_k(ProductArgs p, Epilogu
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    if (c.steps) c.template load<false>(p, lds);
+    if (c.steps) c.load(lds);
     loads_arrived();
     __syncthreads();
     if (second) barrier();
@@ -503,7 +541,7 @@ __global__ __launch_bounds__(512, 2) void product_large_k(ProductArgs p, Epilogu
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) c.fragments(tile, kSteps * part + s, fa[s], fb[s]);
             __builtin_amdgcn_sched_barrier(0);
-            if (part == 0 && i + 1 < c.steps) c.template load<false>(p, lds + ((i + 1) & 1) * C::kTile);
+            if (part == 0 && i + 1 < c.steps) c.load(lds + ((i + 1) & 1) * C::kTile);
             if (part == 1 && second) loads_arrived();
             __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the reads
             barrier();
@@ -546,21 +584,35 @@ __global__ __launch_bounds__(512) void product_run_k(ProductArgs p, Epilogue e) 
     a.places(a_offset);
     b.places(b_offset);
     char* mine = lds + wave * 2 * kTile;
+    // (what goes through registers is put in LDS when the tile before has been multiplied)
+    typename A::Held ha;
+    typename B::Held hb;
     const auto load = [&](int i) __attribute__((always_inline)) {
         char* tile = mine + (i & 1) * kTile;
-        if (Any && !p.a.wide) a.load_any(tile);
+        if (Any && !p.a.wide) a.fetch(ha);
         else a.load(tile, a_offset, 0);
-        if (Any && !p.b.wide) b.load_any(tile + A::kBytes);
+        if (Any && !p.b.wide) b.fetch(hb);
         else b.load(tile + A::kBytes, b_offset, 0);
         a.next();
         b.next();
     };
+    const auto put = [&](int i) __attribute__((always_inline)) {
+        char* tile = mine + (i & 1) * kTile;
+        if (!p.a.wide) a.put(tile, ha);
+        if (!p.b.wide) b.put(tile + A::kBytes, hb);
+    };
     Acc acc = {};
-    if (steps > 0) load(0);
+    if (steps > 0) {
+        load(0);
+        if (Any) put(0);
+    }
     for (int i = 0; i < steps; ++i) {
+        if (Any && (p.a.wide || p.b.wide)) loads_arrived();
         if (i + 1 < steps) load(i + 1);
-        if (i + 1 < steps && !Any) arrived_but<A::kSteps + B::kSteps>();
-        else loads_arrived();
+        if (!Any) {
+            if (i + 1 < steps) arrived_but<A::kSteps + B::kSteps>();
+            else loads_arrived();
+        }
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): stores to LDS, and the reads of the tile before
         asm volatile("" ::: "memory");
         const char* tile = mine + (i & 1) * kTile;
@@ -570,6 +622,7 @@ __global__ __launch_bounds__(512) void product_run_k(ProductArgs p, Epilogue e) 
         // (the next loads write where these reads were)
         __builtin_amdgcn_s_waitcnt(0xc07f);
         asm volatile("" ::: "memory");
+        if (Any && i + 1 < steps) put(i + 1);
     }
     __syncthreads();
     float* sums = reinterpret_cast<float*>(lds);
