@@ -241,12 +241,13 @@ void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
     args.part = reinterpret_cast<float*>(p.work + p.part);
     args.a = product_operand(s.a, s.a_stride, s.a_whole ? s.a_stride : AK ? s.k : s.m, sizeof(T));
     args.b = product_operand(s.b, s.b_stride, s.b_whole ? s.b_stride : BK ? s.k : s.n, sizeof(T));
-    // Operands that are not whole chunks are read by registers, a tile at a time, where few tiles
-    // share them; else they are copied to whole chunks first (a plan whose widths are not whole
-    // eights has room for it).  2,047 -> 2,047, bf16: 128 rows 16.2 us by registers, 17.2 copied, 256
-    // rows 27.2 and 20.6, 1,024 rows 54.9 and 29.9.
+    // Operands that are not whole chunks come through registers, 64 x 64 tiles at a time, where the
+    // product is small or few tiles share them; else they are copied to whole chunks first, for larger
+    // tiles (a plan whose widths are not whole eights has room for it).  2,047 -> 2,047: 256 rows bf16
+    // 14.8 us through registers, 20.7 copied, f32 29.7 and 36.4; 512 rows 27.2 and 25.9, 69.5 and 49.1;
+    // 2,048 rows 51.2 and 39.7, 156 and 124.  130 rows, 2,047 -> 8,191: 30.3 and 33.2, 66 and 84.
     const int64_t m_tiles = ceil_div(s.m, 64), n_tiles = ceil_div(s.n, 64), deep = ceil_div(s.k, kDepth<T>);
-    const bool shared = std::min(m_tiles, n_tiles) > 2 && deep * std::max<int64_t>(1, m_tiles * n_tiles / (4 * d.compute_units)) > 12;
+    const bool shared = std::min(m_tiles, n_tiles) > 3 && deep * m_tiles * n_tiles > 56 * int64_t(d.compute_units);
     if ((!args.a.wide || !args.b.wide) && p.a_copy && shared) {
         const auto copy = [&](Operand& o, const void* x, int64_t stride, int64_t rows, int64_t columns, size_t place) {
             if (o.wide) return;
