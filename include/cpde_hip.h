@@ -508,9 +508,11 @@ int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, c
 /* The gradients of x, W and bias from y's (the residual's is y's own): with
  * dz = dy activation'(pre), dx = dz W, dW = dz^T x, dbias = the sum of dz's rows.  Any of
  * dx, dweight and dbias may be NULL, and is then not computed; x is read for dweight only,
- * weight for dx only, pre (else NULL) where there is an activation.  With 16-bit tensors dz
- * is rounded to their type, once, before the two products.  accumulate=1 adds dweight and
- * dbias onto what is there, 0 overwrites them. */
+ * weight for dx only, pre (else NULL) where there is an activation.  With 16-bit tensors and
+ * an activation dz is rounded to their type, once, before the two products; gradients of at
+ * most 2^17 values, from matrices of at most 2^20 (rows and columns to whole eights), take it
+ * as a sum of two such values, where an infinity in x or W may give NaN.  accumulate=1 adds
+ * dweight and dbias onto what is there, 0 overwrites them. */
 int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, const cpde_rows* weight,
                          const cpde_rows* pre, const cpde_rows* dy, const cpde_rows* dx, const cpde_rows* dweight,
                          void* dbias, int accumulate);

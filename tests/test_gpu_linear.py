@@ -257,6 +257,27 @@ def test_odd_widths(device, dtype, rows, inputs, outputs, kind):
     plan.destroy()
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('rows,inputs,outputs', [(33, 35, 41), (70, 9, 8), (66, 71, 65), (300, 129, 67), (3, 1031, 70), (129, 7, 200)])
+def test_ends_of_odd_rows(device, dtype, rows, inputs, outputs):
+    """Rows that end inside 16 bytes, NaN between them and around: none comes into a sum."""
+    print(f'[case] linear {dtype} {rows}x{inputs}x{outputs} among NaN', flush=True)
+
+    def among(rows, columns, seed):
+        flat = torch.full((rows * (columns + 3) + 16,), math.nan, device='cuda', dtype=TYPES[dtype][0])
+        t = flat[7:7 + rows * (columns + 3)].view(rows, columns + 3)[:, :columns]
+        return t.copy_(matrix(rows, columns, dtype, seed=seed))
+
+    x, w, dy = among(rows, inputs, 1), among(outputs, inputs, 2), among(rows, outputs, 5)
+    for kind in ('none', 'silu'):
+        plan = plan_of(device, dtype, rows, inputs, outputs, kind)
+        y, z = forward(device, plan, x, w, None, None, pad=1)
+        want = linear(x.cpu(), w.cpu(), None, None, kind, dtype)
+        check(y, *want['y'], 'y')
+        gradient(device, plan, x, w, z, dy, kind, dtype, True)
+        plan.destroy()
+
+
 @pytest.mark.parametrize('dtype', ['f16', 'bf16'])
 @pytest.mark.parametrize('plan_rows,rows,inputs,outputs,kind,few', [
     (63, 63, 31, 61, 'gelu', 'both'), (400, 300, 40, 16, 'silu', 'both'), (16, 16, 2000, 24, 'relu', 'both'),
