@@ -20,13 +20,14 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 // 32 bits, and the operands hold zeros there: a row's diagonal is the largest of it, and
 // alike in all rows of a matrix with even singular values, so that its rounding would move
 // all of them one way (4 x 15 x 526: 0.0026 from the exact values for 0.0017, which is the
-// type's own rounding).  With A = D + O: A^2 = D^2 + D O + O D + O^2.
+// type's own rounding).  Small matrices have them apart whatever the type (f32: half the error,
+// for 0.8 us a step).  With A = D + O: A^2 = D^2 + D O + O D + O^2.
 constexpr float kUp = 4096.f, kDown = 1.f / (4096.f * 4096.f);
 
-// b A + c A^2 of an entry from A and A^2; with one plane from O^2, less the diagonal's share.
-template <int PLANES>
+// b A + c A^2 of an entry from A and A^2; with the diagonal apart from O^2.
+template <bool Apart>
 __device__ inline float poly_of(float a, float square, bool diagonal, float row, float column) {
-    if (PLANES == 1) square += a * (diagonal ? a : row + column);
+    if (Apart) square += a * (diagonal ? a : row + column);
     return kB * a + kC * square;
 }
 
@@ -197,7 +198,7 @@ struct PolyEpilogue {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const bool one = PLANES == 1 && m == n + j;
-            v[j] = j < count ? poly_of<PLANES>(one ? row : a[j], v[j] * kDown, one, row, column.d[j]) : 0.f;
+            v[j] = j < count ? poly_of<PLANES == 1>(one ? row : a[j], v[j] * kDown, one, row, column.d[j]) : 0.f;
             if (one) {
                 poly_diagonal[batch * side + m] = v[j];
                 v[j] = 0;
@@ -251,7 +252,7 @@ struct StepEpilogue {
 // the matrix lying so that it is at least as wide as high; its sixteen waves hold a 32 x 32
 // of X and of A in registers.  Symmetric products are made by the waves of the blocks on and
 // below the diagonal and stored twice.  Bound: the products of one CU (128 x 128 f32: 1.3 us
-// each at the matrix unit's rate) and the barriers between them: 7 us a step; in launches
+// each at the matrix unit's rate) and the barriers between them: 8 us a step; in launches
 // of their own the three products of a step take 13.
 constexpr int kSmall = 128;
 // X's row in LDS, in columns.
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
     __shared__ __align__(16) char x_lds[2 * kPlane];       // X; at the end the result in floats
     __shared__ __align__(16) char g_lds[PLANES * kPlane];
     __shared__ double sums[16];
-    __shared__ float diagonal[kSmall];  // with one plane: of A, then of b A + c A^2
+    __shared__ float diagonal[kSmall];  // of A, then of b A + c A^2
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, matrix = blockIdx.x;
     const bool tall = p.rows > p.columns;
     const int high = min(p.rows, p.columns), wide = max(p.rows, p.columns);
@@ -415,8 +416,8 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
         for (int j = 0; j < 4; ++j) x[4 * g + j] = (float(hi[j]) + float(lo[j])) * (1.f / kUp);
     }
     const int side_steps = (high + 15) / 16, wide_steps = (wide + 15) / 16;
-    const auto on_diagonal = [&](int e) { return PLANES == 1 && ba.row == ba.column + 8 * (e >> 2) + (e & 3); };
-    // a symmetric matrix's block into LDS; with one plane its diagonal apart, zeros in its place
+    const auto on_diagonal = [&](int e) { return ba.row == ba.column + 8 * (e >> 2) + (e & 3); };
+    // a symmetric matrix's block into LDS; its diagonal apart, zeros in its place
     const auto put_square = [&](Acc v) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -435,11 +436,11 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
         __syncthreads();
         if (square) {
             c = product(g_lds, kG, g_lds, kG, ba, side_steps, std::true_type{});
-            const float row = PLANES == 1 ? diagonal[ba.row] : 0;
+            const float row = diagonal[ba.row];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float column = PLANES == 1 ? diagonal[ba.column + 8 * (e >> 2) + (e & 3)] : 0;
-                c[e] = poly_of<PLANES>(a[e], c[e] * kDown, on_diagonal(e), row, column);
+                const float column = diagonal[ba.column + 8 * (e >> 2) + (e & 3)];
+                c[e] = poly_of<true>(a[e], c[e] * kDown, on_diagonal(e), row, column);
             }
         }
         __syncthreads();
@@ -447,7 +448,7 @@ __global__ __launch_bounds__(1024) void orthogonal_small_k(Source<T> s, SmallArg
         __syncthreads();
         if (live) {
             c = product(g_lds, kG, x_lds, kX, bx, side_steps, std::false_type{});
-            x = (kA + (PLANES == 1 ? diagonal[bx.row] : 0.f)) * x + kDown * c;
+            x = (kA + diagonal[bx.row]) * x + kDown * c;
         }
         __syncthreads();
         if (step + 1 < p.steps) {

@@ -89,6 +89,25 @@ def test_even_singular_values(device, count, rows, columns):
     assert far < 1.25 * least, (far, least)
 
 
+@pytest.mark.parametrize('count,rows,columns', [(2, 8, 32), (1, 16, 64), (4, 128, 128), (2, 60, 61)])
+def test_small_float_matrices(device, count, rows, columns):
+    """No further off than five steps of float products: those round A, b A + c A^2 and X to
+    2^-24, where here diagonals and X itself are held so, and what is off the diagonal (a
+    row of it about as large) to 2^-23 with two products in 2^-22 left out.  Over six matrices."""
+    print(f'[case] orthogonal f32 {count}x{rows}x{columns}, small', flush=True)
+    own = plain = 0.0
+    for seed in range(6):
+        x = matrices(count, rows, columns, 'f32', seed=seed)
+        want = orthogonal(x, 5)
+        y = (x.double() / x.double().square().sum((1, 2), keepdim=True).sqrt()).float()
+        for _ in range(5):
+            gram = y @ y.transpose(1, 2).contiguous()
+            y = 3.4445 * y + (-4.7750 * gram + 2.0315 * (gram @ gram)) @ y
+        own += float((forward(device, x, 'f32', 5).double() - want).norm())
+        plain += float((y.double() - want).norm())
+    assert own < 1.5 * plain, (own, plain)
+
+
 def test_singular_values(device):
     """What it is for: singular vectors stay, values come into 0.68..1.13 (and the type's rounding)."""
     for dtype in ('f32', 'bf16'):
