@@ -597,6 +597,7 @@ int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int
         *out = nullptr;
         check_dtype(dtype);
         require(count >= 0 && rows >= 0 && columns >= 0, "negative size");
+        // (rows of 2^20 pairs are the longest that products take: no call is refused once it has begun)
         require(count <= 1024 && rows <= 1 << 20 && columns <= 1 << 20, "too many or too large matrices");
         require(steps >= 1 && steps <= 32, "1 to 32 steps");
         require(!dev->capturing, "a capture is open on this device");

@@ -801,12 +801,13 @@ inline size_t product_part(int compute_units, int64_t batch, int64_t m, int64_t 
     return size_t(std::min<int64_t>(kPartTiles * compute_units * 128 * 128, kMostSplits * batch * m * ((n + 7) / 8 * 8)));
 }
 
-// An operand of rows of `columns` values of `size` bytes.
+// An operand of rows of `columns` values of `size` bytes.  (A tile of 256 rows 2^22 bytes apart
+// ends within 2^31 of its start.)
 inline Operand product_operand(const void* data, int64_t stride, int64_t columns, size_t size) {
     Operand o{};
     o.data = static_cast<const char*>(data);
     o.stride = stride * int64_t(size);
-    o.wide = wide(data, stride, size) && columns * size % 16 == 0 && o.stride < (int64_t(1) << 22);
+    o.wide = wide(data, stride, size) && columns * size % 16 == 0 && o.stride <= (int64_t(1) << 22);
     return o;
 }
 
