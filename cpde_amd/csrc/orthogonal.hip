@@ -492,8 +492,15 @@ void check_matrices(const Orthogonal& p, const cpde_matrices* x, bool output) {
     require(x->matrix >= 0 && x->row >= 0, "negative stride");
     require(x->matrix <= int64_t(1) << 40 && x->row <= int64_t(1) << 40, "invalid stride");
     if (!output) return;
-    require(p.rows == 1 || x->row >= p.columns, "output elements overlap");
-    require(p.count == 1 || x->matrix >= (p.rows - 1) * (p.rows > 1 ? x->row : 0) + p.columns, "output elements overlap");
+    // (either axis may be the inner one: matrices may take turns row by row)
+    std::pair<int64_t, int64_t> axes[] = {{x->matrix, p.count}, {x->row, p.rows}};
+    if (axes[0] > axes[1]) std::swap(axes[0], axes[1]);
+    int64_t extent = p.columns;
+    for (const auto& [stride, count] : axes) {
+        if (count == 1) continue;
+        require(stride >= extent, "output elements overlap");
+        extent += stride * (count - 1);
+    }
 }
 template <class T>
 Matrices<T> matrices(const cpde_matrices* x) {
