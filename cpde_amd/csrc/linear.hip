@@ -230,9 +230,19 @@ struct Sides {
     int n;
     bool a_whole, b_whole;  // its rows go on in zeros to whole chunks
 };
+// A product of a plan's, as it is launched, and the operands that are copied for it before.
+struct Prepared {
+    Product product;
+    struct {
+        const void* from;  // (null: not copied)
+        void* to;
+        CopyArgs args;
+    } copy[2];
+};
 template <bool AK, bool BK, class T>
-void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
-    Device& d = *p.dev;
+Prepared prepare(const Linear& p, const Sides& s) {
+    const Device& d = *p.dev;
+    Prepared r{};
     ProductArgs args{};
     args.m = int(s.m);
     args.n = s.n;
@@ -249,17 +259,23 @@ void product(const Linear& p, const Sides& s, const LinearEpilogue<T>& e) {
     const int64_t m_tiles = ceil_div(s.m, 64), n_tiles = ceil_div(s.n, 64), deep = ceil_div(s.k, kDepth<T>);
     const bool shared = std::min(m_tiles, n_tiles) > 3 && deep * m_tiles * n_tiles > 56 * int64_t(d.compute_units);
     if ((!args.a.wide || !args.b.wide) && p.a_copy && shared) {
-        const auto copy = [&](Operand& o, const void* x, int64_t stride, int64_t rows, int64_t columns, size_t place) {
+        const auto copy = [&](int i, Operand& o, const void* x, int64_t stride, int64_t rows, int64_t columns, size_t place) {
             if (o.wide) return;
             const int pitch = pitch_of(columns);
-            T* to = reinterpret_cast<T*>(p.work + place);
-            copy_rows<T>(d, x, to, {stride, rows, rows, int(columns), pitch, 1, 0});
-            o = product_operand(to, pitch, pitch, sizeof(T));
+            r.copy[i] = {x, p.work + place, {stride, rows, rows, int(columns), pitch, 1, 0}};
+            o = product_operand(r.copy[i].to, pitch, pitch, sizeof(T));
         };
-        copy(args.a, s.a, s.a_stride, AK ? s.m : s.k, AK ? s.k : s.m, p.a_copy);
-        copy(args.b, s.b, s.b_stride, BK ? s.n : s.k, BK ? s.k : s.n, p.b_copy);
+        copy(0, args.a, s.a, s.a_stride, AK ? s.m : s.k, AK ? s.k : s.m, p.a_copy);
+        copy(1, args.b, s.b, s.b_stride, BK ? s.n : s.k, BK ? s.k : s.n, p.b_copy);
     }
-    launch_product<T, AK, BK>(d, args, e);
+    r.product = cut_for<T, AK, BK>(d, args);
+    return r;
+}
+template <bool AK, bool BK, class T>
+void launch(const Linear& p, const Prepared& r, const LinearEpilogue<T>& e) {
+    for (const auto& c : r.copy)
+        if (c.from) copy_rows<T>(*p.dev, c.from, static_cast<T*>(c.to), c.args);
+    launch_product<T, AK, BK>(*p.dev, r.product, e);
 }
 
 // A matrix argument of `rows` x `columns`; an output's rows do not overlap.
@@ -371,7 +387,8 @@ int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, c
                 e.pre_stride = pre->stride;
             }
             e.activation = p.activation;
-            product<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs, false, false}, e);
+            launch<true, true, T>(
+                p, prepare<true, true, T>(p, {x->data, weight->data, x->stride, weight->stride, rows, p.inputs, p.outputs, false, false}), e);
         });
     });
 }
@@ -402,13 +419,23 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
         TraceScope trace(d, kTraceLinearGradient, 2.0 * ((dx != nullptr) + (dweight != nullptr)) * rows * p.inputs * p.outputs);
         with_type(p.dtype, [&](auto element) {
             using T = decltype(element);
-            const void* dz = dy->data;
-            int64_t dz_stride = dy->stride;  // (of the plan's own: whole chunks, zeros behind the columns)
             const int in = pitch_of(p.inputs), o = pitch_of(p.outputs);
             // (rows and widths to whole chunks are what is written)
             const bool two = bent && sizeof(T) == 2 && rows * o <= kFewInner;
             const bool two_x = two && dx && rows * in <= kFew && int64_t(o) * in <= kFewInner;
             const bool two_w = two && dweight && int64_t(o) * in <= kFew && rows * in <= kFewInner;
+            const void* dz = bent ? p.work + p.dz : dy->data;  // (the plan's own: whole chunks, zeros behind the columns)
+            const int64_t dz_stride = !bent ? dy->stride : two_x || two_w ? 2 * o : o;
+            // both products are cut before the first launch: a refused call writes nothing
+            Prepared for_x, for_w;
+            if (dx)
+                for_x = prepare<true, false, T>(
+                    p, two_x ? Sides{dz, p.work + p.twice[0], dz_stride, in, rows, 2 * o, p.inputs, true, true}
+                             : Sides{dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs, bent, false});
+            if (dweight)
+                for_w = prepare<false, false, T>(
+                    p, two_w ? Sides{dz, p.work + p.twice[1], o, in, p.outputs, 2 * rows, p.inputs, true, true}
+                             : Sides{dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs, bent, false});
             if ((bent || dbias) && p.outputs) {
                 SlopeArgs a{};
                 a.dy = dy->data;
@@ -420,10 +447,8 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     a.pre = pre->data;
                     a.pre_stride = pre->stride;
                     a.dz = p.work + p.dz;
-                    a.dz_stride = two_x || two_w ? 2 * o : o;
+                    a.dz_stride = int(dz_stride);
                     a.low = two_x || two_w ? o : 0;
-                    dz = a.dz;
-                    dz_stride = a.dz_stride;
                 }
                 if (dbias) a.part = reinterpret_cast<float*>(p.work + p.bias_part);
                 // strips of 32 rows at least, and workgroups for the whole device
@@ -453,14 +478,11 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     HIP_CHECK(hipGetLastError());
                 }
             }
-            if (dx && rows) {
+            if (dx) {
                 LinearEpilogue<T> e{};
                 e.y = static_cast<T*>(dx->data);
                 e.y_stride = dx->stride;
-                if (two_x)
-                    product<true, false, T>(p, {dz, p.work + p.twice[0], dz_stride, in, rows, 2 * o, p.inputs, true, true}, e);
-                else
-                    product<true, false, T>(p, {dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs, bent, false}, e);
+                launch<true, false, T>(p, for_x, e);
             }
             if (dweight) {
                 LinearEpilogue<T> e{};
@@ -470,10 +492,7 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     e.residual = e.y;
                     e.residual_stride = e.y_stride;
                 }
-                if (two_w)
-                    product<false, false, T>(p, {dz, p.work + p.twice[1], o, in, p.outputs, 2 * rows, p.inputs, true, true}, e);
-                else
-                    product<false, false, T>(p, {dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs, bent, false}, e);
+                launch<false, false, T>(p, for_w, e);
             }
         });
     });

@@ -811,48 +811,70 @@ inline Operand product_operand(const void* data, int64_t stride, int64_t columns
     return o;
 }
 
-// A launch of one of the kernels of tiles of `side`.
-template <class K, class E>
-void launch_tiles(Device& d, K kernel, int side, int threads, ProductArgs p, const E& e, size_t lds = 0) {
-    p.m_tiles = ceil_div(p.m, side);
-    p.n_tiles = ceil_div(p.n, side);
+// A product as it is launched: with its cut.
+struct Product {
+    ProductArgs args;
+    ProductCut cut;
+    bool wide;
+    bool empty() const { return !args.m || !args.n || !args.batch; }
+};
+// Columns of a wave's part of a 128 x 128 tile: eight waves, or four where a fragment costs more:
+// floats' splits (1,024 tiles, k = 1024: 185 us for 199), transposing reads of both operands (4096 x
+// 2048, k = 8192, bf16: 133 for 156; of neither, 128 tiles, k = 1024: 13.7, and 11.9 by eight)
+template <class T, bool AK, bool BK>
+constexpr int kWave128 = std::is_same_v<T, float> || (!AK && !BK) ? 64 : 32;
+
+// p: the operands, sizes and batch.  Its cut is made here, and a launch of too many workgroups
+// refused, so that a call of several launches can cut all of them before its first one.
+template <class T, bool AK, bool BK>
+Product cut_for(const Device& d, ProductArgs p) {
+    Product q{p, {}, p.a.wide && p.b.wide};
+    if (q.empty()) return q;
+    const ProductCut c = q.cut = cut_product<T>(d.compute_units, p.batch, p.m, p.n, p.k, q.wide, p.symmetric);
+    const int deep = std::max(1, ceil_div(p.k, kDepth<T>));
+    p.span = ceil_div(deep, std::min(c.splits, deep));
+    p.splits = ceil_div(deep, p.span);
+    if (c.side == 32) p.symmetric = 0;  // (whole tiles of both halves)
+    p.m_tiles = ceil_div(p.m, c.side);
+    p.n_tiles = ceil_div(p.n, c.side);
+    q.args = p;
+    const int threads = c.side == 32 ? 64 * c.waves : c.side == 64 ? 256 : c.side == 128 ? 256 * 64 / kWave128<T, AK, BK> : 512;
     const int64_t tiles = p.symmetric ? int64_t(p.m_tiles) * (p.m_tiles + 1) / 2 : int64_t(p.m_tiles) * p.n_tiles;
     require(tiles * threads < (int64_t(1) << 31) && int64_t(p.splits) * p.batch < 65536, "too many workgroups");
+    return q;
+}
+
+// A launch of one of the kernels of tiles.
+template <class K, class E>
+void launch_tiles(Device& d, K kernel, int threads, const ProductArgs& p, const E& e, size_t lds = 0) {
+    const int tiles = p.symmetric ? p.m_tiles * (p.m_tiles + 1) / 2 : p.m_tiles * p.n_tiles;
     hipLaunchKernelGGL(kernel, dim3(unsigned(tiles), unsigned(p.splits) * p.batch), threads, lds, d.stream, p, e);
     HIP_CHECK(hipGetLastError());
 }
 
-// p: the operands, sizes and batch; its cut is made here.
 template <class T, bool AK, bool BK, class E>
-void launch_product(Device& d, ProductArgs p, const E& e) {
-    if (!p.m || !p.n || !p.batch) return;
+void launch_product(Device& d, const Product& q, const E& e) {
+    if (q.empty()) return;
     constexpr bool kAny = E::kAny;  // (whether operands may be of any alignment)
-    const bool wide = p.a.wide && p.b.wide;
-    require(wide || kAny, "operands of products are aligned");
-    const ProductCut c = cut_product<T>(d.compute_units, p.batch, p.m, p.n, p.k, wide, p.symmetric);
-    const int deep = std::max(1, ceil_div(p.k, kDepth<T>));
-    p.span = ceil_div(deep, std::min(c.splits, deep));
-    p.splits = ceil_div(deep, p.span);
+    const ProductArgs& p = q.args;
+    const ProductCut& c = q.cut;
+    require(q.wide || kAny, "operands of products are aligned");
     if (c.side == 32) {
         const size_t lds = c.waves * kRunBytes<T>;
-        p.symmetric = 0;  // (whole tiles of both halves)
-        if (wide) {
-            launch_tiles(d, product_run_k<T, AK, BK, false, E>, 32, 64 * c.waves, p, e, lds);
+        if (q.wide) {
+            launch_tiles(d, product_run_k<T, AK, BK, false, E>, 64 * c.waves, p, e, lds);
         } else {
-            if constexpr (kAny) launch_tiles(d, product_run_k<T, AK, BK, true, E>, 32, 64 * c.waves, p, e, lds);
+            if constexpr (kAny) launch_tiles(d, product_run_k<T, AK, BK, true, E>, 64 * c.waves, p, e, lds);
         }
-    } else if (!wide) {
-        if constexpr (kAny) launch_tiles(d, product_k<T, AK, BK, 64, 32, 32, 1, 2, true, E>, 64, 256, p, e);
+    } else if (!q.wide) {
+        if constexpr (kAny) launch_tiles(d, product_k<T, AK, BK, 64, 32, 32, 1, 2, true, E>, 256, p, e);
     } else if (c.side == 64) {
-        launch_tiles(d, product_k<T, AK, BK, 64, 32, 32, 3, 2, false, E>, 64, 256, p, e);
+        launch_tiles(d, product_k<T, AK, BK, 64, 32, 32, 3, 2, false, E>, 256, p, e);
     } else if (c.side == 128) {
-        // eight waves, or four where a fragment costs more: floats' splits (1,024 tiles, k = 1024:
-        // 185 us for 199), transposing reads of both operands (4096 x 2048, k = 8192, bf16: 133 for 156;
-        // of neither, 128 tiles, k = 1024: 13.7, and 11.9 by eight)
-        constexpr int kWave = std::is_same_v<T, float> || (!AK && !BK) ? 64 : 32;
-        launch_tiles(d, product_k<T, AK, BK, 128, 64, kWave, 2, 128 / kWave, false, E>, 128, 256 * 64 / kWave, p, e);
+        constexpr int kWave = kWave128<T, AK, BK>;
+        launch_tiles(d, product_k<T, AK, BK, 128, 64, kWave, 2, 128 / kWave, false, E>, 256 * 64 / kWave, p, e);
     } else {
-        launch_tiles(d, product_large_k<T, AK, BK, E>, 256, 512, p, e);
+        launch_tiles(d, product_large_k<T, AK, BK, E>, 512, p, e);
     }
     if (p.splits > 1) {
         if constexpr (E::kSymmetric)
@@ -867,6 +889,10 @@ void launch_product(Device& d, ProductArgs p, const E& e) {
         hipLaunchKernelGGL((product_join_k<E>), unsigned((lanes + 255) / 256), 256, 0, d.stream, p, e);
         HIP_CHECK(hipGetLastError());
     }
+}
+template <class T, bool AK, bool BK, class E>
+void launch_product(Device& d, const ProductArgs& p, const E& e) {
+    launch_product<T, AK, BK>(d, cut_for<T, AK, BK>(d, p), e);
 }
 
 }  // namespace

@@ -490,8 +490,9 @@ int cpde_dropout(cpde_device* dev, int dtype, int64_t rows, int64_t columns, con
  * z / (1 + exp(-z)).  Products are summed in 32 bits.  Floats may be multiplied as exact
  * sums of three bf16 values, whose least products (2^-21 of the factors' at most) are left
  * out: about as exact as rounded floats, but an infinity in x, W or dz may give NaN where
- * the float instruction would give an infinity.  A call of more than 2^31 / 256 tiles of
- * 64 x 64 results is refused.  backward = 0: cpde_linear_backward will not be called. */
+ * the float instruction would give an infinity.  A call one of whose products has 2^23 tiles
+ * of 64 x 64 results or more may be refused, and then writes nothing.  backward = 0:
+ * cpde_linear_backward will not be called. */
 #define CPDE_NONE 0
 #define CPDE_SIGMOID 1
 #define CPDE_RELU 2
