@@ -10,18 +10,23 @@ namespace {
 // ---- activations ------------------------------------------------------------------------
 __device__ inline float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 __device__ inline float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-z)); }
-// The normal distribution's integral up to z, (1 + erf(z / sqrt 2)) / 2.  For 16-bit tensors
-// by the formula 7.1.26 of M. Abramowitz, I. Stegun, "Handbook of mathematical functions"
-// (1964), off by at most 1.5e-7, which takes a third of the instructions.
+// The normal distribution's integral up to z, (1 + erf(z / sqrt 2)) / 2.  For 16-bit tensors by
+// exp(z^2 / 2) times the integral up to -|z|, which is t P(t) with t = 1 / (1 + 0.2634 |z|) and P
+// of degree six, fitted here for the least relative error over |z| <= 13.5 (5.4e-7): off by at most
+// 4e-7, and, with its exponential's rounding, by 1e-5 of its value as far out as that is normal,
+// so that small values have all the digits of their type.  It takes a third of the instructions of
+// erfcf.
 template <class T>
 __device__ inline float normal_integral(float z) {
     if (sizeof(T) == 4) return 0.5f * erfcf(z * -0.70710678118654752440f);
-    const float x = fabsf(z) * 0.70710678118654752440f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    q *= 0.5f * t * exp_fast(-x * x);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.26339728f, fabsf(z), 1.f));
+    float q = fmaf(-0.069694854f, t, 0.20668863f);
+    q = fmaf(q, t, -0.079968646f);
+    q = fmaf(q, t, 0.15077229f);
+    q = fmaf(q, t, 0.07958568f);
+    q = fmaf(q, t, 0.107690774f);
+    q = fmaf(q, t, 0.10492611f);
+    q *= t * __builtin_amdgcn_exp2f(z * z * -0.72134752044448170368f);
     return z < 0 ? q : 1 - q;
 }
 
