@@ -28,8 +28,9 @@ class Product(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, plan, bent):
-        rows = x.reshape(-1, x.shape[-1])
-        residual = None if residual is None else residual.reshape(-1, weight.shape[0])
+        # (columns that repeat a value have a stride of zero)
+        rows = x.reshape(-1, x.shape[-1]).contiguous()
+        residual = None if residual is None else residual.reshape(-1, weight.shape[0]).contiguous()
         y = torch.empty((rows.shape[0], weight.shape[0]), device=x.device, dtype=x.dtype)
         pre = torch.empty_like(y) if bent else None
         plan.forward(rows.shape[0], hip.Rows.of(rows), hip.Rows.of(weight), hip.Rows.of(y), bias=bias,
@@ -43,7 +44,7 @@ class Product(torch.autograd.Function):
     @once
     def backward(ctx, dy):
         rows, weight, pre = ctx.saved_tensors
-        flat = dy.reshape(rows.shape[0], -1)
+        flat = dy.reshape(rows.shape[0], -1).contiguous()  # (a sum's gradient repeats one value)
         dx, dweight = torch.empty_like(rows), torch.empty_like(weight)
         dbias = torch.empty(weight.shape[0], device=dy.device, dtype=dy.dtype) if ctx.has[0] else None
         ctx.plan.backward(rows.shape[0], hip.Rows.of(rows), hip.Rows.of(weight), hip.Rows.of(flat),
@@ -57,6 +58,7 @@ class Rotate(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, plan):
+        q, k = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k))
         q_out, k_out = torch.empty(q.shape, device=q.device), torch.empty(k.shape, device=k.device)
         plan.forward(*(hip.Heads.of(t) for t in (q, k, q_out, k_out)), q_weight, k_weight)
         ctx.plan = plan
