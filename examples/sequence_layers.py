@@ -36,7 +36,7 @@ class Product(torch.autograd.Function):
         plan.forward(rows.shape[0], hip.Rows.of(rows), hip.Rows.of(weight), hip.Rows.of(y), bias=bias,
                      residual=None if residual is None else hip.Rows.of(residual),
                      pre=None if pre is None else hip.Rows.of(pre))
-        ctx.plan, ctx.shape, ctx.has = plan, x.shape, (bias is not None, residual is not None)
+        ctx.plan, ctx.shape = plan, x.shape
         ctx.save_for_backward(rows, weight, pre)
         return y.view(*x.shape[:-1], -1)
 
@@ -45,12 +45,13 @@ class Product(torch.autograd.Function):
     def backward(ctx, dy):
         rows, weight, pre = ctx.saved_tensors
         flat = dy.reshape(rows.shape[0], -1).contiguous()  # (a sum's gradient repeats one value)
-        dx, dweight = torch.empty_like(rows), torch.empty_like(weight)
-        dbias = torch.empty(weight.shape[0], device=dy.device, dtype=dy.dtype) if ctx.has[0] else None
+        dx, dweight = (torch.empty_like(t) if n else None for t, n in zip((rows, weight), ctx.needs_input_grad))
+        dbias = torch.empty(weight.shape[0], device=dy.device, dtype=dy.dtype) if ctx.needs_input_grad[2] else None
         ctx.plan.backward(rows.shape[0], hip.Rows.of(rows), hip.Rows.of(weight), hip.Rows.of(flat),
-                          pre=None if pre is None else hip.Rows.of(pre), dx=hip.Rows.of(dx), dweight=hip.Rows.of(dweight),
-                          dbias=dbias)
-        return dx.view(ctx.shape), dweight, dbias, dy if ctx.has[1] else None, None, None
+                          pre=None if pre is None else hip.Rows.of(pre), dx=None if dx is None else hip.Rows.of(dx),
+                          dweight=None if dweight is None else hip.Rows.of(dweight), dbias=dbias)
+        return (None if dx is None else dx.view(ctx.shape), dweight, dbias, dy if ctx.needs_input_grad[3] else None, None,
+                None)
 
 
 class Rotate(torch.autograd.Function):

@@ -56,3 +56,15 @@ def test_inputs_that_repeat_a_column():
     assert plan.asked == {'dx', 'dweight'}
     q, k = leaf(1, 3, 2, 1).expand(1, 3, 2, 8), leaf(1, 3, 2, 1).expand(1, 3, 2, 8)
     sum(t.sum() for t in example.Rotate.apply(q, k, leaf(8), leaf(8), plan)).backward()
+
+
+@pytest.mark.parametrize('needed', range(1, 16))
+def test_only_gradients_that_are_needed(needed):
+    """What no gradient is asked of costs no product."""
+    has = [bool(needed >> i & 1) for i in range(4)]
+    shapes = (3, 8), (4, 8), (4,), (3, 4)
+    x, w, b, r = leaves = [leaf(*s, grad=h) for s, h in zip(shapes, has)]
+    plan = Plan()
+    example.Product.apply(x, w, b, r, plan, True).sum().backward()
+    assert (plan.asked or set()) == {n for n, h in zip(('dx', 'dweight', 'dbias'), has) if h}
+    assert [t.grad is not None for t in leaves] == has
