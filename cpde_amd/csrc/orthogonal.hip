@@ -624,19 +624,26 @@ int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int
             at += (bytes + 255) / 256 * 256;
             return here;
         };
-        const bool small = is_small(rows, columns);
-        if (!small) {
-            p->sums = place(sizeof(double) * n * p->blocks);
+        if (!is_small(rows, columns)) {
             for (auto& x : p->x) x = place(2 * 2 * n * rows * pitch);
             p->gram = place(2 * p->planes() * n * side * side_pitch);
             p->poly = place(2 * p->planes() * n * side * side_pitch);
+        }
+        const size_t operands = at;
+        if (operands) {
+            p->sums = place(sizeof(double) * n * p->blocks);
             p->diagonal = place(sizeof(float) * 2 * n * side);
             p->part = place(sizeof(float) * std::max(product_part(dev->compute_units, count, side, side),
                                                  product_part(dev->compute_units, count, rows, columns)));
         }
         HIP_CHECK(hipMalloc(&p->work, std::max<size_t>(at, 256)));
-        // (what stands behind the matrices' columns is never written: zeros)
-        if (!small) launch_fill(*dev, reinterpret_cast<float*>(p->work), at / sizeof(float), 0.f);
+        try {
+            // (what stands behind the operands' columns is never written: zeros)
+            if (operands) launch_fill(*dev, reinterpret_cast<float*>(p->work), operands / sizeof(float), 0.f);
+        } catch (...) {
+            (void)hipFree(p->work);
+            throw;
+        }
         *out = p.release();
     });
 }
