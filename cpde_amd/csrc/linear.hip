@@ -283,6 +283,48 @@ void launch(const Linear& p, const Prepared& r, const LinearEpilogue<T>& e) {
     launch_product<T, AK, BK>(*p.dev, r.product, e);
 }
 
+// A gradient's products (those that are wanted), cut before the first launch: a refused call
+// writes nothing.
+struct Gradient {
+    bool two_x, two_w;  // dz goes as two values
+    const void* dz;     // (the plan's own: whole chunks, zeros behind the columns)
+    int64_t dz_stride;
+    Prepared dx, dweight;
+};
+template <class T>
+Gradient prepare_gradient(const Linear& p, int64_t rows, const cpde_rows* x, const cpde_rows* weight, const cpde_rows& dy, bool dx,
+                          bool dweight) {
+    const bool bent = p.activation != CPDE_NONE;
+    // (rows and widths to whole chunks are what is written)
+    const int in = pitch_of(p.inputs), o = pitch_of(p.outputs);
+    const bool two = bent && sizeof(T) == 2 && rows * o <= kFewInner;
+    Gradient g{};
+    g.two_x = two && dx && rows * in <= kFew && int64_t(o) * in <= kFewInner;
+    g.two_w = two && dweight && int64_t(o) * in <= kFew && rows * in <= kFewInner;
+    g.dz = bent ? p.work + p.dz : dy.data;
+    g.dz_stride = !bent ? dy.stride : g.two_x || g.two_w ? 2 * o : o;
+    if (dx)
+        g.dx = prepare<true, false, T>(
+            p, g.two_x ? Sides{g.dz, p.work + p.twice[0], g.dz_stride, in, rows, 2 * o, p.inputs, true, true}
+                       : Sides{g.dz, weight->data, g.dz_stride, weight->stride, rows, p.outputs, p.inputs, bent, false});
+    if (dweight)
+        g.dweight = prepare<false, false, T>(
+            p, g.two_w ? Sides{g.dz, p.work + p.twice[1], o, in, p.outputs, 2 * rows, p.inputs, true, true}
+                       : Sides{g.dz, x->data, g.dz_stride, x->stride, p.outputs, rows, p.inputs, bent, false});
+    return g;
+}
+
+// What runs for a product.
+std::string describe(const Prepared& r) {
+    const auto& [args, cut, wide] = r.product;
+    if (r.product.empty()) return "nothing";
+    std::string s = std::string(cut.side == 32 ? "product_run_k " : cut.side == 256 ? "product_large_k " : "product_k ") +
+                    std::to_string(cut.side) + " splits " + std::to_string(args.splits);
+    if (!wide) s += " through registers";
+    if (r.copy[0].from || r.copy[1].from) s += " copied";
+    return s;
+}
+
 // A matrix argument of `rows` x `columns`; an output's rows do not overlap.
 void check_rows(const cpde_rows* r, int64_t rows, int64_t columns, bool output) {
     require(r, "null argument");
@@ -361,6 +403,26 @@ int cpde_linear_destroy(cpde_linear* linear) {
     });
 }
 
+int cpde_linear_info(cpde_linear* linear, int64_t rows, int aligned, char* text, size_t capacity) {
+    return guarded([&] {
+        require(linear && text && capacity, "null argument");
+        const Linear& p = *linear;
+        require(rows >= 0 && rows <= p.rows, "more rows than the plan's");
+        with_type(p.dtype, [&](auto element) {
+            using T = decltype(element);
+            // (addresses are looked at, and not used)
+            const auto of = [&](int columns) { return cpde_rows{reinterpret_cast<void*>(aligned ? 256 : 256 + sizeof(T)), columns}; };
+            const cpde_rows x = of(p.inputs), dy = of(p.outputs);
+            std::string s = "forward " + describe(prepare<true, true, T>(p, {x.data, x.data, x.stride, x.stride, rows, p.inputs, p.outputs, false, false}));
+            if (p.backward) {
+                const Gradient g = prepare_gradient<T>(p, rows, &x, &x, dy, true, true);
+                s += ", dx " + describe(g.dx) + ", dweight " + describe(g.dweight);
+            }
+            std::snprintf(text, capacity, "%s", s.c_str());
+        });
+    });
+}
+
 int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, const cpde_rows* weight, const void* bias,
                         const cpde_rows* residual, const cpde_rows* y, const cpde_rows* pre) {
     return guarded([&] {
@@ -424,23 +486,8 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
         TraceScope trace(d, kTraceLinearGradient, 2.0 * ((dx != nullptr) + (dweight != nullptr)) * rows * p.inputs * p.outputs);
         with_type(p.dtype, [&](auto element) {
             using T = decltype(element);
+            const Gradient g = prepare_gradient<T>(p, rows, x, weight, *dy, dx != nullptr, dweight != nullptr);
             const int in = pitch_of(p.inputs), o = pitch_of(p.outputs);
-            // (rows and widths to whole chunks are what is written)
-            const bool two = bent && sizeof(T) == 2 && rows * o <= kFewInner;
-            const bool two_x = two && dx && rows * in <= kFew && int64_t(o) * in <= kFewInner;
-            const bool two_w = two && dweight && int64_t(o) * in <= kFew && rows * in <= kFewInner;
-            const void* dz = bent ? p.work + p.dz : dy->data;  // (the plan's own: whole chunks, zeros behind the columns)
-            const int64_t dz_stride = !bent ? dy->stride : two_x || two_w ? 2 * o : o;
-            // both products are cut before the first launch: a refused call writes nothing
-            Prepared for_x, for_w;
-            if (dx)
-                for_x = prepare<true, false, T>(
-                    p, two_x ? Sides{dz, p.work + p.twice[0], dz_stride, in, rows, 2 * o, p.inputs, true, true}
-                             : Sides{dz, weight->data, dz_stride, weight->stride, rows, p.outputs, p.inputs, bent, false});
-            if (dweight)
-                for_w = prepare<false, false, T>(
-                    p, two_w ? Sides{dz, p.work + p.twice[1], o, in, p.outputs, 2 * rows, p.inputs, true, true}
-                             : Sides{dz, x->data, dz_stride, x->stride, p.outputs, rows, p.inputs, bent, false});
             if ((bent || dbias) && p.outputs) {
                 SlopeArgs a{};
                 a.dy = dy->data;
@@ -452,8 +499,8 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     a.pre = pre->data;
                     a.pre_stride = pre->stride;
                     a.dz = p.work + p.dz;
-                    a.dz_stride = int(dz_stride);
-                    a.low = two_x || two_w ? o : 0;
+                    a.dz_stride = int(g.dz_stride);
+                    a.low = g.two_x || g.two_w ? o : 0;
                 }
                 if (dbias) a.part = reinterpret_cast<float*>(p.work + p.bias_part);
                 // strips of 32 rows at least, and workgroups for the whole device
@@ -463,17 +510,17 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                 const int strips = a.strips = std::max(1, ceil_div(rows, a.strip));
                 // weights again below themselves, where dz and what it leaves stand side by side; rows of
                 // x in turn with themselves, where those are rows of o
-                if (two_x) {
+                if (g.two_x) {
                     a.from[0] = weight->data;
                     a.to[0] = p.work + p.twice[0];
                     a.copy[0] = {weight->stride, p.outputs, o, p.inputs, in, 1, o};
                 }
-                if (two_w) {
+                if (g.two_w) {
                     a.from[1] = x->data;
                     a.to[1] = p.work + p.twice[1];
                     a.copy[1] = {x->stride, rows, rows, p.inputs, in, 2, 1};
                 }
-                const int64_t chunks = std::max(two_x ? int64_t(o) * in : 0, two_w ? rows * in : 0) / 8;
+                const int64_t chunks = std::max(g.two_x ? int64_t(o) * in : 0, g.two_w ? rows * in : 0) / 8;
                 const int copiers = int(std::min<int64_t>(ceil_div(chunks, 256 * column_blocks), most));
                 hipLaunchKernelGGL((linear_slope_k<T>), dim3(column_blocks, strips + copiers), 256, 0, d.stream, a);
                 HIP_CHECK(hipGetLastError());
@@ -487,7 +534,7 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                 LinearEpilogue<T> e{};
                 e.y = static_cast<T*>(dx->data);
                 e.y_stride = dx->stride;
-                launch<true, false, T>(p, for_x, e);
+                launch<true, false, T>(p, g.dx, e);
             }
             if (dweight) {
                 LinearEpilogue<T> e{};
@@ -497,7 +544,7 @@ int cpde_linear_backward(cpde_linear* linear, int64_t rows, const cpde_rows* x, 
                     e.residual = e.y;
                     e.residual_stride = e.y_stride;
                 }
-                launch<false, false, T>(p, for_w, e);
+                launch<false, false, T>(p, g.dweight, e);
             }
         });
     });

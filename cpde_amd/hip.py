@@ -218,6 +218,7 @@ SIGNATURES = {
     'cpde_dropout': (i32, [vp, i32, i64, i64, rows_p, rows_p, rows_p, ctypes.c_double, u64, u64]),
     'cpde_linear_create': (i32, [vp, i32, i64, i32, i32, i32, i32, ctypes.POINTER(vp)]),
     'cpde_linear_destroy': (i32, [vp]),
+    'cpde_linear_info': (i32, [vp, i64, i32, ctypes.c_char_p, ctypes.c_size_t]),
     'cpde_linear_forward': (i32, [vp, i64, rows_p, rows_p, vp, rows_p, rows_p, rows_p]),
     'cpde_linear_backward': (i32, [vp, i64, rows_p, rows_p, rows_p, rows_p, rows_p, rows_p, vp, i32]),
     'cpde_rotation_create': (i32, [vp, ctypes.POINTER(RotationShape), ctypes.POINTER(vp)]),
@@ -708,6 +709,13 @@ class Linear:
         for name, a in bias.items():
             if a is not None:
                 _list_holds(name, a, self.element, gpu, self.outputs)
+
+    def info(self, rows, aligned=True):
+        """The kernels that calls of `rows` rows run on contiguous matrices (aligned: from whole
+        16 bytes on), their tiles and splits."""
+        text = ctypes.create_string_buffer(256)
+        check(load().cpde_linear_info(self.handle, rows, int(aligned), text, 256))
+        return text.value.decode()
 
     def forward(self, rows, x, weight, y, bias=None, residual=None, pre=None):
         self._check(rows, {'x': x}, {'y': y, 'residual': residual, 'pre': pre}, {'weight': weight}, {'bias': bias})

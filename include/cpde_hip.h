@@ -501,6 +501,11 @@ int cpde_dropout(cpde_device* dev, int dtype, int64_t rows, int64_t columns, con
 int cpde_linear_create(cpde_device* dev, int dtype, int64_t rows, int inputs, int outputs, int activation, int backward,
                        cpde_linear** out);
 int cpde_linear_destroy(cpde_linear* linear);
+/* The kernels that calls of `rows` rows run on contiguous matrices that start at whole 16 bytes
+ * (aligned = 1) or do not, the side of their tiles and over how many splits of the inner axis:
+ * "forward product_k 64 splits 1 through registers" and, with a backward,
+ * ", dx product_large_k 256 splits 1, dweight product_k 128 splits 3 copied". */
+int cpde_linear_info(cpde_linear* linear, int64_t rows, int aligned, char* text, size_t capacity);
 /* bias and residual may be NULL, and residual may be y.  pre (may be NULL) gets
  * x W^T + bias, rounded to the type, which the backward of a plan with an activation
  * needs. */
