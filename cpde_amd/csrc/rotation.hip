@@ -54,14 +54,17 @@ __device__ inline float sum_group(float x) {
     return x;
 }
 
-// What a lane holds of a head's vector: four pairs of columns.  WIDE: two runs of four
-// columns, from `first` and from `second` (interleaved: one run of eight); otherwise
-// single columns, -1 where there is none.  Columns that are not turned are pairs of an
-// angle of zero.
+// What a lane holds of a head's vector: pairs of columns.  WIDE: four of them, as two runs of
+// four columns, from `first` and from `second` (interleaved: one run of eight); otherwise two,
+// single columns, -1 where there is none (64 lanes hold the widest head).  Columns that are not
+// turned are pairs of an angle of zero.
+template <bool WIDE>
+constexpr int kPairs = WIDE ? 4 : 2;
 template <bool WIDE>
 struct Columns {
-    int first[WIDE ? 1 : 4], second[WIDE ? 1 : 4];
-    int unit[4];  // number of the pair, -1 where it is not turned
+    static constexpr int N = kPairs<WIDE>;
+    int first[WIDE ? 1 : N], second[WIDE ? 1 : N];
+    int unit[N];  // number of the pair, -1 where it is not turned
     bool live;
     __device__ void start(const RotationArgs& a, int lane) {
         if constexpr (WIDE) {
@@ -70,11 +73,11 @@ struct Columns {
             first[0] = turned && !a.interleaved ? 4 * lane : 8 * lane;
             second[0] = turned && !a.interleaved ? a.pairs + 4 * lane : 8 * lane + 4;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) unit[j] = turned ? 4 * lane + j : -1;
+            for (int j = 0; j < N; ++j) unit[j] = turned ? 4 * lane + j : -1;
         } else {
             live = true;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < N; ++j) {
                 const int u = lane + 64 * j;
                 unit[j] = u < a.pairs ? u : -1;
                 first[j] = u < a.pairs ? (a.interleaved ? 2 * u : u) : 2 * u;  // (2 pairs + 2 (u - pairs))
@@ -85,7 +88,7 @@ struct Columns {
         }
     }
     template <class T>
-    __device__ void load(const T* p, const RotationArgs& a, float (&u)[4], float (&v)[4]) const {
+    __device__ void load(const T* p, const RotationArgs& a, float (&u)[N], float (&v)[N]) const {
         if constexpr (WIDE) {
             vec<T, 4> lo = {}, hi = {};
             if (live) {
@@ -103,14 +106,14 @@ struct Columns {
             v[3] = float(hi[3]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < N; ++j) {
                 u[j] = first[j] >= 0 ? float(p[first[j]]) : 0.f;
                 v[j] = second[j] >= 0 ? float(p[second[j]]) : 0.f;
             }
         }
     }
     template <class T>
-    __device__ void store(T* p, const RotationArgs& a, const float (&u)[4], const float (&v)[4]) const {
+    __device__ void store(T* p, const RotationArgs& a, const float (&u)[N], const float (&v)[N]) const {
         if constexpr (WIDE) {
             if (!live) return;
             const bool across = a.interleaved && unit[0] >= 0;
@@ -120,7 +123,7 @@ struct Columns {
             *reinterpret_cast<vec<T, 4>*>(p + second[0]) = hi;
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < N; ++j) {
                 if (first[j] >= 0) p[first[j]] = T(u[j]);
                 if (second[j] >= 0) p[second[j]] = T(v[j]);
             }
@@ -165,7 +168,8 @@ __device__ inline void start_tokens(const RotationArgs& a, Tokens& t, int64_t fi
 }
 // A lane's cosines and sines of a token.
 template <bool WIDE>
-__device__ inline void turn_of(const Tokens& t, int token, const Columns<WIDE>& columns, float (&c)[4], float (&s)[4]) {
+__device__ inline void turn_of(const Tokens& t, int token, const Columns<WIDE>& columns, float (&c)[kPairs<WIDE>],
+                               float (&s)[kPairs<WIDE>]) {
     if constexpr (WIDE) {
         typedef float Quad __attribute__((ext_vector_type(4)));
         Quad cos = {1, 1, 1, 1}, sin = {};
@@ -180,7 +184,7 @@ __device__ inline void turn_of(const Tokens& t, int token, const Columns<WIDE>& 
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kPairs<WIDE>; ++j) {
             c[j] = columns.unit[j] >= 0 ? t.cos[token][columns.unit[j]] : 1.f;
             s[j] = columns.unit[j] >= 0 ? t.sin[token][columns.unit[j]] : 0.f;
         }
@@ -208,11 +212,12 @@ __device__ __attribute__((always_inline)) inline void each_head(const Side& side
 }
 // A side's weights in a lane's columns; ones where there are none.
 template <class T, bool WIDE>
-__device__ inline void weights_of(const RotationArgs& a, const Side& side, const Columns<WIDE>& columns, float (&u)[4], float (&v)[4]) {
+__device__ inline void weights_of(const RotationArgs& a, const Side& side, const Columns<WIDE>& columns, float (&u)[kPairs<WIDE>],
+                                  float (&v)[kPairs<WIDE>]) {
     if (side.weight) columns.load(reinterpret_cast<const T*>(side.weight), a, u, v);
     else
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = v[j] = 1;
+        for (int j = 0; j < kPairs<WIDE>; ++j) u[j] = v[j] = 1;
 }
 
 // A workgroup takes a few tokens, a group of LANES lanes one head's vector after another.
@@ -222,6 +227,7 @@ __device__ inline void weights_of(const RotationArgs& a, const Side& side, const
 // channels of memory (54 and 69 us).
 template <class T, int LANES, bool WIDE>
 __global__ __launch_bounds__(256) void rotation_forward_k(RotationArgs a) {
+    constexpr int N = kPairs<WIDE>;
     __shared__ __align__(16) Tokens t;
     const int64_t first = int64_t(blockIdx.x) * a.most;
     const int count = int(min(int64_t(a.most), a.count - first));
@@ -232,22 +238,22 @@ __global__ __launch_bounds__(256) void rotation_forward_k(RotationArgs a) {
     for (int k = 0; k < 2; ++k) {
         const Side& side = a.side[k];
         if (!side.heads) continue;
-        float wu[4], wv[4];
+        float wu[N], wv[N];
         weights_of<T>(a, side, columns, wu, wv);
         each_head<LANES>(side, count, [&](int token, int head) __attribute__((always_inline)) {
-            float u[4] = {}, v[4] = {};
+            float u[N] = {}, v[N] = {};
             if (t.position[token] >= 0) {  // (a place without a token, whose row is zeros, is not read)
                 columns.load(reinterpret_cast<const T*>(side.x) + t.x[k][token] + head * side.x_head, a, u, v);
-                float up = 1, c[4], s[4];
+                float up = 1, c[N], s[N];
                 if (a.norm) {
                     float square = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) square += u[j] * u[j] + v[j] * v[j];
+                    for (int j = 0; j < N; ++j) square += u[j] * u[j] + v[j] * v[j];
                     up = 1.f / sqrtf(sum_group<LANES>(square) / a.dim + a.eps);
                 }
                 turn_of(t, token, columns, c, s);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < N; ++j) {
                     const float x = u[j] * up * wu[j], y = v[j] * up * wv[j];
                     u[j] = x * c[j] - y * s[j];
                     v[j] = x * s[j] + y * c[j];
@@ -263,13 +269,13 @@ __global__ __launch_bounds__(256) void rotation_forward_k(RotationArgs a) {
 // through the tokens with a stride; their sums are joined in fixed order.
 template <class T, int LANES, bool WIDE>
 __global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
-    constexpr int kGroups = 256 / LANES;
+    constexpr int kGroups = 256 / LANES, N = kPairs<WIDE>;
     __shared__ __align__(16) Tokens t;
-    __shared__ float sums[kGroups][LANES * 8 + 1];
+    __shared__ float sums[kGroups][LANES * 2 * N + 1];
     const int lane = threadIdx.x % LANES;
     Columns<WIDE> columns;
     columns.start(a, lane);
-    float du[2][4] = {}, dv[2][4] = {};
+    float du[2][N] = {}, dv[2][N] = {};
     for (int64_t first = int64_t(blockIdx.x) * a.most; first < a.count; first += int64_t(gridDim.x) * a.most) {
         const int count = int(min(int64_t(a.most), a.count - first));
         __syncthreads();
@@ -278,17 +284,17 @@ __global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
         for (int k = 0; k < 2; ++k) {
             const Side& side = a.side[k];
             if (!side.heads) continue;
-            float wu[4], wv[4];
+            float wu[N], wv[N];
             weights_of<T>(a, side, columns, wu, wv);
             each_head<LANES>(side, count, [&](int token, int head) __attribute__((always_inline)) {
-                float u[4] = {}, v[4] = {}, gu[4] = {}, gv[4] = {};
+                float u[N] = {}, v[N] = {}, gu[N] = {}, gv[N] = {};
                 if (t.position[token] >= 0) {
                     columns.load(reinterpret_cast<const T*>(side.x) + t.x[k][token] + head * side.x_head, a, u, v);
                     columns.load(reinterpret_cast<const T*>(side.dy) + t.dy[k][token] + head * side.dy_head, a, gu, gv);
-                    float c[4], s[4], square = 0, dot = 0;
+                    float c[N], s[N], square = 0, dot = 0;
                     turn_of(t, token, columns, c, s);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < N; ++j) {
                         const float back = gu[j] * c[j] + gv[j] * s[j];
                         gv[j] = gv[j] * c[j] - gu[j] * s[j];
                         gu[j] = back;
@@ -296,7 +302,7 @@ __global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
                     }
                     const float up = a.norm ? 1.f / sqrtf(sum_group<LANES>(square) / a.dim + a.eps) : 1.f;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < N; ++j) {
                         u[j] *= up;
                         v[j] *= up;
                         du[k][j] += gu[j] * u[j];
@@ -307,7 +313,7 @@ __global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
                     }
                     const float mean = a.norm ? sum_group<LANES>(dot) / a.dim : 0.f;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < N; ++j) {
                         gu[j] = up * (gu[j] - u[j] * mean);
                         gv[j] = up * (gv[j] - v[j] * mean);
                     }
@@ -320,16 +326,16 @@ __global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
     for (int keys = 0; keys < 2; ++keys) {
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            sums[threadIdx.x / LANES][lane * 8 + j] = du[keys][j];
-            sums[threadIdx.x / LANES][lane * 8 + 4 + j] = dv[keys][j];
+        for (int j = 0; j < N; ++j) {
+            sums[threadIdx.x / LANES][lane * 2 * N + j] = du[keys][j];
+            sums[threadIdx.x / LANES][lane * 2 * N + N + j] = dv[keys][j];
         }
         __syncthreads();
         // (in the order of the lanes' places; rotation_weights_k undoes it)
-        for (int i = threadIdx.x; i < LANES * 8; i += 256) {
+        for (int i = threadIdx.x; i < LANES * 2 * N; i += 256) {
             float total = 0;
             for (int g = 0; g < kGroups; ++g) total += sums[g][i];
-            a.part[(int64_t(blockIdx.x) * 2 + keys) * (LANES * 8) + i] = total;
+            a.part[(int64_t(blockIdx.x) * 2 + keys) * (LANES * 2 * N) + i] = total;
         }
     }
 }
@@ -337,18 +343,19 @@ __global__ __launch_bounds__(256) void rotation_gradient_k(RotationArgs a) {
 // The workgroups' sums in order: 16 places and 64 runs of workgroups a workgroup.
 template <class T, int LANES, bool WIDE>
 __global__ __launch_bounds__(1024) void rotation_weights_k(RotationArgs a, int blocks, T* dq_weight, T* dk_weight) {
+    constexpr int N = kPairs<WIDE>;
     __shared__ float sums[64][17];
     const int keys = blockIdx.y, in = threadIdx.x & 15, run = threadIdx.x >> 4, place = blockIdx.x * 16 + in;
     const int per = (blocks + 63) / 64;
     float total = 0;
-    for (int b = run * per; b < min(blocks, (run + 1) * per); ++b) total += a.part[(int64_t(b) * 2 + keys) * (LANES * 8) + place];
+    for (int b = run * per; b < min(blocks, (run + 1) * per); ++b) total += a.part[(int64_t(b) * 2 + keys) * (LANES * 2 * N) + place];
     sums[run][in] = total;
     __syncthreads();
     T* to = keys ? dk_weight : dq_weight;
     if (run || !to) return;
     for (int r = 1; r < 64; ++r) total += sums[r][in];
-    const int lane = place / 8, j = place & 3;
-    const bool second = place & 4;
+    const int lane = place / (2 * N), j = place % N;
+    const bool second = place & N;
     Columns<WIDE> columns;
     columns.start(a, lane);
     int column;
@@ -474,7 +481,7 @@ int cpde_rotation_create(cpde_device* dev, const cpde_rotation_shape* shape, cpd
         p->dev = dev;
         p->shape = s;
         p->blocks = dev->compute_units * kGradientBlocks;
-        const size_t pairs = size_t(s.rotated / 2), part = s.backward ? size_t(p->blocks) * 2 * 64 * 8 : 0;
+        const size_t pairs = size_t(s.rotated / 2), part = s.backward ? size_t(p->blocks) * 2 * kMaxDim : 0;
         char* memory = nullptr;
         HIP_CHECK(hipMalloc(&memory, kMaxDim * sizeof(double) + part * sizeof(float)));
         p->rates = reinterpret_cast<double*>(memory);
@@ -579,7 +586,7 @@ int cpde_rotation_backward(cpde_rotation* rotation, const cpde_heads* q, const c
                 hipLaunchKernelGGL((rotation_gradient_k<T, L, W>), blocks, 256, 0, d.stream, a);
                 HIP_CHECK(hipGetLastError());
                 if (a.part)
-                    hipLaunchKernelGGL((rotation_weights_k<T, L, W>), dim3(L * 8 / 16, 2), 1024, 0, d.stream, a, blocks,
+                    hipLaunchKernelGGL((rotation_weights_k<T, L, W>), dim3(L * 2 * kPairs<W> / 16, 2), 1024, 0, d.stream, a, blocks,
                                        static_cast<T*>(dq_weight), static_cast<T*>(dk_weight));
             });
         });
