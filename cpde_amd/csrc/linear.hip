@@ -209,8 +209,8 @@ constexpr int kStrips = 256;  // of a bias's gradient
 // Gradients of at most kFew values, from matrices of at most kFewInner, take a 16-bit dz as a
 // sum of two values (the inner axis twice as long, its other operand written twice by
 // linear_slope_k), and are as exact as the type.  Such calls wait for launches more than for
-// products (256 -> 256, 256 rows: 13.5 us with and without; 128 -> 128, 1,000 rows: 16.4 for
-// 13.5; 64 -> 64, 16,384 rows: 33 for 27).  Beyond, dz is rounded once and the products run at
+// products (256 -> 256, 256 rows: 12.9 us for 10.9; 128 -> 128, 1,000 rows: 16.4 for 12.6; 64 -> 64,
+// 16,384 rows: 32.5 for 27.3).  Beyond, dz is rounded once and the products run at
 // the matrix units' rate: the results lie 1.4 times as far from the exact ones.
 constexpr int64_t kFew = 1 << 17, kFewInner = 1 << 20;
 
@@ -259,8 +259,8 @@ Prepared prepare(const Linear& p, const Sides& s) {
     // Operands that are not whole chunks come through registers, 64 x 64 tiles at a time, where the
     // product is small or few tiles share them; else they are copied to whole chunks first, for larger
     // tiles (a plan whose widths are not whole eights has room for it).  2,047 -> 2,047: 256 rows bf16
-    // 14.8 us through registers, 20.7 copied, f32 29.7 and 36.4; 512 rows 27.2 and 25.9, 69.5 and 49.1;
-    // 2,048 rows 51.2 and 39.7, 156 and 124.  130 rows, 2,047 -> 8,191: 30.3 and 33.2, 66 and 84.
+    // 13.8 us through registers, 19.2 copied, f32 31.6 and 35.9; 512 rows 20.0 and 25.1, 71.0 and 47.8;
+    // 2,048 rows 47.8 and 40.9, 155 and 116.  130 rows, 2,047 -> 8,191: 27.5 and 31.5, 67 and 82.
     const int64_t m_tiles = ceil_div(s.m, 64), n_tiles = ceil_div(s.n, 64), deep = ceil_div(s.k, kDepth<T>);
     const bool shared = std::min(m_tiles, n_tiles) > 3 && deep * m_tiles * n_tiles > 56 * int64_t(d.compute_units);
     if ((!args.a.wide || !args.b.wide) && p.a_copy && shared) {

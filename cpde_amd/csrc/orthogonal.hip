@@ -12,9 +12,12 @@ namespace {
 // after a few steps, where s was not too small.
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 // The products' operands are f16, times 2^12: entries of X, A and b A + c A^2 lie below 4,
-// and those down to 2^-26 stay in the type's normal range.  f32 and f16 matrices go as sums
-// of two f16 values (22 bits; three of the four products, to 2^-22), so that the products
-// stay as exact as the type; bf16 ones as one.  X itself is kept as a sum of two whatever the
+// and one value has its 11 bits down to 2^-26.  f32 and f16 matrices go as sums of two f16
+// values, three of the four products: off by 2^-22 of an entry, or by 2^-37, the second one's
+// smallest steps, where the entry is below 2^-15.  That is of matrices of norm one: the sums of
+// (b A + c A^2) X take it `side` times, 2^-24 of X up to a side of 8,192, and X's own entries
+// are 2^-13 or more in the mean up to 8,192 x 8,192.  So the products stay as exact as the type; bf16
+// matrices go as one value.  X itself is kept as a sum of two whatever the
 // type: its roundings pass through all later steps, which multiply small singular values by
 // up to 485.  With one value an operand the diagonals D of A and of b A + c A^2 stay apart in
 // 32 bits, and the operands hold zeros there: a row's diagonal is the largest of it, and

@@ -81,7 +81,8 @@ __device__ inline auto part(const F& f) {
     else return f;
 }
 
-// A sum of two f16 values, 22 bits together.  Matrices of them hold 32 first parts and then
+// A sum of two f16 values, 22 bits together where the second is one of the type's normal values
+// (smaller sums are off by 2^-25 at most).  Matrices of them hold 32 first parts and then
 // the 32 second ones, and so on, in rows of whole such groups.  Three of the four products
 // are exact to 2^-21 of the factors'.
 struct Pair {

@@ -508,7 +508,9 @@ int cpde_linear_destroy(cpde_linear* linear);
 int cpde_linear_info(cpde_linear* linear, int64_t rows, int aligned, char* text, size_t capacity);
 /* bias and residual may be NULL, and residual may be y.  pre (may be NULL) gets
  * x W^T + bias, rounded to the type, which the backward of a plan with an activation
- * needs. */
+ * needs.  Matrices that start at whole 16 bytes, in rows of whole 16 bytes up to 4 MiB apart,
+ * run fastest; of a plan whose widths are whole eights, others run on tiles of 64 x 64 whatever
+ * the size. */
 int cpde_linear_forward(cpde_linear* linear, int64_t rows, const cpde_rows* x, const cpde_rows* weight, const void* bias,
                         const cpde_rows* residual, const cpde_rows* y, const cpde_rows* pre);
 /* The gradients of x, W and bias from y's (the residual's is y's own): with
@@ -542,7 +544,8 @@ int cpde_rotation_destroy(cpde_rotation* rotation);
  * the tensors' type, NULL for ones.  positions: int32 [batch][tokens] on the device, NULL
  * for the token's number; a negative one marks a place without a token, whose results are
  * zeros whatever stands there.  q_out may be q, and k_out k.  Angles are taken in 64 bits
- * at every position. */
+ * at every position; a head's squares are summed in 32 (columns beyond 10^18 may give
+ * zeros). */
 int cpde_rotation_forward(cpde_rotation* rotation, const cpde_heads* q, const cpde_heads* k, const void* q_weight,
                           const void* k_weight, const int32_t* positions, const cpde_heads* q_out,
                           const cpde_heads* k_out);
@@ -554,7 +557,8 @@ int cpde_rotation_backward(cpde_rotation* rotation, const cpde_heads* q, const c
                            const cpde_heads* dk_out, const cpde_heads* dq, const cpde_heads* dk, void* dq_weight,
                            void* dk_weight);
 
-/* `count` matrices [rows][columns] by their strides in elements, columns contiguous. */
+/* `count` matrices [rows][columns] by their strides in elements, columns contiguous.  Those
+ * written do not overlap, but may lie between one another's rows. */
 typedef struct {
     void* data;
     int64_t matrix, row;
@@ -564,13 +568,14 @@ typedef struct {
  * X <- a X + b (X X^T) X + c (X X^T)^2 X with (a, b, c) = (3.4445, -4.7750, 2.0315), which
  * keeps the singular vectors and takes the singular values into 0.68..1.13 (five steps: those
  * above about 0.003 of |x|).  The products run on f16 operands: f32 and f16 matrices as sums of two
- * (22 bits), bf16 ones as one.  A matrix of zeros gives zeros. */
+ * (off by 2^-22 of an entry, or 2^-37 of |x| where that is more), bf16 ones as one.  A matrix of
+ * zeros gives zeros.  At most 1,024 matrices of at most 2^20 rows and columns, 1 to 32 steps. */
 int cpde_orthogonal_create(cpde_device* dev, int dtype, int count, int rows, int columns, int steps, cpde_orthogonal** out);
 int cpde_orthogonal_destroy(cpde_orthogonal* orthogonal);
 /* out = O(x); out may be x. */
 int cpde_orthogonal_forward(cpde_orthogonal* orthogonal, const cpde_matrices* x, const cpde_matrices* out);
-/* One step of an optimizer (beside cpde_rprop and cpde_adam) on weights of any layers of
- * one shape: momentum <- factor momentum + gradient, u = momentum (nesterov = 1:
+/* One step of an optimizer on the caller's weights, of any layers of one shape (cpde_rprop and
+ * cpde_adam are those of a cpde_net's own): momentum <- factor momentum + gradient, u = momentum (nesterov = 1:
  * gradient + factor momentum), weight <- (1 - rate decay) weight -
  * rate sqrt(max(1, rows / columns)) O(u).  gradient and weight are of the plan's type, the
  * momentum is float whatever that is. */
