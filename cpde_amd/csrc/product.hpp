@@ -234,7 +234,7 @@ struct TileSide {
     // Through registers, for any other, by 16-byte loads of any alignment, all under way at
     // once.  16-bit chunks over the end of a row are loaded as far ahead as they go over it, and
     // moved back (gradients of 8,192 rows, 255 -> 255: 44 us; value by value 110).  Floats there,
-    // and rows shorter than a chunk, go value by value (the same in floats: 56 us; moved 62).
+    // and rows shorter than a chunk, go value by value (the same in floats: 53 us; moved 62).
     using Chunk = vec<std::conditional_t<std::is_same_v<T, Pair>, float, T>, kChunk>;
     using Held = Chunk[kSteps];
     // Of eight 16-bit values those from `by` (0 to 8) on, then zeros.
